@@ -17,6 +17,7 @@
 #include "../../include/lily_sampler.h"
 #include "../../include/lily_sampler_math.h"
 #include "api_internal.h"
+#include "device_scope.h"
 #include "launch.h"
 
 using namespace lily;
@@ -45,28 +46,6 @@ int hip_fail(hipError_t e, const char* what) {
         }                                  \
     } while (0)
 
-// Makes `device` the calling thread's current device for the rest of the enclosing scope and
-// puts the caller's own choice back on the way out: a library call must not leave the host
-// thread on another GPU than it came with.
-struct DeviceScope {
-    int before = -1;
-    bool switched = false;
-    hipError_t err = hipSuccess;
-    explicit DeviceScope(int device) {
-        err = hipGetDevice(&before);
-        if (err == hipSuccess && before != device) {
-            err = hipSetDevice(device);
-            switched = err == hipSuccess;
-        }
-    }
-    ~DeviceScope() {
-        if (switched) {
-            DeviceScope device_scope_(before);
-        }
-    }
-    DeviceScope(const DeviceScope&) = delete;
-    DeviceScope& operator=(const DeviceScope&) = delete;
-};
 #define ON_DEVICE(device)                 \
     DeviceScope device_scope_(device);    \
     HIP_TRY(device_scope_.err)
