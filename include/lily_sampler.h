@@ -43,7 +43,9 @@ typedef enum lily_status {
     LILY_ERR_RANGE = -6        /* index or size beyond a stated limit */
 } lily_status;
 
-typedef enum lily_dtype { LILY_F32 = 0, LILY_BF16 = 1 } lily_dtype;
+/* LILY_E4M3 (8-bit floats, 4 exponent and 3 fraction bits, largest finite value 448, no infinities) is a
+ * type of the operators around the head (lily_rms_norm, lily_project), not of logits. */
+typedef enum lily_dtype { LILY_F32 = 0, LILY_BF16 = 1, LILY_E4M3 = 2 } lily_dtype;
 
 /* src/kernels/sample.rs:21-31 SamplingParams, field for field (top_k as u32). */
 typedef struct lily_sampling_params {
@@ -500,6 +502,46 @@ int lily_sample_rows_tiled(lily_sampler_t* s, const lily_rows* batch, const floa
 /* Both, in the sampler's stream: batch->logits_dev is where the logits are written (it is
  * written to although the field is const), batch->vocab and batch->rows size the product. */
 int lily_lm_head_sample_rows(lily_sampler_t* s, const lily_lm_head* head, const lily_rows* batch);
+
+/* ---- Around the head: the norm in front of it.
+ *
+ * The residual's addition and the root-mean-square norm that hand the head (or a projection) its
+ * hidden rows:
+ *     h = x + residual, rounded to stream_dtype (h = x where residual_dev is NULL)
+ *     y = h / sqrt(mean(h^2) + eps) * (weight + weight_offset)
+ * in f32.  h goes to sum_dev where that is given, y to out_dev: f32, bf16 (nearest even) or, for
+ * an 8-bit product, E4M3 with one f32 scale a row: scale = max|y| / 448, q = E4M3(y / scale).  A row
+ * whose largest |y| lies below 2^-116 has scale 0 and zeros; a row with a value that is not finite
+ * has what the formula gives, and in 8 bits a NaN scale.
+ *
+ * Rows hold d (1 .. LILY_NORM_MAX_D) elements, strides count elements and may be anything from d on;
+ * rows that start at multiples of 16 bytes in every array, with d a multiple of 8, go the fast way.
+ * sum_dev may be x_dev or residual_dev, and out_dev may be either, each with the same type and stride;
+ * other overlaps are refused, as far as they can be told from pointers, strides and sizes (arrays of one
+ * stride that lie side by side in wider rows do not overlap).  Enqueued on the sampler's stream; no
+ * workspace. */
+#define LILY_NORM_MAX_D 32768u
+typedef struct lily_norm {
+    uint32_t rows;
+    uint32_t d;
+    const void* x_dev;            /* [rows][x_stride] of x_dtype */
+    uint64_t x_stride;
+    const void* residual_dev;     /* [rows][residual_stride] of stream_dtype, or NULL */
+    uint64_t residual_stride;
+    void* sum_dev;                /* [rows][sum_stride] of stream_dtype, or NULL; only with a residual */
+    uint64_t sum_stride;
+    const void* weight_dev;       /* [d] of weight_dtype, or NULL (ones, and no weight_offset) */
+    void* out_dev;                /* [rows][out_stride] of out_dtype */
+    uint64_t out_stride;
+    float* scales_dev;            /* [rows]; with LILY_E4M3 only, and required there */
+    uint32_t x_dtype;             /* LILY_F32 or LILY_BF16, as stream_dtype and weight_dtype */
+    uint32_t stream_dtype;
+    uint32_t weight_dtype;
+    uint32_t out_dtype;           /* LILY_F32, LILY_BF16 or LILY_E4M3 */
+    float eps;                    /* finite, >= 0 */
+    float weight_offset;          /* 0, or 1 where the weights are stored less one */
+} lily_norm;
+int lily_rms_norm(lily_sampler_t* s, const lily_norm* norm);
 
 #ifdef __cplusplus
 }

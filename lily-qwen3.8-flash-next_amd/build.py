@@ -49,7 +49,9 @@ def units():
     out.append(("rows_tiles.hip", "rows_tiles.o", []))
     out.append(("rows_wide.hip", "rows_wide.o", []))
     out.append(("rows_argmax.hip", "rows_argmax.o", []))
+    out.append(("norm.hip", "norm.o", []))
     out.append(("sampler_api.cpp", "sampler_api.o", []))
+    out.append(("operators_api.cpp", "operators_api.o", []))
     return out
 
 

@@ -34,4 +34,8 @@ int scratch_device(const lily_scratch_t* sc);
 // draw finds it done.
 int static_scratch_init(int device);
 
+// What an operator's entry point needs of a sampler.
+int sampler_device(const lily_sampler_t* s);
+hipStream_t sampler_stream(const lily_sampler_t* s);
+
 }  // namespace lily

@@ -1,0 +1,14 @@
+// operators.h - host-callable launchers of the operators around the head.
+#pragma once
+
+#include <hip/hip_runtime_api.h>
+
+#include "../../include/lily_sampler.h"
+
+namespace lily {
+
+// The norm (norm.hip).  `pieces`: rows start at multiples of 16 bytes in every array and d is a
+// multiple of 8.
+hipError_t launch_rms_norm(hipStream_t stream, const lily_norm& norm, bool pieces);
+
+}  // namespace lily

@@ -1024,6 +1024,9 @@ int api_fail(int code, const char* fmt, ...) {
 
 int scratch_device(const lily_scratch_t* sc) { return sc->s->device; }
 
+int sampler_device(const lily_sampler_t* s) { return s->device; }
+hipStream_t sampler_stream(const lily_sampler_t* s) { return s->stream; }
+
 int sample_row_with_workspace(int device, hipStream_t stream, const Workspace& ws, const float* logits,
                               uint32_t vocab, lily_scratch_t* scratch,
                               const lily_sampling_params* params, uint32_t step, uint32_t* out) {

@@ -23,7 +23,8 @@ CTRL_STRIDE = 4
 SLOT_ACCEPTED = 0
 SLOT_KEEP = 1
 NO_TOKEN = 0xFFFFFFFF
-F32, BF16 = 0, 1
+F32, BF16, E4M3 = 0, 1, 2
+DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3}
 
 
 class SamplerError(RuntimeError):
@@ -105,6 +106,18 @@ class _LmHead(C.Structure):
                 ("group_size", C.c_uint32), ("logits_f32", C.c_uint32)]
 
 
+class _Norm(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("d", C.c_uint32),
+                ("x_dev", C.c_void_p), ("x_stride", C.c_uint64),
+                ("residual_dev", C.c_void_p), ("residual_stride", C.c_uint64),
+                ("sum_dev", C.c_void_p), ("sum_stride", C.c_uint64),
+                ("weight_dev", C.c_void_p),
+                ("out_dev", C.c_void_p), ("out_stride", C.c_uint64),
+                ("scales_dev", C.c_void_p),
+                ("x_dtype", C.c_uint32), ("stream_dtype", C.c_uint32), ("weight_dtype", C.c_uint32),
+                ("out_dtype", C.c_uint32), ("eps", C.c_float), ("weight_offset", C.c_float)]
+
+
 class QuantWeights:
     """The reference's affine weights (src/weights.rs:27-36): codes int32 [out, in * bits / 32]
     (u32 words, the lowest code first), scales and biases bf16 [out, in / group_size]."""
@@ -119,6 +132,7 @@ class QuantWeights:
 
 
 LOGIT_TILE_COLS = 128
+NORM_MAX_D = 32768
 
 
 def _load():
@@ -184,6 +198,7 @@ def _load():
         "lily_sample_rows_tiled": [vp, C.POINTER(_Rows), vp, vp],
         "lily_lm_head_sample_rows": [vp, C.POINTER(_LmHead), C.POINTER(_Rows)],
     }
+    sigs["lily_rms_norm"] = [vp, C.POINTER(_Norm)]
     L.lily_insertions_create.restype = C.c_int
     L.lily_insertions_create.argtypes = [u32, C.POINTER(vp)]
     L.lily_insertions_push.restype = C.c_int
@@ -536,6 +551,53 @@ class Sampler:
         h = self._head(hidden, weight, tile_max, tile_sum, logits)
         _check(_lib.lily_lm_head_sample_rows(self._h, C.byref(h), C.byref(r)))
         return keep
+
+
+    # -- around the head
+    def _matrix(self, t, rows, columns, name):
+        """(address, stride, type) of a [rows, columns] operand whose rows are contiguous."""
+        code = DTYPES.get(t.dtype)
+        if code is None:
+            raise SamplerError(-1, f"{name} must be F32, BF16 or E4M3, got {t.dtype}")
+        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != columns or (t.stride(1) != 1 and columns > 1):
+            raise SamplerError(-1, f"{name} must be [{rows}, {columns}], rows contiguous")
+        if not t.is_cuda or t.device.index != self.device:
+            raise SamplerError(-1, f"{name} must live on the sampler's device")
+        return t.data_ptr(), t.stride(0), code
+
+    def _vector(self, t, n, name):
+        """(address, type) of a contiguous vector of n elements, or nothing."""
+        if t is None:
+            return None, F32
+        code = DTYPES.get(t.dtype)
+        if code is None or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+            raise SamplerError(-1, f"{name} must be [{n}], contiguous")
+        if not t.is_cuda or t.device.index != self.device:
+            raise SamplerError(-1, f"{name} must live on the sampler's device")
+        return t.data_ptr(), code
+
+    def _scales(self, t, n, name):
+        at, code = self._vector(t, n, name)
+        if code != F32:
+            raise SamplerError(-1, f"{name} must be F32")
+        return at
+
+    def rms_norm(self, x, weight, out, eps=1e-6, residual=None, summed=None, weight_offset=0.0, scales=None):
+        """lily_rms_norm: out = (h / sqrt(mean(h^2) + eps)) * (weight + weight_offset), h = x + residual, h to
+        `summed`.  out: f32, bf16, or float8_e4m3fn with `scales` [rows] f32."""
+        if x.dim() != 2:
+            raise SamplerError(-1, "x must be [rows, d], rows contiguous")
+        rows, d = x.shape
+        xp, xs, xt = self._matrix(x, rows, d, "x")
+        op, os_, ot = self._matrix(out, rows, d, "out")
+        wp, wt = self._vector(weight, d, "weight")
+        rp, rs, rt = self._matrix(residual, rows, d, "residual") if residual is not None else (None, 0, F32)
+        sp, ss, st = self._matrix(summed, rows, d, "summed") if summed is not None else (None, 0, rt)
+        if st != rt:
+            raise SamplerError(-1, "summed must have the residual's type")
+        _check(_lib.lily_rms_norm(self._h, C.byref(_Norm(
+            rows, d, xp, xs, rp, rs, sp, ss, wp, op, os_, self._scales(scales, rows, "scales"), xt, rt, wt, ot,
+            eps, weight_offset))))
 
 
 class Plan:

@@ -1,0 +1,93 @@
+"""What the operators around the head refuse, told from the descriptor alone: no GPU needed (the
+descriptor is looked at before the sampler, so the calls are made without one; a call with nothing wrong
+answers that the sampler is missing)."""
+import ctypes as C
+
+import pytest
+
+import lily_sampler as LS
+
+INVALID, RANGE = -1, -6
+L = LS._lib
+
+
+def _said(rc):
+    return rc, L.lily_last_error().decode()
+
+
+def _norm(**over):
+    kw = dict(rows=4, d=64, x_dev=0x10000, x_stride=64, residual_dev=0x20000, residual_stride=64, sum_dev=0x30000,
+              sum_stride=64, weight_dev=0x40000, out_dev=0x50000, out_stride=64, scales_dev=None, x_dtype=LS.BF16,
+              stream_dtype=LS.BF16, weight_dtype=LS.F32, out_dtype=LS.BF16, eps=1e-6, weight_offset=0.0)
+    kw.update(over)
+    n = LS._Norm()
+    for k, v in kw.items():
+        setattr(n, k, v)
+    return n
+
+
+@pytest.mark.parametrize("over", [
+    dict(),
+    dict(rows=1, x_stride=0, residual_stride=0, sum_stride=0, out_stride=0),      # one row: strides say nothing
+    dict(residual_dev=None, sum_dev=None),
+    dict(weight_dev=None),
+    dict(weight_offset=1.0, eps=0.0),
+    dict(out_dtype=LS.E4M3, scales_dev=0x60000),
+    dict(sum_dev=0x20000),                                                        # in place of the residual
+    dict(sum_dev=0x10000, out_dev=0x20000),                                       # in place of both inputs
+    dict(d=63, x_dev=0x10002),
+    dict(d=LS.NORM_MAX_D, **{k: LS.NORM_MAX_D for k in ("x_stride", "residual_stride", "sum_stride", "out_stride")},
+         rows=1, weight_dtype=LS.BF16),
+    # columns side by side of one wide buffer
+    dict(x_dev=0x10000, residual_dev=0x10080, sum_dev=0x10100, out_dev=0x10180,
+         **{k: 256 for k in ("x_stride", "residual_stride", "sum_stride", "out_stride")}),
+])
+def test_a_sound_norm_only_lacks_the_sampler(over):
+    rc, text = _said(L.lily_rms_norm(None, C.byref(_norm(**over))))
+    assert rc == INVALID and text == "sampler is null"
+
+
+@pytest.mark.parametrize("over, code, word", [
+    (dict(x_dev=None), INVALID, "required"),
+    (dict(out_dev=None), INVALID, "required"),
+    (dict(rows=0), INVALID, "positive"),
+    (dict(d=0), INVALID, "positive"),
+    (dict(d=LS.NORM_MAX_D + 1), RANGE, "elements"),
+    (dict(rows=0x80000000), RANGE, "elements"),
+    (dict(x_dtype=LS.E4M3), INVALID, "LILY_BF16"),
+    (dict(stream_dtype=3), INVALID, "LILY_BF16"),
+    (dict(weight_dtype=LS.E4M3), INVALID, "LILY_BF16"),
+    (dict(out_dtype=3), INVALID, "out is"),
+    (dict(out_dtype=LS.E4M3), INVALID, "scales"),
+    (dict(scales_dev=0x60000), INVALID, "scales"),
+    (dict(residual_dev=None), INVALID, "needs a residual"),
+    (dict(eps=-1e-6), INVALID, "eps"),
+    (dict(eps=float("nan")), INVALID, "eps"),
+    (dict(eps=float("inf")), INVALID, "eps"),
+    (dict(weight_offset=float("nan")), INVALID, "eps"),
+    (dict(weight_dev=None, weight_offset=1.0), INVALID, "needs weights"),
+    (dict(x_stride=63), INVALID, "shorter"),
+    (dict(residual_stride=63), INVALID, "shorter"),
+    (dict(sum_stride=0), INVALID, "shorter"),
+    (dict(out_stride=63), INVALID, "shorter"),
+    (dict(x_dev=0x10001), INVALID, "multiple"),
+    (dict(weight_dev=0x40002), INVALID, "multiple"),
+    (dict(x_stride=1 << 62), RANGE, "address"),
+    (dict(x_dev=(1 << 63) - 64), RANGE, "address"),
+    (dict(sum_dev=0x10002), INVALID, "overlaps an input"),                   # shifted by one element
+    (dict(out_dev=0x10000, out_dtype=LS.F32), INVALID, "overlaps an input"),  # another type in the same place
+    (dict(out_dev=0x10000, out_stride=128), INVALID, "overlaps an input"),
+    (dict(out_dev=0x40000), INVALID, "weights"),
+    (dict(out_dev=0x30000), INVALID, "sum and out"),
+    (dict(out_dtype=LS.E4M3, scales_dev=0x50004), INVALID, "scales"),
+    (dict(out_dtype=LS.E4M3, scales_dev=0x10000), INVALID, "scales"),
+    (dict(x_dev=0x10000, out_dev=0x10080 - 2, x_stride=256, out_stride=256), INVALID, "overlaps an input"),
+    (dict(x_dev=0x10100, out_dev=0x10000, x_stride=160, out_stride=160), INVALID, "overlaps an input"),
+])
+def test_what_a_norm_refuses(over, code, word):
+    rc, text = _said(L.lily_rms_norm(None, C.byref(_norm(**over))))
+    assert rc == code and word in text, (rc, text)
+
+
+def test_a_missing_descriptor():
+    assert _said(L.lily_rms_norm(None, None))[0] == INVALID
