@@ -543,6 +543,38 @@ typedef struct lily_norm {
 } lily_norm;
 int lily_rms_norm(lily_sampler_t* s, const lily_norm* norm);
 
+/* ---- Processed logits: penalties, bias lists and masks applied to whole rows, and written out.
+ *
+ * The draws form these values for their candidates only; a host that scores tokens, ranks beams, draws
+ * by itself or returns log-probabilities needs the rows.  Of row r of the batch, for every id:
+ *     a = (l + its biases in list order; -inf where the mask bars it; else, if its count c > 0, the
+ *          repetition penalty and - (presence + frequency * c)) / T
+ * in f32, operation for operation as the draws form it (a NaN is worth -inf; T is what
+ * lily_params_effective reports, 1 for a greedy row), so a draw from the written f32 row with neutral
+ * settings is the draw from the raw row with the batch's.  log_sum_exp = log(sum of exp(a)); the
+ * log-probability is a - log_sum_exp, formed as (a - top) - log(sum of exp(a - top)), top the row's largest
+ * value.  A row in which nothing is left has a log_sum_exp of -inf and
+ * log-probabilities of -inf; one that holds +inf has +inf, and what the difference then gives.
+ *
+ * Of the batch: rows, vocab, dtype, logits_dev, row_stride, params, scratch, allow_dev, allow_stride,
+ * bias_dev and bias_offsets are looked at, the rest is not (no token is drawn, none is counted, forced
+ * tokens have no part in a row's distribution); out_ids_dev may be NULL, and rows under penalties may share a
+ * scratch, whose counts are only read.  out_dev may be logits_dev with the same type and stride; any other
+ * overlap of the two is refused.  Vocabularies up to 2^24 (LILY_ERR_RANGE beyond).  The sums of a row cut
+ * into slices pass through the sampler's workspace: graphs captured from one sampler are replayed one after
+ * the other.  More than eight rows are staged as lily_sample_rows stages them; a call that is to be captured
+ * into a graph goes through a plan. */
+typedef struct lily_logits_out {
+    void* out_dev;            /* [rows][out_stride] of out_dtype */
+    uint64_t out_stride;      /* elements */
+    uint32_t out_dtype;       /* LILY_F32 or LILY_BF16 (nearest even) */
+    uint32_t logprobs;        /* 0 = the adjusted logits, 1 = log-probabilities */
+    float* log_sum_exp_dev;   /* [rows] or NULL */
+} lily_logits_out;
+int lily_process_logits(lily_sampler_t* s, const lily_rows* batch, const lily_logits_out* out);
+/* The same of a resident batch: one or two launches, nothing staged. */
+int lily_plan_process_logits(lily_plan_t* p, const lily_logits_out* out);
+
 #ifdef __cplusplus
 }
 #endif

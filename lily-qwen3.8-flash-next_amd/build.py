@@ -50,6 +50,7 @@ def units():
     out.append(("rows_wide.hip", "rows_wide.o", []))
     out.append(("rows_argmax.hip", "rows_argmax.o", []))
     out.append(("norm.hip", "norm.o", []))
+    out.append(("logits_rows.hip", "logits_rows.o", []))
     out.append(("sampler_api.cpp", "sampler_api.o", []))
     out.append(("operators_api.cpp", "operators_api.o", []))
     return out

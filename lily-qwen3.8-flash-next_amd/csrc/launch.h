@@ -155,6 +155,24 @@ struct WideLooks {
 hipError_t launch_rows_wide(hipStream_t stream, int dtype, bool lse, uint32_t rows, const LaunchCfg& cfg,
                             const InlineRows* inline_rows, float* lane_max, uint32_t* count, uint64_t* bounds,
                             const WideLooks& looks);
+// Adjusted rows written out (logits_rows.hip): the rows of `table` (device) or `few` (at most INLINE_ROWS,
+// with the launch), RowArgs::row the row of `out`.  Vocabularies up to LOGITS_MAX_VOCAB.
+constexpr uint32_t LOGITS_SLICE_MAX = 262144;   // ids of a slice under a bias list (a bit each in LDS)
+constexpr uint32_t LOGITS_MAX_VOCAB = LOGITS_SLICE_MAX * MAX_SLICES;
+struct LogitsRows {
+    void* out = nullptr;
+    uint64_t stride = 0;       // elements
+    uint32_t out_dtype = 0;
+    bool logprobs = false;     // else the adjusted logits
+    bool biased = false;       // some row has a bias list
+    float* lse = nullptr;      // [rows of out] or null
+    Handed<double> part;       // workspace: [max_rows][MAX_SLICES][2]
+    uint32_t* ticket = nullptr;   // [max_rows], zero between launches
+    uint32_t max_rows = 0;
+    uint32_t handover = 0;     // 0 = by the launch's size, 1 = strict, 2 = relaxed
+};
+hipError_t launch_logits_rows(hipStream_t stream, int dtype, uint32_t rows, uint32_t vocab, const RowArgs* table,
+                              const InlineRows* few, const LogitsRows& w);
 // `bytes` (a multiple of 16) from pinned host memory, mapped into the device at src, to dst.
 hipError_t launch_copy_pieces(hipStream_t stream, const void* src, void* dst, size_t bytes);
 // The same of up to sizeof(PlacedPieces) bytes from any host memory, through the launch's arguments.

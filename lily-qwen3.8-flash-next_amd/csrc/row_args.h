@@ -69,7 +69,7 @@ struct alignas(16) RowArgs {
     const uint32_t* sel_row;
     const uint32_t* sel_step;
     uint64_t sel_stride;
-    uint64_t pad2;
+    uint64_t row;              // the row's number in its batch (a table may be reordered)
 };
 static_assert(sizeof(RowArgs) == 224, "RowArgs layout");
 

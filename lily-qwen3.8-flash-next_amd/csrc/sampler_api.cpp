@@ -19,6 +19,7 @@
 #include "api_internal.h"
 #include "device_scope.h"
 #include "launch.h"
+#include "operand_span.h"
 
 using namespace lily;
 
@@ -180,6 +181,10 @@ struct lily_plan {
     LaunchPart parts[2];                     // the batch's one or two launches
     uint32_t n_parts = 0;
     uint32_t runs = 0;                       // launches since the table was packed
+    // what lily_plan_process_logits asks of the batch
+    const void* logits = nullptr;
+    uint64_t row_stride = 0;
+    bool biased = false;
 };
 
 namespace {
@@ -845,8 +850,8 @@ int one_row(lily_sampler* s, const void* logits, int dtype, uint32_t vocab, lily
     return launch_inline(s, dtype, vocab, rows, 1);
 }
 
-// Packs a lily_rows batch into `table[0..rows)`.
-int pack_batch(const lily_rows* b, RowArgs* table) {
+// Packs a lily_rows batch into `table[0..rows)`.  `draws`: the rows draw, and count what they draw.
+int pack_batch(const lily_rows* b, RowArgs* table, bool draws = true) {
     if (b == nullptr || b->rows == 0) {
         return fail(LILY_ERR_INVALID_ARG, "empty batch");
     }
@@ -864,7 +869,7 @@ int pack_batch(const lily_rows* b, RowArgs* table) {
     }
     const size_t es = b->dtype == LILY_BF16 ? 2 : 4;
     const uint32_t words = (b->vocab + 31u) / 32u;
-    if (b->scratch != nullptr) {
+    if (b->scratch != nullptr && draws) {
         // No row under penalties may share its scratch with an earlier row: the rows of a launch
         // run side by side.  Sorted by scratch, sharers are neighbours.
         static thread_local std::vector<std::pair<uintptr_t, uint32_t>> owners;
@@ -941,8 +946,13 @@ int pack_batch(const lily_rows* b, RowArgs* table) {
                               nullptr, x)) {
             return rc;
         }
+        table[r].row = r;
     }
     return LILY_OK;
+}
+
+bool any_biased(const RowArgs* rows, uint32_t n) {
+    return std::any_of(rows, rows + n, [](const RowArgs& r) { return r.n_bias != 0u; });
 }
 
 int ensure_table(lily_sampler* s, uint32_t rows) {
@@ -2389,6 +2399,9 @@ int lily_plan_set(lily_plan_t* p, const lily_rows* b) {
     p->vocab = b->vocab;
     p->dtype = b->dtype;
     p->runs = 0;
+    p->logits = b->logits_dev;
+    p->row_stride = b->row_stride;
+    p->biased = any_biased(table.data(), b->rows);
     return LILY_OK;
 }
 
@@ -2404,6 +2417,126 @@ int lily_plan_run(lily_plan_t* p, uint32_t step_delta) {
         }
     }
     p->runs += 1;
+    return LILY_OK;
+}
+
+// ---- processed logits
+
+static int check_logits_out(const lily_logits_out* o, const void* logits, uint64_t row_stride, uint32_t rows,
+                            uint32_t vocab, uint32_t dtype) {
+    if (o == nullptr || o->out_dev == nullptr) {
+        return fail(LILY_ERR_INVALID_ARG, "an output is required");
+    }
+    if (o->out_dtype > LILY_BF16) {
+        return fail(LILY_ERR_INVALID_ARG, "processed logits are LILY_F32 or LILY_BF16");
+    }
+    if (o->logprobs > 1u) {
+        return fail(LILY_ERR_INVALID_ARG, "logprobs is 0 or 1");
+    }
+    if (rows > 1u && o->out_stride < vocab) {
+        return fail(LILY_ERR_INVALID_ARG, "out_stride is shorter than the vocabulary");
+    }
+    if (vocab > LOGITS_MAX_VOCAB || rows > (1u << 24)) {
+        return fail(LILY_ERR_RANGE, "processed logits: vocabularies of up to %u, 2^24 rows", LOGITS_MAX_VOCAB);
+    }
+    const Span in = span(logits, rows, vocab, row_stride, dtype), out = span(o->out_dev, rows, vocab, o->out_stride, o->out_dtype);
+    const Span sums = span(o->log_sum_exp_dev, 1, rows, rows, LILY_F32);
+    for (const Span* q : {&in, &out, &sums}) {
+        if (!fits(*q)) {
+            return fail(LILY_ERR_RANGE, "rows and strides reach beyond the address space");
+        }
+        if (q->rows != 0u && q->at % size_of(q->dtype) != 0u) {
+            return fail(LILY_ERR_INVALID_ARG, "an array does not start at a multiple of its element's size");
+        }
+    }
+    if ((overlap(out, in) && !same(out, in)) || overlap(sums, in) || overlap(sums, out)) {
+        return fail(LILY_ERR_INVALID_ARG, "an output overlaps the logits or another output");
+    }
+    return LILY_OK;
+}
+
+static LogitsRows logits_rows_of(const lily_sampler* s, const lily_logits_out* o, bool biased) {
+    LogitsRows w;
+    w.out = o->out_dev;
+    w.stride = o->out_stride;
+    w.out_dtype = o->out_dtype;
+    w.logprobs = o->logprobs != 0u;
+    w.biased = biased;
+    w.lse = o->log_sum_exp_dev;
+    w.part = Handed<double>{s->ws_lse};
+    w.ticket = s->ws_ticket;
+    w.max_rows = s->ws_rows;
+    w.handover = s->handover;
+    return w;
+}
+
+int lily_process_logits(lily_sampler_t* s, const lily_rows* b, const lily_logits_out* o) {
+    if (b == nullptr || b->rows == 0 || b->vocab == 0) {
+        return fail(LILY_ERR_INVALID_ARG, "empty batch");
+    }
+    if (b->dtype != LILY_F32 && b->dtype != LILY_BF16) {
+        return fail(LILY_ERR_INVALID_ARG, "dtype must be LILY_F32 or LILY_BF16");
+    }
+    if (b->logits_dev == nullptr || b->params == nullptr) {
+        return fail(LILY_ERR_INVALID_ARG, "logits and params are required");
+    }
+    if (int rc = check_logits_out(o, b->logits_dev, b->row_stride, b->rows, b->vocab, b->dtype)) {
+        return rc;
+    }
+    // the part of the batch that has a meaning here (the row's id would go to a place of the output that
+    // no kernel of this call writes an id to)
+    lily_rows q = *b;
+    q.steps = nullptr;
+    q.forced = nullptr;
+    q.uniforms = nullptr;
+    q.out_ids_dev = reinterpret_cast<uint32_t*>(o->out_dev);
+    q.out_logprobs_dev = nullptr;
+    q.dbg_ids_dev = nullptr;
+    q.dbg_probs_dev = nullptr;
+    q.dbg_counts_dev = nullptr;
+    if (b->rows <= (uint32_t)INLINE_ROWS) {
+        InlineRows rows = {};
+        if (int rc = pack_batch(&q, rows.r, false)) {
+            return rc;
+        }
+        if (s == nullptr) {
+            return fail(LILY_ERR_INVALID_ARG, "sampler is null");
+        }
+        ON_DEVICE(s->device);
+        HIP_TRY(launch_logits_rows(s->stream, (int)b->dtype, b->rows, b->vocab, nullptr, &rows,
+                                   logits_rows_of(s, o, any_biased(rows.r, b->rows))));
+        return LILY_OK;
+    }
+    if (s == nullptr) {
+        return fail(LILY_ERR_INVALID_ARG, "sampler is null");
+    }
+    ON_DEVICE(s->device);
+    uint32_t slot = 0;
+    if (int rc = stage_acquire(s, b->rows, &slot)) {
+        return rc;
+    }
+    if (int rc = pack_batch(&q, s->stage[slot], false)) {
+        return rc;
+    }
+    const bool biased = any_biased(s->stage[slot], b->rows);
+    if (int rc = stage_commit(s, slot, (size_t)b->rows * sizeof(RowArgs))) {
+        return rc;
+    }
+    HIP_TRY(launch_logits_rows(s->stream, (int)b->dtype, b->rows, b->vocab, s->table_dev, nullptr,
+                               logits_rows_of(s, o, biased)));
+    return LILY_OK;
+}
+
+int lily_plan_process_logits(lily_plan_t* p, const lily_logits_out* o) {
+    if (p == nullptr || p->rows == 0) {
+        return fail(LILY_ERR_INVALID_ARG, "plan is null or not set");
+    }
+    if (int rc = check_logits_out(o, p->logits, p->row_stride, p->rows, p->vocab, p->dtype)) {
+        return rc;
+    }
+    ON_DEVICE(p->s->device);
+    HIP_TRY(launch_logits_rows(p->s->stream, (int)p->dtype, p->rows, p->vocab, p->table_dev, nullptr,
+                               logits_rows_of(p->s, o, p->biased)));
     return LILY_OK;
 }
 

@@ -118,6 +118,11 @@ class _Norm(C.Structure):
                 ("out_dtype", C.c_uint32), ("eps", C.c_float), ("weight_offset", C.c_float)]
 
 
+class _LogitsOut(C.Structure):
+    _fields_ = [("out_dev", C.c_void_p), ("out_stride", C.c_uint64), ("out_dtype", C.c_uint32),
+                ("logprobs", C.c_uint32), ("log_sum_exp_dev", C.c_void_p)]
+
+
 class QuantWeights:
     """The reference's affine weights (src/weights.rs:27-36): codes int32 [out, in * bits / 32]
     (u32 words, the lowest code first), scales and biases bf16 [out, in / group_size]."""
@@ -199,6 +204,8 @@ def _load():
         "lily_lm_head_sample_rows": [vp, C.POINTER(_LmHead), C.POINTER(_Rows)],
     }
     sigs["lily_rms_norm"] = [vp, C.POINTER(_Norm)]
+    sigs["lily_process_logits"] = [vp, C.POINTER(_Rows), C.POINTER(_LogitsOut)]
+    sigs["lily_plan_process_logits"] = [vp, C.POINTER(_LogitsOut)]
     L.lily_insertions_create.restype = C.c_int
     L.lily_insertions_create.argtypes = [u32, C.POINTER(vp)]
     L.lily_insertions_push.restype = C.c_int
@@ -600,6 +607,19 @@ class Sampler:
             eps, weight_offset))))
 
 
+    def _logits_out(self, rows, vocab, out, log_sum_exp, logprobs):
+        at, stride, code = self._matrix(out, rows, vocab, "out")
+        return _LogitsOut(at, stride, code, 1 if logprobs else 0, self._scales(log_sum_exp, rows, "log_sum_exp"))
+
+    def process_logits(self, logits, params, out, log_sum_exp=None, logprobs=False, scratch=None, allow=None, bias=None):
+        """lily_process_logits: the rows with penalties, biases and masks applied, as adjusted logits or
+        log-probabilities, into `out` (f32 or bf16; `logits` itself too)."""
+        r, keep = self._rows(logits, params, [0] * logits.shape[0], None, scratch=scratch, allow=allow, bias=bias)
+        _check(_lib.lily_process_logits(self._h, C.byref(r),
+                                        C.byref(self._logits_out(*logits.shape, out, log_sum_exp, logprobs))))
+        return keep
+
+
 class Plan:
     """A resident batch: packed and uploaded once, one launch per run."""
 
@@ -608,12 +628,18 @@ class Plan:
         h = C.c_void_p()
         _check(_lib.lily_plan_create(sampler._h, logits.shape[0], C.byref(h)))
         self._h = h
+        self._shape = tuple(logits.shape)
         sampler._children.add(self)
         r, self._keep = sampler._rows(logits, params, steps, out_ids, **kw)
         _check(_lib.lily_plan_set(self._h, C.byref(r)))
 
     def run(self, step_delta=0):
         _check(_lib.lily_plan_run(self._h, step_delta))
+
+    def process_logits(self, out, log_sum_exp=None, logprobs=False):
+        """lily_plan_process_logits: the plan's rows as Sampler.process_logits writes them."""
+        _check(_lib.lily_plan_process_logits(
+            self._h, C.byref(self._s._logits_out(*self._shape, out, log_sum_exp, logprobs))))
 
     def close(self):
         if self._h:

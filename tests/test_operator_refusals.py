@@ -73,6 +73,7 @@ def test_a_sound_norm_only_lacks_the_sampler(over):
     (dict(x_dev=0x10001), INVALID, "multiple"),
     (dict(weight_dev=0x40002), INVALID, "multiple"),
     (dict(x_stride=1 << 62), RANGE, "address"),
+    (dict(x_stride=1 << 63), RANGE, "address"),
     (dict(x_dev=(1 << 63) - 64), RANGE, "address"),
     (dict(sum_dev=0x10002), INVALID, "overlaps an input"),                   # shifted by one element
     (dict(out_dev=0x10000, out_dtype=LS.F32), INVALID, "overlaps an input"),  # another type in the same place
@@ -91,3 +92,68 @@ def test_what_a_norm_refuses(over, code, word):
 
 def test_a_missing_descriptor():
     assert _said(L.lily_rms_norm(None, None))[0] == INVALID
+
+
+# ---- processed logits
+
+
+def _process(rows_over, out_over):
+    kw = dict(rows=2, vocab=100, dtype=LS.F32, logits_dev=0x10000, row_stride=100)
+    kw.update(rows_over)
+    b = LS._Rows()
+    n = max(1, min(kw["rows"], 64))
+    params = (LS.SamplingParams * n)(*[LS.SamplingParams.greedy() for _ in range(n)])
+    b.params = params
+    for k, v in kw.items():
+        setattr(b, k, v)
+    kw = dict(out_dev=0x20000, out_stride=100, out_dtype=LS.F32, logprobs=0, log_sum_exp_dev=None)
+    kw.update(out_over)
+    o = LS._LogitsOut()
+    for k, v in kw.items():
+        setattr(o, k, v)
+    return _said(L.lily_process_logits(None, C.byref(b), C.byref(o)))
+
+
+@pytest.mark.parametrize("rows_over, out_over", [
+    ({}, {}),
+    ({}, dict(log_sum_exp_dev=0x30000, logprobs=1)),
+    ({}, dict(out_dev=0x10000)),                                  # in place
+    (dict(rows=9, row_stride=101), dict(out_stride=103)),
+    (dict(rows=1, row_stride=100), dict(out_stride=0)),
+    (dict(dtype=LS.BF16), dict(out_dtype=LS.BF16)),
+    (dict(row_stride=200), dict(out_dev=0x10000 + 400, out_stride=200)),   # side by side in wider rows
+])
+def test_a_sound_call_for_processed_logits_only_lacks_the_sampler(rows_over, out_over):
+    rc, text = _process(rows_over, out_over)
+    assert rc == INVALID and text == "sampler is null", text
+
+
+@pytest.mark.parametrize("rows_over, out_over, code, word", [
+    (dict(rows=0), {}, INVALID, "empty"),
+    (dict(vocab=0), {}, INVALID, "empty"),
+    (dict(dtype=LS.E4M3), {}, INVALID, "dtype"),
+    (dict(logits_dev=None), {}, INVALID, "required"),
+    (dict(row_stride=99), {}, INVALID, "row_stride"),
+    ({}, dict(out_dev=None), INVALID, "output"),
+    ({}, dict(out_dtype=LS.E4M3), INVALID, "processed logits"),
+    ({}, dict(logprobs=2), INVALID, "logprobs"),
+    ({}, dict(out_stride=99), INVALID, "out_stride"),
+    (dict(vocab=(1 << 24) + 1, row_stride=1 << 25), dict(out_stride=1 << 25), RANGE, "vocabularies"),
+    (dict(row_stride=1 << 62), {}, RANGE, "address"),
+    (dict(logits_dev=0x10002), {}, INVALID, "multiple"),
+    ({}, dict(out_dev=0x20001), INVALID, "multiple"),
+    ({}, dict(log_sum_exp_dev=0x30001), INVALID, "multiple"),
+    ({}, dict(out_dev=0x10004), INVALID, "overlaps"),
+    ({}, dict(out_dev=0x10000, out_dtype=LS.BF16), INVALID, "overlaps"),
+    ({}, dict(out_dev=0x10000, out_stride=120), INVALID, "overlaps"),
+    ({}, dict(log_sum_exp_dev=0x10000), INVALID, "overlaps"),
+    ({}, dict(log_sum_exp_dev=0x20004), INVALID, "overlaps"),
+    (dict(bias_dev=0x40000), {}, INVALID, "bias_offsets"),
+])
+def test_what_processed_logits_refuse(rows_over, out_over, code, word):
+    rc, text = _process(rows_over, out_over)
+    assert rc == code and word in text, (rc, text)
+
+
+def test_a_plan_that_is_missing():
+    assert _said(L.lily_plan_process_logits(None, None))[0] == INVALID
