@@ -543,6 +543,52 @@ typedef struct lily_norm {
 } lily_norm;
 int lily_rms_norm(lily_sampler_t* s, const lily_norm* norm);
 
+/* ---- Around the head: a matrix product with bias, activation and residual in its epilogue.
+ *
+ *     out[r][v] = residual[r][v] + act(x_scales[r] * weight_scales[v] * sum_i x[r][i] * weight[v][i] + bias[v])
+ * The block of a draft head (residual + silu(W x + b)), a projection ahead of the head, or a head held in
+ * 8-bit floats (its logits then in f32 or bf16, without the summaries of lily_lm_head_bf16).  x and weight are
+ * both bf16 or both E4M3 (what lily_rms_norm leaves, its scales as x_scales), contiguous along d, products
+ * and sums in f32 on the matrix cores, the epilogue in f32, one rounding to out_dtype.  Any number of
+ * rows and outputs, d a multiple of 8 (bf16) or 16 (E4M3) elements, rows of x and weight at multiples of 16
+ * bytes, at most 2^23 bytes apart.  out_dev may be residual_dev with the same type and stride; other overlaps of
+ * out with an operand are refused.  Enqueued on the sampler's stream.  Where few tiles span the chip the parts
+ * of d meet in the sampler's workspace, added in a fixed order: graphs captured from one sampler are replayed one
+ * after the other.
+ * E4M3 operands: with an f32 output, and for up to 16 rows, the products and sums are as bf16 has them (each E4M3
+ * value is one of bf16).  More rows with a bf16 output take the matrix cores' 8-bit products, at twice the rate:
+ * of every eight neighbouring elements' products they drop what lies 2^-13 below the largest one, some 6e-5 of the
+ * result. */
+typedef enum lily_activation {
+    LILY_ACT_NONE = 0,
+    LILY_ACT_SILU = 1,        /* v / (1 + exp(-v)) */
+    LILY_ACT_GELU = 2,        /* v * Phi(v) */
+    LILY_ACT_GELU_TANH = 3,   /* v / 2 * (1 + tanh(sqrt(2 / pi) * (v + 0.044715 v^3))) */
+    LILY_ACT_RELU = 4
+} lily_activation;
+typedef struct lily_projection {
+    uint32_t rows;
+    uint32_t n;                       /* outputs */
+    uint32_t d;
+    uint32_t dtype;                   /* of x and weight: LILY_BF16 or LILY_E4M3 */
+    const void* x_dev;                /* [rows][x_stride] */
+    uint64_t x_stride;                /* elements, as every stride here */
+    const void* weight_dev;           /* [n][weight_stride], row v the weights of output v */
+    uint64_t weight_stride;
+    const float* x_scales_dev;        /* [rows] or NULL (ones) */
+    const float* weight_scales_dev;   /* [n] or NULL (ones) */
+    const void* bias_dev;             /* [n] of bias_dtype, or NULL */
+    const void* residual_dev;         /* [rows][residual_stride] of residual_dtype, or NULL */
+    uint64_t residual_stride;
+    void* out_dev;                    /* [rows][out_stride] of out_dtype */
+    uint64_t out_stride;
+    uint32_t bias_dtype;              /* LILY_F32 or LILY_BF16, as residual_dtype and out_dtype */
+    uint32_t residual_dtype;
+    uint32_t out_dtype;
+    uint32_t activation;              /* lily_activation */
+} lily_projection;
+int lily_project(lily_sampler_t* s, const lily_projection* p);
+
 /* ---- Processed logits: penalties, bias lists and masks applied to whole rows, and written out.
  *
  * The draws form these values for their candidates only; a host that scores tokens, ranks beams, draws

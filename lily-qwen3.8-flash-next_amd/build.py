@@ -51,6 +51,8 @@ def units():
     out.append(("rows_argmax.hip", "rows_argmax.o", []))
     out.append(("norm.hip", "norm.o", []))
     out.append(("logits_rows.hip", "logits_rows.o", []))
+    out.append(("project_few.hip", "project_few.o", []))
+    out.append(("project_tiles.hip", "project_tiles.o", []))
     out.append(("sampler_api.cpp", "sampler_api.o", []))
     out.append(("operators_api.cpp", "operators_api.o", []))
     return out

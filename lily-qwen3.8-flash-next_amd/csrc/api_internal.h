@@ -37,5 +37,7 @@ int static_scratch_init(int device);
 // What an operator's entry point needs of a sampler.
 int sampler_device(const lily_sampler_t* s);
 hipStream_t sampler_stream(const lily_sampler_t* s);
+struct ProjectWorkspace;
+void sampler_project_workspace(const lily_sampler_t* s, ProjectWorkspace* ws);
 
 }  // namespace lily

@@ -97,6 +97,65 @@ int check_norm(const lily_norm* n, bool* pieces) {
     return LILY_OK;
 }
 
+int check_projection(const lily_projection* p) {
+    if (p == nullptr || p->x_dev == nullptr || p->weight_dev == nullptr || p->out_dev == nullptr) {
+        return api_fail(LILY_ERR_INVALID_ARG, "projection, x, weight and out are required");
+    }
+    if (p->rows == 0u || p->n == 0u || p->d == 0u) {
+        return api_fail(LILY_ERR_INVALID_ARG, "rows, n and d must be positive");
+    }
+    if (p->dtype != LILY_BF16 && p->dtype != LILY_E4M3) {
+        return api_fail(LILY_ERR_INVALID_ARG, "x and weight are LILY_BF16 or LILY_E4M3");
+    }
+    if (p->bias_dtype > LILY_BF16 || p->residual_dtype > LILY_BF16 || p->out_dtype > LILY_BF16) {
+        return api_fail(LILY_ERR_INVALID_ARG, "bias, residual and out are LILY_F32 or LILY_BF16");
+    }
+    if (p->activation > LILY_ACT_RELU) {
+        return api_fail(LILY_ERR_INVALID_ARG, "unknown activation %u", p->activation);
+    }
+    const uint64_t e = size_of(p->dtype);
+    if (p->d * e % 16u != 0u) {
+        return api_fail(LILY_ERR_INVALID_ARG, "d must be a multiple of 16 bytes: of 8 in bf16, of 16 in E4M3");
+    }
+    if (p->d > 0xffffff80u / e || p->rows > (1u << 24) || p->n > (1u << 30)) {
+        return api_fail(LILY_ERR_RANGE, "a product takes up to 2^24 rows, 2^30 outputs and rows of 2^32 - 128 bytes");
+    }
+    if ((p->rows > 1u && (p->x_stride < p->d || p->out_stride < p->n || (p->residual_dev != nullptr && p->residual_stride < p->n))) ||
+        (p->n > 1u && p->weight_stride < p->d)) {
+        return api_fail(LILY_ERR_INVALID_ARG, "a stride is shorter than its row");
+    }
+    const Span x = span(p->x_dev, p->rows, p->d, p->x_stride, p->dtype);
+    const Span w = span(p->weight_dev, p->n, p->d, p->weight_stride, p->dtype);
+    const Span out = span(p->out_dev, p->rows, p->n, p->out_stride, p->out_dtype);
+    const Span res = span(p->residual_dev, p->rows, p->n, p->residual_stride, p->residual_dtype);
+    const Span bias = span(p->bias_dev, 1, p->n, p->n, p->bias_dtype);
+    const Span xs = span(p->x_scales_dev, 1, p->rows, p->rows, LILY_F32);
+    const Span ws = span(p->weight_scales_dev, 1, p->n, p->n, LILY_F32);
+    if (!aligned(x) || !aligned(w)) {
+        return api_fail(LILY_ERR_INVALID_ARG, "rows of x and weight must start at multiples of 16 bytes");
+    }
+    if ((p->rows > 1u && x.stride > (1u << 23)) || (p->n > 1u && w.stride > (1u << 23))) {
+        return api_fail(LILY_ERR_RANGE, "rows of x and weight lie at most 2^23 bytes apart");
+    }
+    for (const Span* s : {&x, &w, &out, &res, &bias, &xs, &ws}) {
+        if (!fits(*s)) {
+            return api_fail(LILY_ERR_RANGE, "rows and strides reach beyond the address space");
+        }
+        if (s->rows != 0u && (s->at % size_of(s->dtype) != 0u)) {
+            return api_fail(LILY_ERR_INVALID_ARG, "an array does not start at a multiple of its element's size");
+        }
+    }
+    for (const Span* i : {&x, &w, &bias, &xs, &ws}) {
+        if (overlap(out, *i)) {
+            return api_fail(LILY_ERR_INVALID_ARG, "out overlaps an operand");
+        }
+    }
+    if (overlap(out, res) && !same(out, res)) {
+        return api_fail(LILY_ERR_INVALID_ARG, "out overlaps the residual without being it");
+    }
+    return LILY_OK;
+}
+
 int need_sampler(const lily_sampler_t* s) {
     return s != nullptr ? LILY_OK : api_fail(LILY_ERR_INVALID_ARG, "sampler is null");
 }
@@ -115,6 +174,20 @@ int lily_rms_norm(lily_sampler_t* s, const lily_norm* norm) {
     }
     ON_DEVICE(sampler_device(s));
     HIP_TRY(launch_rms_norm(sampler_stream(s), *norm, pieces));
+    return LILY_OK;
+}
+
+int lily_project(lily_sampler_t* s, const lily_projection* p) {
+    if (int rc = check_projection(p)) {
+        return rc;
+    }
+    if (int rc = need_sampler(s)) {
+        return rc;
+    }
+    ON_DEVICE(sampler_device(s));
+    ProjectWorkspace ws;
+    sampler_project_workspace(s, &ws);
+    HIP_TRY(launch_project(sampler_stream(s), *p, ws));
     return LILY_OK;
 }
 

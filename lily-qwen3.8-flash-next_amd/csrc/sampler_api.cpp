@@ -20,6 +20,7 @@
 #include "device_scope.h"
 #include "launch.h"
 #include "operand_span.h"
+#include "operators.h"
 
 using namespace lily;
 
@@ -1036,6 +1037,14 @@ int scratch_device(const lily_scratch_t* sc) { return sc->s->device; }
 
 int sampler_device(const lily_sampler_t* s) { return s->device; }
 hipStream_t sampler_stream(const lily_sampler_t* s) { return s->stream; }
+// (the candidates' slots: no two launches of a stream use them at once)
+void sampler_project_workspace(const lily_sampler_t* s, ProjectWorkspace* ws) {
+    ws->part = s->ws_cand;
+    ws->part_words = s->ws_slots;
+    ws->ticket = s->ws_ticket;
+    ws->tickets = s->ws_rows;
+    ws->handover = s->handover;
+}
 
 int sample_row_with_workspace(int device, hipStream_t stream, const Workspace& ws, const float* logits,
                               uint32_t vocab, lily_scratch_t* scratch,

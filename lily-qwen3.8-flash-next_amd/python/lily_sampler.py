@@ -118,6 +118,20 @@ class _Norm(C.Structure):
                 ("out_dtype", C.c_uint32), ("eps", C.c_float), ("weight_offset", C.c_float)]
 
 
+class _Projection(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("n", C.c_uint32), ("d", C.c_uint32), ("dtype", C.c_uint32),
+                ("x_dev", C.c_void_p), ("x_stride", C.c_uint64),
+                ("weight_dev", C.c_void_p), ("weight_stride", C.c_uint64),
+                ("x_scales_dev", C.c_void_p), ("weight_scales_dev", C.c_void_p), ("bias_dev", C.c_void_p),
+                ("residual_dev", C.c_void_p), ("residual_stride", C.c_uint64),
+                ("out_dev", C.c_void_p), ("out_stride", C.c_uint64),
+                ("bias_dtype", C.c_uint32), ("residual_dtype", C.c_uint32), ("out_dtype", C.c_uint32),
+                ("activation", C.c_uint32)]
+
+
+ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4}
+
+
 class _LogitsOut(C.Structure):
     _fields_ = [("out_dev", C.c_void_p), ("out_stride", C.c_uint64), ("out_dtype", C.c_uint32),
                 ("logprobs", C.c_uint32), ("log_sum_exp_dev", C.c_void_p)]
@@ -204,6 +218,7 @@ def _load():
         "lily_lm_head_sample_rows": [vp, C.POINTER(_LmHead), C.POINTER(_Rows)],
     }
     sigs["lily_rms_norm"] = [vp, C.POINTER(_Norm)]
+    sigs["lily_project"] = [vp, C.POINTER(_Projection)]
     sigs["lily_process_logits"] = [vp, C.POINTER(_Rows), C.POINTER(_LogitsOut)]
     sigs["lily_plan_process_logits"] = [vp, C.POINTER(_LogitsOut)]
     L.lily_insertions_create.restype = C.c_int
@@ -606,6 +621,27 @@ class Sampler:
             rows, d, xp, xs, rp, rs, sp, ss, wp, op, os_, self._scales(scales, rows, "scales"), xt, rt, wt, ot,
             eps, weight_offset))))
 
+
+    def project(self, x, weight, out, x_scales=None, weight_scales=None, bias=None, activation="none", residual=None):
+        """lily_project: out = residual + activation(x_scales * weight_scales * (x @ weight.T) + bias); x [rows, d]
+        and weight [n, d] both bf16 or both float8_e4m3fn."""
+        if x.dim() != 2 or weight.dim() != 2:
+            raise SamplerError(-1, "x must be [rows, d] and weight [n, d], rows contiguous")
+        rows, d = x.shape
+        n = weight.shape[0]
+        xp, xs, xt = self._matrix(x, rows, d, "x")
+        wp, ws, wt = self._matrix(weight, n, d, "weight")
+        op, os_, ot = self._matrix(out, rows, n, "out")
+        if xt != wt:
+            raise SamplerError(-1, "x and weight must have one type")
+        act = ACTIVATIONS.get(activation)
+        if act is None:
+            raise SamplerError(-1, f"activation must be one of {', '.join(ACTIVATIONS)}")
+        bp, bt = self._vector(bias, n, "bias")
+        rp, rs, rt = self._matrix(residual, rows, n, "residual") if residual is not None else (None, 0, F32)
+        _check(_lib.lily_project(self._h, C.byref(_Projection(
+            rows, n, d, xt, xp, xs, wp, ws, self._scales(x_scales, rows, "x_scales"),
+            self._scales(weight_scales, n, "weight_scales"), bp, rp, rs, op, os_, bt, rt, ot, act))))
 
     def _logits_out(self, rows, vocab, out, log_sum_exp, logprobs):
         at, stride, code = self._matrix(out, rows, vocab, "out")

@@ -157,3 +157,77 @@ def test_what_processed_logits_refuse(rows_over, out_over, code, word):
 
 def test_a_plan_that_is_missing():
     assert _said(L.lily_plan_process_logits(None, None))[0] == INVALID
+
+
+# ---- the product with an epilogue
+
+
+def _project(**over):
+    kw = dict(rows=4, n=48, d=64, dtype=LS.BF16, x_dev=0x10000, x_stride=64, weight_dev=0x20000, weight_stride=64,
+              x_scales_dev=None, weight_scales_dev=None, bias_dev=0x30000, residual_dev=0x40000, residual_stride=48,
+              out_dev=0x50000, out_stride=48, bias_dtype=LS.F32, residual_dtype=LS.BF16, out_dtype=LS.BF16, activation=1)
+    kw.update(over)
+    p = LS._Projection()
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return _said(L.lily_project(None, C.byref(p)))
+
+
+@pytest.mark.parametrize("over", [
+    dict(), dict(dtype=LS.E4M3, x_scales_dev=0x60000, weight_scales_dev=0x61000), dict(bias_dev=None), dict(residual_dev=None),
+    dict(rows=1, x_stride=0, residual_stride=0, out_stride=0), dict(n=1, weight_stride=0),
+    dict(out_dev=0x40000), dict(residual_dev=0x50000 + 96, residual_stride=96, out_stride=96),
+    dict(activation=4), dict(d=8, x_stride=8, weight_stride=8), dict(out_dev=0x50002), dict(bias_dtype=LS.BF16, bias_dev=0x30002),
+])
+def test_a_sound_product_only_lacks_the_sampler(over):
+    rc, text = _project(**over)
+    assert rc == INVALID and text == "sampler is null", text
+
+
+@pytest.mark.parametrize("over, code, word", [
+    (dict(x_dev=None), INVALID, "required"),
+    (dict(weight_dev=None), INVALID, "required"),
+    (dict(out_dev=None), INVALID, "required"),
+    (dict(rows=0), INVALID, "positive"),
+    (dict(n=0), INVALID, "positive"),
+    (dict(d=0), INVALID, "positive"),
+    (dict(dtype=LS.F32), INVALID, "x and weight are"),
+    (dict(dtype=3), INVALID, "x and weight are"),
+    (dict(bias_dtype=2), INVALID, "bias, residual"),
+    (dict(residual_dtype=2), INVALID, "bias, residual"),
+    (dict(out_dtype=2), INVALID, "bias, residual"),
+    (dict(activation=5), INVALID, "activation"),
+    (dict(d=60), INVALID, "16 bytes"),
+    (dict(dtype=LS.E4M3, d=56), INVALID, "16 bytes"),
+    (dict(d=0x80000000, x_stride=0x80000000, weight_stride=0x80000000), RANGE, "up to"),
+    (dict(rows=(1 << 24) + 1), RANGE, "up to"),
+    (dict(n=(1 << 30) + 1), RANGE, "up to"),
+    (dict(x_stride=56), INVALID, "shorter"),
+    (dict(weight_stride=56), INVALID, "shorter"),
+    (dict(out_stride=47), INVALID, "shorter"),
+    (dict(residual_stride=47), INVALID, "shorter"),
+    (dict(x_dev=0x10008), INVALID, "16 bytes"),
+    (dict(x_stride=68), INVALID, "16 bytes"),
+    (dict(weight_stride=68), INVALID, "16 bytes"),
+    (dict(weight_stride=(1 << 22) + 8), RANGE, "apart"),
+    (dict(x_stride=(1 << 22) + 8), RANGE, "apart"),
+    (dict(out_stride=1 << 62), RANGE, "address"),
+    (dict(out_dev=0x50001), INVALID, "multiple"),
+    (dict(bias_dev=0x30002), INVALID, "multiple"),
+    (dict(x_scales_dev=0x60002), INVALID, "multiple"),
+    (dict(out_dev=0x10000), INVALID, "operand"),
+    (dict(out_dev=0x20000), INVALID, "operand"),
+    (dict(out_dev=0x30000), INVALID, "operand"),
+    (dict(x_scales_dev=0x50000), INVALID, "operand"),
+    (dict(weight_scales_dev=0x50010), INVALID, "operand"),
+    (dict(out_dev=0x40002), INVALID, "residual"),
+    (dict(out_dev=0x40000, out_dtype=LS.F32), INVALID, "residual"),
+    (dict(out_dev=0x40000, out_stride=50), INVALID, "residual"),
+])
+def test_what_a_product_refuses(over, code, word):
+    rc, text = _project(**over)
+    assert rc == code and word in text, (rc, text)
+
+
+def test_a_product_without_a_descriptor():
+    assert _said(L.lily_project(None, None))[0] == INVALID
