@@ -27,12 +27,61 @@ namespace {
 
 __device__ const uint4 line_of_zeros = {0u, 0u, 0u, 0u};   // what lies beyond d
 
-template <int WM_, int WN_, int MT_, int NT_, int RESIDENT_>
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// A block of S x S sums: its operands' pieces, its products one by one, where a lane's sums lie in it.  The wide
+// form has a quarter of the instructions and of the separately tracked sums (with 16 x 16 blocks a wave's 256
+// registers of sums kept the compiler moving them around: 2 450 us where this takes a tenth).
+template <int S>
+struct Block;
+template <>
+struct Block<16> {
+    typedef f32x4 Sums;
+    static constexpr int PIECES = 2, GROUPS = 1;   // pieces a lane of a line; runs of four neighbouring outputs a lane
+    u32x4 p[PIECES];
+    static __device__ __forceinline__ uint32_t first_piece(uint32_t lane) { return lane >> 4; }   // then every fourth
+    static constexpr uint32_t NEXT_PIECE = 64;     // in bytes of a staged row, by exclusive or
+    static __device__ __forceinline__ uint32_t output(uint32_t lane, int) { return (lane >> 4) * 4u; }
+    static __device__ __forceinline__ Sums product(bf16x8 w, bf16x8 x, Sums c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x, c, 0, 0, 0); }
+    static __device__ __forceinline__ Sums product(i32x8 w, i32x8 x, Sums c) {
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, 0, 0, 0, 0, 0);
+    }
+};
+template <>
+struct Block<32> {
+    typedef f32x16 Sums;
+    static constexpr int PIECES = 4, GROUPS = 4;
+    u32x4 p[PIECES];
+    static __device__ __forceinline__ uint32_t first_piece(uint32_t lane) { return lane >> 5; }   // then every second
+    static constexpr uint32_t NEXT_PIECE = 32;
+    static __device__ __forceinline__ uint32_t output(uint32_t lane, int q) { return (uint32_t)q * 8u + (lane >> 5) * 4u; }
+    static __device__ __forceinline__ Sums product(bf16x8 w, bf16x8 x, Sums c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, x, c, 0, 0, 0); }
+    static __device__ __forceinline__ Sums product(i32x8 w, i32x8 x, Sums c) {
+        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 0, 0, 0, 0, 0, 0);
+    }
+};
+// Products a line of a block takes, and the q-th of them.
+template <Products P, int S>
+constexpr int STEPS = P == PRODUCT_BF16 ? Block<S>::PIECES : P == PRODUCT_E4M3 ? Block<S>::PIECES / 2 : Block<S>::PIECES * 2;
+template <Products P, int S>
+__device__ __forceinline__ typename Block<S>::Sums step(const Block<S>& w, const Block<S>& x, typename Block<S>::Sums c, int q) {
+    if constexpr (P == PRODUCT_BF16) {
+        return Block<S>::product(__builtin_bit_cast(bf16x8, w.p[q]), __builtin_bit_cast(bf16x8, x.p[q]), c);
+    } else if constexpr (P == PRODUCT_E4M3) {
+        return Block<S>::product(__builtin_bit_cast(i32x8, __builtin_shufflevector(w.p[2 * q], w.p[2 * q + 1], 0, 1, 2, 3, 4, 5, 6, 7)),
+                                 __builtin_bit_cast(i32x8, __builtin_shufflevector(x.p[2 * q], x.p[2 * q + 1], 0, 1, 2, 3, 4, 5, 6, 7)), c);
+    } else {
+        const int e = (q & 1) * 2;
+        return Block<S>::product(widened(w.p[q >> 1][e], w.p[q >> 1][e + 1]), widened(x.p[q >> 1][e], x.p[q >> 1][e + 1]), c);
+    }
+}
+
+template <int S_, int WM_, int WN_, int MT_, int NT_, int RESIDENT_>
 struct Tile {
-    static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, RESIDENT = RESIDENT_;
-    static constexpr int MH = MT / 2, NH = NT / 2;                     // products of a half
-    static constexpr int BM = WM * MT * 16, BN = WN * NT * 16;
-    static constexpr int XR = WM * MH * 16, WR = WN * NH * 16;         // rows of a unit: of x, of the weights
+    static constexpr int S = S_, WM = WM_, WN = WN_, MT = MT_, NT = NT_, RESIDENT = RESIDENT_;
+    static constexpr int MH = MT / 2, NH = NT / 2;                     // blocks of a half
+    static constexpr int BM = WM * MT * S, BN = WN * NT * S;
+    static constexpr int XR = WM * MH * S, WR = WN * NH * S;           // rows of a unit: of x, of the weights
     static constexpr int UNIT = (XR + WR) * (int)LINE;
     static constexpr int XL = XR / 32, WL = WR / 32, LOADS = XL + WL;  // loads of a wave and unit
     static constexpr int LDS_BYTES = 4 * UNIT;
@@ -46,11 +95,13 @@ struct Parity {
 
 template <Products P, class T>
 __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const ProjectArgs a, uint32_t m_tiles, uint32_t n_tiles) {
-    constexpr int MH = T::MH, NH = T::NH;
+    constexpr int MH = T::MH, NH = T::NH, S = T::S;
+    typedef Block<S> Operand;
+    typedef typename Operand::Sums Sums;
     extern __shared__ __align__(16) char lds[];
     __shared__ uint32_t last;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-    const uint32_t wm = wave / T::WN, wn = wave % T::WN, g = lane >> 4, r16 = lane & 15u;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+    const uint32_t wm = wave / T::WN, wn = wave % T::WN, r_in = lane % (uint32_t)S;
     // Consecutive workgroups go to consecutive XCDs: each XCD gets a run of tiles of its own (they share
     // its L2), in groups of four tiles of rows.
     const uint32_t tiles = m_tiles * n_tiles, all = tiles * a.splits;
@@ -69,16 +120,15 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
     // Where a lane's pieces come from: 32-bit offsets from the tile's first rows, for both halves.
     const char* x_rows = a.x + (uint64_t)m0 * a.x_stride;
     const char* w_rows = a.w + (uint64_t)n0 * a.w_stride;
-    uint32_t x_at[2][T::XL], w_at[2][T::WL], k_at[T::LOADS];
+    uint32_t x_at[2][T::XL], w_at[2][T::WL];
 #pragma unroll
     for (int i = 0; i < T::LOADS; ++i) {
         const bool is_x = i < T::XL;
         const uint32_t row = (uint32_t)((is_x ? i : i - T::XL) * 32) + wave * 8u + (lane >> 3);   // of the unit's part
         const uint32_t piece = (lane & 7u) ^ ((row >> 1) & 7u);
-        k_at[i] = piece * 16u;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t half = is_x ? (uint32_t)MH * 16u : (uint32_t)NH * 16u;
+            const uint32_t half = is_x ? (uint32_t)(MH * S) : (uint32_t)(NH * S);
             const uint32_t tile_row = row / half * (2u * half) + (uint32_t)h * half + row % half;
             if (is_x) {
                 x_at[h][i] = min(tile_row, a.rows - 1u - m0) * (uint32_t)a.x_stride + piece * 16u;
@@ -90,74 +140,93 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
     typedef __attribute__((address_space(1))) const void* gptr;
     typedef __attribute__((address_space(3))) void* lptr;
     // Asks for a unit of stage s: rows' half hx, outputs' half hw, into LDS place `unit`.
+    // (buffer loads: a lane's offset and the stage's are added by the load itself; the last 32 bits of the resource
+    // are a raw buffer's, and nothing is ever asked beyond the rows)
+    auto x_buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(x_rows), 0, -1, 0x00020000);
+    auto w_buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(w_rows), 0, -1, 0x00020000);
+    auto load = [&](uint32_t s, int hx, int hw, int unit, int i) {
+        const uint32_t k0 = (first + s) * LINE;
+        char* base = lds + unit * T::UNIT + wave * 1024u + i * 4096;
+        if (i < T::XL) {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(x_buffer, (lptr)base, 16, (int)x_at[hx][i < T::XL ? i : 0], (int)k0, 0, 0);
+        } else {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(w_buffer, (lptr)base, 16, (int)w_at[hw][i < T::XL ? 0 : i - T::XL], (int)k0, 0, 0);
+        }
+    };
     auto ask = [&](uint32_t s, int hx, int hw, int unit) {
         const uint32_t k0 = (first + s) * LINE;
-        char* base = lds + unit * T::UNIT + wave * 1024u;
         if (k0 + LINE <= a.d_bytes) {
-            const char* xk = x_rows + k0;
-            const char* wk = w_rows + k0;
-#pragma unroll
-            for (int i = 0; i < T::XL; ++i) {
-                __builtin_amdgcn_global_load_lds((gptr)(xk + (uint64_t)x_at[hx][i]), (lptr)(base + i * 4096), 16, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < T::WL; ++i) {
-                __builtin_amdgcn_global_load_lds((gptr)(wk + (uint64_t)w_at[hw][i]), (lptr)(base + (T::XL + i) * 4096), 16, 0, 0);
-            }
-        } else {   // the stage that d ends in: pieces beyond it are zeros
-            const char* zeros = reinterpret_cast<const char*>(&line_of_zeros);
 #pragma unroll
             for (int i = 0; i < T::LOADS; ++i) {
-                const char* from = i < T::XL ? x_rows + k0 + (uint64_t)x_at[hx][i < T::XL ? i : 0]
-                                             : w_rows + k0 + (uint64_t)w_at[hw][i < T::XL ? 0 : i - T::XL];
-                from = k0 + k_at[i] < a.d_bytes ? from : zeros;
-                __builtin_amdgcn_global_load_lds((gptr)from, (lptr)(base + i * 4096), 16, 0, 0);
+                load(s, hx, hw, unit, i);
             }
+            return;
+        }
+        // the stage that d ends in: pieces beyond it are zeros
+        char* base = lds + unit * T::UNIT + wave * 1024u;
+        const char* zeros = reinterpret_cast<const char*>(&line_of_zeros);
+#pragma unroll
+        for (int i = 0; i < T::LOADS; ++i) {
+            const char* from = i < T::XL ? x_rows + k0 + (uint64_t)x_at[hx][i < T::XL ? i : 0]
+                                         : w_rows + k0 + (uint64_t)w_at[hw][i < T::XL ? 0 : i - T::XL];
+            const uint32_t row = (uint32_t)((i < T::XL ? i : i - T::XL) * 32) + wave * 8u + (lane >> 3);
+            from = k0 + ((lane & 7u) ^ ((row >> 1) & 7u)) * 16u < a.d_bytes ? from : zeros;
+            __builtin_amdgcn_global_load_lds((gptr)from, (lptr)(base + i * 4096), 16, 0, 0);
         }
     };
     // A lane's operands out of a unit.
-    const uint32_t off = r16 * LINE + ((g ^ (r16 >> 1)) << 4);
-    const uint32_t x_off = wm * (uint32_t)(MH * 16) * LINE + off, w_off = (uint32_t)T::XR * LINE + wn * (uint32_t)(NH * 16) * LINE + off;
-    Frag fx[2][MH], fw[2][NH];
-    auto read_x = [&](int h, int unit) {
-#pragma unroll
-        for (int i = 0; i < MH; ++i) {
-            const uint32_t at = (uint32_t)(unit * T::UNIT + i * 16 * (int)LINE) + x_off;
-            fx[h][i].lo = *reinterpret_cast<const u32x4*>(lds + at);
-            fx[h][i].hi = *reinterpret_cast<const u32x4*>(lds + (at ^ 64u));
-        }
+    const uint32_t off = r_in * LINE + ((Operand::first_piece(lane) ^ ((r_in >> 1) & 7u)) << 4);
+    const uint32_t x_off = wm * (uint32_t)(MH * S) * LINE + off, w_off = (uint32_t)T::XR * LINE + wn * (uint32_t)(NH * S) * LINE + off;
+    Operand fx[2][MH], fw[2][NH];
+    // the k-th read of a half
+    constexpr int XREADS = MH * Operand::PIECES, WREADS = NH * Operand::PIECES;
+    auto read = [&](Operand* f, uint32_t from, int k) {
+        const int i = k / Operand::PIECES, q = k % Operand::PIECES;
+        f[i].p[q] = *reinterpret_cast<const u32x4*>(lds + ((from + (uint32_t)(i * S * (int)LINE)) ^ ((uint32_t)q * Operand::NEXT_PIECE)));
     };
-    auto read_w = [&](int h, int unit) {
+    auto read_x = [&](int h, int unit, int k) { read(fx[h], (uint32_t)(unit * T::UNIT) + x_off, k); };
+    auto read_w = [&](int h, int unit, int k) { read(fw[h], (uint32_t)(unit * T::UNIT) + w_off, k); };
+    Sums acc[2][MH][2][NH];
+    auto clear = [&] {
 #pragma unroll
-        for (int i = 0; i < NH; ++i) {
-            const uint32_t at = (uint32_t)(unit * T::UNIT + i * 16 * (int)LINE) + w_off;
-            fw[h][i].lo = *reinterpret_cast<const u32x4*>(lds + at);
-            fw[h][i].hi = *reinterpret_cast<const u32x4*>(lds + (at ^ 64u));
-        }
-    };
-    f32x4 acc[2][MH][2][NH];
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+            for (int i = 0; i < MH; ++i) {
 #pragma unroll
-        for (int i = 0; i < MH; ++i) {
+                for (int e = 0; e < 2; ++e) {
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-#pragma unroll
-                for (int j = 0; j < NH; ++j) {
-                    acc[h][i][q][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int j = 0; j < NH; ++j) {
+                        acc[h][i][e][j] = Sums(0.0f);
+                    }
                 }
             }
         }
-    }
-    auto quarter = [&](int hx, int hw) {
+    };
+    clear();
+    // A quarter's products, one by one, `reads` reads and `loads` loads spread between the first of them: the
+    // matrix pipe is never without work while they are issued.
+    auto quarter = [&](int hx, int hw, int reads, auto&& read_one, int loads, auto&& load_one) {
+        constexpr int STEP = STEPS<P, S>, ALL = STEP * MH * NH;
 #pragma unroll
-        for (int i = 0; i < MH; ++i) {
+        for (int t = 0; t < ALL; ++t) {
+            const int q = t / (MH * NH), i = t / NH % MH, j = t % NH;
 #pragma unroll
-            for (int j = 0; j < NH; ++j) {
-                acc[hx][i][hw][j] = product<P>(fw[hw][j], fx[hx][i], acc[hx][i][hw][j]);
+            for (int k = 0; k < reads; ++k) {
+                if (k * ALL / reads / 2 == t) {
+                    read_one(k);
+                }
             }
+#pragma unroll
+            for (int k = 0; k < loads; ++k) {
+                if (k * ALL / loads == t) {
+                    load_one(k);
+                }
+            }
+            acc[hx][i][hw][j] = step<P, S>(fw[hw][j], fx[hx][i], acc[hx][i][hw][j], q);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
+    auto nothing = [](int) {};
     // Waits until this wave's reads are done and all but the `later` youngest of its loads have landed, then
     // for the other waves.
     auto meet = [&](bool two_units_behind) {
@@ -169,103 +238,68 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
         }
         __builtin_amdgcn_sched_barrier(0);
     };
-    // Units: Y of an even stage 0, X 1; of an odd stage 2 and 3.
-    auto stage = [&](uint32_t s, auto parity) {
+    // Units: Y of an even stage 0, X 1; of an odd stage 2 and 3.  `inner`: two more whole stages follow.
+    // (The reads of a stage past the last find what lies there; nothing is made of them.)
+    auto stage = [&](uint32_t s, auto parity, auto inner) {
         constexpr int p = decltype(parity)::value, Y = 2 * p, X = Y + 1, Y_NEXT = 2 - 2 * p;
-        meet(s + 1u < steps);                       // X of this stage has landed; Y's place is free
-        if (s + 2u < steps) {
-            ask(s + 2u, 0, p, Y);
+        constexpr bool INNER = decltype(inner)::value != 0;
+        constexpr int LOADS = INNER ? T::LOADS : 0;
+        meet(INNER || s + 1u < steps);              // X of this stage has landed; Y's place is free
+        if constexpr (!INNER) {
+            if (s + 2u < steps) {
+                ask(s + 2u, 0, p, Y);
+            }
         }
-        read_w(1 - p, X);
-        __builtin_amdgcn_sched_barrier(0);
-        quarter(0, p);
-        __builtin_amdgcn_sched_barrier(0);
-        read_x(1, X);
-        __builtin_amdgcn_sched_barrier(0);
-        quarter(0, 1 - p);
-        __builtin_amdgcn_sched_barrier(0);
-        meet(s + 2u < steps);                       // Y of the next stage has landed; X's place is free
-        if (s + 2u < steps) {
-            ask(s + 2u, 1, 1 - p, X);
+        quarter(0, p, WREADS, [&](int k) { read_w(1 - p, X, k); }, LOADS, [&](int k) { load(s + 2u, 0, p, Y, k); });
+        quarter(0, 1 - p, XREADS, [&](int k) { read_x(1, X, k); }, 0, nothing);
+        meet(INNER || s + 2u < steps);              // Y of the next stage has landed; X's place is free
+        if constexpr (!INNER) {
+            if (s + 2u < steps) {
+                ask(s + 2u, 1, 1 - p, X);
+            }
         }
-        if (s + 1u < steps) {
-            read_x(0, Y_NEXT);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        quarter(1, 1 - p);
-        __builtin_amdgcn_sched_barrier(0);
-        if (s + 1u < steps) {
-            read_w(1 - p, Y_NEXT);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        quarter(1, p);
-        __builtin_amdgcn_sched_barrier(0);
+        quarter(1, 1 - p, XREADS, [&](int k) { read_x(0, Y_NEXT, k); }, LOADS, [&](int k) { load(s + 2u, 1, 1 - p, X, k); });
+        quarter(1, p, WREADS, [&](int k) { read_w(1 - p, Y_NEXT, k); }, 0, nothing);
     };
-    if (steps != 0u) {
-        ask(0, 0, 0, 0);
-        ask(0, 1, 1, 1);
-        if (steps > 1u) {
-            ask(1, 0, 1, 2);
-            ask(1, 1, 0, 3);
-            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * T::LOADS) : "memory");
-        } else {
-            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        }
-        read_x(0, 0);
-        read_w(0, 0);
-        uint32_t s = 0;
-        for (; s + 1u < steps; s += 2u) {
-            stage(s, Parity<0>{});
-            stage(s + 1u, Parity<1>{});
-        }
-        if (s < steps) {
-            stage(s, Parity<0>{});
+    typedef Parity<1> Inner;
+    typedef Parity<0> Outer;
+    ask(0, 0, 0, 0);
+    ask(0, 1, 1, 1);
+    if (steps > 1u) {
+        ask(1, 0, 1, 2);
+        ask(1, 1, 0, 3);
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * T::LOADS) : "memory");
+    } else {
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+#pragma unroll
+    for (int k = 0; k < XREADS; ++k) {
+        read_x(0, 0, k);
+    }
+#pragma unroll
+    for (int k = 0; k < WREADS; ++k) {
+        read_w(0, 0, k);
+    }
+    uint32_t s = 0;
+    for (; s + 4u < steps; s += 2u) {   // (stage s + 3 is whole: the one that d may end in is a later one)
+        stage(s, Parity<0>{}, Inner{});
+        stage(s + 1u, Parity<1>{}, Inner{});
+    }
+    for (; s < steps; s += 2u) {
+        stage(s, Parity<0>{}, Outer{});
+        if (s + 1u < steps) {
+            stage(s + 1u, Parity<1>{}, Outer{});
         }
     }
+    __syncthreads();   // (the stages' place is the epilogue's)
 
     if (a.splits > 1u) {
         // The parts' sums meet in the workspace, a lane's where its lane of every other part finds them; the
         // last part to arrive adds them in order.
         const uint64_t block = (uint64_t)T::BM * T::BN / 2u;   // 64-bit words
         const uint64_t mine = ((uint64_t)tile * a.splits + split) * block + (uint64_t)tid;
-        uint32_t q = 0;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int i = 0; i < MH; ++i) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                    for (int j = 0; j < NH; ++j) {
-                        const f32x4 v = acc[h][i][e][j];
-                        handed_store(a.part, mine + (uint64_t)q * 512u,
-                                     (uint64_t)lilym_f32_bits(v[0]) | (uint64_t)lilym_f32_bits(v[1]) << 32);
-                        handed_store(a.part, mine + (uint64_t)q * 512u + 256u,
-                                     (uint64_t)lilym_f32_bits(v[2]) | (uint64_t)lilym_f32_bits(v[3]) << 32);
-                        ++q;
-                    }
-                }
-            }
-        }
-        if (!last_to_arrive(a.ticket + tile, a.splits, last, a.relaxed != 0u)) {
-            return;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int i = 0; i < MH; ++i) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                    for (int j = 0; j < NH; ++j) {
-                        acc[h][i][e][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                    }
-                }
-            }
-        }
-        for (uint32_t part = 0; part < a.splits; ++part) {
-            const uint64_t at = ((uint64_t)tile * a.splits + part) * block + (uint64_t)tid;
-            q = 0;
+        auto each = [&](auto&& f) {   // four sums of the lane and their place
+            uint32_t q = 0;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -274,33 +308,69 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
                     for (int e = 0; e < 2; ++e) {
 #pragma unroll
                         for (int j = 0; j < NH; ++j) {
-                            const uint64_t u = handed_load(a.part, at + (uint64_t)q * 512u);
-                            const uint64_t v = handed_load(a.part, at + (uint64_t)q * 512u + 256u);
-                            acc[h][i][e][j] += f32x4{lilym_bits_f32((uint32_t)u), lilym_bits_f32((uint32_t)(u >> 32)),
-                                                     lilym_bits_f32((uint32_t)v), lilym_bits_f32((uint32_t)(v >> 32))};
-                            ++q;
+#pragma unroll
+                            for (int v = 0; v < Operand::GROUPS * 4; v += 2) {
+                                f(acc[h][i][e][j], v, (uint64_t)q * 256u);
+                                ++q;
+                            }
                         }
                     }
                 }
             }
+        };
+        each([&](Sums& c, int v, uint64_t at) {
+            handed_store(a.part, mine + at, (uint64_t)lilym_f32_bits(c[v]) | (uint64_t)lilym_f32_bits(c[v + 1]) << 32);
+        });
+        if (!last_to_arrive(a.ticket + tile, a.splits, last, a.relaxed != 0u)) {
+            return;
+        }
+        clear();
+        for (uint32_t part = 0; part < a.splits; ++part) {
+            const uint64_t from = ((uint64_t)tile * a.splits + part) * block + (uint64_t)tid;
+            each([&](Sums& c, int v, uint64_t at) {
+                const uint64_t u = handed_load(a.part, from + at);
+                c[v] += lilym_bits_f32((uint32_t)u);
+                c[v + 1] += lilym_bits_f32((uint32_t)(u >> 32));
+            });
         }
     }
+    // A quarter at a time through the wave's own part of LDS, so that a lane ends with four neighbouring
+    // outputs and NH * S / 4 lanes with a row's: whole lines are stored.
+    constexpr int ROW = NH * S + 4;   // floats of a row there (a step of four banks from row to row)
+    static_assert(4 * MH * S * ROW * 4 <= T::LDS_BYTES, "a quarter of every wave");
+    constexpr int LANES = NH * S / 4, AT_ONCE = 64 / LANES;
+    float* mine = reinterpret_cast<float*>(lds) + wave * (uint32_t)(MH * S * ROW);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int j = 0; j < NH; ++j) {
-            const uint32_t v = n0 + wn * (uint32_t)(T::NT * 16) + (uint32_t)((e * NH + j) * 16) + g * 4u;
-            const Columns c = columns_at(a, v);
+        for (int e = 0; e < 2; ++e) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int i = 0; i < MH; ++i) {
 #pragma unroll
-                for (int i = 0; i < MH; ++i) {
-                    const uint32_t r = m0 + wm * (uint32_t)(T::MT * 16) + (uint32_t)((h * MH + i) * 16) + r16;
-                    if (r < a.rows) {
-                        finish(a, r, v, c, a.x_scales != nullptr ? gload(a.x_scales + r) : 1.0f, acc[h][i][e][j]);
+                for (int j = 0; j < NH; ++j) {
+#pragma unroll
+                    for (int q = 0; q < Operand::GROUPS; ++q) {
+                        const Sums& c = acc[h][i][e][j];
+                        *reinterpret_cast<f32x4*>(mine + ((uint32_t)(i * S) + r_in) * ROW + j * S + Operand::output(lane, q)) =
+                            f32x4{c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]};
                     }
                 }
             }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const uint32_t column = (lane % LANES) * 4u;
+            const uint32_t v = n0 + wn * (uint32_t)(T::NT * S) + (uint32_t)(e * NH * S) + column;
+            const Columns c = columns_at(a, v);
+            const uint32_t r0 = m0 + wm * (uint32_t)(T::MT * S) + (uint32_t)(h * MH * S);
+#pragma unroll 2
+            for (uint32_t q = lane / LANES; q < (uint32_t)(MH * S); q += AT_ONCE) {
+                const f32x4 sum = *reinterpret_cast<const f32x4*>(mine + q * ROW + column);
+                if (r0 + q < a.rows) {
+                    finish(a, r0 + q, v, c, a.x_scales != nullptr ? gload(a.x_scales + r0 + q) : 1.0f, sum);
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
     }
 }
@@ -354,12 +424,12 @@ hipError_t launch_project_tiles(hipStream_t stream, ProjectArgs& a, bool e4m3, u
                                 uint32_t handover) {
     const uint64_t big = (uint64_t)((a.rows + 255u) / 256u) * ((a.n + 255u) / 256u);
     if (a.rows > 128u && big >= 128u) {
-        return launch_tile<Tile<2, 2, 8, 8, 1>>(stream, a, e4m3, part_words, tickets, handover);
+        return launch_tile<Tile<32, 2, 2, 4, 4, 1>>(stream, a, e4m3, part_words, tickets, handover);
     }
     if (a.rows > 64u) {
-        return launch_tile<Tile<2, 2, 4, 4, 2>>(stream, a, e4m3, part_words, tickets, handover);
+        return launch_tile<Tile<16, 2, 2, 4, 4, 2>>(stream, a, e4m3, part_words, tickets, handover);
     }
-    return launch_tile<Tile<1, 4, 4, 2, 2>>(stream, a, e4m3, part_words, tickets, handover);
+    return launch_tile<Tile<16, 1, 4, 4, 2, 2>>(stream, a, e4m3, part_words, tickets, handover);
 }
 
 }  // namespace lily
