@@ -165,11 +165,13 @@ struct LogitsRows {
     uint32_t out_dtype = 0;
     bool logprobs = false;     // else the adjusted logits
     bool biased = false;       // some row has a bias list
+    bool in_place = false;     // out is where the logits are
     float* lse = nullptr;      // [rows of out] or null
-    Handed<double> part;       // workspace: [max_rows][MAX_SLICES][2]
-    uint32_t* ticket = nullptr;   // [max_rows], zero between launches
+    // workspace, all of it 0 between launches
+    Handed<uint64_t> word;     // [max_rows][MAX_SLICES]
+    uint32_t* done = nullptr;  // [max_rows]
     uint32_t max_rows = 0;
-    uint32_t handover = 0;     // 0 = by the launch's size, 1 = strict, 2 = relaxed
+    uint32_t looks = 0;        // at the words of a row's other slices, before a slice forms them itself
 };
 hipError_t launch_logits_rows(hipStream_t stream, int dtype, uint32_t rows, uint32_t vocab, const RowArgs* table,
                               const InlineRows* few, const LogitsRows& w);

@@ -2464,18 +2464,19 @@ static int check_logits_out(const lily_logits_out* o, const void* logits, uint64
     return LILY_OK;
 }
 
-static LogitsRows logits_rows_of(const lily_sampler* s, const lily_logits_out* o, bool biased) {
+static LogitsRows logits_rows_of(lily_sampler* s, const lily_logits_out* o, bool biased, const void* logits) {
     LogitsRows w;
+    w.in_place = o->out_dev == logits;
     w.out = o->out_dev;
     w.stride = o->out_stride;
     w.out_dtype = o->out_dtype;
     w.logprobs = o->logprobs != 0u;
     w.biased = biased;
     w.lse = o->log_sum_exp_dev;
-    w.part = Handed<double>{s->ws_lse};
-    w.ticket = s->ws_ticket;
-    w.max_rows = s->ws_rows;
-    w.handover = s->handover;
+    w.word = Handed<uint64_t>{s->wide_bounds};
+    w.done = s->wide_count;
+    w.max_rows = WS_ROWS;
+    w.looks = looks_of_launch(s).keys;
     return w;
 }
 
@@ -2513,7 +2514,7 @@ int lily_process_logits(lily_sampler_t* s, const lily_rows* b, const lily_logits
         }
         ON_DEVICE(s->device);
         HIP_TRY(launch_logits_rows(s->stream, (int)b->dtype, b->rows, b->vocab, nullptr, &rows,
-                                   logits_rows_of(s, o, any_biased(rows.r, b->rows))));
+                                   logits_rows_of(s, o, any_biased(rows.r, b->rows), b->logits_dev)));
         return LILY_OK;
     }
     if (s == nullptr) {
@@ -2532,7 +2533,7 @@ int lily_process_logits(lily_sampler_t* s, const lily_rows* b, const lily_logits
         return rc;
     }
     HIP_TRY(launch_logits_rows(s->stream, (int)b->dtype, b->rows, b->vocab, s->table_dev, nullptr,
-                               logits_rows_of(s, o, biased)));
+                               logits_rows_of(s, o, biased, b->logits_dev)));
     return LILY_OK;
 }
 
@@ -2545,7 +2546,7 @@ int lily_plan_process_logits(lily_plan_t* p, const lily_logits_out* o) {
     }
     ON_DEVICE(p->s->device);
     HIP_TRY(launch_logits_rows(p->s->stream, (int)p->dtype, p->rows, p->vocab, p->table_dev, nullptr,
-                               logits_rows_of(p->s, o, p->biased)));
+                               logits_rows_of(p->s, o, p->biased, p->logits)));
     return LILY_OK;
 }
 

@@ -578,23 +578,23 @@ class Sampler:
     # -- around the head
     def _matrix(self, t, rows, columns, name):
         """(address, stride, type) of a [rows, columns] operand whose rows are contiguous."""
-        code = DTYPES.get(t.dtype)
+        code, shape, stride = DTYPES.get(t.dtype), t.shape, t.stride()
         if code is None:
             raise SamplerError(-1, f"{name} must be F32, BF16 or E4M3, got {t.dtype}")
-        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != columns or (t.stride(1) != 1 and columns > 1):
+        if len(shape) != 2 or shape[0] != rows or shape[1] != columns or (stride[1] != 1 and columns > 1):
             raise SamplerError(-1, f"{name} must be [{rows}, {columns}], rows contiguous")
-        if not t.is_cuda or t.device.index != self.device:
+        if t.get_device() != self.device:
             raise SamplerError(-1, f"{name} must live on the sampler's device")
-        return t.data_ptr(), t.stride(0), code
+        return t.data_ptr(), stride[0], code
 
     def _vector(self, t, n, name):
         """(address, type) of a contiguous vector of n elements, or nothing."""
         if t is None:
             return None, F32
-        code = DTYPES.get(t.dtype)
-        if code is None or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        code, shape = DTYPES.get(t.dtype), t.shape
+        if code is None or len(shape) != 1 or shape[0] != n or (t.stride(0) != 1 and n > 1):
             raise SamplerError(-1, f"{name} must be [{n}], contiguous")
-        if not t.is_cuda or t.device.index != self.device:
+        if t.get_device() != self.device:
             raise SamplerError(-1, f"{name} must live on the sampler's device")
         return t.data_ptr(), code
 

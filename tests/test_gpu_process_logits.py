@@ -4,7 +4,7 @@ Bar:
   * adjusted f32 values bit-exact against the draws' arithmetic restated in numpy f32 (biases in list
     order, mask, penalties, IEEE division by T; NaN worth -inf); bf16 output: those rounded to nearest even;
   * log_sum_exp against f64 over the reference's f32 values: a thread adds n <= max(8, V / 1024) terms
-    (rows here have 1 024 threads or slices of 2 048 ids), each addition, each raise of its reference (one
+    (slices of 2 048 to 8 192 ids, 32 a thread at most, or of a 64th of a long row), each addition, each raise of its reference (one
     in four) and each term (exponent formed with three roundings of at most |x| e^-|x| <= 0.37 weight, the
     exponential 2 steps) rounded: (1.25 n + 8) 2^-24 relative to the sum, so absolute in its logarithm,
     and one rounding of the result;
@@ -301,6 +301,63 @@ def test_a_draw_from_the_written_row_is_the_draw_from_the_raw_one(sampler):
         assert torch.equal(ids, raw_ids), step
         sampler.process_logits(logits, params, written, log_sum_exp=lse, scratch=scratch, allow=a, bias=lists)
         del keep
+
+
+@pytest.mark.parametrize("looks", ["0,0,1000000", "1,1,1000000"])
+def test_slices_that_do_not_wait_for_each_other(monkeypatch, looks):
+    """A slice that does not find the words of its row's other slices forms them itself: the same bits, in place of
+    the logits too, and the workspace is clean for the calls that follow."""
+    patient = LS.Sampler(0)
+    monkeypatch.setenv("LILY_SAMPLER_WIDE_LOOKS", looks)
+    hasty = LS.Sampler(0)
+    monkeypatch.delenv("LILY_SAMPLER_WIDE_LOOKS")
+    rng = np.random.default_rng(31)
+    for rows, vocab in ((1, 151936), (7, 50257), (70, 30000)):
+        x, kws, _, allow, lists, _ = _case(None, rng, rows, vocab, "f32", False, "rows", 9, [0.7, 1.0])
+        logits, a = upload_logits(x), torch.from_numpy(allow.view(np.int32)).to(dev())
+        params = [ls_params(**k) for k in kws]
+        for logprobs in (False, True):
+            outs = []
+            for s, place in ((patient, False), (hasty, False), (patient, True), (hasty, True), (hasty, False)):
+                out = logits.clone() if place else torch.empty_like(logits)
+                lse = torch.zeros(rows, device=dev())
+                torch.cuda.synchronize()
+                keep = s.process_logits(out if place else logits, params, out, log_sum_exp=lse, logprobs=logprobs, allow=a, bias=lists)
+                s.synchronize()
+                outs.append((out.cpu().numpy().view(np.uint32), lse.cpu().numpy().view(np.uint32)))
+                del keep
+            for o in outs[1:]:
+                assert np.array_equal(outs[0][0], o[0]) and np.array_equal(outs[0][1], o[1]), (rows, vocab, logprobs)
+        # the draws of many candidates use the same workspace
+        ids = [torch.zeros(rows, dtype=torch.int32, device=dev()) for _ in range(2)]
+        torch.cuda.synchronize()
+        for s, out in ((patient, ids[0]), (hasty, ids[1])):
+            s.sample_rows(logits, [ls_params(temperature=0.9, top_k=0, seed=r) for r in range(rows)], [3] * rows, out)
+            s.synchronize()
+        assert torch.equal(ids[0], ids[1])
+    patient.close()
+    hasty.close()
+
+
+def test_rows_longer_than_the_slices_that_are_held(sampler):
+    rng = np.random.default_rng(77)
+    rows, vocab = 2, 600001
+    x, kws, scratch, allow, lists, want = _case(sampler, rng, rows, vocab, "bf16", True, "rows", 30, [0.8])
+    _, logits = _place(x, "bf16", 1, 0)
+    a = torch.from_numpy(allow.view(np.int32)).to(dev())
+    out, lse = torch.empty(rows, vocab, device=dev()), torch.empty(rows, device=dev())
+    for logprobs in (False, True, False):
+        torch.cuda.synchronize()
+        keep = sampler.process_logits(logits, [ls_params(**k) for k in kws], out, log_sum_exp=lse, logprobs=logprobs,
+                                      scratch=scratch, allow=a, bias=lists)
+        sampler.synchronize()
+        _check(out, lse, want, logprobs, vocab)
+        del keep
+    short = torch.empty(rows, 5000, device=dev())   # the words these rows left are gone
+    torch.cuda.synchronize()
+    sampler.process_logits(upload_logits(x[:, :5000].astype(F)), [ls_params()] * rows, short, log_sum_exp=lse)
+    sampler.synchronize()
+    _check(short, lse, [_adjusted(x[r, :5000], {}) for r in range(rows)], False, 5000)
 
 
 def test_rows_that_share_a_scratch_and_leave_its_counts_alone(sampler):
