@@ -13,11 +13,8 @@ hipError_t launch_rms_norm(hipStream_t stream, const lily_norm& norm, bool piece
 
 // The matrix product with an epilogue (project_few.hip, project_tiles.hip); the workspace is the sampler's.
 struct ProjectWorkspace {
-    uint64_t* part;
-    uint64_t part_words;
-    uint32_t* ticket;   // zero between launches
-    uint32_t tickets;
-    uint32_t handover;  // 0 = by the launch's size, 1 = strict, 2 = relaxed
+    float* part;            // sums of parts of d, in 16-byte units
+    uint64_t part_floats;
 };
 hipError_t launch_project(hipStream_t stream, const lily_projection& p, const ProjectWorkspace& ws);
 

@@ -36,12 +36,11 @@ struct ProjectArgs {
     uint64_t residual_stride, out_stride;      // elements
     uint32_t rows, n, d_bytes;
     uint32_t bias_bf16, residual_bf16, out_bf16, act;
-    uint32_t wide;              // four neighbouring outputs (and residuals) start at multiples of their size
     uint32_t splits;            // parts of d, each a workgroup's
-    uint32_t relaxed;           // the form of their hand-over
-    Handed<uint64_t> part;      // their sums
-    uint32_t* ticket;           // [tiles], zero between launches
+    float* part;                // their sums, [splits][rows][part_stride(n)]
 };
+
+__host__ __device__ constexpr uint32_t part_stride(uint32_t n) { return (n + 3u) / 4u * 4u; }
 
 // The operand of a lane: two pieces.
 struct Frag {
@@ -92,20 +91,28 @@ __device__ __forceinline__ f32x4 product(const Frag& w, const Frag& x, f32x4 c) 
 __device__ __forceinline__ float logistic(float v) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * v));
 }
-__device__ __forceinline__ float activated(float v, uint32_t act) {
-    switch (act) {
-    case LILY_ACT_SILU:
-        return v * logistic(v);
-    case LILY_ACT_GELU:
-        return 0.5f * v * erfcf(-0.70710678118654752f * v);
-    case LILY_ACT_GELU_TANH: {
-        const float u = 1.5957691216057308f * (v + 0.044715f * v * v * v);   // 2 sqrt(2 / pi) (v + ...)
-        return v * logistic(u);
-    }
-    case LILY_ACT_RELU:
-        return v > 0.0f || v != v ? v : 0.0f;
-    default:
-        return v;
+template <int N>
+__device__ __forceinline__ void activate(float (&v)[N], uint32_t act) {   // (one branch for all of them)
+    if (act == LILY_ACT_SILU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            v[j] *= logistic(v[j]);
+        }
+    } else if (N <= 4 && act == LILY_ACT_GELU) {   // (some eighty instructions a value: a row at a time only)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            v[j] = 0.5f * v[j] * erfcf(-0.70710678118654752f * v[j]);
+        }
+    } else if (act == LILY_ACT_GELU_TANH) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            v[j] *= logistic(1.5957691216057308f * (v[j] + 0.044715f * v[j] * v[j] * v[j]));   // 2 sqrt(2 / pi) (v + ...)
+        }
+    } else if (act == LILY_ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            v[j] = v[j] > 0.0f || v[j] != v[j] ? v[j] : 0.0f;
+        }
     }
 }
 
@@ -115,82 +122,129 @@ __device__ __forceinline__ uint32_t pj_bf16_pair(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((pj_f32x2{a, b}), pj_bf16x2));
 }
 
-// What the epilogue knows of four neighbouring columns before it sees a row.
+// What the epilogue knows of four neighbouring columns before it sees a row.  (As it lies in memory: values are
+// widened where they are used, so that nobody waits for them before.)
 struct Columns {
-    float scale[4], bias[4];
-};
-__device__ __forceinline__ Columns columns_at(const ProjectArgs& a, uint32_t v0) {
-    Columns c;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint32_t v = min(v0 + (uint32_t)j, a.n - 1u);
-        c.scale[j] = a.w_scales != nullptr ? gload(a.w_scales + v) : 1.0f;
-        c.bias[j] = a.bias == nullptr ? 0.0f
-                    : a.bias_bf16     ? lilym_bits_f32((uint32_t)gload(static_cast<const uint16_t*>(a.bias) + v) << 16)
-                                      : gload(static_cast<const float*>(a.bias) + v);
-    }
-    return c;
-}
-
-// Sums of row r (< rows), columns v0 .. v0 + 3, finished and stored.
-__device__ __forceinline__ void finish(const ProjectArgs& a, uint32_t r, uint32_t v0, const Columns& c, float x_scale, f32x4 sum) {
-    if (v0 >= a.n) {
-        return;
-    }
-    float v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        v[j] = sum[j] * x_scale * c.scale[j] + c.bias[j];
-    }
-    if (a.act != LILY_ACT_NONE) {
+    float scale[4];
+    uint32_t raw[4];
+    __device__ __forceinline__ void load(const ProjectArgs& a, uint32_t v0) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            v[j] = activated(v[j], a.act);
+            const uint32_t v = min(v0 + (uint32_t)j, a.n - 1u);
+            scale[j] = 1.0f;
+            raw[j] = 0u;
+            if (a.w_scales != nullptr) {
+                scale[j] = gload(a.w_scales + v);
+            }
+            if (a.bias != nullptr) {
+                raw[j] = a.bias_bf16 ? (uint32_t)gload(static_cast<const uint16_t*>(a.bias) + v)
+                                     : gload(static_cast<const uint32_t*>(a.bias) + v);
+            }
         }
     }
-    const uint64_t at = (uint64_t)r * a.out_stride + v0, from = (uint64_t)r * a.residual_stride + v0;
-    if (a.wide && v0 + 4u <= a.n) {
-        if (a.residual != nullptr) {
-            if (a.residual_bf16) {
-                const pj_u32x2 q = gload(reinterpret_cast<const pj_u32x2*>(static_cast<const uint16_t*>(a.residual) + from));
-                v[0] += lilym_bits_f32(q.x << 16);
-                v[1] += lilym_bits_f32(q.x & 0xffff0000u);
-                v[2] += lilym_bits_f32(q.y << 16);
-                v[3] += lilym_bits_f32(q.y & 0xffff0000u);
-            } else {
-                const f32x4 q = gload(reinterpret_cast<const f32x4*>(static_cast<const float*>(a.residual) + from));
+    __device__ __forceinline__ float bias(const ProjectArgs& a, int j) const {
+        return lilym_bits_f32(a.bias_bf16 ? raw[j] << 16 : raw[j]);
+    }
+};
+
+// (rows of any alignment: the hardware takes wide accesses at any element)
+typedef pj_u32x2 pj_u32x2_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+typedef u32x4 pj_u32x4_any __attribute__((aligned(4)));
+
+// N rows r0, r0 + step, ... (those below a.rows count) of columns v0 .. v0 + 3 (v0 < n): load() asks for what the
+// epilogue reads of them, store() finishes their sums.
+template <int N>
+struct Finish {
+    float scale[N];
+    u32x4 res[N];   // two bf16 a word, or f32
+    __device__ __forceinline__ void load(const ProjectArgs& a, uint32_t r0, uint32_t step, uint32_t v0) {
+        const uint32_t top = a.rows - 1u;
+        const bool whole = v0 + 4u <= a.n;
+        if (a.x_scales != nullptr) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    v[j] += q[j];
+            for (int q = 0; q < N; ++q) {
+                scale[q] = gload(a.x_scales + min(r0 + (uint32_t)q * step, top));
+            }
+        }
+        if (a.residual != nullptr) {
+#pragma unroll
+            for (int q = 0; q < N; ++q) {
+                const uint64_t from = (uint64_t)min(r0 + (uint32_t)q * step, top) * a.residual_stride + v0;
+                if (whole && a.residual_bf16) {
+                    const pj_u32x2 t = *(const LILY_GLOBAL pj_u32x2_any*)(static_cast<const uint16_t*>(a.residual) + from);
+                    res[q] = u32x4{t.x, t.y, 0u, 0u};
+                } else if (whole) {
+                    res[q] = *(const LILY_GLOBAL pj_u32x4_any*)(static_cast<const uint32_t*>(a.residual) + from);
+                } else {
+                    uint32_t t[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint64_t at = from + min((uint32_t)j, a.n - 1u - v0);
+                        t[j] = a.residual_bf16 ? (uint32_t)gload(static_cast<const uint16_t*>(a.residual) + at)
+                                               : gload(static_cast<const uint32_t*>(a.residual) + at);
+                    }
+                    res[q] = a.residual_bf16 ? u32x4{t[0] | t[1] << 16, t[2] | t[3] << 16, 0u, 0u} : u32x4{t[0], t[1], t[2], t[3]};
                 }
             }
         }
-        if (a.out_bf16) {
-            *(LILY_GLOBAL pj_u32x2*)(static_cast<uint16_t*>(a.out) + at) =
-                pj_u32x2{pj_bf16_pair(v[0], v[1]), pj_bf16_pair(v[2], v[3])};
-        } else {
-            *(LILY_GLOBAL f32x4*)(static_cast<float*>(a.out) + at) = f32x4{v[0], v[1], v[2], v[3]};
-        }
-        return;
     }
+    __device__ __forceinline__ float residual(const ProjectArgs& a, int q, int j) const {
+        const u32x4 w = res[q];
+        const uint32_t half = (j & 1) ? w[j / 2] & 0xffff0000u : w[j / 2] << 16;
+        return lilym_bits_f32(a.residual_bf16 ? half : w[j]);
+    }
+    __device__ __forceinline__ void store(const ProjectArgs& a, uint32_t r0, uint32_t step, uint32_t v0, const Columns& c,
+                                          const f32x4 (&sums)[N]) const {
+        float v[4 * N];
+        const bool whole = v0 + 4u <= a.n;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (v0 + (uint32_t)j < a.n) {
-            if (a.residual != nullptr) {
-                v[j] += a.residual_bf16 ? load_logit<LILY_BF16>(static_cast<const uint16_t*>(a.residual) + from, (uint32_t)j)
-                                        : load_logit<LILY_F32>(static_cast<const float*>(a.residual) + from, (uint32_t)j);
+        for (int q = 0; q < N; ++q) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float t = a.x_scales != nullptr ? sums[q][j] * scale[q] : sums[q][j];
+                v[4 * q + j] = t * c.scale[j] + c.bias(a, j);
             }
-            if (a.out_bf16) {
-                *(LILY_GLOBAL uint16_t*)(static_cast<uint16_t*>(a.out) + at + j) = (uint16_t)pj_bf16_pair(v[j], 0.0f);
-            } else {
-                *(LILY_GLOBAL float*)(static_cast<float*>(a.out) + at + j) = v[j];
+        }
+        activate(v, a.act);
+        if (a.residual != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 4 * N; ++e) {
+                v[e] += residual(a, e / 4, e % 4);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+            const uint32_t r = r0 + (uint32_t)q * step;
+            if (r < a.rows) {
+                store_row(a, (uint64_t)r * a.out_stride + v0, v0, f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]});
             }
         }
     }
-}
+    static __device__ __forceinline__ void store_row(const ProjectArgs& a, uint64_t at, uint32_t v0, f32x4 v) {
+        if (v0 + 4u <= a.n) {
+            if (a.out_bf16) {
+                *(LILY_GLOBAL pj_u32x2_any*)(static_cast<uint16_t*>(a.out) + at) = pj_u32x2{pj_bf16_pair(v[0], v[1]), pj_bf16_pair(v[2], v[3])};
+            } else {
+                *(LILY_GLOBAL f32x4_any*)(static_cast<float*>(a.out) + at) = v;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (v0 + (uint32_t)j < a.n) {
+                    if (a.out_bf16) {
+                        *(LILY_GLOBAL uint16_t*)(static_cast<uint16_t*>(a.out) + at + j) = (uint16_t)pj_bf16_pair(v[j], 0.0f);
+                    } else {
+                        *(LILY_GLOBAL float*)(static_cast<float*>(a.out) + at + j) = v[j];
+                    }
+                }
+            }
+        }
+    }
+};
 
 hipError_t launch_project_few(hipStream_t stream, const ProjectArgs& a, bool e4m3);
-hipError_t launch_project_tiles(hipStream_t stream, ProjectArgs& a, bool e4m3, uint64_t part_words, uint32_t tickets,
-                                uint32_t handover);
+// `tile`: 64, 128 or 256 rows and outputs; a.splits parts of d.
+hipError_t launch_project_tiles(hipStream_t stream, const ProjectArgs& a, bool e4m3, uint32_t tile);
 
 }  // namespace lily

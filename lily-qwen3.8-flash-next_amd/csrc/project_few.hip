@@ -1,88 +1,211 @@
-// project_few.hip - the matrix product with an epilogue for up to 16 rows: the weights are read once at
-// the speed of memory, the matrix cores idle.
+// project_few.hip - the matrix product with an epilogue for few rows: the weights are read once at the speed of
+// memory, the matrix cores idle.
 //
-// A workgroup takes 16 outputs' weight rows; its waves share d, a run of whole lines (128 bytes a row)
-// each, so that a layer of a few thousand outputs already keeps every compute unit's memory path busy without
-// a join between workgroups.  A wave asks for its lines straight into the registers the product takes them
-// from, AHEAD of them at a time (16 rows x 64 bytes an instruction, the line's other half with the next).
-// The waves' sums meet in LDS.
+// A workgroup takes 16 outputs' weight rows; its waves share d, a run of whole lines (128 bytes a row) each, so that
+// a layer of a few thousand outputs already keeps every compute unit's memory path busy without a join between
+// workgroups.  A wave works alone: its lines arrive in a ring of its own in LDS, loads that write LDS themselves, eight
+// whole lines an instruction (a lane that loads what the product wants of it touches 16 lines with every 16
+// lanes: 16 bytes a clock and compute unit, whatever is in flight), and it waits for its own loads only.  The
+// waves' sums meet in LDS.
+#include <algorithm>
+
+#include "launch.h"
 #include "project.h"
 
 namespace lily {
 
 namespace {
 
-constexpr int FEW_AHEAD = 8;   // lines of a wave in flight
+__device__ const uint4 few_zeros = {0u, 0u, 0u, 0u};   // what lies beyond d
 
-template <Products P>
-__global__ void __launch_bounds__(512) k_project_few(const ProjectArgs a) {
+// RT: blocks of 16 rows of x; DEPTH: lines of a wave in flight.
+template <Products P, int RT, int WAVES, int DEPTH>
+__global__ void __launch_bounds__(WAVES * 64) k_project_few(const ProjectArgs a) {
+    constexpr uint32_t ROWS = 16 + 16 * RT, SLOT = ROWS * LINE, LOADS = ROWS / 8;
     extern __shared__ __align__(16) char lds[];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, waves = blockDim.x >> 6;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const uint32_t g = lane >> 4, r = lane & 15u, v0 = blockIdx.x * 16u;
     const uint32_t lines = (a.d_bytes + LINE - 1u) / LINE;
-    const uint32_t per = (lines + waves - 1u) / waves, from = min(wave * per, lines), to = min(from + per, lines);
-    const char* w = a.w + (uint64_t)min(v0 + r, a.n - 1u) * a.w_stride;
-    const char* x = a.x + (uint64_t)min(r, a.rows - 1u) * a.x_stride;
-    // (a row beyond the last is the last one's values: its sums go nowhere)
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    auto piece = [&](const char* row, uint32_t at) -> u32x4 {
-        // beyond d: zeros, in both operands (what lies behind a row may be anything)
-        const u32x4 p = gload(reinterpret_cast<const u32x4*>(row + min(at, a.d_bytes - 16u)));
-        return at < a.d_bytes ? p : u32x4{0u, 0u, 0u, 0u};
-    };
-    for (uint32_t l0 = from; l0 < to; l0 += FEW_AHEAD) {
-        Frag fw[FEW_AHEAD], fx[FEW_AHEAD];
+    const uint32_t per = lines / WAVES, over = lines % WAVES;
+    const uint32_t from = wave * per + min(wave, over), count = per + (wave < over ? 1u : 0u);
+    // The wave that finishes asks for what the epilogue reads before anything else: behind the sums it would be
+    // another trip to memory.
+    const uint32_t v = v0 + g * 4u, row0 = wave * 16u + r;
+    Columns columns;
+    Finish<1> finish;
+    const bool finishes = wave < (uint32_t)RT && v < a.n && row0 < a.rows;
+    if (finishes) {
+        columns.load(a, v);
+        finish.load(a, row0, 1u, v);
+    }
+    // Instruction i brings rows 8 i .. 8 i + 7 of a line (16 of the weights, then x), a lane the piece that
+    // belongs in its place: the pieces of a row change places by the row's number, so that 16 lanes that read one
+    // piece of 16 rows meet 16 groups of banks.  (A row beyond the last is the last one's values: its sums go nowhere.)
+    const char* src[LOADS];
 #pragma unroll
-        for (int u = 0; u < FEW_AHEAD; ++u) {
-            // (a line past the wave's last is its last again, and its product is left out)
-            const uint32_t at = min(l0 + (uint32_t)u, to - 1u) * LINE + g * 16u;
-            fw[u].lo = piece(w, at);
-            fw[u].hi = piece(w, at + 64u);
-            fx[u].lo = piece(x, at);
-            fx[u].hi = piece(x, at + 64u);
-        }
+    for (uint32_t i = 0; i < LOADS; ++i) {
+        const uint32_t row = i * 8u + (lane >> 3), piece = (lane & 7u) ^ ((row >> 1) & 7u);
+        src[i] = (i < 2u ? a.w + (uint64_t)min(v0 + row, a.n - 1u) * a.w_stride
+                         : a.x + (uint64_t)min(row - 16u, a.rows - 1u) * a.x_stride) + piece * 16u + from * LINE;
+    }
+    typedef __attribute__((address_space(1))) const void* gptr;
+    typedef __attribute__((address_space(3))) void* lptr;
+    char* ring = lds + wave * (DEPTH * SLOT);
+    auto ask = [&](uint32_t l, uint32_t slot) {
+        char* base = ring + slot * SLOT;
+        const uint32_t at = l * LINE;
+        if ((from + l + 1u) * LINE <= a.d_bytes) {
 #pragma unroll
-        for (int u = 0; u < FEW_AHEAD; ++u) {
-            if (l0 + (uint32_t)u < to) {
-                acc = product<P>(fw[u], fx[u], acc);
+            for (uint32_t i = 0; i < LOADS; ++i) {
+                __builtin_amdgcn_global_load_lds((gptr)(src[i] + at), (lptr)(base + i * 1024u), 16, 0, 0);
+            }
+        } else {   // the line that d ends in: pieces beyond it are zeros, in both operands
+            const char* zeros = reinterpret_cast<const char*>(&few_zeros);
+#pragma unroll
+            for (uint32_t i = 0; i < LOADS; ++i) {
+                const uint32_t piece = (lane & 7u) ^ (((i * 8u + (lane >> 3)) >> 1) & 7u);
+                const char* p = (from + l) * LINE + piece * 16u < a.d_bytes ? src[i] + at : zeros;
+                __builtin_amdgcn_global_load_lds((gptr)p, (lptr)(base + i * 1024u), 16, 0, 0);
             }
         }
+    };
+#pragma unroll
+    for (uint32_t j = 0; j < DEPTH; ++j) {
+        if (j < count) {
+            ask(j, j);
+        }
     }
+    f32x4 acc[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const uint32_t off = r * LINE + ((g ^ (r >> 1)) << 4);
+    uint32_t slot = 0;
+    for (uint32_t l = 0; l < count; ++l) {
+        if (l + DEPTH <= count) {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * LOADS) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        const char* base = ring + slot * SLOT + off;
+        auto frag = [&](uint32_t block) {
+            Frag f;
+            f.lo = *reinterpret_cast<const u32x4*>(base + block * 16u * LINE);
+            f.hi = *reinterpret_cast<const u32x4*>(lds + ((uint32_t)(base - lds) ^ 64u) + block * 16u * LINE);
+            return f;
+        };
+        const Frag fw = frag(0);
+        Frag fx[RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            fx[t] = frag(1u + (uint32_t)t);
+        }
+        __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): the slot has been read
+        __builtin_amdgcn_sched_barrier(0);
+        if (l + DEPTH < count) {
+            ask(l + DEPTH, slot);
+        }
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            acc[t] = product<P>(fw, fx[t], acc[t]);
+        }
+        slot = slot + 1u == DEPTH ? 0u : slot + 1u;
+    }
+    __syncthreads();   // (every ring is the sums' place now)
     f32x4* sums = reinterpret_cast<f32x4*>(lds);
-    if (waves > 1u) {
-        if (wave != 0u) {
-            sums[(wave - 1u) * 64u + lane] = acc;
-        }
-        __syncthreads();
-        if (wave != 0u) {
-            return;
-        }
-        for (uint32_t q = 0; q + 1u < waves; ++q) {
-            acc += sums[q * 64u + lane];
-        }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        sums[(wave * RT + (uint32_t)t) * 64u + lane] = acc[t];
     }
-    if (r < a.rows) {
-        const uint32_t v = v0 + g * 4u;
-        finish(a, r, v, columns_at(a, v), a.x_scales != nullptr ? gload(a.x_scales + r) : 1.0f, acc);
+    __syncthreads();
+    if (finishes) {   // block `wave` of the rows
+        f32x4 sum[1] = {sums[wave * 64u + lane]};
+#pragma unroll
+        for (uint32_t q = 1; q < WAVES; ++q) {
+            sum[0] += sums[(q * RT + wave) * 64u + lane];
+        }
+        finish.store(a, row0, 1u, v, columns, sum);
     }
+}
+
+template <int RT, int WAVES, int DEPTH>
+hipError_t launch_few(hipStream_t stream, const ProjectArgs& a, bool e4m3) {
+    constexpr uint32_t lds = WAVES * DEPTH * (16 + 16 * RT) * LINE;
+    static_assert(lds >= WAVES * RT * 1024, "the sums' place");
+    const dim3 grid((a.n + 15u) / 16u), block(WAVES * 64);
+    static LdsAllowed allowed[2];
+    const void* kernel = e4m3 ? (const void*)k_project_few<PRODUCT_E4M3_WIDE, RT, WAVES, DEPTH>
+                              : (const void*)k_project_few<PRODUCT_BF16, RT, WAVES, DEPTH>;
+    if (const hipError_t e = allowed[e4m3 ? 1 : 0].say(kernel, lds); e != hipSuccess) {
+        return e;
+    }
+    if (e4m3) {
+        hipLaunchKernelGGL((k_project_few<PRODUCT_E4M3_WIDE, RT, WAVES, DEPTH>), grid, block, lds, stream, a);
+    } else {
+        hipLaunchKernelGGL((k_project_few<PRODUCT_BF16, RT, WAVES, DEPTH>), grid, block, lds, stream, a);
+    }
+    return hipGetLastError();
 }
 
 }  // namespace
 
+// (waves x lines of a wave in flight, d = 4096 bf16, n = 4096 / 151 936 in E4M3, us: 8 x 2 7.5 / 105, 8 x 4 7.7 / 150, 4 x 4
+// 7.8 / 103; 64 rows 4 x 2 10.1, 8 x 1 10.3, 4 x 4 10.4)
 hipError_t launch_project_few(hipStream_t stream, const ProjectArgs& a, bool e4m3) {
+    return a.rows <= 16u   ? launch_few<1, 8, 2>(stream, a, e4m3)
+           : a.rows <= 32u ? launch_few<2, 8, 2>(stream, a, e4m3)
+                           : launch_few<4, 4, 2>(stream, a, e4m3);
+}
+
+// Which kernel, and how many parts of d: by an estimate of each one's time in us, from what they take on the chip
+// (rows x n x d in bf16, the estimate in brackets):
+//   few rows     a compute unit takes in 85 GB/s through LDS: 64 x 4096 x 4096 10.1 (10.5), 64 x 16384 x 2048 19.4 (18.2)
+//   64 x 64      a line of d 0.27 a round of one tile a compute unit, 0.21 where it has several: 256 x 4096 x 4096 18.4
+//                (20.3), 512 x 4096 x 4096 29.8 (29.9), 64 x 16384 x 2048 16.4 (15.2: memory)
+//   128 x 128    0.51 a tile of a compute unit: 1024 x 4096 x 4096 .. 8192 x 4096 x 4096 271 (267)
+//   256 x 256    1.45 a tile, and 15 for every tile's epilogue, which nothing hides: 8192 x 4096 x 4096 242 (218), where
+//                128 x 128 would take 271
+// Parts of d: a launch more (3, with what the parts' sums cost to write and read at 4 TB/s): 64 x 1000 x 8192 in eight 10.6
+// (11.3) against 25.5 in one; memory at 5.6 TB/s bounds all of them.
+struct ProjectPlan {
+    uint32_t tile = 0;     // 0: few rows
+    uint32_t splits = 1;
+};
+static ProjectPlan project_plan(const ProjectArgs& a, uint64_t part_floats) {
+    const double rows = a.rows, n = a.n, bytes = a.d_bytes;
     const uint32_t lines = (a.d_bytes + LINE - 1u) / LINE;
-    uint32_t waves = 1;
-    while (waves < 8u && waves * (uint32_t)FEW_AHEAD < lines) {
-        waves *= 2u;
+    const double memory = ((rows + n) * bytes + rows * n * (a.out_bf16 ? 2.0 : 4.0)) / 5.6e6;
+    auto over = [](uint32_t x, uint32_t y) { return (x + y - 1u) / y; };
+    auto rounds = [](uint64_t tiles) { return (double)((tiles + 255u) / 256u); };
+    ProjectPlan best;
+    double least = 1e30;
+    auto offer = [&](uint32_t tile, uint32_t splits, double us) {
+        if (us < least) {
+            least = us;
+            best.tile = tile;
+            best.splits = splits;
+        }
+    };
+    if (a.rows <= 64u) {
+        const double blocks = a.rows <= 16u ? 2.0 : a.rows <= 32u ? 3.0 : 5.0;   // of 16 rows a workgroup takes in
+        offer(0u, 1u, 2.8 + std::max(memory, rounds(over(a.n, 16u)) * blocks * 16.0 * bytes / 85e3));
+        if (a.rows <= 16u) {
+            return best;   // (nothing else reads the weights once)
+        }
     }
-    const dim3 grid((a.n + 15u) / 16u), block(waves * 64u);
-    const size_t lds = (size_t)(waves - 1u) * 1024u;
-    if (e4m3) {
-        hipLaunchKernelGGL((k_project_few<PRODUCT_E4M3_WIDE>), grid, block, lds, stream, a);
-    } else {
-        hipLaunchKernelGGL((k_project_few<PRODUCT_BF16>), grid, block, lds, stream, a);
+    const uint64_t t64 = (uint64_t)over(a.rows, 64u) * over(a.n, 64u), t128 = (uint64_t)over(a.rows, 128u) * over(a.n, 128u),
+                   t256 = (uint64_t)over(a.rows, 256u) * over(a.n, 256u);
+    for (uint32_t k = 1; k <= 16u; k *= 2u) {
+        if (k > 1u && (lines < 4u * k || (double)k * rows * part_stride(a.n) > (double)part_floats)) {
+            break;
+        }
+        const double us = lines / (double)k * std::max(0.27, 0.21 * rounds(t64 * k));
+        offer(64u, k, 3.0 + std::max(memory, us) + (k > 1u ? 3.0 + k * rows * n * 8.0 / 4e6 : 0.0));
     }
-    return hipGetLastError();
+    offer(128u, 1u, 6.0 + std::max(memory, lines * 0.51 * rounds(t128)));
+    offer(256u, 1u, 2.0 + std::max(memory, rounds(t256) * (15.0 + lines * 1.45)));
+    return best;
 }
 
 hipError_t launch_project(hipStream_t stream, const lily_projection& p, const ProjectWorkspace& ws) {
@@ -106,18 +229,12 @@ hipError_t launch_project(hipStream_t stream, const lily_projection& p, const Pr
     a.residual_bf16 = p.residual_dtype == LILY_BF16;
     a.out_bf16 = p.out_dtype == LILY_BF16;
     a.act = p.activation;
-    const uint64_t out_size = a.out_bf16 ? 8u : 16u, res_size = a.residual_bf16 ? 8u : 16u;   // of four elements
-    a.wide = reinterpret_cast<uintptr_t>(p.out_dev) % out_size == 0u && (p.rows == 1u || p.out_stride % 4u == 0u) &&
-             (p.residual_dev == nullptr || (reinterpret_cast<uintptr_t>(p.residual_dev) % res_size == 0u &&
-                                            (p.rows == 1u || p.residual_stride % 4u == 0u)));
     a.splits = 1;
-    a.part = Handed<uint64_t>{ws.part};
-    a.ticket = ws.ticket;
+    a.part = ws.part;
     const bool e4m3 = p.dtype == LILY_E4M3;
-    if (p.rows <= 16u) {
-        return launch_project_few(stream, a, e4m3);
-    }
-    return launch_project_tiles(stream, a, e4m3, ws.part_words, ws.tickets, ws.handover);
+    const ProjectPlan plan = project_plan(a, ws.part_floats);
+    a.splits = plan.splits;
+    return plan.tile == 0u ? launch_project_few(stream, a, e4m3) : launch_project_tiles(stream, a, e4m3, plan.tile);
 }
 
 }  // namespace lily

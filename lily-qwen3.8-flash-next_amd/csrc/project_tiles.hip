@@ -76,30 +76,31 @@ __device__ __forceinline__ typename Block<S>::Sums step(const Block<S>& w, const
     }
 }
 
-template <int S_, int WM_, int WN_, int MT_, int NT_, int RESIDENT_>
+template <int S_, int WM_, int WN_, int MT_, int NT_, int RESIDENT_, int DEPTH_>
 struct Tile {
-    static constexpr int S = S_, WM = WM_, WN = WN_, MT = MT_, NT = NT_, RESIDENT = RESIDENT_;
+    // DEPTH: stages in LDS (an even number), RESIDENT: workgroups a compute unit is to hold
+    static constexpr int S = S_, WM = WM_, WN = WN_, MT = MT_, NT = NT_, RESIDENT = RESIDENT_, DEPTH = DEPTH_;
     static constexpr int MH = MT / 2, NH = NT / 2;                     // blocks of a half
     static constexpr int BM = WM * MT * S, BN = WN * NT * S;
     static constexpr int XR = WM * MH * S, WR = WN * NH * S;           // rows of a unit: of x, of the weights
     static constexpr int UNIT = (XR + WR) * (int)LINE;
     static constexpr int XL = XR / 32, WL = WR / 32, LOADS = XL + WL;  // loads of a wave and unit
-    static constexpr int LDS_BYTES = 4 * UNIT;
+    static constexpr int LDS_BYTES = 2 * DEPTH * UNIT;
+    static_assert(DEPTH % 2 == 0 && (2 * DEPTH - 1) * LOADS < 64, "loads in flight are counted in six bits");
     static_assert(WM * WN == 4 && XR % 32 == 0 && WR % 32 == 0, "whole loads a wave");
 };
 
 template <int V>
-struct Parity {
+struct Constant {
     static constexpr int value = V;
 };
 
 template <Products P, class T>
 __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const ProjectArgs a, uint32_t m_tiles, uint32_t n_tiles) {
-    constexpr int MH = T::MH, NH = T::NH, S = T::S;
+    constexpr int MH = T::MH, NH = T::NH, S = T::S, DEPTH = T::DEPTH;
     typedef Block<S> Operand;
     typedef typename Operand::Sums Sums;
     extern __shared__ __align__(16) char lds[];
-    __shared__ uint32_t last;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const uint32_t wm = wave / T::WN, wn = wave % T::WN, r_in = lane % (uint32_t)S;
     // Consecutive workgroups go to consecutive XCDs: each XCD gets a run of tiles of its own (they share
@@ -227,48 +228,67 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
         }
     };
     auto nothing = [](int) {};
-    // Waits until this wave's reads are done and all but the `later` youngest of its loads have landed, then
-    // for the other waves.
-    auto meet = [&](bool two_units_behind) {
+    // Waits until this wave's reads are done and all but the youngest of its loads have landed (those of the
+    // DEPTH - 1 stages behind; `full` false: all of them), then for the other waves.
+    auto meet = [&](bool full) {
         __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
-        if (two_units_behind) {
-            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * T::LOADS) : "memory");
+        if (full) {
+            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * (DEPTH - 1) * T::LOADS) : "memory");
         } else {
             asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
         }
         __builtin_amdgcn_sched_barrier(0);
     };
-    // Units: Y of an even stage 0, X 1; of an odd stage 2 and 3.  `inner`: two more whole stages follow.
+    // Stage s, at place `at` of the DEPTH stages: unit Y at 2 at, X behind it.  `inner`: DEPTH more whole stages follow.
     // (The reads of a stage past the last find what lies there; nothing is made of them.)
-    auto stage = [&](uint32_t s, auto parity, auto inner) {
-        constexpr int p = decltype(parity)::value, Y = 2 * p, X = Y + 1, Y_NEXT = 2 - 2 * p;
+    auto stage = [&](uint32_t s, auto place, auto inner) {
+        constexpr int at = decltype(place)::value, p = at & 1, Y = 2 * at, X = Y + 1, Y_NEXT = 2 * ((at + 1) % DEPTH);
         constexpr bool INNER = decltype(inner)::value != 0;
         constexpr int LOADS = INNER ? T::LOADS : 0;
-        meet(INNER || s + 1u < steps);              // X of this stage has landed; Y's place is free
+        constexpr uint32_t D = DEPTH;
+        meet(INNER || s + D <= steps);              // X of this stage has landed; Y's place is free
         if constexpr (!INNER) {
-            if (s + 2u < steps) {
-                ask(s + 2u, 0, p, Y);
+            if (s + D < steps) {
+                ask(s + D, 0, p, Y);
             }
         }
-        quarter(0, p, WREADS, [&](int k) { read_w(1 - p, X, k); }, LOADS, [&](int k) { load(s + 2u, 0, p, Y, k); });
+        quarter(0, p, WREADS, [&](int k) { read_w(1 - p, X, k); }, LOADS, [&](int k) { load(s + D, 0, p, Y, k); });
         quarter(0, 1 - p, XREADS, [&](int k) { read_x(1, X, k); }, 0, nothing);
-        meet(INNER || s + 2u < steps);              // Y of the next stage has landed; X's place is free
+        meet(INNER || s + D < steps);               // Y of the next stage has landed; X's place is free
         if constexpr (!INNER) {
-            if (s + 2u < steps) {
-                ask(s + 2u, 1, 1 - p, X);
+            if (s + D < steps) {
+                ask(s + D, 1, 1 - p, X);
             }
         }
-        quarter(1, 1 - p, XREADS, [&](int k) { read_x(0, Y_NEXT, k); }, LOADS, [&](int k) { load(s + 2u, 1, 1 - p, X, k); });
+        quarter(1, 1 - p, XREADS, [&](int k) { read_x(0, Y_NEXT, k); }, LOADS, [&](int k) { load(s + D, 1, 1 - p, X, k); });
         quarter(1, p, WREADS, [&](int k) { read_w(1 - p, Y_NEXT, k); }, 0, nothing);
     };
-    typedef Parity<1> Inner;
-    typedef Parity<0> Outer;
-    ask(0, 0, 0, 0);
-    ask(0, 1, 1, 1);
-    if (steps > 1u) {
-        ask(1, 0, 1, 2);
-        ask(1, 1, 0, 3);
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * T::LOADS) : "memory");
+    // (everything that has to be a constant of a stage is one: DEPTH stages one after the other)
+    auto stages = [&](uint32_t s, auto inner) {
+        auto one = [&](auto place) {
+            if constexpr (decltype(place)::value < DEPTH) {
+                if (decltype(inner)::value != 0 || s + (uint32_t)decltype(place)::value < steps) {
+                    stage(s + (uint32_t)decltype(place)::value, place, inner);
+                }
+            }
+        };
+        one(Constant<0>{});
+        one(Constant<1>{});
+        one(Constant<2>{});
+        one(Constant<3>{});
+        one(Constant<4>{});
+        one(Constant<5>{});
+    };
+    static_assert(DEPTH <= 6, "stages() lists six");
+#pragma unroll
+    for (int j = 0; j < DEPTH; ++j) {
+        if ((uint32_t)j < steps) {
+            ask((uint32_t)j, 0, j & 1, 2 * j);
+            ask((uint32_t)j, 1, 1 - (j & 1), 2 * j + 1);
+        }
+    }
+    if (steps >= (uint32_t)DEPTH) {
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((2 * DEPTH - 1) * T::LOADS) : "memory");
     } else {
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     }
@@ -281,115 +301,137 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
         read_w(0, 0, k);
     }
     uint32_t s = 0;
-    for (; s + 4u < steps; s += 2u) {   // (stage s + 3 is whole: the one that d may end in is a later one)
-        stage(s, Parity<0>{}, Inner{});
-        stage(s + 1u, Parity<1>{}, Inner{});
+    for (; s + 2u * DEPTH < steps; s += DEPTH) {   // (what these ask for is whole: the stage that d may end in is a later one)
+        stages(s, Constant<1>{});
     }
-    for (; s < steps; s += 2u) {
-        stage(s, Parity<0>{}, Outer{});
-        if (s + 1u < steps) {
-            stage(s + 1u, Parity<1>{}, Outer{});
-        }
+    for (; s < steps; s += DEPTH) {
+        stages(s, Constant<0>{});
     }
     __syncthreads();   // (the stages' place is the epilogue's)
 
-    if (a.splits > 1u) {
-        // The parts' sums meet in the workspace, a lane's where its lane of every other part finds them; the
-        // last part to arrive adds them in order.
-        const uint64_t block = (uint64_t)T::BM * T::BN / 2u;   // 64-bit words
-        const uint64_t mine = ((uint64_t)tile * a.splits + split) * block + (uint64_t)tid;
-        auto each = [&](auto&& f) {   // four sums of the lane and their place
-            uint32_t q = 0;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int i = 0; i < MH; ++i) {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                        for (int j = 0; j < NH; ++j) {
-#pragma unroll
-                            for (int v = 0; v < Operand::GROUPS * 4; v += 2) {
-                                f(acc[h][i][e][j], v, (uint64_t)q * 256u);
-                                ++q;
-                            }
-                        }
-                    }
-                }
-            }
-        };
-        each([&](Sums& c, int v, uint64_t at) {
-            handed_store(a.part, mine + at, (uint64_t)lilym_f32_bits(c[v]) | (uint64_t)lilym_f32_bits(c[v + 1]) << 32);
-        });
-        if (!last_to_arrive(a.ticket + tile, a.splits, last, a.relaxed != 0u)) {
-            return;
-        }
-        clear();
-        for (uint32_t part = 0; part < a.splits; ++part) {
-            const uint64_t from = ((uint64_t)tile * a.splits + part) * block + (uint64_t)tid;
-            each([&](Sums& c, int v, uint64_t at) {
-                const uint64_t u = handed_load(a.part, from + at);
-                c[v] += lilym_bits_f32((uint32_t)u);
-                c[v + 1] += lilym_bits_f32((uint32_t)(u >> 32));
-            });
-        }
-    }
     // A quarter at a time through the wave's own part of LDS, so that a lane ends with four neighbouring
-    // outputs and NH * S / 4 lanes with a row's: whole lines are stored.
+    // outputs and NH * S / 4 lanes with a row's: whole lines are stored.  What the next quarter's epilogue reads is on its
+    // way meanwhile (nothing else hides it where the tile fills a compute unit: 8192 x 12288 x 4096 in E4M3 with a
+    // residual 572 us without).
     constexpr int ROW = NH * S + 4;   // floats of a row there (a step of four banks from row to row)
     static_assert(4 * MH * S * ROW * 4 <= T::LDS_BYTES, "a quarter of every wave");
-    constexpr int LANES = NH * S / 4, AT_ONCE = 64 / LANES;
+    constexpr int LANES = NH * S / 4, AT_ONCE = 64 / LANES;                     // lanes of a row, rows at once
+    constexpr int TURNS = MH * S / AT_ONCE, BATCH = TURNS < 8 ? TURNS : 8, BATCHES = TURNS / BATCH;
     float* mine = reinterpret_cast<float*>(lds) + wave * (uint32_t)(MH * S * ROW);
+    const uint32_t column = (lane % LANES) * 4u;
+    auto output_of = [&](int qd) { return n0 + wn * (uint32_t)(T::NT * S) + (uint32_t)((qd & 1) * NH * S) + column; };
+    auto row_of = [&](int qd) { return m0 + wm * (uint32_t)(T::MT * S) + (uint32_t)((qd >> 1) * MH * S) + lane / LANES; };
+    const bool batches = a.splits == 1u && a.act != LILY_ACT_GELU;
+    Columns columns[2];
+    Finish<BATCH> finish[2][BATCHES];
+    auto ahead = [&](auto which) {
+        constexpr int qd = decltype(which)::value;
+        if (batches && output_of(qd) < a.n) {
+            columns[qd & 1].load(a, output_of(qd));
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+            for (int b = 0; b < BATCHES; ++b) {
+                finish[qd & 1][b].load(a, row_of(qd) + (uint32_t)(b * BATCH * AT_ONCE), AT_ONCE, output_of(qd));
+            }
+        }
+    };
+    auto give = [&](auto which) {
+        constexpr int qd = decltype(which)::value, h = qd >> 1, e = qd & 1;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int i = 0; i < MH; ++i) {
 #pragma unroll
-            for (int i = 0; i < MH; ++i) {
+            for (int j = 0; j < NH; ++j) {
 #pragma unroll
-                for (int j = 0; j < NH; ++j) {
-#pragma unroll
-                    for (int q = 0; q < Operand::GROUPS; ++q) {
-                        const Sums& c = acc[h][i][e][j];
-                        *reinterpret_cast<f32x4*>(mine + ((uint32_t)(i * S) + r_in) * ROW + j * S + Operand::output(lane, q)) =
-                            f32x4{c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]};
-                    }
+                for (int q = 0; q < Operand::GROUPS; ++q) {
+                    const Sums& c = acc[h][i][e][j];
+                    *reinterpret_cast<f32x4*>(mine + ((uint32_t)(i * S) + r_in) * ROW + j * S + Operand::output(lane, q)) =
+                        f32x4{c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]};
                 }
             }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            const uint32_t column = (lane % LANES) * 4u;
-            const uint32_t v = n0 + wn * (uint32_t)(T::NT * S) + (uint32_t)(e * NH * S) + column;
-            const Columns c = columns_at(a, v);
-            const uint32_t r0 = m0 + wm * (uint32_t)(T::MT * S) + (uint32_t)(h * MH * S);
-#pragma unroll 2
-            for (uint32_t q = lane / LANES; q < (uint32_t)(MH * S); q += AT_ONCE) {
-                const f32x4 sum = *reinterpret_cast<const f32x4*>(mine + q * ROW + column);
-                if (r0 + q < a.rows) {
-                    finish(a, r0 + q, v, c, a.x_scales != nullptr ? gload(a.x_scales + r0 + q) : 1.0f, sum);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if constexpr (qd < 3) {
+            ahead(Constant<qd + 1>{});
+        }
+        const uint32_t v = output_of(qd), r0 = row_of(qd);
+        const float* from = mine + (lane / LANES) * ROW + column;
+        if (v >= a.n) {
+        } else if (batches) {
+#pragma unroll
+            for (int b = 0; b < BATCHES; ++b) {
+                f32x4 sums[BATCH];
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    sums[k] = *reinterpret_cast<const f32x4*>(from + (b * BATCH + k) * AT_ONCE * ROW);
+                }
+                finish[qd & 1][b].store(a, r0 + (uint32_t)(b * BATCH * AT_ONCE), AT_ONCE, v, columns[qd & 1], sums);
+            }
+        } else if (a.splits > 1u) {   // a part's sums as they are; k_project_join does the rest
+            for (uint32_t q = 0; q < TURNS; ++q) {
+                const uint32_t r = r0 + q * AT_ONCE;
+                if (r < a.rows) {
+                    *(LILY_GLOBAL f32x4*)(a.part + ((uint64_t)split * a.rows + r) * part_stride(a.n) + v) =
+                        *reinterpret_cast<const f32x4*>(from + q * AT_ONCE * ROW);
                 }
             }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+        } else {   // (GELU: a row at a time)
+            Columns c;
+            c.load(a, v);
+            for (uint32_t q = 0; q < TURNS; ++q) {
+                const uint32_t r = r0 + q * AT_ONCE;
+                if (r < a.rows) {
+                    const f32x4 sum[1] = {*reinterpret_cast<const f32x4*>(from + q * AT_ONCE * ROW)};
+                    Finish<1> f;
+                    f.load(a, r, 1u, v);
+                    f.store(a, r, 1u, v, c, sum);
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    ahead(Constant<0>{});
+    give(Constant<0>{});
+    give(Constant<1>{});
+    give(Constant<2>{});
+    give(Constant<3>{});
+}
+
+// The parts of d joined: a thread adds four neighbouring outputs of a row over the parts, in order, and finishes them.
+__global__ void __launch_bounds__(256) k_project_join(const ProjectArgs a) {
+    const uint32_t fours = part_stride(a.n) / 4u;
+    const uint64_t at = (uint64_t)blockIdx.x * 256u + threadIdx.x;
+    if (at >= (uint64_t)fours * a.rows) {
+        return;
+    }
+    const uint32_t r = (uint32_t)(at / fours), v = (uint32_t)(at % fours) * 4u;
+    Columns c;
+    Finish<1> f;
+    c.load(a, v);
+    f.load(a, r, 1u, v);
+    const float* from = a.part + (uint64_t)r * part_stride(a.n) + v;
+    const uint64_t next = (uint64_t)a.rows * part_stride(a.n);
+    f32x4 sum[1] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+    for (uint32_t q = 0; q < a.splits; q += 4u) {
+        f32x4 p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            p[j] = gload(reinterpret_cast<const f32x4*>(from + min(q + (uint32_t)j, a.splits - 1u) * next));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (q + (uint32_t)j < a.splits) {
+                sum[0] += p[j];
+            }
         }
     }
+    f.store(a, r, 1u, v, c, sum);
 }
 
 template <class T>
-hipError_t launch_tile(hipStream_t stream, ProjectArgs& a, bool e4m3, uint64_t part_words, uint32_t tickets, uint32_t handover) {
+hipError_t launch_tile(hipStream_t stream, const ProjectArgs& a, bool e4m3) {
     const uint32_t m_tiles = (a.rows + T::BM - 1u) / T::BM, n_tiles = (a.n + T::BN - 1u) / T::BN;
-    const uint64_t tiles = (uint64_t)m_tiles * n_tiles;
-    const uint32_t stages = (a.d_bytes + LINE - 1u) / LINE;
-    // Parts of d: enough to fill the chip once, none shorter than eight stages, what the workspace holds.
-    uint32_t splits = 1;
-    const uint32_t places = 256u * T::RESIDENT;
-    while (splits < 16u && tiles * splits * 2u <= places && stages / (splits * 2u) >= 8u && tiles <= tickets &&
-           tiles * (splits * 2u) * (T::BM * T::BN / 2u) <= part_words) {
-        splits *= 2u;
-    }
-    a.splits = splits;
-    a.relaxed = handover == 2u || (handover == 0u && tiles * splits > 256u) ? 1u : 0u;
-    const dim3 grid((uint32_t)(tiles * splits)), block(256);
+    const dim3 grid(m_tiles * n_tiles * a.splits), block(256);
     auto go = [&](const void* kernel, LdsAllowed& allowed, auto launch) -> hipError_t {
         const hipError_t e = allowed.say(kernel, T::LDS_BYTES);
         if (e == hipSuccess) {
@@ -415,21 +457,19 @@ hipError_t launch_tile(hipStream_t stream, ProjectArgs& a, bool e4m3, uint64_t p
     if (e != hipSuccess) {
         return e;
     }
+    if (a.splits > 1u) {
+        const uint64_t threads = (uint64_t)a.rows * (part_stride(a.n) / 4u);
+        hipLaunchKernelGGL(k_project_join, dim3((uint32_t)((threads + 255u) / 256u)), dim3(256), 0, stream, a);
+    }
     return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_project_tiles(hipStream_t stream, ProjectArgs& a, bool e4m3, uint64_t part_words, uint32_t tickets,
-                                uint32_t handover) {
-    const uint64_t big = (uint64_t)((a.rows + 255u) / 256u) * ((a.n + 255u) / 256u);
-    if (a.rows > 128u && big >= 128u) {
-        return launch_tile<Tile<32, 2, 2, 4, 4, 1>>(stream, a, e4m3, part_words, tickets, handover);
-    }
-    if (a.rows > 64u) {
-        return launch_tile<Tile<16, 2, 2, 4, 4, 2>>(stream, a, e4m3, part_words, tickets, handover);
-    }
-    return launch_tile<Tile<16, 1, 4, 4, 2, 2>>(stream, a, e4m3, part_words, tickets, handover);
+hipError_t launch_project_tiles(hipStream_t stream, const ProjectArgs& a, bool e4m3, uint32_t tile) {
+    return tile == 256u   ? launch_tile<Tile<32, 2, 2, 4, 4, 1, 2>>(stream, a, e4m3)
+           : tile == 128u ? launch_tile<Tile<16, 2, 2, 4, 4, 2, 2>>(stream, a, e4m3)
+                          : launch_tile<Tile<16, 2, 2, 2, 2, 2, 4>>(stream, a, e4m3);
 }
 
 }  // namespace lily

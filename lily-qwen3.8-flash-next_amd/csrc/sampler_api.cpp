@@ -1039,11 +1039,8 @@ int sampler_device(const lily_sampler_t* s) { return s->device; }
 hipStream_t sampler_stream(const lily_sampler_t* s) { return s->stream; }
 // (the candidates' slots: no two launches of a stream use them at once)
 void sampler_project_workspace(const lily_sampler_t* s, ProjectWorkspace* ws) {
-    ws->part = s->ws_cand;
-    ws->part_words = s->ws_slots;
-    ws->ticket = s->ws_ticket;
-    ws->tickets = s->ws_rows;
-    ws->handover = s->handover;
+    ws->part = reinterpret_cast<float*>(s->ws_cand);
+    ws->part_floats = (uint64_t)s->ws_slots * 2u;
 }
 
 int sample_row_with_workspace(int device, hipStream_t stream, const Workspace& ws, const float* logits,
