@@ -514,8 +514,7 @@ int lily_lm_head_sample_rows(lily_sampler_t* s, const lily_lm_head* head, const 
  * whose largest |y| lies below 2^-116 has scale 0 and zeros; a row with a value that is not finite
  * has what the formula gives, and in 8 bits a NaN scale.
  *
- * Rows hold d (1 .. LILY_NORM_MAX_D) elements, strides count elements and may be anything from d on;
- * rows that start at multiples of 16 bytes in every array, with d a multiple of 8, go the fast way.
+ * Rows hold d (1 .. LILY_NORM_MAX_D) elements, strides count elements and may be anything from d on.
  * sum_dev may be x_dev or residual_dev, and out_dev may be either, each with the same type and stride;
  * other overlaps are refused, as far as they can be told from pointers, strides and sizes (arrays of one
  * stride that lie side by side in wider rows do not overlap).  Enqueued on the sampler's stream; no

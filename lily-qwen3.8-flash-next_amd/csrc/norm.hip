@@ -39,19 +39,24 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 
-// Eight elements as they lie in memory: two pieces of 16 bytes of f32, one of bf16.
+// Eight elements as they lie in memory: two pieces of 16 bytes of f32, one of bf16.  (Rows may start at any
+// element: the hardware takes wide accesses there.)
 struct Raw {
     u32x4 a, b;
 };
+typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
+typedef u32x4 u32x4_at4 __attribute__((aligned(4)));
+typedef f32x4 f32x4_at4 __attribute__((aligned(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 u32x2_at1 __attribute__((aligned(1)));
 __device__ __forceinline__ Raw load8(const void* row, uint32_t i, bool bf16) {
     Raw r;
     if (bf16) {
-        r.a = gload(reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(row) + i));
+        r.a = *(const LILY_GLOBAL u32x4_at2*)(static_cast<const uint16_t*>(row) + i);
         r.b = r.a;
     } else {
-        const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const float*>(row) + i);
-        r.a = gload(p);
-        r.b = gload(p + 1);
+        r.a = *(const LILY_GLOBAL u32x4_at4*)(static_cast<const uint32_t*>(row) + i);
+        r.b = *(const LILY_GLOBAL u32x4_at4*)(static_cast<const uint32_t*>(row) + i + 4);
     }
     return r;
 }
@@ -84,11 +89,11 @@ __device__ __forceinline__ void store1(void* row, uint32_t i, float v, uint32_t 
 }
 __device__ __forceinline__ void store8(void* row, uint32_t i, const float (&v)[8], uint32_t dtype) {
     if (dtype == LILY_F32) {
-        f32x4* p = reinterpret_cast<f32x4*>(static_cast<float*>(row) + i);
+        LILY_GLOBAL f32x4_at4* p = (LILY_GLOBAL f32x4_at4*)(static_cast<float*>(row) + i);
         p[0] = f32x4{v[0], v[1], v[2], v[3]};
         p[1] = f32x4{v[4], v[5], v[6], v[7]};
     } else if (dtype == LILY_BF16) {
-        *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(row) + i) =
+        *(LILY_GLOBAL u32x4_at2*)(static_cast<uint16_t*>(row) + i) =
             u32x4{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])};
     } else {
         // (nearest even by the conversion; |v| <= 448 (1 + 2^-22), which rounds to 448)
@@ -96,7 +101,7 @@ __device__ __forceinline__ void store8(void* row, uint32_t i, const float (&v)[8
         lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
         int hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
         hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], hi, true);
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(row) + i) = make_uint2((uint32_t)lo, (uint32_t)hi);
+        *(LILY_GLOBAL u32x2_at1*)(static_cast<uint8_t*>(row) + i) = u32x2{(uint32_t)lo, (uint32_t)hi};
     }
 }
 
@@ -118,10 +123,9 @@ __device__ __forceinline__ float wave_sum_f(float v) {
     return t;
 }
 
-// CH: pieces of eight elements a thread holds (CH * 8 * blockDim.x >= d).  PIECES: every row starts at a
-// multiple of 16 bytes and d is a multiple of 8; otherwise a thread's elements lie blockDim.x apart and
-// go one by one.
-template <int CH, bool PIECES>
+// CH: pieces of eight elements a thread holds (CH * 8 * blockDim.x >= d).  RAGGED: d is no multiple of 8, and the
+// last piece goes element by element.
+template <int CH, bool RAGGED>
 __global__ void __launch_bounds__(1024) k_rms_norm(const NormArgs a) {
     __shared__ float part[16];
     __shared__ uint32_t top_of[16];
@@ -133,81 +137,83 @@ __global__ void __launch_bounds__(1024) k_rms_norm(const NormArgs a) {
     char* out = static_cast<char*>(a.out) + row * a.out_stride * (a.out_dtype == LILY_F32 ? 4u : a.out_dtype == LILY_BF16 ? 2u : 1u);
     const bool with_residual = a.residual != nullptr;
     float h[CH][8], w[CH][8];
+    auto at = [&](int c) { return ((uint32_t)c * nt + tid) * 8u; };
+    auto whole = [&](int c) { return RAGGED ? at(c) + 8u <= a.d : at(c) < a.d; };
 
-    if constexpr (PIECES) {
-        // Everything the row needs is asked for before any of it is looked at (the weights too: they
-        // are the same for all rows and come from the L2).  A piece beyond the row is the row's last
-        // one again, worth zeros.
-        Raw rx[CH], rr[CH], rw[CH];
-        const uint32_t last = a.d - 8u;
+    // Everything the row needs is asked for before any of it is looked at (the weights too: they are the same for all
+    // rows and come from the L2).  What is not there is worth zeros.
+    Raw rx[CH], rr[CH], rw[CH];
+    auto from = [&](int c) { return RAGGED ? at(c) : min(at(c), a.d - 8u); };   // (no branch around a load where none is needed)
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        if (!RAGGED || whole(c)) {
+            rx[c] = load8(x, from(c), a.x_bf16);
+        }
+    }
+    if (with_residual) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            rx[c] = load8(x, min(((uint32_t)c * nt + tid) * 8u, last), a.x_bf16);
-        }
-        if (with_residual) {
-#pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                rr[c] = load8(res, min(((uint32_t)c * nt + tid) * 8u, last), a.stream_bf16);
+            if (!RAGGED || whole(c)) {
+                rr[c] = load8(res, from(c), a.stream_bf16);
             }
         }
-        if (a.weight != nullptr) {
-#pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                rw[c] = load8(a.weight, min(((uint32_t)c * nt + tid) * 8u, last), a.weight_bf16);
-            }
-        }
+    }
+    if (a.weight != nullptr) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const uint32_t i = ((uint32_t)c * nt + tid) * 8u;
+            if (!RAGGED || whole(c)) {
+                rw[c] = load8(a.weight, from(c), a.weight_bf16);
+            }
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const uint32_t i = at(c);
+        float r[8];
+        if (!RAGGED || whole(c)) {
             widen(rx[c], a.x_bf16, h[c]);
             if (with_residual) {
-                float r[8];
                 widen(rr[c], a.stream_bf16, r);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    h[c][j] = rounded(h[c][j] + r[j], a.stream_bf16);
-                }
-                if (a.sum != nullptr && i < a.d) {
-                    store8(sum, i, h[c], a.stream_bf16 ? LILY_BF16 : LILY_F32);
-                }
             }
             if (a.weight != nullptr) {
                 widen(rw[c], a.weight_bf16, w[c]);
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                h[c][j] = i < a.d ? h[c][j] : 0.0f;
-                w[c][j] = i < a.d ? (a.weight != nullptr ? w[c][j] + a.offset : 1.0f) : 0.0f;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t i = (uint32_t)(c * 8 + j) * nt + tid, at = min(i, a.d - 1u);
-                float v = load1(x, at, a.x_bf16);
-                if (with_residual) {
-                    v = rounded(v + load1(res, at, a.stream_bf16), a.stream_bf16);
-                }
-                h[c][j] = i < a.d ? v : 0.0f;
-                w[c][j] = i < a.d ? (a.weight != nullptr ? load1(a.weight, at, a.weight_bf16) + a.offset : 1.0f) : 0.0f;
-            }
-        }
-        // (the row has been read whole before any of it is written: the sum may lie where x lies, one
-        // thread's elements being its own, and an element beyond the row reads the last one's)
-        __syncthreads();
-        if (with_residual && a.sum != nullptr) {
-#pragma unroll
-            for (int c = 0; c < CH; ++c) {
+            if (!RAGGED && i >= a.d) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const uint32_t i = (uint32_t)(c * 8 + j) * nt + tid;
-                    if (i < a.d) {
-                        store1(sum, i, h[c][j], a.stream_bf16 ? LILY_BF16 : LILY_F32);
+                    h[c][j] = r[j] = w[c][j] = 0.0f;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool there = i + (uint32_t)j < a.d;
+                h[c][j] = there ? load1(x, i + (uint32_t)j, a.x_bf16) : 0.0f;
+                r[j] = there && with_residual ? load1(res, i + (uint32_t)j, a.stream_bf16) : 0.0f;
+                w[c][j] = there && a.weight != nullptr ? load1(a.weight, i + (uint32_t)j, a.weight_bf16) : 0.0f;
+            }
+        }
+        if (with_residual) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                h[c][j] = rounded(h[c][j] + r[j], a.stream_bf16);
+            }
+            if (a.sum != nullptr) {   // (it may lie where x or the residual lies: the thread has read its own elements)
+                if (whole(c)) {
+                    store8(sum, i, h[c], a.stream_bf16 ? LILY_BF16 : LILY_F32);
+                } else if (RAGGED) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        if (i + (uint32_t)j < a.d) {
+                            store1(sum, i + (uint32_t)j, h[c][j], a.stream_bf16 ? LILY_BF16 : LILY_F32);
+                        }
                     }
                 }
             }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            w[c][j] = a.weight != nullptr ? w[c][j] + a.offset : 1.0f;
         }
     }
 
@@ -264,17 +270,14 @@ __global__ void __launch_bounds__(1024) k_rms_norm(const NormArgs a) {
     }
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        if constexpr (PIECES) {
-            const uint32_t i = ((uint32_t)c * nt + tid) * 8u;
-            if (i < a.d) {
-                store8(out, i, h[c], a.out_dtype);
-            }
-        } else {
+        const uint32_t i = at(c);
+        if (whole(c)) {
+            store8(out, i, h[c], a.out_dtype);
+        } else if (RAGGED) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const uint32_t i = (uint32_t)(c * 8 + j) * nt + tid;
-                if (i < a.d) {
-                    store1(out, i, h[c][j], a.out_dtype);
+                if (i + (uint32_t)j < a.d) {
+                    store1(out, i + (uint32_t)j, h[c][j], a.out_dtype);
                 }
             }
         }
@@ -283,7 +286,7 @@ __global__ void __launch_bounds__(1024) k_rms_norm(const NormArgs a) {
 
 }  // namespace
 
-hipError_t launch_rms_norm(hipStream_t stream, const lily_norm& n, bool pieces) {
+hipError_t launch_rms_norm(hipStream_t stream, const lily_norm& n) {
     NormArgs a = {};
     a.x = n.x_dev;
     a.residual = n.residual_dev;
@@ -307,7 +310,7 @@ hipError_t launch_rms_norm(hipStream_t stream, const lily_norm& n, bool pieces) 
     const uint32_t threads = ((held + ch - 1u) / ch + 63u) / 64u * 64u;
     const dim3 grid(n.rows), block(threads);
 #define LILY_NORM(CH)                                                              \
-    if (pieces) {                                                                  \
+    if (n.d % 8u != 0u) {                                                          \
         hipLaunchKernelGGL((k_rms_norm<CH, true>), grid, block, 0, stream, a);     \
     } else {                                                                       \
         hipLaunchKernelGGL((k_rms_norm<CH, false>), grid, block, 0, stream, a);    \

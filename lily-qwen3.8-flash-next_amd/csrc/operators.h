@@ -7,9 +7,8 @@
 
 namespace lily {
 
-// The norm (norm.hip).  `pieces`: rows start at multiples of 16 bytes in every array and d is a
-// multiple of 8.
-hipError_t launch_rms_norm(hipStream_t stream, const lily_norm& norm, bool pieces);
+// The norm (norm.hip).
+hipError_t launch_rms_norm(hipStream_t stream, const lily_norm& norm);
 
 // The matrix product with an epilogue (project_few.hip, project_tiles.hip); the workspace is the sampler's.
 struct ProjectWorkspace {

@@ -26,7 +26,7 @@ namespace {
     DeviceScope device_scope_(device);    \
     HIP_TRY(device_scope_.err)
 
-int check_norm(const lily_norm* n, bool* pieces) {
+int check_norm(const lily_norm* n) {
     if (n == nullptr || n->x_dev == nullptr || n->out_dev == nullptr) {
         return api_fail(LILY_ERR_INVALID_ARG, "norm, x and out are required");
     }
@@ -91,9 +91,6 @@ int check_norm(const lily_norm* n, bool* pieces) {
     if (overlap(sum, out)) {
         return api_fail(LILY_ERR_INVALID_ARG, "sum and out overlap");
     }
-    *pieces = n->d % 8u == 0u && aligned(x) && aligned(res) && aligned(sum) && w.at % 16u == 0u &&
-              out.at % (n->out_dtype == LILY_E4M3 ? 8u : 16u) == 0u &&
-              out.stride % (n->out_dtype == LILY_E4M3 ? 8u : 16u) == 0u;
     return LILY_OK;
 }
 
@@ -165,15 +162,14 @@ int need_sampler(const lily_sampler_t* s) {
 extern "C" {
 
 int lily_rms_norm(lily_sampler_t* s, const lily_norm* norm) {
-    bool pieces = false;
-    if (int rc = check_norm(norm, &pieces)) {
+    if (int rc = check_norm(norm)) {
         return rc;
     }
     if (int rc = need_sampler(s)) {
         return rc;
     }
     ON_DEVICE(sampler_device(s));
-    HIP_TRY(launch_rms_norm(sampler_stream(s), *norm, pieces));
+    HIP_TRY(launch_rms_norm(sampler_stream(s), *norm));
     return LILY_OK;
 }
 
