@@ -197,7 +197,6 @@ struct Finish {
     __device__ __forceinline__ void store(const ProjectArgs& a, uint32_t r0, uint32_t step, uint32_t v0, const Columns& c,
                                           const f32x4 (&sums)[N]) const {
         float v[4 * N];
-        const bool whole = v0 + 4u <= a.n;
 #pragma unroll
         for (int q = 0; q < N; ++q) {
 #pragma unroll

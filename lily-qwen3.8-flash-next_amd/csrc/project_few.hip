@@ -161,13 +161,14 @@ hipError_t launch_project_few(hipStream_t stream, const ProjectArgs& a, bool e4m
 // Which kernel, and how many parts of d: by an estimate of each one's time in us, from what they take on the chip
 // (rows x n x d in bf16, the estimate in brackets):
 //   few rows     a compute unit takes in 85 GB/s through LDS: 64 x 4096 x 4096 10.1 (10.5), 64 x 16384 x 2048 19.4 (18.2)
-//   64 x 64      a line of d 0.27 a round of one tile a compute unit, 0.21 where it has several: 256 x 4096 x 4096 18.4
-//                (20.3), 512 x 4096 x 4096 29.8 (29.9), 64 x 16384 x 2048 16.4 (15.2: memory)
-//   128 x 128    0.51 a tile of a compute unit: 1024 x 4096 x 4096 .. 8192 x 4096 x 4096 271 (267)
+//   64 x 64      a line of d 0.22 where a compute unit has one tile, 0.21 a round of tiles: 256 x 4096 x 4096 17.8 (18.1),
+//                512 x 4096 x 4096 28.6 (30.9), 64 x 16384 x 2048 16.4 (16.2: memory)
+//   128 x 128    a line 0.51 a round, 0.38 where tiles are few: 1024 x 4096 x 4096 36.7 (38.6), 8192 x 4096 x 4096 271 (267)
 //   256 x 256    1.45 a tile, and 15 for every tile's epilogue, which nothing hides: 8192 x 4096 x 4096 242 (218), where
 //                128 x 128 would take 271
-// Parts of d: a launch more (3, with what the parts' sums cost to write and read at 4 TB/s): 64 x 1000 x 8192 in eight 10.6
-// (11.3) against 25.5 in one; memory at 5.6 TB/s bounds all of them.
+// Parts of d: a launch more (1.5), and the parts' sums written and read at 5.5 TB/s: 64 x 1000 x 8192 in eight 10.6 (10.5)
+// against 25.5 in one; 300 x 4096 x 4096 in two of 128 x 128 22.2 (23.3), where 64 x 64 takes 28.1 in one and 25.9 in two
+// and 128 x 128 30.4 in one; 512 x 4096 x 4096 25.9 (29.9).  Memory at 5.6 TB/s bounds all of them.
 struct ProjectPlan {
     uint32_t tile = 0;     // 0: few rows
     uint32_t splits = 1;
@@ -200,10 +201,11 @@ static ProjectPlan project_plan(const ProjectArgs& a, uint64_t part_floats) {
         if (k > 1u && (lines < 4u * k || (double)k * rows * part_stride(a.n) > (double)part_floats)) {
             break;
         }
-        const double us = lines / (double)k * std::max(0.27, 0.21 * rounds(t64 * k));
-        offer(64u, k, 3.0 + std::max(memory, us) + (k > 1u ? 3.0 + k * rows * n * 8.0 / 4e6 : 0.0));
+        const double each = lines / (double)k, join = k > 1u ? 1.5 + k * rows * n * 8.0 / 5.5e6 : 0.0;
+        offer(64u, k, 4.0 + std::max(memory, each * std::max(0.22, 0.21 * rounds(t64 * k))) + join);
+        const double turns = t128 * k <= 256u ? (double)(t128 * k) / 256.0 : rounds(t128 * k);
+        offer(128u, k, 6.0 + std::max(memory, each * std::max(0.38, 0.51 * turns)) + join);
     }
-    offer(128u, 1u, 6.0 + std::max(memory, lines * 0.51 * rounds(t128)));
     offer(256u, 1u, 2.0 + std::max(memory, rounds(t256) * (15.0 + lines * 1.45)));
     return best;
 }

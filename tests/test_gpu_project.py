@@ -244,3 +244,11 @@ def test_what_the_python_mirror_refuses(sampler):
         kw.update(bad)
         with pytest.raises(LS.SamplerError):
             sampler.project(**kw)
+
+
+# d shared between workgroups by tiles of both sizes: two, four and sixteen parts, even and uneven, ragged edges
+@pytest.mark.parametrize("rows, n, d", [(300, 4096, 4096), (500, 4000, 2064), (257, 3000, 4096), (100, 10007, 4096), (600, 500, 8192),
+                                        (140, 1000, 4112), (17, 130, 8192)])
+@pytest.mark.parametrize("dtype, out", [("bf16", "bf16"), ("e4m3", "bf16"), ("e4m3", "f32")])
+def test_parts_of_the_rows(sampler, rows, n, d, dtype, out):
+    _run(sampler, rows, n, d, dtype, out, "gelu_tanh", "bf16", "bf16")
