@@ -517,8 +517,9 @@ int lily_lm_head_sample_rows(lily_sampler_t* s, const lily_lm_head* head, const 
  * Rows hold d (1 .. LILY_NORM_MAX_D) elements, strides count elements and may be anything from d on.
  * sum_dev may be x_dev or residual_dev, and out_dev may be either, each with the same type and stride;
  * other overlaps are refused, as far as they can be told from pointers, strides and sizes (arrays of one
- * stride that lie side by side in wider rows do not overlap).  Enqueued on the sampler's stream; no
- * workspace. */
+ * stride that lie side by side in wider rows do not overlap).  Up to 4 194 303 rows of any width, more of
+ * rows below 8 192 elements (LILY_ERR_RANGE beyond: a launch has 2^32 - 1 threads, a row the eighth of its
+ * elements).  Enqueued on the sampler's stream; no workspace. */
 #define LILY_NORM_MAX_D 32768u
 typedef struct lily_norm {
     uint32_t rows;
@@ -548,8 +549,8 @@ int lily_rms_norm(lily_sampler_t* s, const lily_norm* norm);
  * The block of a draft head (residual + silu(W x + b)), a projection ahead of the head, or a head held in
  * 8-bit floats (its logits then in f32 or bf16, without the summaries of lily_lm_head_bf16).  x and weight are
  * both bf16 or both E4M3 (what lily_rms_norm leaves, its scales as x_scales), contiguous along d, products
- * and sums in f32 on the matrix cores, the epilogue in f32, one rounding to out_dtype.  Any number of
- * rows and outputs, d a multiple of 8 (bf16) or 16 (E4M3) elements, rows of x and weight at multiples of 16
+ * and sums in f32 on the matrix cores, the epilogue in f32, one rounding to out_dtype.  Up to
+ * 2^24 rows, 2^26 outputs and 2^24 - 1 tiles of 64 x 64 of both (LILY_ERR_RANGE beyond), d a multiple of 8 (bf16) or 16 (E4M3) elements, rows of x and weight at multiples of 16
  * bytes, at most 2^23 bytes apart.  out_dev may be residual_dev with the same type and stride; other overlaps of
  * out with an operand are refused.  Enqueued on the sampler's stream, one launch or two.  Where few tiles span the
  * chip the parts of d meet in the sampler's workspace, added in a fixed order: graphs captured from one sampler are

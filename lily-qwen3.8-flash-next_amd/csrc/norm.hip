@@ -305,10 +305,9 @@ hipError_t launch_rms_norm(hipStream_t stream, const lily_norm& n) {
     a.out_dtype = n.out_dtype;
     a.eps = n.eps;
     a.offset = n.weight_offset;
-    const uint32_t held = (n.d + 7u) / 8u;   // pieces of a row
-    uint32_t ch = held <= 1024u ? 1u : held <= 2048u ? 2u : 4u;
-    const uint32_t threads = ((held + ch - 1u) / ch + 63u) / 64u * 64u;
-    const dim3 grid(n.rows), block(threads);
+    const NormShape shape = norm_shape(n.d);
+    const uint32_t ch = shape.pieces;
+    const dim3 grid(n.rows), block(shape.threads);
 #define LILY_NORM(CH)                                                              \
     if (n.d % 8u != 0u) {                                                          \
         hipLaunchKernelGGL((k_rms_norm<CH, true>), grid, block, 0, stream, a);     \

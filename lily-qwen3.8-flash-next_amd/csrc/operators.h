@@ -7,7 +7,14 @@
 
 namespace lily {
 
-// The norm (norm.hip).
+// The norm (norm.hip): a row is a workgroup of up to 1024 threads, with pieces of eight elements.
+struct NormShape {
+    uint32_t pieces, threads;   // pieces a thread holds
+};
+constexpr NormShape norm_shape(uint32_t d) {
+    const uint32_t held = (d + 7u) / 8u, pieces = held <= 1024u ? 1u : held <= 2048u ? 2u : 4u;
+    return {pieces, ((held + pieces - 1u) / pieces + 63u) / 64u * 64u};
+}
 hipError_t launch_rms_norm(hipStream_t stream, const lily_norm& norm);
 
 // The matrix product with an epilogue (project_few.hip, project_tiles.hip); the workspace is the sampler's.

@@ -26,6 +26,8 @@ namespace {
     DeviceScope device_scope_(device);    \
     HIP_TRY(device_scope_.err)
 
+constexpr uint32_t MAX_THREADS = 0xffffffffu;   // of a launch
+
 int check_norm(const lily_norm* n) {
     if (n == nullptr || n->x_dev == nullptr || n->out_dev == nullptr) {
         return api_fail(LILY_ERR_INVALID_ARG, "norm, x and out are required");
@@ -33,8 +35,11 @@ int check_norm(const lily_norm* n) {
     if (n->rows == 0u || n->d == 0u) {
         return api_fail(LILY_ERR_INVALID_ARG, "rows and d must be positive");
     }
-    if (n->d > LILY_NORM_MAX_D || n->rows > 0x7fffffffu) {
-        return api_fail(LILY_ERR_RANGE, "a norm takes rows of up to %u elements, 2^31 - 1 of them", LILY_NORM_MAX_D);
+    if (n->d > LILY_NORM_MAX_D) {
+        return api_fail(LILY_ERR_RANGE, "a norm takes rows of up to %u elements", LILY_NORM_MAX_D);
+    }
+    if (n->rows > MAX_THREADS / norm_shape(n->d).threads) {
+        return api_fail(LILY_ERR_RANGE, "a norm takes up to %u rows of %u elements", MAX_THREADS / norm_shape(n->d).threads, n->d);
     }
     if (n->x_dtype > LILY_BF16 || n->stream_dtype > LILY_BF16 || n->weight_dtype > LILY_BF16) {
         return api_fail(LILY_ERR_INVALID_ARG, "x, residual and weight are LILY_F32 or LILY_BF16");
@@ -114,8 +119,12 @@ int check_projection(const lily_projection* p) {
     if (p->d * e % 16u != 0u) {
         return api_fail(LILY_ERR_INVALID_ARG, "d must be a multiple of 16 bytes: of 8 in bf16, of 16 in E4M3");
     }
-    if (p->d > 0xffffff80u / e || p->rows > (1u << 24) || p->n > (1u << 30)) {
-        return api_fail(LILY_ERR_RANGE, "a product takes up to 2^24 rows, 2^30 outputs and rows of 2^32 - 128 bytes");
+    if (p->d > 0xffffff80u / e || p->rows > (1u << 24) || p->n > (1u << 26)) {
+        return api_fail(LILY_ERR_RANGE, "a product takes up to 2^24 rows, 2^26 outputs and rows of 2^32 - 128 bytes");
+    }
+    // (the smallest tile that many rows may get: 256 threads for 64 x 64)
+    if (((p->rows + 63ull) / 64u) * ((p->n + 63ull) / 64u) > MAX_THREADS / 256u) {
+        return api_fail(LILY_ERR_RANGE, "a product has up to 2^24 - 1 tiles of 64 x 64 outputs");
     }
     if ((p->rows > 1u && (p->x_stride < p->d || p->out_stride < p->n || (p->residual_dev != nullptr && p->residual_stride < p->n))) ||
         (p->n > 1u && p->weight_stride < p->d)) {

@@ -231,3 +231,30 @@ def test_what_a_product_refuses(over, code, word):
 
 def test_a_product_without_a_descriptor():
     assert _said(L.lily_project(None, None))[0] == INVALID
+
+
+# ---- more than a launch holds (2^32 - 1 threads)
+
+
+@pytest.mark.parametrize("rows, d, sound", [
+    ((1 << 26) - 1, 512, True), (1 << 26, 512, False), ((1 << 26) - 1, 1, True), (1 << 26, 1, False),
+    ((1 << 22) - 1, 8192, True), (1 << 22, 8192, False), ((1 << 22) - 1, 32768, True), (1 << 22, 32768, False),
+    ((1 << 32) - 1, 513, False),
+])
+def test_the_most_rows_of_a_norm(rows, d, sound):
+    far = 1 << 44
+    rc, text = _said(L.lily_rms_norm(None, C.byref(_norm(rows=rows, d=d, x_stride=d, residual_stride=d, sum_stride=d, out_stride=d,
+                                                         x_dev=far, residual_dev=2 * far, sum_dev=3 * far, weight_dev=0x40000,
+                                                         out_dev=4 * far))))
+    assert (rc, text) == (INVALID, "sampler is null") if sound else rc == RANGE and "up to" in text, (rc, text)
+
+
+@pytest.mark.parametrize("rows, n, sound", [
+    (1, 1 << 26, True), (1, (1 << 26) + 1, False), (1 << 24, 64, True), (1 << 24, 63 * 64, True), (1 << 24, 64 * 64, False),
+    (1 << 10, 1 << 26, False), (960, 1 << 26, True), (65, 1 << 26, True),
+])
+def test_the_most_tiles_of_a_product(rows, n, sound):
+    far = 1 << 44
+    rc, text = _project(rows=rows, n=n, x_dev=far, weight_dev=2 * far, residual_dev=3 * far, out_dev=4 * far, residual_stride=n,
+                        out_stride=n, bias_dev=5 * far)
+    assert (rc, text) == (INVALID, "sampler is null") if sound else rc == RANGE and "up to" in text, (rc, text)
