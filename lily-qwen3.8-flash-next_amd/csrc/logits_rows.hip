@@ -16,9 +16,15 @@
 // values stay in registers: each workgroup leaves its (largest value, sum) as one word, which is the whole message,
 // looks for the words of its row's other slices, a bounded number of times, and writes.  Where a word does not
 // come (the other workgroup has no place on the chip yet) it forms the other slices' words itself, by the same
-// operations, so the result is the same.  One pass over the logits: 1 024 rows of 151 936 went twice through a row
-// in 245 us before, and two launches of 64 rows took 25.  Rows too long for that (over 524 288 ids) take a launch
-// for the sums and one that writes.
+// operations, so the result is the same.  Rows too long for that (over 524 288 ids) take a launch for the sums and one
+// that writes.
+//
+// Bound by memory where rows are many: 1 024 rows of 151 936 bf16 to f32 are written, adjusted, in 166 us (933 MB, 5.6
+// TB/s, what a copy reaches) and as log-probabilities in 180; under histories of 2 048 ids in 200 and 215, where the
+// counts of the listed ids, a line each, are 180 MB more.  Operations come next (37 vector instructions an id with such a
+// history; 53, with a division of five operations and a look at the listed ids group by group, took 245 us).  64
+// rows take 21 us, 13 of them for what crosses the memory: a batch that is one round of workgroups reads, waits for its
+// neighbours' words and writes, one after the other.  4 rows take 11, where each step is a latency.
 #include <hip/hip_runtime.h>
 
 #include "device_common.h"
@@ -54,6 +60,7 @@ constexpr bool is_logprobs(int form) { return form == FORM_HELD_LOGPROBS || form
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef u32x4 u32x4_any __attribute__((aligned(4)));
 typedef u32x2 u32x2_any __attribute__((aligned(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4_out __attribute__((ext_vector_type(4), aligned(4)));
 typedef u32x2 u32x2_out __attribute__((aligned(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -68,16 +75,16 @@ struct RawGroup;
 template <>
 struct RawGroup<LILY_F32> {
     u32x4 w;
-    __device__ __forceinline__ void load(const void* row, uint32_t id) {
-        w = *(const LILY_GLOBAL u32x4_any*)(static_cast<const float*>(row) + id);
+    __device__ __forceinline__ void load(const void* from, uint32_t group) {
+        w = *(const LILY_GLOBAL u32x4_any*)(static_cast<const char*>(from) + group * 16u);
     }
     __device__ __forceinline__ float at(int j) const { return lilym_bits_f32(w[j]); }
 };
 template <>
 struct RawGroup<LILY_BF16> {
     u32x2 w;
-    __device__ __forceinline__ void load(const void* row, uint32_t id) {
-        w = *(const LILY_GLOBAL u32x2_any*)(static_cast<const uint16_t*>(row) + id);
+    __device__ __forceinline__ void load(const void* from, uint32_t group) {
+        w = *(const LILY_GLOBAL u32x2_any*)(static_cast<const char*>(from) + group * 8u);
     }
     __device__ __forceinline__ float at(int j) const {
         return lilym_bits_f32((j & 1) ? (w[j >> 1] & 0xffff0000u) : (w[j >> 1] << 16));
@@ -85,11 +92,11 @@ struct RawGroup<LILY_BF16> {
 };
 
 template <int DT>
-__device__ __forceinline__ void store_group(void* row, uint32_t id, const float (&v)[GROUP]) {
+__device__ __forceinline__ void store_group(void* to, uint32_t group, f32x4 v) {
     if (DT == LILY_F32) {
-        *(LILY_GLOBAL f32x4_out*)(static_cast<float*>(row) + id) = f32x4_out{v[0], v[1], v[2], v[3]};
+        *(LILY_GLOBAL f32x4_out*)(static_cast<char*>(to) + group * 16u) = f32x4_out{v[0], v[1], v[2], v[3]};
     } else {
-        *(LILY_GLOBAL u32x2_out*)(static_cast<uint16_t*>(row) + id) = u32x2_out{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
+        *(LILY_GLOBAL u32x2_out*)(static_cast<char*>(to) + group * 8u) = u32x2_out{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
     }
 }
 template <int DT>
@@ -108,7 +115,11 @@ struct SliceBias {
     uint32_t ids[BIAS_PAIRS];
     float deltas[BIAS_PAIRS];
 };
-// A thread's running sum of exp(v - m), m the largest value it has seen.  (The reference is a value, not its
+// (the maximum that hands a NaN on needs no quieted operands: an instruction for three values)
+__device__ __forceinline__ float largest(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float largest(f32x4 v) { return largest(largest(v[0], v[1]), largest(v[2], v[3])); }
+
+// A thread's sum of exp(v - m), m the largest value it has seen.  (The reference is a value, not its
 // multiple by log2 e: rows whose every value is the type's lowest would overflow there.)
 struct RowSum {
     float m, s;
@@ -118,18 +129,51 @@ struct RowSum {
     }
     __device__ __forceinline__ float raise(float top) {
         const float before = m;
-        m = fmaxf(m, top);
-        const float ref = fmaxf(m, F32_LOWEST);   // (nothing but -inf so far: its terms are 0)
+        m = largest(m, top);
+        const float ref = largest(m, F32_LOWEST);   // (nothing but -inf so far: its terms are 0)
         s *= __builtin_amdgcn_exp2f((before - ref) * LOG2E);
         return ref;
     }
     __device__ __forceinline__ void add(float v, float ref) { s += __builtin_amdgcn_exp2f((v - ref) * LOG2E); }
     __device__ __forceinline__ void add1(float v) { add(v, raise(v)); }
-    __device__ __forceinline__ void add4(const float (&v)[GROUP]) {
-        const float ref = raise(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+    __device__ __forceinline__ void add4(f32x4 v) {
+        const float ref = raise(largest(v));
 #pragma unroll
         for (int j = 0; j < GROUP; ++j) {
             add(v[j], ref);
+        }
+    }
+    // All the values a thread holds, in the place of what was summed before.  The exponents are formed in one operation
+    // each, v log2 e - c, c = ref log2 e rounded once: what that rounding took is the same factor for all the terms,
+    // and is given back to their sum.  (Not where the products leave the numbers.)
+    __device__ __forceinline__ void hold(const f32x4 (&v)[HELD], float odd) {
+        m = odd;
+#pragma unroll
+        for (int u = 0; u < HELD; ++u) {
+            m = largest(m, largest(v[u]));
+        }
+        const float ref = largest(m, F32_LOWEST);
+        float part[GROUP] = {};
+        if (fabsf(ref) < 0x1p100f) {
+            const float c = ref * LOG2E;
+#pragma unroll
+            for (int u = 0; u < HELD; ++u) {
+#pragma unroll
+                for (int j = 0; j < GROUP; ++j) {
+                    part[j] += __builtin_amdgcn_exp2f(__builtin_fmaf(v[u][j], LOG2E, -c));
+                }
+            }
+            part[0] += __builtin_amdgcn_exp2f(__builtin_fmaf(odd, LOG2E, -c));
+            s = ((part[0] + part[1]) + (part[2] + part[3])) * __builtin_amdgcn_exp2f(-__builtin_fmaf(ref, LOG2E, -c));
+        } else {
+#pragma unroll
+            for (int u = 0; u < HELD; ++u) {
+#pragma unroll
+                for (int j = 0; j < GROUP; ++j) {
+                    part[j] += __builtin_amdgcn_exp2f((v[u][j] - ref) * LOG2E);
+                }
+            }
+            s = ((part[0] + part[1]) + (part[2] + part[3])) + __builtin_amdgcn_exp2f((odd - ref) * LOG2E);
         }
     }
 };
@@ -183,44 +227,48 @@ __device__ __forceinline__ void list_biases(const RowArgs& a, uint32_t lo, uint3
     __syncthreads();
 }
 
-// The division by the temperature, rounded as IEEE has it.  By its correctly rounded reciprocal r: q0 = l r is
-// within 1.5 units in the last place of l / T, q1 = q0 + (l - q0 T) r within one, its remainder l - q1 T is then
-// exact, and q1 + (l - q1 T) r is the quotient correctly rounded (Markstein 1990) - five operations for the
-// fourteen of a division, as long as nothing on the way leaves the normal numbers: zeros, tiny and huge values and
-// infinities go the long way, a group at a time.
+// The division by the temperature, rounded as IEEE has it, and -inf for a NaN.  With the reciprocal in two parts, r the
+// nearest number and low what is left of it, q = l r + l low is within a unit in the last place of l / T, its remainder l - q T is
+// exact, and q + (l - q T) r is the quotient correctly rounded (Markstein 1990) - four operations for the fourteen of a
+// division, as long as nothing on the way is subnormal or overflows upwards: a group with a zero, a tiny or a huge value goes the long
+// way.  Values far below zero may overflow: what should be -inf comes out as a NaN, and is worth -inf.  (The remainder
+// is formed with the other sign: so zeros would keep theirs.)
 struct Temperature {
-    float t, r;
+    float t, r, low;
     bool one, plain;
 };
 __device__ __forceinline__ Temperature temperature_of(const RowArgs& a) {
     Temperature t;
     t.t = a.temperature;
     t.r = 1.0f / a.temperature;
+    t.low = __builtin_fmaf(-t.r, t.t, 1.0f) * t.r;
     t.one = a.temperature == 1.0f;
-    t.plain = a.temperature > 0x1p-60f && a.temperature < 0x1p60f;
+    t.plain = a.temperature > 0x1p-20f && a.temperature < 0x1p20f;
     return t;
 }
-__device__ __forceinline__ void divide(float (&v)[GROUP], const Temperature& t) {
+__device__ __forceinline__ void divide(f32x4& v, const Temperature& t) {
     if (t.one) {
-        return;
-    }
-    float most = fabsf(v[0]), least = fabsf(v[0]);
-#pragma unroll
-    for (int j = 1; j < GROUP; ++j) {
-        most = fmaxf(most, fabsf(v[j]));
-        least = fminf(least, fabsf(v[j]));
-    }
-    if (t.plain && most < 0x1p60f && least > 0x1p-40f) {
 #pragma unroll
         for (int j = 0; j < GROUP; ++j) {
-            float q = v[j] * t.r;
-            q = __builtin_fmaf(__builtin_fmaf(-q, t.t, v[j]), t.r, q);
-            v[j] = __builtin_fmaf(__builtin_fmaf(-q, t.t, v[j]), t.r, q);
+            v[j] = fmaxf(v[j], NEG_INF);
+        }
+        return;
+    }
+    float least = fabsf(v[0]);
+#pragma unroll
+    for (int j = 1; j < GROUP; ++j) {
+        least = __builtin_elementwise_minimum(least, fabsf(v[j]));
+    }
+    if (t.plain && largest(v) < 0x1p100f && least > 0x1p-100f) {
+#pragma unroll
+        for (int j = 0; j < GROUP; ++j) {
+            const float q = __builtin_fmaf(v[j], t.r, v[j] * t.low), over = __builtin_fmaf(q, t.t, -v[j]);
+            v[j] = fmaxf(__builtin_fmaf(-over, t.r, q), NEG_INF);
         }
     } else {
 #pragma unroll
         for (int j = 0; j < GROUP; ++j) {
-            v[j] /= t.t;
+            v[j] = fmaxf(v[j] / t.t, NEG_INF);
         }
     }
 }
@@ -253,7 +301,7 @@ __device__ __forceinline__ float adjusted(const RowArgs& a, const SliceBias* sb,
 // here and evaluated a lane each (one lane's look at its counts would hold up the other 63), and their values
 // go back to the groups they belong to, which are then stored whole: lines written in part, now and a while later,
 // cost more than everything else (1 024 rows of 151 936 bf16 under 2 048-id histories to f32: +110 us of 192).
-constexpr uint32_t QUEUE = 512;   // ids of a wave; a step has 256 at most
+constexpr uint32_t QUEUE = 512;   // ids of a wave: two groups of every lane at least
 
 // What a workgroup's look at its slice, ids [lo, hi) (lo a multiple of 32), goes by.
 struct Slice {
@@ -285,99 +333,106 @@ __device__ __forceinline__ float odd_value(const Slice& s, uint32_t id) {
     return value_of<DT>(s, id, !s.masked || bit_of(s.a.allow, id));
 }
 
-// The values of N groups of every lane, groups w0 + lane, w0 + lane + nt, ... (w0 the same in the wave); groups
+// The values of N groups of every lane, groups w0 + lane, w0 + lane + 256, ... (w0 the same in the wave); groups
 // from `whole` on hold nothing of use.
 template <int DT, int N>
-__device__ __forceinline__ void groups(const Slice& s, uint32_t w0, float (&v)[N][GROUP]) {
-    const uint32_t lane = threadIdx.x & 63u, nt = blockDim.x;
+__device__ __forceinline__ void groups(const Slice& s, uint32_t w0, f32x4 (&v)[N]) {
+    static_assert(N * GROUP <= 32 && QUEUE >= 2 * GROUP * 64, "a bit an id of a lane");
+    const uint32_t lane = threadIdx.x & 63u, g0 = w0 + lane;
+    const char* from = static_cast<const char*>(s.a.logits) + (size_t)s.lo * (DT == LILY_F32 ? 4u : 2u);
     RawGroup<DT> raw[N];
     uint32_t listed[N], admitted[N];
-    auto id_at = [&](int u) { return s.lo + min(w0 + lane + (uint32_t)u * nt, s.whole - 1u) * GROUP; };
+    auto at = [&](int u) { return min(g0 + (uint32_t)u * 256u, s.whole - 1u); };
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-        raw[u].load(s.a.logits, id_at(u));
+        raw[u].load(from, at(u));
     }
     if (s.pen) {
+        const uint32_t* words = s.a.touched + s.lo / 32u;
 #pragma unroll
         for (int u = 0; u < N; ++u) {
-            listed[u] = gload(s.a.touched + (id_at(u) >> 5));
+            listed[u] = gload(words + at(u) / 8u);
         }
     }
     if (s.masked) {
+        const uint32_t* words = s.a.allow + s.lo / 32u;
 #pragma unroll
         for (int u = 0; u < N; ++u) {
-            admitted[u] = gload(s.a.allow + (id_at(u) >> 5));
+            admitted[u] = gload(words + at(u) / 8u);
         }
     }
-    uint32_t some[N];
+    const uint32_t shift = g0 % 8u * GROUP;   // of the groups' bits in their words, the same for all of them
+    uint32_t some = 0, open = 0xffffffffu;    // bits of the lane's ids: listed or biased, admitted
+    if (s.pen) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            some |= (listed[u] >> shift & 15u) << (u * GROUP);
+        }
+    }
+    if (s.biased) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            some |= (s.bits[at(u) / 8u] >> shift & 15u) << (u * GROUP);
+        }
+    }
+    if (s.masked) {
+        open = 0u;
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            open |= (admitted[u] >> shift & 15u) << (u * GROUP);
+        }
+    }
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-        const uint32_t id = id_at(u);
-        uint32_t word = s.pen ? listed[u] : 0u;
-        if (s.biased) {
-            word |= s.bits[(id - s.lo) >> 5];
-        }
-        const uint32_t open = s.masked ? (admitted[u] >> (id & 31u)) & 15u : 15u;
-        some[u] = w0 + lane + (uint32_t)u * nt < s.whole ? (word >> (id & 31u)) & open : 0u;
 #pragma unroll
         for (int j = 0; j < GROUP; ++j) {
             v[u][j] = raw[u].at(j);
         }
-        if (open != 15u) {
+        divide(v[u], s.temperature);
+        if (s.masked) {
 #pragma unroll
             for (int j = 0; j < GROUP; ++j) {
-                v[u][j] = (open >> j) & 1u ? v[u][j] : NEG_INF;
+                const uint32_t all = (uint32_t)((int32_t)(open << (31 - u * GROUP - j)) >> 31);
+                v[u][j] = lilym_bits_f32((lilym_f32_bits(v[u][j]) & all) | (lilym_f32_bits(NEG_INF) & ~all));
             }
         }
-        divide(v[u], s.temperature);
-#pragma unroll
-        for (int j = 0; j < GROUP; ++j) {
-            v[u][j] = fmaxf(v[u][j], NEG_INF);   // (a NaN is worth -inf)
-        }
     }
-    if (!s.pen && !s.biased) {
+    const uint32_t mine = g0 < s.whole ? (s.whole - g0 + 255u) / 256u : 0u;   // groups that are there
+    some &= open & (mine >= (uint32_t)N ? 0xffffffffu : (1u << (mine * GROUP)) - 1u);
+    if (__ballot(some != 0u) == 0ull) {
         return;
     }
-    // All steps' ids at once, or as many steps' as the queue holds.
-    for (;;) {
-        uint32_t at[N], waiting = 0, taken = 0;
-#pragma unroll
-        for (int u = 0; u < N; ++u) {
-            if (__ballot(some[u] != 0u) != 0u) {
-                const uint32_t n = (uint32_t)__builtin_popcount(some[u]), upto = wave_scan_u32(n);
-                const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-                if (waiting + all <= QUEUE) {
-                    at[u] = waiting + upto - n;
-                    waiting += all;
-                    taken |= 1u << u;
-                    uint32_t k = at[u];
-                    for (uint32_t rest = some[u]; rest != 0u; rest &= rest - 1u) {
-                        s.queue[k++] = id_at(u) + (uint32_t)__builtin_ctz(rest);
-                    }
-                }
-            }
-        }
-        if (taken == 0u) {
-            return;
+    // All of the ids at once, or two groups' after the other where they are too many for the queue.
+    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32((uint32_t)__builtin_popcount(some)), 63);
+    const uint32_t width = all <= QUEUE ? 32u : 2u * GROUP;
+    for (uint32_t b = 0; b < (uint32_t)(N * GROUP); b += width) {
+        const uint32_t part = some & (width == 32u ? 0xffffffffu : ((1u << width) - 1u) << b);
+        const uint32_t n = (uint32_t)__builtin_popcount(part), upto = wave_scan_u32(n);
+        const uint32_t waiting = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+        uint32_t k = upto - n;
+        for (uint32_t rest = part; rest != 0u; rest &= rest - 1u) {
+            const uint32_t c = (uint32_t)__builtin_ctz(rest);
+            s.queue[k++] = s.lo + (g0 + c / GROUP * 256u) * GROUP + c % GROUP;
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        for (uint32_t k = lane; k < waiting; k += 64u) {
-            s.queue[k] = lilym_f32_bits(value_of<DT>(s, s.queue[k], true));
+        for (uint32_t i = lane; i < waiting; i += 64u) {
+            s.queue[i] = lilym_f32_bits(value_of<DT>(s, s.queue[i], true));
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+        k = upto - n;
 #pragma unroll
         for (int u = 0; u < N; ++u) {
-            if (((taken >> u) & 1u) != 0u) {
-                uint32_t k = at[u];
+            const uint32_t bits = part >> (u * GROUP) & 15u;
+            if (__ballot(bits != 0u) != 0ull) {
 #pragma unroll
                 for (int j = 0; j < GROUP; ++j) {
-                    if ((some[u] >> j) & 1u) {
-                        v[u][j] = lilym_bits_f32(s.queue[k++]);
-                    }
+                    const float x = lilym_bits_f32(s.queue[k]);   // (one behind the last may be looked at, and is not taken)
+                    const bool taken = (bits >> j & 1u) != 0u;
+                    v[u][j] = taken ? x : v[u][j];
+                    k += taken ? 1u : 0u;
                 }
-                some[u] = 0u;
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -385,18 +440,18 @@ __device__ __forceinline__ void groups(const Slice& s, uint32_t w0, float (&v)[N
     }
 }
 
-// One pass over the slice: each(id, values of a group), each_one(id, value).
+// One pass over the slice: each(group, its values), each_one(id, value).
 template <int DT, class EACH, class EACH_ONE>
 __device__ __forceinline__ void pass_over(const Slice& s, EACH&& each, EACH_ONE&& each_one) {
-    const uint32_t tid = threadIdx.x, nt = blockDim.x, lane = tid & 63u;
-    for (uint32_t w0 = tid - lane; w0 < s.whole; w0 += nt * AHEAD) {
-        float v[AHEAD][GROUP];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    for (uint32_t w0 = tid - lane; w0 < s.whole; w0 += 256u * AHEAD) {
+        f32x4 v[AHEAD];
         groups<DT>(s, w0, v);
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
-            const uint32_t g = w0 + lane + (uint32_t)u * nt;
+            const uint32_t g = w0 + lane + (uint32_t)u * 256u;
             if (g < s.whole) {
-                each(s.lo + g * GROUP, v[u]);
+                each(g, v[u]);
             }
         }
     }
@@ -404,6 +459,29 @@ __device__ __forceinline__ void pass_over(const Slice& s, EACH&& each, EACH_ONE&
     if (odd_id(s, id)) {
         each_one(id, odd_value<DT>(s, id));
     }
+}
+
+// The slice's values in registers, and the thread's sum of them.
+template <int DT>
+__device__ __forceinline__ RowSum hold(const Slice& s, f32x4 (&v)[HELD], float& odd_v) {
+    const uint32_t tid = threadIdx.x;
+    if (s.whole != 0u) {
+        groups<DT>(s, tid & ~63u, v);
+    }
+#pragma unroll
+    for (int u = 0; u < HELD; ++u) {
+        if (s.whole < (uint32_t)(u + 1) * 256u && tid + (uint32_t)u * 256u >= s.whole) {
+#pragma unroll
+            for (int j = 0; j < GROUP; ++j) {
+                v[u][j] = NEG_INF;
+            }
+        }
+    }
+    uint32_t odd;
+    odd_v = odd_id(s, odd) ? odd_value<DT>(s, odd) : NEG_INF;
+    RowSum sum;
+    sum.hold(v, odd_v);
+    return sum;
 }
 
 struct LogitsLaunch {
@@ -423,14 +501,15 @@ struct LogitsLaunch {
 // (a - top) - log_s, exact where the row's values lie together however large they are (rows masked by the
 // type's lowest value throughout are even, not nothing).
 struct LogSum {
-    float top, log_s;
-    __device__ __forceinline__ float whole() const { return (float)((double)top + (double)log_s); }
-    __device__ __forceinline__ float logprob(float a) const { return a > NEG_INF ? (a - top) - log_s : NEG_INF; }
+    float top, log_s;   // (an empty row has 0 for both: its values stay -inf)
+    float whole;        // the log-sum-exp
+    __device__ __forceinline__ float logprob(float a) const { return (a - top) - log_s; }
 };
 __device__ __forceinline__ LogSum log_sum(double m, double s) {
     LogSum r;
-    r.top = (float)m;
-    r.log_s = s > 0.0 ? (float)log(s) : 0.0f;   // (0: an empty row; NaN: a row that holds +inf)
+    r.top = m > (double)NEG_INF ? (float)m : 0.0f;
+    r.log_s = s > 0.0 ? (float)log(s) : 0.0f;   // (NaN: a row that holds +inf)
+    r.whole = (float)(m + (double)r.log_s);
     return r;
 }
 
@@ -468,7 +547,7 @@ __device__ __forceinline__ void logits_row(const RowArgs& a, uint32_t row_of_lau
     __shared__ SliceBias sb;
     __shared__ Sums sh;
     __shared__ uint32_t wave_count[4];
-    __shared__ uint32_t queues[4][QUEUE];
+    __shared__ uint32_t queues[4][QUEUE + 1];
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
     uint32_t* queue = queues[tid >> 6];
     uint32_t* bits = reinterpret_cast<uint32_t*>(dyn_lds);
@@ -483,12 +562,13 @@ __device__ __forceinline__ void logits_row(const RowArgs& a, uint32_t row_of_lau
         return Slice(a, &sb, bits, queue, lo, hi);
     };
     const Slice mine = take(slice);
-    LogSum lse = {0.0f, 0.0f};
+    LogSum lse = {0.0f, 0.0f, 0.0f};
     auto worth = [&](float v) { return is_logprobs(FORM) ? lse.logprob(v) : v; };
     auto write_one = [&](uint32_t id, float v) { store_one<OT>(out, id, worth(v)); };
-    auto write = [&](uint32_t id, const float (&v)[GROUP]) {
-        const float p[GROUP] = {worth(v[0]), worth(v[1]), worth(v[2]), worth(v[3])};
-        store_group<OT>(out, id, p);
+    char* out_slice = static_cast<char*>(out) + (size_t)mine.lo * (OT == LILY_F32 ? 4u : 2u);
+    auto write = [&](uint32_t group, f32x4 v) {
+        const f32x4 p = {worth(v[0]), worth(v[1]), worth(v[2]), worth(v[3])};
+        store_group<OT>(out_slice, group, p);
     };
     if constexpr (FORM == FORM_ADJUSTED) {
         pass_over<DT>(mine, write, write_one);
@@ -496,7 +576,7 @@ __device__ __forceinline__ void logits_row(const RowArgs& a, uint32_t row_of_lau
         RowSum sum;
         sum.init();
         pass_over<DT>(
-            mine, [&](uint32_t, const float (&v)[GROUP]) { sum.add4(v); }, [&](uint32_t, float v) { sum.add1(v); });
+            mine, [&](uint32_t, f32x4 v) { sum.add4(v); }, [&](uint32_t, float v) { sum.add1(v); });
         const uint64_t word = merge_threads(sum, sh);
         if (tid == 0u) {
             handed_store(q.word, first + slice, word);
@@ -506,28 +586,14 @@ __device__ __forceinline__ void logits_row(const RowArgs& a, uint32_t row_of_lau
         merge_slices(lane < q.slices ? handed_load(q.word, first + lane) : 0ull, q.slices, m, s);
         lse = log_sum(m, s);
         if (q.lse != nullptr && slice == 0u && tid == 0u) {
-            q.lse[row] = lse.whole();
+            q.lse[row] = lse.whole;
         }
         pass_over<DT>(mine, write, write_one);
     } else {
         // The slice's values in registers, and its word.
-        float v[HELD][GROUP], odd_v = NEG_INF;
-        uint32_t odd;
-        RowSum sum;
-        sum.init();
-        if (mine.whole != 0u) {
-            groups<DT>(mine, tid - lane, v);
-        }
-#pragma unroll
-        for (int u = 0; u < HELD; ++u) {
-            if (tid + (uint32_t)u * 256u < mine.whole) {
-                sum.add4(v[u]);
-            }
-        }
-        if (odd_id(mine, odd)) {
-            odd_v = odd_value<DT>(mine, odd);
-            sum.add1(odd_v);
-        }
+        f32x4 v[HELD];
+        float odd_v;
+        const RowSum sum = hold<DT>(mine, v, odd_v);
         const uint64_t word = merge_threads(sum, sh);
         if (q.slices > 1u && tid == 0u) {
             handed_store(q.word, first + slice, word);
@@ -537,10 +603,11 @@ __device__ __forceinline__ void logits_row(const RowArgs& a, uint32_t row_of_lau
             for (int u = 0; u < HELD; ++u) {
                 const uint32_t g = tid + (uint32_t)u * 256u;
                 if (g < mine.whole) {
-                    write(mine.lo + g * GROUP, v[u]);
+                    write(g, v[u]);
                 }
             }
-            if (odd < mine.hi) {
+            uint32_t odd;
+            if (odd_id(mine, odd)) {
                 write_one(odd, odd_v);
             }
         };
@@ -574,29 +641,27 @@ __device__ __forceinline__ void logits_row(const RowArgs& a, uint32_t row_of_lau
             __syncthreads();
             if (sh.missing != 0u) {
                 // Somebody has no place on the chip yet: the words that are missing from here, the same ones (the
-                // threads add the same values in the same order).
+                // threads add the same values in the same order), and then this slice again.
                 for (uint32_t other = 0; other < q.slices; ++other) {
                     if (sh.words[other] != 0ull) {
                         continue;
                     }
-                    RowSum again;
-                    again.init();
-                    pass_over<DT>(
-                        take(other), [&](uint32_t, const float (&w)[GROUP]) { again.add4(w); },
-                        [&](uint32_t, float w) { again.add1(w); });
-                    const uint64_t formed = merge_threads(again, sh);
+                    const uint64_t formed = merge_threads(hold<DT>(take(other), v, odd_v), sh);
                     if (tid == 0u) {
                         const uint64_t come = handed_load(q.word, first + other);
                         sh.words[other] = come != 0ull ? come : formed;
                     }
                     __syncthreads();
                 }
+                if (is_logprobs(FORM)) {
+                    hold<DT>(take(slice), v, odd_v);
+                }
             }
             double m, s;
             merge_slices(sh.words[lane], q.slices, m, s);
             lse = log_sum(m, s);
             if (q.lse != nullptr && slice == 0u && tid == 0u) {
-                q.lse[row] = lse.whole();
+                q.lse[row] = lse.whole;
             }
         }
         if (is_logprobs(FORM)) {
@@ -627,16 +692,14 @@ __device__ __forceinline__ RowArgs row_of(const LILY_CONST RowArgs* p) {
     return a;
 }
 
-// (five waves a SIMD where values are held: by itself the compiler takes the registers of four; 276 -> 246 us for
-// 1 024 rows of bf16 log-probabilities.  Six spill: 339)
 template <int DT, int OT, int FORM>
-__global__ void __launch_bounds__(256, is_held(FORM) ? 5 : 1) k_logits_rows_table(const RowArgs* table, LogitsLaunch q) {
+__global__ void __launch_bounds__(256) k_logits_rows_table(const RowArgs* table, LogitsLaunch q) {
     const uint32_t row = blockIdx.x / q.slices, slice = blockIdx.x % q.slices;
     const RowArgs a = row_of((const LILY_CONST RowArgs*)table + row);
     logits_row<DT, OT, FORM>(a, row, slice, q);
 }
 template <int DT, int OT, int FORM>
-__global__ void __launch_bounds__(256, is_held(FORM) ? 5 : 1) k_logits_rows_inline(InlineRows rows, LogitsLaunch q) {
+__global__ void __launch_bounds__(256) k_logits_rows_inline(InlineRows rows, LogitsLaunch q) {
     const LILY_CONST RowArgs* table = (const LILY_CONST RowArgs*)__builtin_amdgcn_kernarg_segment_ptr();
     const uint32_t row = blockIdx.x / q.slices, slice = blockIdx.x % q.slices;
     const RowArgs a = row_of(table + row);

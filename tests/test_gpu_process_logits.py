@@ -428,3 +428,68 @@ def test_what_the_python_mirror_refuses(sampler):
         kw.update(bad)
         with pytest.raises(LS.SamplerError):
             sampler.process_logits(**kw)
+
+
+@pytest.mark.parametrize("temperature", [0.7, 1.3, 0.1, 1.9999999, 0.50000006, 3.0, 1e-5, 9e5, 2e6, 1e-7])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_the_division_is_ieee_s(sampler, temperature, dtype):
+    """Quotients bit for bit: ordinary values, zeros of both signs, subnormal, tiny and huge ones, values that overflow on
+    either side, infinities and NaN (worth -inf), each among ordinary neighbours and by itself."""
+    rng = np.random.default_rng(5)
+    vocab = 40003
+    x = (rng.normal(0, 4, (3, vocab)) * np.exp2(rng.integers(-3, 4, (3, vocab)))).astype(F)
+    odd = np.array([0.0, -0.0, 1e-45, -1e-45, 1.1754944e-38, -3e-39, 7.9e-31, 1e-30, -1e-30, 2.0 ** -100, -(2.0 ** -101), 1.2e30, 1.3e30,
+                    -1.3e30, 2.0 ** 100, -(2.0 ** 101), 3.4028235e38, -3.4028235e38, -3.3895314e38, 1e38, -1e38, np.inf, -np.inf, np.nan], F)
+    x[1, 100:4100:7] = odd[rng.integers(0, len(odd), 572)]
+    x[2, : 4 * len(odd)] = np.repeat(odd, 4)
+    if dtype == "bf16":
+        x = W.bf16_bits_to_f32(W.to_bf16_bits(x))
+    logits = upload_logits(x) if dtype == "f32" else torch.from_numpy(x).to(dev()).bfloat16()
+    out, lse = torch.empty(3, vocab, device=dev()), torch.empty(3, device=dev())
+    kws = [dict(temperature=temperature, top_k=5, seed=r) for r in range(3)]
+    params = [ls_params(**k) for k in kws]
+    want = [_adjusted(x[r], kws[r]) for r in range(3)]
+    assert params[0].effective()[0] == F(temperature)
+    torch.cuda.synchronize()
+    for sums in (None, lse):
+        keep = sampler.process_logits(logits, params, out, log_sum_exp=sums)
+        sampler.synchronize()
+        for r in range(3):
+            assert np.array_equal(out[r].cpu().numpy().view(np.uint32), want[r].view(np.uint32)), (r, sums is None)
+        del keep
+    ref = _lse(want[0])
+    assert abs(float(lse[0]) - ref) <= (1.25 * max(8, vocab / 1024) + 8 + abs(ref)) * U
+    assert float(lse[2]) == np.inf
+
+
+@pytest.mark.parametrize("vocab", [4, 1029, 8200, 30001])
+@pytest.mark.parametrize("what", ["counts", "biases", "both"])
+@pytest.mark.parametrize("with_sum", [False, True])
+def test_every_id_is_listed(sampler, vocab, what, with_sum):
+    """More ids of a wave than it gathers at once: every id counted, biased, or both, under a mask that leaves three of four."""
+    rng = np.random.default_rng(vocab)
+    rows = 2
+    x = rng.normal(0, 3, (rows, vocab)).astype(F)
+    penalties = dict(repetition_penalty=1.2, presence_penalty=0.4, frequency_penalty=0.1) if what != "biases" else {}
+    kws = [dict(temperature=0.9, top_k=5, seed=r, **penalties) for r in range(rows)]
+    counts, scratch = None, None
+    if what != "biases":
+        counts = rng.integers(1, 9, (rows, vocab)).astype(np.int32)
+        scratch = [LS.SamplerScratch(sampler, vocab) for _ in range(rows)]
+        for r in range(rows):
+            scratch[r].write_counts(torch.from_numpy(counts[r]))
+    lists = None
+    if what != "counts":
+        n = min(vocab, 400)   # in a run, so that a lane's ids are all of them
+        lists = [[(int(i), float(d)) for i, d in zip(range(r, n), rng.normal(0, 2, n - r))] for r in range(rows)]
+    allow = np.zeros((rows, (vocab + 31) // 32), np.uint32)
+    allow[:] = 0xEEEEEEEE
+    a = torch.from_numpy(allow.view(np.int32)).to(dev())
+    logits, out = upload_logits(x), torch.empty(rows, vocab, device=dev())
+    lse = torch.empty(rows, device=dev()) if with_sum else None
+    torch.cuda.synchronize()
+    keep = sampler.process_logits(logits, [ls_params(**k) for k in kws], out, log_sum_exp=lse, scratch=scratch, allow=a, bias=lists)
+    sampler.synchronize()
+    want = [_adjusted(x[r], kws[r], None if counts is None else counts[r], allow[r], None if lists is None else lists[r]) for r in range(rows)]
+    _check(out, lse, want, False, vocab)
+    del keep
