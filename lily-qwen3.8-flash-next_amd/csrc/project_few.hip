@@ -168,7 +168,10 @@ hipError_t launch_project_few(hipStream_t stream, const ProjectArgs& a, bool e4m
 //                128 x 128 would take 271
 // Parts of d: a launch more (1.5), and the parts' sums written and read at 5.5 TB/s: 64 x 1000 x 8192 in eight 10.6 (10.5)
 // against 25.5 in one; 300 x 4096 x 4096 in two of 128 x 128 22.2 (23.3), where 64 x 64 takes 28.1 in one and 25.9 in two
-// and 128 x 128 30.4 in one; 512 x 4096 x 4096 25.9 (29.9).  Memory at 5.6 TB/s bounds all of them.
+// and 128 x 128 30.4 in one; 512 x 4096 x 4096 25.9 (29.9); 100 x 10 007 x 4096 in E4M3, 79 tiles of 128 x 128, in two
+// 16.6 (16.5), in three 16.9 (16.9), in four, a second round, 20.0 (21.5).  Memory at 5.6 TB/s bounds all of them.
+// Rows that do not start at lines of 128 bytes cost 1.4 times as much a line of d, two requests: the same with rows of 4128
+// bytes 19.3 in three parts (18.9), 20.2 in two (18.9), 23.4 in one of 64 x 64 (22.8).
 struct ProjectPlan {
     uint32_t tile = 0;     // 0: few rows
     uint32_t splits = 1;
@@ -179,6 +182,8 @@ static ProjectPlan project_plan(const ProjectArgs& a, uint64_t part_floats) {
     const double memory = ((rows + n) * bytes + rows * n * (a.out_bf16 ? 2.0 : 4.0)) / 5.6e6;
     auto over = [](uint32_t x, uint32_t y) { return (x + y - 1u) / y; };
     auto rounds = [](uint64_t tiles) { return (double)((tiles + 255u) / 256u); };
+    auto straight = [](const char* p, uint64_t stride) { return (reinterpret_cast<uintptr_t>(p) | stride) % LINE == 0u; };
+    const double crossed = straight(a.x, a.x_stride) && straight(a.w, a.w_stride) ? 1.0 : 1.4;
     ProjectPlan best;
     double least = 1e30;
     auto offer = [&](uint32_t tile, uint32_t splits, double us) {
@@ -197,14 +202,14 @@ static ProjectPlan project_plan(const ProjectArgs& a, uint64_t part_floats) {
     }
     const uint64_t t64 = (uint64_t)over(a.rows, 64u) * over(a.n, 64u), t128 = (uint64_t)over(a.rows, 128u) * over(a.n, 128u),
                    t256 = (uint64_t)over(a.rows, 256u) * over(a.n, 256u);
-    for (uint32_t k = 1; k <= 16u; k *= 2u) {
+    for (uint32_t k = 1; k <= 16u; ++k) {
         if (k > 1u && (lines < 4u * k || (double)k * rows * part_stride(a.n) > (double)part_floats)) {
             break;
         }
-        const double each = lines / (double)k, join = k > 1u ? 1.5 + k * rows * n * 8.0 / 5.5e6 : 0.0;
-        offer(64u, k, 4.0 + std::max(memory, each * std::max(0.22, 0.21 * rounds(t64 * k))) + join);
+        const double each = lines * crossed / (double)k, join = k > 1u ? 1.5 + k * rows * n * 8.0 / 5.5e6 : 0.0;
+        offer(64u, k, std::max(3.0 + memory, 4.0 + each * std::max(0.22, 0.21 * rounds(t64 * k))) + join);
         const double turns = t128 * k <= 256u ? (double)(t128 * k) / 256.0 : rounds(t128 * k);
-        offer(128u, k, 6.0 + std::max(memory, each * std::max(0.38, 0.51 * turns)) + join);
+        offer(128u, k, std::max(3.0 + memory, 6.0 + each * std::max(0.38, 0.51 * turns)) + join);
     }
     offer(256u, 1u, 2.0 + std::max(memory, rounds(t256) * (15.0 + lines * 1.45)));
     return best;
