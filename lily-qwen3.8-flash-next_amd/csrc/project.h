@@ -98,7 +98,7 @@ __device__ __forceinline__ void activate(float (&v)[N], uint32_t act) {   // (on
         for (int j = 0; j < N; ++j) {
             v[j] *= logistic(v[j]);
         }
-    } else if (N <= 4 && act == LILY_ACT_GELU) {   // (some eighty instructions a value: a row at a time only)
+    } else if (N <= 8 && act == LILY_ACT_GELU) {   // (some eighty instructions a value: a row at a time only)
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             v[j] = 0.5f * v[j] * erfcf(-0.70710678118654752f * v[j]);

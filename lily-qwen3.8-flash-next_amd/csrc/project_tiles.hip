@@ -18,6 +18,8 @@
 //
 // A staged row's eight pieces change places by the row's number (piece ^ (row / 2) % 8): the 16 lanes that
 // read one piece of 16 rows then meet 16 different groups of banks.
+#include <utility>
+
 #include "launch.h"
 #include "project.h"
 
@@ -37,11 +39,10 @@ struct Block;
 template <>
 struct Block<16> {
     typedef f32x4 Sums;
-    static constexpr int PIECES = 2, GROUPS = 1;   // pieces a lane of a line; runs of four neighbouring outputs a lane
+    static constexpr int PIECES = 2;               // a lane of a line
     u32x4 p[PIECES];
     static __device__ __forceinline__ uint32_t first_piece(uint32_t lane) { return lane >> 4; }   // then every fourth
     static constexpr uint32_t NEXT_PIECE = 64;     // in bytes of a staged row, by exclusive or
-    static __device__ __forceinline__ uint32_t output(uint32_t lane, int) { return (lane >> 4) * 4u; }
     static __device__ __forceinline__ Sums product(bf16x8 w, bf16x8 x, Sums c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x, c, 0, 0, 0); }
     static __device__ __forceinline__ Sums product(i32x8 w, i32x8 x, Sums c) {
         return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, 0, 0, 0, 0, 0);
@@ -50,11 +51,10 @@ struct Block<16> {
 template <>
 struct Block<32> {
     typedef f32x16 Sums;
-    static constexpr int PIECES = 4, GROUPS = 4;
+    static constexpr int PIECES = 4;
     u32x4 p[PIECES];
     static __device__ __forceinline__ uint32_t first_piece(uint32_t lane) { return lane >> 5; }   // then every second
     static constexpr uint32_t NEXT_PIECE = 32;
-    static __device__ __forceinline__ uint32_t output(uint32_t lane, int q) { return (uint32_t)q * 8u + (lane >> 5) * 4u; }
     static __device__ __forceinline__ Sums product(bf16x8 w, bf16x8 x, Sums c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, x, c, 0, 0, 0); }
     static __device__ __forceinline__ Sums product(i32x8 w, i32x8 x, Sums c) {
         return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 0, 0, 0, 0, 0, 0);
@@ -85,7 +85,8 @@ struct Tile {
     static constexpr int XR = WM * MH * S, WR = WN * NH * S;           // rows of a unit: of x, of the weights
     static constexpr int UNIT = (XR + WR) * (int)LINE;
     static constexpr int XL = XR / 32, WL = WR / 32, LOADS = XL + WL;  // loads of a wave and unit
-    static constexpr int LDS_BYTES = 2 * DEPTH * UNIT;
+    static constexpr int STAGES = 2 * DEPTH * UNIT, HALVES = 4 * MH * S * (NT * S + 4) * 4;   // bytes; the epilogue's, by halves
+    static constexpr int LDS_BYTES = S == 32 && HALVES > STAGES ? HALVES : STAGES;
     static_assert(DEPTH % 2 == 0 && (2 * DEPTH - 1) * LOADS < 64, "loads in flight are counted in six bits");
     static_assert(WM * WN == 4 && XR % 32 == 0 && WR % 32 == 0, "whole loads a wave");
 };
@@ -94,6 +95,259 @@ template <int V>
 struct Constant {
     static constexpr int value = V;
 };
+// f of the constants 0 .. N - 1
+template <class F, int... I>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
+    (f(Constant<I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+    each_of(f, std::make_integer_sequence<int, N>{});
+}
+
+// The epilogue of the large tile, which nothing else hides: half of a wave's rows at a time through its part of LDS, so
+// that a lane has eight neighbouring outputs and 16 lanes a row's 256 bytes of bf16.  Its outputs are the same in every
+// row: their scales and biases are read once, the rows go by a loop of few operations a value, what
+// the next four rows read is on its way meanwhile.  (Quarters of four outputs a lane, rows unrolled, took 39 000 cycles a
+// tile of bf16 without operands, a fifth of a tile with d = 4096, and 64 000 with a bias, SiLU and a residual.)
+// A row's 16-byte pieces from the 16th on change places in pairs: lanes 8 to 15 then read the groups of banks that lanes
+// 0 to 7 leave.
+struct Rows {     // what four rows read
+    float scale[4];
+    u32x4 lo[4];  // the residual as it lies in memory: eight bf16, or the first four f32
+};
+typedef u32x4 pj_u32x4_out __attribute__((aligned(2)));
+template <class T>
+__device__ __forceinline__ void give_halves(const ProjectArgs& a, const f32x16 (&acc)[2][T::MH][2][T::NH], char* lds, uint32_t m, uint32_t n,
+                                            uint32_t wave, uint32_t lane) {
+    static_assert(T::S == 32 && T::MT == 4 && T::NT == 4, "four blocks of 32 both ways");
+    constexpr uint32_t ROW = 132;   // floats (a step of four banks from row to row)
+    float* mine = reinterpret_cast<float*>(lds) + wave * (64u * ROW);
+    const uint32_t v0 = n + lane % 16u * 8u, r0 = m + lane / 16u;
+    const bool whole = v0 + 8u <= a.n;
+    float scale[8];
+    uint32_t raw[8];   // of the bias
+    each<8>([&](auto k) {
+        const uint32_t v = min(v0 + k.value, a.n - 1u);
+        scale[k.value] = a.w_scales != nullptr ? gload(a.w_scales + v) : 1.0f;
+        raw[k.value] = 0u;
+        if (a.bias != nullptr) {
+            raw[k.value] = a.bias_bf16 ? (uint32_t)gload(static_cast<const uint16_t*>(a.bias) + v) << 16 : gload(static_cast<const uint32_t*>(a.bias) + v);
+        }
+    });
+    // Rows r0 + 4 turn, + 4, + 8, + 12; and the residual's last four outputs in f32.
+    auto residual_at = [&](uint32_t r, uint32_t first) {
+        const uint64_t from = (uint64_t)min(r, a.rows - 1u) * a.residual_stride + v0 + first;
+        const uint16_t* half = static_cast<const uint16_t*>(a.residual) + from;
+        const uint32_t* word = static_cast<const uint32_t*>(a.residual) + from;
+        u32x4 w;
+        if (whole && a.residual_bf16) {
+            w = *(const LILY_GLOBAL pj_u32x4_out*)half;
+        } else if (whole) {
+            w = *(const LILY_GLOBAL pj_u32x4_any*)word;
+        } else {
+            uint32_t e[8];
+            each<8>([&](auto k) {   // (what lies behind the last output is not read)
+                const uint32_t j = min((uint32_t)k.value, a.n - 1u - v0 - min(first, a.n - 1u - v0));
+                e[k.value] = a.residual_bf16 ? (uint32_t)gload(half + j) : first + j < a.n - v0 ? gload(word + j) : 0u;
+            });
+            w = a.residual_bf16 ? u32x4{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16} : u32x4{e[0], e[1], e[2], e[3]};
+        }
+        return w;
+    };
+    auto rows_at = [&](Rows& l, uint32_t turn) {
+        if (a.x_scales != nullptr) {
+            each<4>([&](auto t) { l.scale[t.value] = gload(a.x_scales + min(r0 + (turn + t.value) * 4u, a.rows - 1u)); });
+        }
+        if (a.residual != nullptr) {
+            each<4>([&](auto t) { l.lo[t.value] = residual_at(r0 + (turn + t.value) * 4u, 0u); });
+        }
+    };
+    u32x4 hi[4];
+    auto last_at = [&](uint32_t turn) {
+        if (a.residual != nullptr && !a.residual_bf16) {
+            each<4>([&](auto t) { hi[t.value] = residual_at(r0 + (turn + t.value) * 4u, 4u); });
+        }
+    };
+    const uint32_t at = lane / 16u * ROW + ((lane % 16u * 2u) ^ (lane % 16u >> 3)) * 4u, other = (lane % 16u >> 3) != 0u ? (uint32_t)-4 : 4u;
+    // N rows r0 + 4 (turn + first), + 4, ...: their sums lie from row `from` of the half on
+    auto give = [&](const Rows& l, uint32_t turn, auto first, auto rows) {
+        constexpr int F = decltype(first)::value, N = decltype(rows)::value;
+        float v[8 * N];
+        each<N>([&](auto t) {
+            const float* p = mine + ((turn + F + t.value) % 16u * 4u) * ROW + at;
+            const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + (int32_t)other);
+            each<8>([&](auto k) {
+                const float sum = k.value < 4 ? x[k.value % 4] : y[k.value % 4];
+                v[t.value * 8 + k.value] = sum * l.scale[F + t.value] * scale[k.value] + lilym_bits_f32(raw[k.value]);
+            });
+        });
+        activate(v, a.act);
+        if (a.residual != nullptr && a.residual_bf16) {
+            each<8 * N>([&](auto e) {
+                const uint32_t w = l.lo[F + e.value / 8][e.value % 8 / 2];
+                v[e.value] += lilym_bits_f32((e.value & 1) ? w & 0xffff0000u : w << 16);
+            });
+        } else if (a.residual != nullptr) {
+            each<8 * N>([&](auto e) {
+                v[e.value] += lilym_bits_f32(e.value % 8 < 4 ? l.lo[F + e.value / 8][e.value % 4] : hi[F + e.value / 8][e.value % 4]);
+            });
+        }
+        each<N>([&](auto t) {
+            constexpr int e = t.value * 8;
+            const uint32_t r = r0 + (turn + F + t.value) * 4u;
+            if (r < a.rows) {
+                const uint64_t to = (uint64_t)r * a.out_stride + v0;
+                if (!whole) {
+                    each<7>([&](auto k) {
+                        if (v0 + k.value < a.n) {
+                            if (a.out_bf16) {
+                                *(LILY_GLOBAL uint16_t*)(static_cast<uint16_t*>(a.out) + to + k.value) = (uint16_t)pj_bf16_pair(v[e + k.value], 0.0f);
+                            } else {
+                                *(LILY_GLOBAL float*)(static_cast<float*>(a.out) + to + k.value) = v[e + k.value];
+                            }
+                        }
+                    });
+                } else if (a.out_bf16) {
+                    *(LILY_GLOBAL pj_u32x4_out*)(static_cast<uint16_t*>(a.out) + to) =
+                        u32x4{pj_bf16_pair(v[e], v[e + 1]), pj_bf16_pair(v[e + 2], v[e + 3]), pj_bf16_pair(v[e + 4], v[e + 5]),
+                              pj_bf16_pair(v[e + 6], v[e + 7])};
+                } else {
+                    *(LILY_GLOBAL f32x4_any*)(static_cast<float*>(a.out) + to) = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+                    *(LILY_GLOBAL f32x4_any*)(static_cast<float*>(a.out) + to + 4) = f32x4{v[e + 4], v[e + 5], v[e + 6], v[e + 7]};
+                }
+            }
+        });
+    };
+    // (a loop, and one copy of it: unrolled it runs once a tile and waits for its own instructions, 346 -> 400 us for 8192 x
+    // 12288 x 4096 in E4M3.  More rows ahead than the next four change nothing.)
+    Rows l[2] = {};
+    each<2>([&](auto b) { each<4>([&](auto t) { l[b.value].scale[t.value] = 1.0f; }); });
+    if (v0 < a.n) {
+        rows_at(l[0], 0u);
+        last_at(0u);
+    }
+    __syncthreads();   // (the stages' place is the epilogue's)
+    auto spread = [&](auto h) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        each<32>([&](auto b) {
+            constexpr int i = b.value / 16, e = b.value / 8 % 2, j = b.value / 4 % 2, q = b.value % 4;
+            const f32x16& c = acc[h.value][i][e][j];
+            const uint32_t piece = (uint32_t)(e * 16 + j * 8 + q * 2) + ((lane >> 5) ^ (uint32_t)e);
+            *reinterpret_cast<f32x4*>(mine + ((uint32_t)(i * 32) + lane % 32u) * ROW + piece * 4u) =
+                f32x4{c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]};
+        });
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    spread(Constant<0>{});
+#pragma unroll 1
+    for (uint32_t turn = 0; turn < 32u; turn += 4u) {
+        if (turn == 16u) {
+            spread(Constant<1>{});
+        }
+        if (v0 < a.n) {
+            rows_at(l[1], min(turn + 4u, 28u));
+            if (a.act != LILY_ACT_GELU) {
+                give(l[0], turn, Constant<0>{}, Constant<4>{});
+            } else {   // (some eighty instructions a value)
+                each<4>([&](auto t) { give(l[0], turn, t, Constant<1>{}); });
+            }
+            l[0] = l[1];
+            last_at(min(turn + 4u, 28u));
+        }
+    }
+}
+
+// The epilogue of the smaller tiles.
+template <class T>
+__device__ __forceinline__ void give_quarters(const ProjectArgs& a, const typename Block<T::S>::Sums (&acc)[2][T::MH][2][T::NH], char* lds,
+                                              uint32_t m0, uint32_t n0, uint32_t wave, uint32_t lane, uint32_t split) {
+    constexpr int MH = T::MH, NH = T::NH, S = T::S;
+    const uint32_t wm = wave / T::WN, wn = wave % T::WN, r_in = lane % (uint32_t)S;
+    // A quarter at a time through the wave's own part of LDS, so that a lane ends with four neighbouring
+    // outputs and NH * S / 4 lanes with a row's: whole lines are stored.  What the next quarter's epilogue reads is on its
+    // way meanwhile (nothing else hides it where the tile fills a compute unit: 8192 x 12288 x 4096 in E4M3 with a
+    // residual 572 us without).
+    constexpr int ROW = NH * S + 4;   // floats of a row there (a step of four banks from row to row)
+    static_assert(4 * MH * S * ROW * 4 <= T::LDS_BYTES, "a quarter of every wave");
+    constexpr int LANES = NH * S / 4, AT_ONCE = 64 / LANES;                     // lanes of a row, rows at once
+    constexpr int TURNS = MH * S / AT_ONCE, BATCH = TURNS < 8 ? TURNS : 8, BATCHES = TURNS / BATCH;
+    float* mine = reinterpret_cast<float*>(lds) + wave * (uint32_t)(MH * S * ROW);
+    const uint32_t column = (lane % LANES) * 4u;
+    auto output_of = [&](int qd) { return n0 + wn * (uint32_t)(T::NT * S) + (uint32_t)((qd & 1) * NH * S) + column; };
+    auto row_of = [&](int qd) { return m0 + wm * (uint32_t)(T::MT * S) + (uint32_t)((qd >> 1) * MH * S) + lane / LANES; };
+    const bool batches = a.splits == 1u && a.act != LILY_ACT_GELU;
+    Columns columns[2];
+    Finish<BATCH> finish[2][BATCHES];
+    auto ahead = [&](auto which) {
+        constexpr int qd = decltype(which)::value;
+        if (batches && output_of(qd) < a.n) {
+            columns[qd & 1].load(a, output_of(qd));
+#pragma unroll
+            for (int b = 0; b < BATCHES; ++b) {
+                finish[qd & 1][b].load(a, row_of(qd) + (uint32_t)(b * BATCH * AT_ONCE), AT_ONCE, output_of(qd));
+            }
+        }
+    };
+    auto give = [&](auto which) {
+        constexpr int qd = decltype(which)::value, h = qd >> 1, e = qd & 1;
+#pragma unroll
+        for (int i = 0; i < MH; ++i) {
+#pragma unroll
+            for (int j = 0; j < NH; ++j) {
+*reinterpret_cast<f32x4*>(mine + ((uint32_t)(i * S) + r_in) * ROW + j * S + (lane >> 4) * 4u) = acc[h][i][e][j];
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if constexpr (qd < 3) {
+            ahead(Constant<qd + 1>{});
+        }
+        const uint32_t v = output_of(qd), r0 = row_of(qd);
+        const float* from = mine + (lane / LANES) * ROW + column;
+        if (v >= a.n) {
+        } else if (batches) {
+#pragma unroll
+            for (int b = 0; b < BATCHES; ++b) {
+                f32x4 sums[BATCH];
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    sums[k] = *reinterpret_cast<const f32x4*>(from + (b * BATCH + k) * AT_ONCE * ROW);
+                }
+                finish[qd & 1][b].store(a, r0 + (uint32_t)(b * BATCH * AT_ONCE), AT_ONCE, v, columns[qd & 1], sums);
+            }
+        } else if (a.splits > 1u) {   // a part's sums as they are; k_project_join does the rest
+            for (uint32_t q = 0; q < TURNS; ++q) {
+                const uint32_t r = r0 + q * AT_ONCE;
+                if (r < a.rows) {
+                    *(LILY_GLOBAL f32x4*)(a.part + ((uint64_t)split * a.rows + r) * part_stride(a.n) + v) =
+                        *reinterpret_cast<const f32x4*>(from + q * AT_ONCE * ROW);
+                }
+            }
+        } else {   // (GELU: a row at a time)
+            Columns c;
+            c.load(a, v);
+            for (uint32_t q = 0; q < TURNS; ++q) {
+                const uint32_t r = r0 + q * AT_ONCE;
+                if (r < a.rows) {
+                    const f32x4 sum[1] = {*reinterpret_cast<const f32x4*>(from + q * AT_ONCE * ROW)};
+                    Finish<1> f;
+                    f.load(a, r, 1u, v);
+                    f.store(a, r, 1u, v, c, sum);
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    ahead(Constant<0>{});
+    give(Constant<0>{});
+    give(Constant<1>{});
+    give(Constant<2>{});
+    give(Constant<3>{});
+}
 
 template <Products P, class T>
 __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const ProjectArgs a, uint32_t m_tiles, uint32_t n_tiles) {
@@ -301,100 +555,40 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
         read_w(0, 0, k);
     }
     uint32_t s = 0;
+    // The residual's lines are asked for, to nobody's use, ten stages before the epilogue reads them: all tiles read and write
+    // at once there, and what comes from memory then is waited for (8192 x 4096 x 4096 bf16 with bias, SiLU and residual
+    // 254 us without, 249 at the tile's beginning, 245 so).  What they fetch goes to a place of LDS that only the epilogue has
+    // a use for, behind the last stages' wait for every load; the waits before count them as loads, and so wait for more.
+    constexpr uint32_t TOUCH = 10;
+    const bool touches = a.residual != nullptr && m0 + (uint32_t)T::BM <= a.rows && n0 + (uint32_t)T::BN <= a.n;
+    auto touch = [&] {
+        static_assert(T::STAGES + 1024 <= T::LDS_BYTES || S != 32, "a place for them");
+        const uint32_t e = a.residual_bf16 ? 2u : 4u, lines = e;   // lines of a wave's 128 outputs of a row
+        for (uint32_t k = 0; k < 2u * lines; ++k) {
+            const uint32_t at = k * 64u + lane, row = m0 + wm * 128u + at / lines;
+            const char* p = static_cast<const char*>(a.residual) + ((uint64_t)row * a.residual_stride + n0 + wn * 128u) * e + at % lines * LINE;
+            __builtin_amdgcn_global_load_lds((gptr)p, (lptr)(lds + T::STAGES + wave * 256u), 4, 0, 0);
+        }
+    };
+    const uint32_t touch_at = steps > TOUCH ? (steps - TOUCH) / DEPTH * DEPTH : 0u;
     for (; s + 2u * DEPTH < steps; s += DEPTH) {   // (what these ask for is whole: the stage that d may end in is a later one)
         stages(s, Constant<1>{});
+        if constexpr (S == 32) {
+            if (s == touch_at && touches) {
+                touch();
+            }
+        }
     }
     for (; s < steps; s += DEPTH) {
         stages(s, Constant<0>{});
     }
-    __syncthreads();   // (the stages' place is the epilogue's)
-
-    // A quarter at a time through the wave's own part of LDS, so that a lane ends with four neighbouring
-    // outputs and NH * S / 4 lanes with a row's: whole lines are stored.  What the next quarter's epilogue reads is on its
-    // way meanwhile (nothing else hides it where the tile fills a compute unit: 8192 x 12288 x 4096 in E4M3 with a
-    // residual 572 us without).
-    constexpr int ROW = NH * S + 4;   // floats of a row there (a step of four banks from row to row)
-    static_assert(4 * MH * S * ROW * 4 <= T::LDS_BYTES, "a quarter of every wave");
-    constexpr int LANES = NH * S / 4, AT_ONCE = 64 / LANES;                     // lanes of a row, rows at once
-    constexpr int TURNS = MH * S / AT_ONCE, BATCH = TURNS < 8 ? TURNS : 8, BATCHES = TURNS / BATCH;
-    float* mine = reinterpret_cast<float*>(lds) + wave * (uint32_t)(MH * S * ROW);
-    const uint32_t column = (lane % LANES) * 4u;
-    auto output_of = [&](int qd) { return n0 + wn * (uint32_t)(T::NT * S) + (uint32_t)((qd & 1) * NH * S) + column; };
-    auto row_of = [&](int qd) { return m0 + wm * (uint32_t)(T::MT * S) + (uint32_t)((qd >> 1) * MH * S) + lane / LANES; };
-    const bool batches = a.splits == 1u && a.act != LILY_ACT_GELU;
-    Columns columns[2];
-    Finish<BATCH> finish[2][BATCHES];
-    auto ahead = [&](auto which) {
-        constexpr int qd = decltype(which)::value;
-        if (batches && output_of(qd) < a.n) {
-            columns[qd & 1].load(a, output_of(qd));
-#pragma unroll
-            for (int b = 0; b < BATCHES; ++b) {
-                finish[qd & 1][b].load(a, row_of(qd) + (uint32_t)(b * BATCH * AT_ONCE), AT_ONCE, output_of(qd));
-            }
-        }
-    };
-    auto give = [&](auto which) {
-        constexpr int qd = decltype(which)::value, h = qd >> 1, e = qd & 1;
-#pragma unroll
-        for (int i = 0; i < MH; ++i) {
-#pragma unroll
-            for (int j = 0; j < NH; ++j) {
-#pragma unroll
-                for (int q = 0; q < Operand::GROUPS; ++q) {
-                    const Sums& c = acc[h][i][e][j];
-                    *reinterpret_cast<f32x4*>(mine + ((uint32_t)(i * S) + r_in) * ROW + j * S + Operand::output(lane, q)) =
-                        f32x4{c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]};
-                }
-            }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        if constexpr (qd < 3) {
-            ahead(Constant<qd + 1>{});
-        }
-        const uint32_t v = output_of(qd), r0 = row_of(qd);
-        const float* from = mine + (lane / LANES) * ROW + column;
-        if (v >= a.n) {
-        } else if (batches) {
-#pragma unroll
-            for (int b = 0; b < BATCHES; ++b) {
-                f32x4 sums[BATCH];
-#pragma unroll
-                for (int k = 0; k < BATCH; ++k) {
-                    sums[k] = *reinterpret_cast<const f32x4*>(from + (b * BATCH + k) * AT_ONCE * ROW);
-                }
-                finish[qd & 1][b].store(a, r0 + (uint32_t)(b * BATCH * AT_ONCE), AT_ONCE, v, columns[qd & 1], sums);
-            }
-        } else if (a.splits > 1u) {   // a part's sums as they are; k_project_join does the rest
-            for (uint32_t q = 0; q < TURNS; ++q) {
-                const uint32_t r = r0 + q * AT_ONCE;
-                if (r < a.rows) {
-                    *(LILY_GLOBAL f32x4*)(a.part + ((uint64_t)split * a.rows + r) * part_stride(a.n) + v) =
-                        *reinterpret_cast<const f32x4*>(from + q * AT_ONCE * ROW);
-                }
-            }
-        } else {   // (GELU: a row at a time)
-            Columns c;
-            c.load(a, v);
-            for (uint32_t q = 0; q < TURNS; ++q) {
-                const uint32_t r = r0 + q * AT_ONCE;
-                if (r < a.rows) {
-                    const f32x4 sum[1] = {*reinterpret_cast<const f32x4*>(from + q * AT_ONCE * ROW)};
-                    Finish<1> f;
-                    f.load(a, r, 1u, v);
-                    f.store(a, r, 1u, v, c, sum);
-                }
-            }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-    };
-    ahead(Constant<0>{});
-    give(Constant<0>{});
-    give(Constant<1>{});
-    give(Constant<2>{});
-    give(Constant<3>{});
+    if constexpr (S == 32) {
+        give_halves<T>(a, acc, lds, m0 + wm * (uint32_t)(T::MT * S), n0 + wn * (uint32_t)(T::NT * S), wave, lane);
+        return;
+    } else {
+        __syncthreads();   // (the stages' place is the epilogue's)
+        give_quarters<T>(a, acc, lds, m0, n0, wave, lane, split);
+    }
 }
 
 // The parts of d joined: a thread adds four neighbouring outputs of a row over the parts, in order, and finishes them.

@@ -252,3 +252,33 @@ def test_what_the_python_mirror_refuses(sampler):
 @pytest.mark.parametrize("dtype, out", [("bf16", "bf16"), ("e4m3", "bf16"), ("e4m3", "f32")])
 def test_parts_of_the_rows(sampler, rows, n, d, dtype, out):
     _run(sampler, rows, n, d, dtype, out, "gelu_tanh", "bf16", "bf16")
+
+
+# the large tile's epilogue: whole and ragged tiles, every residual and activation, odd strides, in place
+@pytest.mark.parametrize("rows, n, d, start", [(2048, 4096, 2048, 0), (2051, 4100, 1040, 3)])
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("out, act, bias, residual, scales", [
+    ("bf16", "gelu", "f32", "bf16", True), ("f32", "gelu", None, "f32", False), ("f32", "gelu_tanh", "bf16", "f32", True),
+    ("bf16", "silu", "bf16", "f32", False), ("f32", "relu", "f32", "bf16", True), ("f32", "none", None, None, False),
+    ("bf16", "none", None, None, True),
+])
+def test_the_large_tile_s_epilogue(sampler, rows, n, d, start, dtype, out, act, bias, residual, scales):
+    if dtype == "e4m3":
+        scales = True   # (the bound of the 8-bit products asks for them)
+    _run(sampler, rows, n, d, dtype, out, act, bias, residual, scales, start=start)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_a_large_product_in_place_of_the_residual(sampler, dtype):
+    g = torch.Generator(device=dev())
+    g.manual_seed(8)
+    x, w = _rows(g, 2048, 2048, "bf16")[1], _rows(g, 4096, 2048, "bf16", 0, 0.02)[1]
+    res = _rows(g, 2048, 4096, dtype)[1]
+    want, tol = _formula(x, w, None, None, None, "silu", res)
+    apart = torch.empty_like(res)
+    torch.cuda.synchronize()
+    sampler.project(x, w, apart, activation="silu", residual=res)
+    sampler.project(x, w, res, activation="silu", residual=res)
+    sampler.synchronize()
+    _check(res, want, tol)
+    assert torch.equal(apart, res)
