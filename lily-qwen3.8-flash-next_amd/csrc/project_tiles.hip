@@ -1,7 +1,7 @@
 // project_tiles.hip - the matrix product with an epilogue for more rows: tiles on the matrix cores.
 //
-// Four waves share a tile of rows x outputs, each a block of MT x NT products of 16 x 16.  d goes by stages of
-// 128 bytes a row.  A wave's block is taken in quarters, two halves of its rows against two halves of its
+// Four waves share a tile of rows x outputs, each MT x NT blocks of 16 x 16 or, in the large tile, 32 x 32.  d goes by
+// stages of 128 bytes a row.  A wave's block is taken in quarters, two halves of its rows against two halves of its
 // outputs, so that half the operands a stage needs are in registers while the other half is on its way
 // from LDS:
 //
@@ -18,6 +18,11 @@
 //
 // A staged row's eight pieces change places by the row's number (piece ^ (row / 2) % 8): the 16 lanes that
 // read one piece of 16 rows then meet 16 different groups of banks.
+//
+// Measured (cycles of a 256 x 256 tile, 8192 x 4096 x 4096 in bf16): 4 300 until the first stage is there, 146 000 for 64
+// stages, of which the matrix pipe is busy 131 000, and the epilogue, in which all compute units write at once.  224 us, 1.23
+// PFLOP/s, at 1.8 GHz (the clock follows the power the products take; a large library product runs at 1.59 PFLOP/s);
+// 8192 x 8192 x 8192 808 us, 1.36; 8192 x 12 288 x 4096 in E4M3 339 us, 2.43 (3.21).
 #include <utility>
 
 #include "launch.h"
