@@ -87,9 +87,27 @@ __device__ __forceinline__ f32x4 product(const Frag& w, const Frag& x, f32x4 c) 
 }
 
 // The activations, f32.  The reciprocal is the hardware's (1 ulp); none of the forms cancels: GELU's
-// tail comes from erfc, the other two are v times a logistic function.
+// tail is formed by itself, the other two are v times a logistic function.
 __device__ __forceinline__ float logistic(float v) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * v));
+}
+// The normal distribution's tail beyond |v|, exp(-v^2 / 2) t Q(t) with t = 1 / (1 + 0.36 |v|): Q is the polynomial of degree 9
+// that is nearest to exp(v^2 / 2) Phi(-|v|) / t relatively, over |v| <= 14.5, where the tail leaves the numbers (a least-squares fit on
+// Chebyshev points, its weights raised where it is worst: 2e-8).  With its roundings within (8 + v^2) 2^-24 of the tail.
+// 26 operations a value where erfc takes some eighty: 8192 x 4096 x 4096 bf16 266 us with that, a row at a time.
+__device__ __forceinline__ float tail_beyond(float v) {
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.36f, fabsf(v), 1.0f));
+    float q = 0.010566466f;
+    q = __builtin_fmaf(q, t, -0.084390737f);
+    q = __builtin_fmaf(q, t, 0.25836042f);
+    q = __builtin_fmaf(q, t, -0.36961335f);
+    q = __builtin_fmaf(q, t, 0.21752089f);
+    q = __builtin_fmaf(q, t, -0.053044252f);
+    q = __builtin_fmaf(q, t, 0.11190969f);
+    q = __builtin_fmaf(q, t, 0.12111426f);
+    q = __builtin_fmaf(q, t, 0.14397095f);
+    q = __builtin_fmaf(q, t, 0.14360565f);
+    return __builtin_amdgcn_exp2f(v * v * -0.72134752f) * (t * q);
 }
 template <int N>
 __device__ __forceinline__ void activate(float (&v)[N], uint32_t act) {   // (one branch for all of them)
@@ -98,10 +116,11 @@ __device__ __forceinline__ void activate(float (&v)[N], uint32_t act) {   // (on
         for (int j = 0; j < N; ++j) {
             v[j] *= logistic(v[j]);
         }
-    } else if (N <= 8 && act == LILY_ACT_GELU) {   // (some eighty instructions a value: a row at a time only)
+    } else if (act == LILY_ACT_GELU) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            v[j] = 0.5f * v[j] * erfcf(-0.70710678118654752f * v[j]);
+            const float tail = tail_beyond(v[j]);
+            v[j] *= v[j] > 0.0f ? 1.0f - tail : tail;
         }
     } else if (act == LILY_ACT_GELU_TANH) {
 #pragma unroll

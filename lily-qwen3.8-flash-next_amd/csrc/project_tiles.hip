@@ -175,32 +175,31 @@ __device__ __forceinline__ void give_halves(const ProjectArgs& a, const f32x16 (
         }
     };
     const uint32_t at = lane / 16u * ROW + ((lane % 16u * 2u) ^ (lane % 16u >> 3)) * 4u, other = (lane % 16u >> 3) != 0u ? (uint32_t)-4 : 4u;
-    // N rows r0 + 4 (turn + first), + 4, ...: their sums lie from row `from` of the half on
-    auto give = [&](const Rows& l, uint32_t turn, auto first, auto rows) {
-        constexpr int F = decltype(first)::value, N = decltype(rows)::value;
-        float v[8 * N];
-        each<N>([&](auto t) {
-            const float* p = mine + ((turn + F + t.value) % 16u * 4u) * ROW + at;
+    // rows r0 + 4 turn, + 4, + 8, + 12
+    auto give = [&](const Rows& l, uint32_t turn) {
+        float v[32];
+        each<4>([&](auto t) {
+            const float* p = mine + ((turn + t.value) % 16u * 4u) * ROW + at;
             const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + (int32_t)other);
             each<8>([&](auto k) {
                 const float sum = k.value < 4 ? x[k.value % 4] : y[k.value % 4];
-                v[t.value * 8 + k.value] = sum * l.scale[F + t.value] * scale[k.value] + lilym_bits_f32(raw[k.value]);
+                v[t.value * 8 + k.value] = sum * l.scale[t.value] * scale[k.value] + lilym_bits_f32(raw[k.value]);
             });
         });
         activate(v, a.act);
         if (a.residual != nullptr && a.residual_bf16) {
-            each<8 * N>([&](auto e) {
-                const uint32_t w = l.lo[F + e.value / 8][e.value % 8 / 2];
+            each<32>([&](auto e) {
+                const uint32_t w = l.lo[e.value / 8][e.value % 8 / 2];
                 v[e.value] += lilym_bits_f32((e.value & 1) ? w & 0xffff0000u : w << 16);
             });
         } else if (a.residual != nullptr) {
-            each<8 * N>([&](auto e) {
-                v[e.value] += lilym_bits_f32(e.value % 8 < 4 ? l.lo[F + e.value / 8][e.value % 4] : hi[F + e.value / 8][e.value % 4]);
+            each<32>([&](auto e) {
+                v[e.value] += lilym_bits_f32(e.value % 8 < 4 ? l.lo[e.value / 8][e.value % 4] : hi[e.value / 8][e.value % 4]);
             });
         }
-        each<N>([&](auto t) {
+        each<4>([&](auto t) {
             constexpr int e = t.value * 8;
-            const uint32_t r = r0 + (turn + F + t.value) * 4u;
+            const uint32_t r = r0 + (turn + t.value) * 4u;
             if (r < a.rows) {
                 const uint64_t to = (uint64_t)r * a.out_stride + v0;
                 if (!whole) {
@@ -254,11 +253,7 @@ __device__ __forceinline__ void give_halves(const ProjectArgs& a, const f32x16 (
         }
         if (v0 < a.n) {
             rows_at(l[1], min(turn + 4u, 28u));
-            if (a.act != LILY_ACT_GELU) {
-                give(l[0], turn, Constant<0>{}, Constant<4>{});
-            } else {   // (some eighty instructions a value)
-                each<4>([&](auto t) { give(l[0], turn, t, Constant<1>{}); });
-            }
+            give(l[0], turn);
             l[0] = l[1];
             last_at(min(turn + 4u, 28u));
         }
@@ -283,7 +278,7 @@ __device__ __forceinline__ void give_quarters(const ProjectArgs& a, const typena
     const uint32_t column = (lane % LANES) * 4u;
     auto output_of = [&](int qd) { return n0 + wn * (uint32_t)(T::NT * S) + (uint32_t)((qd & 1) * NH * S) + column; };
     auto row_of = [&](int qd) { return m0 + wm * (uint32_t)(T::MT * S) + (uint32_t)((qd >> 1) * MH * S) + lane / LANES; };
-    const bool batches = a.splits == 1u && a.act != LILY_ACT_GELU;
+    const bool batches = a.splits == 1u;
     Columns columns[2];
     Finish<BATCH> finish[2][BATCHES];
     auto ahead = [&](auto which) {
@@ -323,24 +318,12 @@ __device__ __forceinline__ void give_quarters(const ProjectArgs& a, const typena
                 }
                 finish[qd & 1][b].store(a, r0 + (uint32_t)(b * BATCH * AT_ONCE), AT_ONCE, v, columns[qd & 1], sums);
             }
-        } else if (a.splits > 1u) {   // a part's sums as they are; k_project_join does the rest
+        } else {   // a part's sums as they are; k_project_join does the rest
             for (uint32_t q = 0; q < TURNS; ++q) {
                 const uint32_t r = r0 + q * AT_ONCE;
                 if (r < a.rows) {
                     *(LILY_GLOBAL f32x4*)(a.part + ((uint64_t)split * a.rows + r) * part_stride(a.n) + v) =
                         *reinterpret_cast<const f32x4*>(from + q * AT_ONCE * ROW);
-                }
-            }
-        } else {   // (GELU: a row at a time)
-            Columns c;
-            c.load(a, v);
-            for (uint32_t q = 0; q < TURNS; ++q) {
-                const uint32_t r = r0 + q * AT_ONCE;
-                if (r < a.rows) {
-                    const f32x4 sum[1] = {*reinterpret_cast<const f32x4*>(from + q * AT_ONCE * ROW)};
-                    Finish<1> f;
-                    f.load(a, r, 1u, v);
-                    f.store(a, r, 1u, v, c, sum);
                 }
             }
         }

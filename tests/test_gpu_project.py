@@ -4,8 +4,9 @@ Bar, derived from the arithmetic (u = 2^-24): with S = sum |x_i w_i| * xs * ws o
 products is within (d + 16) u S in any order of addition (bf16 and E4M3 products are exact in f32; up to 16
 parts are joined); the scales, the bias and the residual round once each, at most 2 u (S + |bias|) and u of the
 result; an activation moves an error of its argument by at most 1.13 (the largest slope of the four) and
-adds 8 u of its value (exponential, reciprocal, erfc of ocml: 4 ulp) - its exponent's rounding costs |v| u of the
-part that the logistic function still turns, at most 2 u |v|.  Together
+adds 8 u of its value (exponential, reciprocal; GELU's tail is within (8 + v^2) u of itself, and v^2 u |v| Phi(-|v|)
+is below u |v| / 10) - its exponent's rounding costs |v| u of the part that the logistic function still turns, at most
+2 u |v|.  Together
     tol = 1.13 ((d + 24) u S + 4 u |bias|) + 12 u |act| + 2 u |out|   and, for bf16, 2^-8 |out| more.
 
 E4M3 operands with a bf16 output go through the matrix cores' 8-bit products from 17 rows on, which cut each of
@@ -282,3 +283,30 @@ def test_a_large_product_in_place_of_the_residual(sampler, dtype):
     sampler.synchronize()
     _check(res, want, tol)
     assert torch.equal(apart, res)
+
+
+@pytest.mark.parametrize("rows, n, out_dtype", [(1, 200000, "f32"), (100, 20000, "f32"), (2048, 8192, "f32"), (20, 20000, "bf16")])
+def test_gelu_over_its_range(sampler, rows, n, out_dtype):
+    """Rows of zeros, so that the bias is the argument.  With the tail Phi(-|v|) formed within (8 + v^2) u of itself: below
+    zero the product rounds once more, (9 + v^2) u of the result; above, 1 - tail is within (8 + v^2) u of the tail and one
+    rounding, and the product one more.  Where the tail leaves the normal numbers (v < -13) it may be 2^-126 off."""
+    v = torch.cat([torch.linspace(-14, 14, n - 2000, dtype=torch.float64), torch.logspace(-30, 0, 1000, dtype=torch.float64),
+                   -torch.logspace(-30, 0, 1000, dtype=torch.float64)]).float().to(dev())
+    v[7], v[8], v[9], v[10] = 0.0, -0.0, 1e30, float("inf")
+    x = torch.zeros(rows, 64, dtype=torch.bfloat16, device=dev())
+    w = torch.ones(n, 64, dtype=torch.bfloat16, device=dev())
+    out = torch.empty(rows, n, dtype=DT[out_dtype], device=dev())
+    torch.cuda.synchronize()
+    sampler.project(x, w, out, bias=v, activation="gelu")
+    sampler.synchronize()
+    d = v.double()
+    # (by erfc on the host, which keeps the tail: Phi(-12.95) is 1.2e-38, and not 0)
+    low = (0.5 * torch.special.erfc(d.abs().cpu() * math.sqrt(0.5))).to(dev())
+    want, tail = d * torch.where(d > 0, 1.0 - low, low), low
+    want[8], want[10] = 0.0, float("inf")
+    near = 8 + d.square().clamp_max(1e4)
+    tol = torch.where(d < 0, (near + 1) * U * want.abs(), d.abs() * U * (near * tail + 2)) + 2.0 ** -126 * d.abs().clamp_max(100.0)
+    if out_dtype == "bf16":
+        tol = tol + 2.0 ** -8 * want.abs()
+    ok = ((out.double() - want).abs() <= tol) | (out.double() == want)
+    assert bool(ok.all()), (v[~ok.all(0)][:5], out[:, ~ok.all(0)][0, :5], want[~ok.all(0)][:5])
