@@ -171,84 +171,54 @@ typedef pj_u32x2 pj_u32x2_any __attribute__((aligned(2)));
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 typedef u32x4 pj_u32x4_any __attribute__((aligned(4)));
 
-// N rows r0, r0 + step, ... (those below a.rows count) of columns v0 .. v0 + 3 (v0 < n): load() asks for what the
-// epilogue reads of them, store() finishes their sums.
-template <int N>
+// Row r (r < rows) of columns v0 .. v0 + 3 (v0 < n): load() asks for what the epilogue reads of it, store() finishes
+// its sums.
 struct Finish {
-    float scale[N];
-    u32x4 res[N];   // two bf16 a word, or f32
-    __device__ __forceinline__ void load(const ProjectArgs& a, uint32_t r0, uint32_t step, uint32_t v0) {
-        const uint32_t top = a.rows - 1u;
-        const bool whole = v0 + 4u <= a.n;
+    float scale;
+    u32x4 res;   // two bf16 a word, or f32
+    __device__ __forceinline__ void load(const ProjectArgs& a, uint32_t r, uint32_t v0) {
         if (a.x_scales != nullptr) {
-#pragma unroll
-            for (int q = 0; q < N; ++q) {
-                scale[q] = gload(a.x_scales + min(r0 + (uint32_t)q * step, top));
-            }
+            scale = gload(a.x_scales + r);
         }
-        if (a.residual != nullptr) {
-#pragma unroll
-            for (int q = 0; q < N; ++q) {
-                const uint64_t from = (uint64_t)min(r0 + (uint32_t)q * step, top) * a.residual_stride + v0;
-                if (whole && a.residual_bf16) {
-                    const pj_u32x2 t = *(const LILY_GLOBAL pj_u32x2_any*)(static_cast<const uint16_t*>(a.residual) + from);
-                    res[q] = u32x4{t.x, t.y, 0u, 0u};
-                } else if (whole) {
-                    res[q] = *(const LILY_GLOBAL pj_u32x4_any*)(static_cast<const uint32_t*>(a.residual) + from);
-                } else {
-                    uint32_t t[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint64_t at = from + min((uint32_t)j, a.n - 1u - v0);
-                        t[j] = a.residual_bf16 ? (uint32_t)gload(static_cast<const uint16_t*>(a.residual) + at)
-                                               : gload(static_cast<const uint32_t*>(a.residual) + at);
-                    }
-                    res[q] = a.residual_bf16 ? u32x4{t[0] | t[1] << 16, t[2] | t[3] << 16, 0u, 0u} : u32x4{t[0], t[1], t[2], t[3]};
-                }
-            }
+        if (a.residual == nullptr) {
+            return;
         }
-    }
-    __device__ __forceinline__ float residual(const ProjectArgs& a, int q, int j) const {
-        const u32x4 w = res[q];
-        const uint32_t half = (j & 1) ? w[j / 2] & 0xffff0000u : w[j / 2] << 16;
-        return lilym_bits_f32(a.residual_bf16 ? half : w[j]);
-    }
-    __device__ __forceinline__ void store(const ProjectArgs& a, uint32_t r0, uint32_t step, uint32_t v0, const Columns& c,
-                                          const f32x4 (&sums)[N]) const {
-        float v[4 * N];
-#pragma unroll
-        for (int q = 0; q < N; ++q) {
+        const uint64_t from = (uint64_t)r * a.residual_stride + v0;
+        if (v0 + 4u <= a.n && a.residual_bf16) {
+            const pj_u32x2 t = *(const LILY_GLOBAL pj_u32x2_any*)(static_cast<const uint16_t*>(a.residual) + from);
+            res = u32x4{t.x, t.y, 0u, 0u};
+        } else if (v0 + 4u <= a.n) {
+            res = *(const LILY_GLOBAL pj_u32x4_any*)(static_cast<const uint32_t*>(a.residual) + from);
+        } else {
+            uint32_t t[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float t = a.x_scales != nullptr ? sums[q][j] * scale[q] : sums[q][j];
-                v[4 * q + j] = t * c.scale[j] + c.bias(a, j);
+                const uint64_t at = from + min((uint32_t)j, a.n - 1u - v0);
+                t[j] = a.residual_bf16 ? (uint32_t)gload(static_cast<const uint16_t*>(a.residual) + at)
+                                       : gload(static_cast<const uint32_t*>(a.residual) + at);
             }
+            res = a.residual_bf16 ? u32x4{t[0] | t[1] << 16, t[2] | t[3] << 16, 0u, 0u} : u32x4{t[0], t[1], t[2], t[3]};
+        }
+    }
+    __device__ __forceinline__ void store(const ProjectArgs& a, uint32_t r, uint32_t v0, const Columns& c, f32x4 sum) const {
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float t = a.x_scales != nullptr ? sum[j] * scale : sum[j];
+            v[j] = t * c.scale[j] + c.bias(a, j);
         }
         activate(v, a.act);
         if (a.residual != nullptr) {
 #pragma unroll
-            for (int e = 0; e < 4 * N; ++e) {
-                v[e] += residual(a, e / 4, e % 4);
-            }
-        }
-#pragma unroll
-        for (int q = 0; q < N; ++q) {
-            const uint32_t r = r0 + (uint32_t)q * step;
-            if (r < a.rows) {
-                store_row(a, (uint64_t)r * a.out_stride + v0, v0, f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]});
-            }
-        }
-    }
-    static __device__ __forceinline__ void store_row(const ProjectArgs& a, uint64_t at, uint32_t v0, f32x4 v) {
-        if (v0 + 4u <= a.n) {
-            if (a.out_bf16) {
-                *(LILY_GLOBAL pj_u32x2_any*)(static_cast<uint16_t*>(a.out) + at) = pj_u32x2{pj_bf16_pair(v[0], v[1]), pj_bf16_pair(v[2], v[3])};
-            } else {
-                *(LILY_GLOBAL f32x4_any*)(static_cast<float*>(a.out) + at) = v;
-            }
-        } else {
-#pragma unroll
             for (int j = 0; j < 4; ++j) {
+                const uint32_t half = (j & 1) ? res[j / 2] & 0xffff0000u : res[j / 2] << 16;
+                v[j] += lilym_bits_f32(a.residual_bf16 ? half : res[j]);
+            }
+        }
+        const uint64_t at = (uint64_t)r * a.out_stride + v0;
+        if (v0 + 4u > a.n) {
+#pragma unroll
+            for (int j = 0; j < 3; ++j) {
                 if (v0 + (uint32_t)j < a.n) {
                     if (a.out_bf16) {
                         *(LILY_GLOBAL uint16_t*)(static_cast<uint16_t*>(a.out) + at + j) = (uint16_t)pj_bf16_pair(v[j], 0.0f);
@@ -257,6 +227,10 @@ struct Finish {
                     }
                 }
             }
+        } else if (a.out_bf16) {
+            *(LILY_GLOBAL pj_u32x2_any*)(static_cast<uint16_t*>(a.out) + at) = pj_u32x2{pj_bf16_pair(v[0], v[1]), pj_bf16_pair(v[2], v[3])};
+        } else {
+            *(LILY_GLOBAL f32x4_any*)(static_cast<float*>(a.out) + at) = f32x4{v[0], v[1], v[2], v[3]};
         }
     }
 };

@@ -35,11 +35,11 @@ __global__ void __launch_bounds__(WAVES * 64) k_project_few(const ProjectArgs a)
     // another trip to memory.
     const uint32_t v = v0 + g * 4u, row0 = wave * 16u + r;
     Columns columns;
-    Finish<1> finish;
+    Finish finish;
     const bool finishes = wave < (uint32_t)RT && v < a.n && row0 < a.rows;
     if (finishes) {
         columns.load(a, v);
-        finish.load(a, row0, 1u, v);
+        finish.load(a, row0, v);
     }
     // Instruction i brings rows 8 i .. 8 i + 7 of a line (16 of the weights, then x), a lane the piece that
     // belongs in its place: the pieces of a row change places by the row's number, so that 16 lanes that read one
@@ -123,12 +123,12 @@ __global__ void __launch_bounds__(WAVES * 64) k_project_few(const ProjectArgs a)
     }
     __syncthreads();
     if (finishes) {   // block `wave` of the rows
-        f32x4 sum[1] = {sums[wave * 64u + lane]};
+        f32x4 sum = sums[wave * 64u + lane];
 #pragma unroll
         for (uint32_t q = 1; q < WAVES; ++q) {
-            sum[0] += sums[(q * RT + wave) * 64u + lane];
+            sum += sums[(q * RT + wave) * 64u + lane];
         }
-        finish.store(a, row0, 1u, v, columns, sum);
+        finish.store(a, row0, v, columns, sum);
     }
 }
 

@@ -90,8 +90,11 @@ struct Tile {
     static constexpr int XR = WM * MH * S, WR = WN * NH * S;           // rows of a unit: of x, of the weights
     static constexpr int UNIT = (XR + WR) * (int)LINE;
     static constexpr int XL = XR / 32, WL = WR / 32, LOADS = XL + WL;  // loads of a wave and unit
-    static constexpr int STAGES = 2 * DEPTH * UNIT, HALVES = 4 * MH * S * (NT * S + 4) * 4;   // bytes; the epilogue's, by halves
-    static constexpr int LDS_BYTES = S == 32 && HALVES > STAGES ? HALVES : STAGES;
+    // The epilogue's: a wave's rows that lie in LDS at once (half of the large tile's), and floats of a row there (a step of
+    // four banks from row to row).
+    static constexpr int PARTS = S == 32 ? 2 : 1, PART_ROWS = MT * S / PARTS, ROW = NT * S + 4;
+    static constexpr int STAGES = 2 * DEPTH * UNIT, SPREAD = 4 * PART_ROWS * ROW * 4;   // bytes
+    static constexpr int LDS_BYTES = SPREAD > STAGES ? SPREAD : STAGES;
     static_assert(DEPTH % 2 == 0 && (2 * DEPTH - 1) * LOADS < 64, "loads in flight are counted in six bits");
     static_assert(WM * WN == 4 && XR % 32 == 0 && WR % 32 == 0, "whole loads a wave");
 };
@@ -110,26 +113,64 @@ __device__ __forceinline__ void each(F&& f) {
     each_of(f, std::make_integer_sequence<int, N>{});
 }
 
-// The epilogue of the large tile, which nothing else hides: half of a wave's rows at a time through its part of LDS, so
-// that a lane has eight neighbouring outputs and 16 lanes a row's 256 bytes of bf16.  Its outputs are the same in every
-// row: their scales and biases are read once, the rows go by a loop of few operations a value, what
-// the next four rows read is on its way meanwhile.  (Quarters of four outputs a lane, rows unrolled, took 39 000 cycles a
-// tile of bf16 without operands, a fifth of a tile with d = 4096, and 64 000 with a bias, SiLU and a residual.)
+// The epilogue: a wave's rows (of the large tile half of them at a time) through its part of LDS, so that a lane has eight
+// neighbouring outputs, and the lanes of a row store it whole (256 bytes of bf16 in the large tile, where nothing else
+// hides what an epilogue takes).  Its outputs are the same in every row: their scales and biases are read once, the rows go
+// by a loop of few operations a value, and what the next rows read is on its way meanwhile.  (Quarters of four outputs a lane,
+// rows unrolled, took 39 000 cycles a large tile of bf16 without operands, a fifth of a tile with d = 4096, and 64 000 with a
+// bias, SiLU and a residual.)
 // A row's 16-byte pieces from the 16th on change places in pairs: lanes 8 to 15 then read the groups of banks that lanes
 // 0 to 7 leave.
-struct Rows {     // what four rows read
-    float scale[4];
-    u32x4 lo[4];  // the residual as it lies in memory: eight bf16, or the first four f32
+template <int B>
+struct Rows {     // what B rows read
+    float scale[B];
+    u32x4 lo[B];  // the residual as it lies in memory: eight bf16, or the first four f32
 };
 typedef u32x4 pj_u32x4_out __attribute__((aligned(2)));
 template <class T>
-__device__ __forceinline__ void give_halves(const ProjectArgs& a, const f32x16 (&acc)[2][T::MH][2][T::NH], char* lds, uint32_t m, uint32_t n,
-                                            uint32_t wave, uint32_t lane) {
-    static_assert(T::S == 32 && T::MT == 4 && T::NT == 4, "four blocks of 32 both ways");
-    constexpr uint32_t ROW = 132;   // floats (a step of four banks from row to row)
-    float* mine = reinterpret_cast<float*>(lds) + wave * (64u * ROW);
-    const uint32_t v0 = n + lane % 16u * 8u, r0 = m + lane / 16u;
+__device__ __forceinline__ void give_out(const ProjectArgs& a, const typename Block<T::S>::Sums (&acc)[2][T::MH][2][T::NH], char* lds, uint32_t m,
+                                         uint32_t n, uint32_t wave, uint32_t lane, uint32_t split) {
+    constexpr uint32_t ROW = T::ROW, LANES = T::NT * T::S / 8, AT_ONCE = 64 / LANES, TURNS = T::MT * T::S / AT_ONCE;   // lanes of a row, rows at once
+    constexpr int B = TURNS < 4 ? TURNS : 4;                                                                         // of them a batch
+    constexpr uint32_t PART_TURNS = TURNS / T::PARTS;
+    float* mine = reinterpret_cast<float*>(lds) + wave * ((uint32_t)T::PART_ROWS * ROW);
+    const uint32_t in_row = lane % LANES, v0 = n + in_row * 8u, r0 = m + lane / LANES;
     const bool whole = v0 + 8u <= a.n;
+    auto spread = [&](auto part) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        constexpr int H = 2 / T::PARTS;   // halves of the rows
+        each<H * T::MH * 2 * T::NH>([&](auto b) {
+            constexpr int h = b.value / (T::MH * 2 * T::NH), i = b.value / (2 * T::NH) % T::MH, e = b.value / T::NH % 2, j = b.value % T::NH;
+            const auto& c = acc[part.value * H + h][i][e][j];
+            float* row = mine + ((uint32_t)((h * T::MH + i) * T::S) + lane % (uint32_t)T::S) * ROW;
+            each<T::S == 32 ? 4 : 1>([&](auto q) {   // runs of four outputs of a lane
+                const uint32_t piece = T::S == 32 ? (uint32_t)((e * T::NH + j) * 8 + q.value * 2) + ((lane >> 5) ^ (uint32_t)((e * T::NH + j) / 2))
+                                                  : (uint32_t)((e * T::NH + j) * 4) + (lane >> 4);
+                *reinterpret_cast<f32x4*>(row + piece * 4u) = f32x4{c[4 * q.value], c[4 * q.value + 1], c[4 * q.value + 2], c[4 * q.value + 3]};
+            });
+        });
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    if constexpr (T::PARTS == 1) {
+        if (a.splits > 1u) {   // a part's sums as they are; k_project_join does the rest
+            __syncthreads();   // (the stages' place is the epilogue's)
+            spread(Constant<0>{});
+#pragma unroll 4
+            for (uint32_t turn = 0; turn < TURNS; ++turn) {
+                const uint32_t r = r0 + turn * AT_ONCE;
+                each<2>([&](auto q) {
+                    const uint32_t piece = in_row + q.value * LANES, v = n + piece * 4u;
+                    if (r < a.rows && v < a.n) {
+                        *(LILY_GLOBAL f32x4*)(a.part + ((uint64_t)split * a.rows + r) * part_stride(a.n) + v) =
+                            *reinterpret_cast<const f32x4*>(mine + (turn * AT_ONCE + lane / LANES) * ROW + piece * 4u);
+                    }
+                });
+            }
+            return;
+        }
+    }
     float scale[8];
     uint32_t raw[8];   // of the bias
     each<8>([&](auto k) {
@@ -140,7 +181,7 @@ __device__ __forceinline__ void give_halves(const ProjectArgs& a, const f32x16 (
             raw[k.value] = a.bias_bf16 ? (uint32_t)gload(static_cast<const uint16_t*>(a.bias) + v) << 16 : gload(static_cast<const uint32_t*>(a.bias) + v);
         }
     });
-    // Rows r0 + 4 turn, + 4, + 8, + 12; and the residual's last four outputs in f32.
+    // Rows r0 + AT_ONCE turn and B - 1 after it; and the residual's last four outputs in f32.
     auto residual_at = [&](uint32_t r, uint32_t first) {
         const uint64_t from = (uint64_t)min(r, a.rows - 1u) * a.residual_stride + v0 + first;
         const uint16_t* half = static_cast<const uint16_t*>(a.residual) + from;
@@ -160,27 +201,28 @@ __device__ __forceinline__ void give_halves(const ProjectArgs& a, const f32x16 (
         }
         return w;
     };
-    auto rows_at = [&](Rows& l, uint32_t turn) {
+    auto rows_at = [&](Rows<B>& l, uint32_t turn) {
         if (a.x_scales != nullptr) {
-            each<4>([&](auto t) { l.scale[t.value] = gload(a.x_scales + min(r0 + (turn + t.value) * 4u, a.rows - 1u)); });
+            each<B>([&](auto t) { l.scale[t.value] = gload(a.x_scales + min(r0 + (turn + t.value) * AT_ONCE, a.rows - 1u)); });
         }
         if (a.residual != nullptr) {
-            each<4>([&](auto t) { l.lo[t.value] = residual_at(r0 + (turn + t.value) * 4u, 0u); });
+            each<B>([&](auto t) { l.lo[t.value] = residual_at(r0 + (turn + t.value) * AT_ONCE, 0u); });
         }
     };
-    u32x4 hi[4];
+    u32x4 hi[B];
     auto last_at = [&](uint32_t turn) {
         if (a.residual != nullptr && !a.residual_bf16) {
-            each<4>([&](auto t) { hi[t.value] = residual_at(r0 + (turn + t.value) * 4u, 4u); });
+            each<B>([&](auto t) { hi[t.value] = residual_at(r0 + (turn + t.value) * AT_ONCE, 4u); });
         }
     };
-    const uint32_t at = lane / 16u * ROW + ((lane % 16u * 2u) ^ (lane % 16u >> 3)) * 4u, other = (lane % 16u >> 3) != 0u ? (uint32_t)-4 : 4u;
-    // rows r0 + 4 turn, + 4, + 8, + 12
-    auto give = [&](const Rows& l, uint32_t turn) {
-        float v[32];
-        each<4>([&](auto t) {
-            const float* p = mine + ((turn + t.value) % 16u * 4u) * ROW + at;
-            const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + (int32_t)other);
+    const uint32_t turned = in_row * 2u >> 4;
+    const float* first = mine + lane / LANES * ROW + ((in_row * 2u) ^ turned) * 4u;
+    const int32_t other = turned != 0u ? -4 : 4;
+    auto give = [&](const Rows<B>& l, uint32_t turn) {
+        float v[8 * B];
+        each<B>([&](auto t) {
+            const float* p = first + ((turn + t.value) % PART_TURNS * AT_ONCE) * ROW;
+            const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + other);
             each<8>([&](auto k) {
                 const float sum = k.value < 4 ? x[k.value % 4] : y[k.value % 4];
                 v[t.value * 8 + k.value] = sum * l.scale[t.value] * scale[k.value] + lilym_bits_f32(raw[k.value]);
@@ -188,18 +230,18 @@ __device__ __forceinline__ void give_halves(const ProjectArgs& a, const f32x16 (
         });
         activate(v, a.act);
         if (a.residual != nullptr && a.residual_bf16) {
-            each<32>([&](auto e) {
+            each<8 * B>([&](auto e) {
                 const uint32_t w = l.lo[e.value / 8][e.value % 8 / 2];
                 v[e.value] += lilym_bits_f32((e.value & 1) ? w & 0xffff0000u : w << 16);
             });
         } else if (a.residual != nullptr) {
-            each<32>([&](auto e) {
+            each<8 * B>([&](auto e) {
                 v[e.value] += lilym_bits_f32(e.value % 8 < 4 ? l.lo[e.value / 8][e.value % 4] : hi[e.value / 8][e.value % 4]);
             });
         }
-        each<4>([&](auto t) {
+        each<B>([&](auto t) {
             constexpr int e = t.value * 8;
-            const uint32_t r = r0 + (turn + t.value) * 4u;
+            const uint32_t r = r0 + (turn + t.value) * AT_ONCE;
             if (r < a.rows) {
                 const uint64_t to = (uint64_t)r * a.out_stride + v0;
                 if (!whole) {
@@ -225,116 +267,39 @@ __device__ __forceinline__ void give_halves(const ProjectArgs& a, const f32x16 (
     };
     // (a loop, and one copy of it: unrolled it runs once a tile and waits for its own instructions, 346 -> 400 us for 8192 x
     // 12288 x 4096 in E4M3.  More rows ahead than the next four change nothing.)
-    Rows l[2] = {};
-    each<2>([&](auto b) { each<4>([&](auto t) { l[b.value].scale[t.value] = 1.0f; }); });
-    if (v0 < a.n) {
-        rows_at(l[0], 0u);
-        last_at(0u);
+    Rows<B> now = {}, next = {};
+    each<B>([&](auto t) { now.scale[t.value] = next.scale[t.value] = 1.0f; });
+    auto begin = [&] {
+        if (v0 < a.n) {
+            rows_at(now, 0u);
+            last_at(0u);
+        }
+    };
+    if constexpr (T::PARTS == 2) {   // (the sums are in registers of their own there; the smaller tiles' would be in the way)
+        begin();
     }
     __syncthreads();   // (the stages' place is the epilogue's)
-    auto spread = [&](auto h) {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        each<32>([&](auto b) {
-            constexpr int i = b.value / 16, e = b.value / 8 % 2, j = b.value / 4 % 2, q = b.value % 4;
-            const f32x16& c = acc[h.value][i][e][j];
-            const uint32_t piece = (uint32_t)(e * 16 + j * 8 + q * 2) + ((lane >> 5) ^ (uint32_t)e);
-            *reinterpret_cast<f32x4*>(mine + ((uint32_t)(i * 32) + lane % 32u) * ROW + piece * 4u) =
-                f32x4{c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]};
-        });
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-    };
     spread(Constant<0>{});
+    if constexpr (T::PARTS == 1) {
+        begin();
+    }
 #pragma unroll 1
-    for (uint32_t turn = 0; turn < 32u; turn += 4u) {
-        if (turn == 16u) {
-            spread(Constant<1>{});
+    for (uint32_t at = 0; at < TURNS; at += (uint32_t)B) {
+        uint32_t turn = at;
+        asm("" : "+s"(turn));   // (an address is computed where it is used: 64 that grow with the loop took 340 registers)
+        if constexpr (T::PARTS == 2) {
+            if (turn == PART_TURNS) {
+                spread(Constant<1>{});
+            }
         }
         if (v0 < a.n) {
-            rows_at(l[1], min(turn + 4u, 28u));
-            give(l[0], turn);
-            l[0] = l[1];
-            last_at(min(turn + 4u, 28u));
+            const uint32_t then = min(turn + (uint32_t)B, TURNS - (uint32_t)B);
+            rows_at(next, then);
+            give(now, turn);
+            now = next;
+            last_at(then);
         }
     }
-}
-
-// The epilogue of the smaller tiles.
-template <class T>
-__device__ __forceinline__ void give_quarters(const ProjectArgs& a, const typename Block<T::S>::Sums (&acc)[2][T::MH][2][T::NH], char* lds,
-                                              uint32_t m0, uint32_t n0, uint32_t wave, uint32_t lane, uint32_t split) {
-    constexpr int MH = T::MH, NH = T::NH, S = T::S;
-    const uint32_t wm = wave / T::WN, wn = wave % T::WN, r_in = lane % (uint32_t)S;
-    // A quarter at a time through the wave's own part of LDS, so that a lane ends with four neighbouring
-    // outputs and NH * S / 4 lanes with a row's: whole lines are stored.  What the next quarter's epilogue reads is on its
-    // way meanwhile (nothing else hides it where the tile fills a compute unit: 8192 x 12288 x 4096 in E4M3 with a
-    // residual 572 us without).
-    constexpr int ROW = NH * S + 4;   // floats of a row there (a step of four banks from row to row)
-    static_assert(4 * MH * S * ROW * 4 <= T::LDS_BYTES, "a quarter of every wave");
-    constexpr int LANES = NH * S / 4, AT_ONCE = 64 / LANES;                     // lanes of a row, rows at once
-    constexpr int TURNS = MH * S / AT_ONCE, BATCH = TURNS < 8 ? TURNS : 8, BATCHES = TURNS / BATCH;
-    float* mine = reinterpret_cast<float*>(lds) + wave * (uint32_t)(MH * S * ROW);
-    const uint32_t column = (lane % LANES) * 4u;
-    auto output_of = [&](int qd) { return n0 + wn * (uint32_t)(T::NT * S) + (uint32_t)((qd & 1) * NH * S) + column; };
-    auto row_of = [&](int qd) { return m0 + wm * (uint32_t)(T::MT * S) + (uint32_t)((qd >> 1) * MH * S) + lane / LANES; };
-    const bool batches = a.splits == 1u;
-    Columns columns[2];
-    Finish<BATCH> finish[2][BATCHES];
-    auto ahead = [&](auto which) {
-        constexpr int qd = decltype(which)::value;
-        if (batches && output_of(qd) < a.n) {
-            columns[qd & 1].load(a, output_of(qd));
-#pragma unroll
-            for (int b = 0; b < BATCHES; ++b) {
-                finish[qd & 1][b].load(a, row_of(qd) + (uint32_t)(b * BATCH * AT_ONCE), AT_ONCE, output_of(qd));
-            }
-        }
-    };
-    auto give = [&](auto which) {
-        constexpr int qd = decltype(which)::value, h = qd >> 1, e = qd & 1;
-#pragma unroll
-        for (int i = 0; i < MH; ++i) {
-#pragma unroll
-            for (int j = 0; j < NH; ++j) {
-*reinterpret_cast<f32x4*>(mine + ((uint32_t)(i * S) + r_in) * ROW + j * S + (lane >> 4) * 4u) = acc[h][i][e][j];
-            }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        if constexpr (qd < 3) {
-            ahead(Constant<qd + 1>{});
-        }
-        const uint32_t v = output_of(qd), r0 = row_of(qd);
-        const float* from = mine + (lane / LANES) * ROW + column;
-        if (v >= a.n) {
-        } else if (batches) {
-#pragma unroll
-            for (int b = 0; b < BATCHES; ++b) {
-                f32x4 sums[BATCH];
-#pragma unroll
-                for (int k = 0; k < BATCH; ++k) {
-                    sums[k] = *reinterpret_cast<const f32x4*>(from + (b * BATCH + k) * AT_ONCE * ROW);
-                }
-                finish[qd & 1][b].store(a, r0 + (uint32_t)(b * BATCH * AT_ONCE), AT_ONCE, v, columns[qd & 1], sums);
-            }
-        } else {   // a part's sums as they are; k_project_join does the rest
-            for (uint32_t q = 0; q < TURNS; ++q) {
-                const uint32_t r = r0 + q * AT_ONCE;
-                if (r < a.rows) {
-                    *(LILY_GLOBAL f32x4*)(a.part + ((uint64_t)split * a.rows + r) * part_stride(a.n) + v) =
-                        *reinterpret_cast<const f32x4*>(from + q * AT_ONCE * ROW);
-                }
-            }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-    };
-    ahead(Constant<0>{});
-    give(Constant<0>{});
-    give(Constant<1>{});
-    give(Constant<2>{});
-    give(Constant<3>{});
 }
 
 template <Products P, class T>
@@ -570,13 +535,7 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
     for (; s < steps; s += DEPTH) {
         stages(s, Constant<0>{});
     }
-    if constexpr (S == 32) {
-        give_halves<T>(a, acc, lds, m0 + wm * (uint32_t)(T::MT * S), n0 + wn * (uint32_t)(T::NT * S), wave, lane);
-        return;
-    } else {
-        __syncthreads();   // (the stages' place is the epilogue's)
-        give_quarters<T>(a, acc, lds, m0, n0, wave, lane, split);
-    }
+    give_out<T>(a, acc, lds, m0 + wm * (uint32_t)(T::MT * S), n0 + wn * (uint32_t)(T::NT * S), wave, lane, split);
 }
 
 // The parts of d joined: a thread adds four neighbouring outputs of a row over the parts, in order, and finishes them.
@@ -588,12 +547,12 @@ __global__ void __launch_bounds__(256) k_project_join(const ProjectArgs a) {
     }
     const uint32_t r = (uint32_t)(at / fours), v = (uint32_t)(at % fours) * 4u;
     Columns c;
-    Finish<1> f;
+    Finish f;
     c.load(a, v);
-    f.load(a, r, 1u, v);
+    f.load(a, r, v);
     const float* from = a.part + (uint64_t)r * part_stride(a.n) + v;
     const uint64_t next = (uint64_t)a.rows * part_stride(a.n);
-    f32x4 sum[1] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t q = 0; q < a.splits; q += 4u) {
         f32x4 p[4];
 #pragma unroll
@@ -603,11 +562,11 @@ __global__ void __launch_bounds__(256) k_project_join(const ProjectArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (q + (uint32_t)j < a.splits) {
-                sum[0] += p[j];
+                sum += p[j];
             }
         }
     }
-    f.store(a, r, 1u, v, c, sum);
+    f.store(a, r, v, c, sum);
 }
 
 template <class T>
