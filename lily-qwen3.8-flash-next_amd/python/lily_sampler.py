@@ -576,27 +576,30 @@ class Sampler:
 
 
     # -- around the head
-    def _matrix(self, t, rows, columns, name):
-        """(address, stride, type) of a [rows, columns] operand whose rows are contiguous."""
-        code, shape, stride = DTYPES.get(t.dtype), t.shape, t.stride()
-        if code is None:
-            raise SamplerError(-1, f"{name} must be F32, BF16 or E4M3, got {t.dtype}")
-        if len(shape) != 2 or shape[0] != rows or shape[1] != columns or (stride[1] != 1 and columns > 1):
-            raise SamplerError(-1, f"{name} must be [{rows}, {columns}], rows contiguous")
-        if t.get_device() != self.device:
-            raise SamplerError(-1, f"{name} must live on the sampler's device")
+    def _matrix(self, t, shape, name):
+        """(address, stride, type) of an operand of `shape` ([rows, columns]) whose rows are contiguous."""
+        code, stride = DTYPES.get(t.dtype), t.stride()
+        if code is None or t.shape != shape or stride[1] != 1 or t.get_device() != self.device:
+            self._must(code is not None, name, f"F32, BF16 or E4M3, got {t.dtype}")
+            self._must(t.shape == shape and (stride[1] == 1 or shape[1] <= 1), name, f"[{shape[0]}, {shape[1]}], rows contiguous")
+            self._must(t.get_device() == self.device, name, "on the sampler's device")
         return t.data_ptr(), stride[0], code
 
     def _vector(self, t, n, name):
         """(address, type) of a contiguous vector of n elements, or nothing."""
         if t is None:
             return None, F32
-        code, shape = DTYPES.get(t.dtype), t.shape
-        if code is None or len(shape) != 1 or shape[0] != n or (t.stride(0) != 1 and n > 1):
-            raise SamplerError(-1, f"{name} must be [{n}], contiguous")
-        if t.get_device() != self.device:
-            raise SamplerError(-1, f"{name} must live on the sampler's device")
+        code, stride = DTYPES.get(t.dtype), t.stride()
+        if code is None or stride != (1,) or t.shape[0] != n or t.get_device() != self.device:
+            self._must(code is not None and len(t.shape) == 1 and t.shape[0] == n and (stride[0] == 1 or n <= 1), name,
+                       f"[{n}], contiguous")
+            self._must(t.get_device() == self.device, name, "on the sampler's device")
         return t.data_ptr(), code
+
+    @staticmethod
+    def _must(holds, name, what):
+        if not holds:
+            raise SamplerError(-1, f"{name} must be {what}")
 
     def _scales(self, t, n, name):
         at, code = self._vector(t, n, name)
@@ -607,14 +610,15 @@ class Sampler:
     def rms_norm(self, x, weight, out, eps=1e-6, residual=None, summed=None, weight_offset=0.0, scales=None):
         """lily_rms_norm: out = (h / sqrt(mean(h^2) + eps)) * (weight + weight_offset), h = x + residual, h to
         `summed`.  out: f32, bf16, or float8_e4m3fn with `scales` [rows] f32."""
-        if x.dim() != 2:
+        shape = x.shape
+        if len(shape) != 2:
             raise SamplerError(-1, "x must be [rows, d], rows contiguous")
-        rows, d = x.shape
-        xp, xs, xt = self._matrix(x, rows, d, "x")
-        op, os_, ot = self._matrix(out, rows, d, "out")
+        rows, d = shape
+        xp, xs, xt = self._matrix(x, shape, "x")
+        op, os_, ot = self._matrix(out, shape, "out")
         wp, wt = self._vector(weight, d, "weight")
-        rp, rs, rt = self._matrix(residual, rows, d, "residual") if residual is not None else (None, 0, F32)
-        sp, ss, st = self._matrix(summed, rows, d, "summed") if summed is not None else (None, 0, rt)
+        rp, rs, rt = self._matrix(residual, shape, "residual") if residual is not None else (None, 0, F32)
+        sp, ss, st = self._matrix(summed, shape, "summed") if summed is not None else (None, 0, rt)
         if st != rt:
             raise SamplerError(-1, "summed must have the residual's type")
         _check(_lib.lily_rms_norm(self._h, C.byref(_Norm(
@@ -629,22 +633,22 @@ class Sampler:
             raise SamplerError(-1, "x must be [rows, d] and weight [n, d], rows contiguous")
         rows, d = x.shape
         n = weight.shape[0]
-        xp, xs, xt = self._matrix(x, rows, d, "x")
-        wp, ws, wt = self._matrix(weight, n, d, "weight")
-        op, os_, ot = self._matrix(out, rows, n, "out")
+        xp, xs, xt = self._matrix(x, (rows, d), "x")
+        wp, ws, wt = self._matrix(weight, (n, d), "weight")
+        op, os_, ot = self._matrix(out, (rows, n), "out")
         if xt != wt:
             raise SamplerError(-1, "x and weight must have one type")
         act = ACTIVATIONS.get(activation)
         if act is None:
             raise SamplerError(-1, f"activation must be one of {', '.join(ACTIVATIONS)}")
         bp, bt = self._vector(bias, n, "bias")
-        rp, rs, rt = self._matrix(residual, rows, n, "residual") if residual is not None else (None, 0, F32)
+        rp, rs, rt = self._matrix(residual, (rows, n), "residual") if residual is not None else (None, 0, F32)
         _check(_lib.lily_project(self._h, C.byref(_Projection(
             rows, n, d, xt, xp, xs, wp, ws, self._scales(x_scales, rows, "x_scales"),
             self._scales(weight_scales, n, "weight_scales"), bp, rp, rs, op, os_, bt, rt, ot, act))))
 
     def _logits_out(self, rows, vocab, out, log_sum_exp, logprobs):
-        at, stride, code = self._matrix(out, rows, vocab, "out")
+        at, stride, code = self._matrix(out, (rows, vocab), "out")
         return _LogitsOut(at, stride, code, 1 if logprobs else 0, self._scales(log_sum_exp, rows, "log_sum_exp"))
 
     def process_logits(self, logits, params, out, log_sum_exp=None, logprobs=False, scratch=None, allow=None, bias=None):
