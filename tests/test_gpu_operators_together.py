@@ -177,3 +177,60 @@ def test_a_captured_step(rows):
         step.s.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(replayed, step.outputs()))
     step.close()
+
+
+FAR = (1 << 31) + 24   # elements between two rows: their bytes, and in f32 their elements' bytes twice over, pass 32 bits
+
+
+def _far(rows, cols, dtype):
+    """[rows, cols] with FAR elements from row to row (what lies between is not touched, nor ever written)."""
+    return torch.as_strided(torch.empty((rows - 1) * FAR + cols, dtype=dtype, device=dev()), (rows, cols), (FAR, 1))
+
+
+def test_rows_that_lie_further_apart_than_32_bits():
+    s = LS.Sampler(0)
+    g = torch.Generator(device=dev())
+    g.manual_seed(5)
+    rows, d, n, vocab = 3, 512, 300, 9000
+    x, h, out = (_far(rows, d, torch.bfloat16) for _ in range(3))
+    x.copy_(torch.randn(rows, d, generator=g, device=dev()))
+    h.copy_(torch.randn(rows, d, generator=g, device=dev()))
+    w = torch.ones(d, device=dev())
+    torch.cuda.synchronize()
+    before = h.clone()
+    s.rms_norm(x, w, out, eps=EPS, residual=h, summed=h)
+    s.synchronize()
+    want_h, y = N._formula(x, before, "bf16", w, 0.0, EPS)
+    assert torch.equal(want_h, h)
+    N._check(y, out, None, "bf16")
+    del x, h
+    torch.cuda.empty_cache()
+    for many in (rows, 20):   # few rows, and tiles (of rows side by side)
+        res, o = _far(rows, n, torch.bfloat16), _far(rows, n, torch.float32)
+        a = out.contiguous() if many == rows else torch.randn(many, d, generator=g, device=dev()).bfloat16()
+        if many != rows:
+            del res, o
+            torch.cuda.empty_cache()
+            stride = (1 << 28) + 8
+            res, o = (torch.as_strided(torch.empty((many - 1) * stride + n, dtype=t, device=dev()), (many, n), (stride, 1))
+                      for t in (torch.bfloat16, torch.float32))
+        res.copy_(torch.randn(many, n, generator=g, device=dev()))
+        weight = (torch.randn(n, d, generator=g, device=dev()) / math.sqrt(d)).bfloat16()
+        torch.cuda.synchronize()
+        s.project(a, weight, o, activation="silu", residual=res)
+        s.synchronize()
+        P._check(o, *P._formula(a, weight, None, None, None, "silu", res))
+        del res, o
+        torch.cuda.empty_cache()
+    logits, adjusted = _far(rows, vocab, torch.bfloat16), _far(rows, vocab, torch.float32)
+    logits.copy_(torch.randn(rows, vocab, generator=g, device=dev()) * 3)
+    lse = torch.empty(rows, device=dev())
+    params = [ls_params(temperature=0.5, top_k=5, seed=r) for r in range(rows)]
+    torch.cuda.synchronize()
+    keep = s.process_logits(logits, params, adjusted, log_sum_exp=lse)
+    s.synchronize()
+    assert torch.equal(adjusted, logits.float() / 0.5)
+    ref = torch.logsumexp(adjusted.double(), 1)
+    assert bool(((lse - ref).abs() <= (1.25 * 9 + 8 + ref.abs()) * 2.0 ** -24).all())
+    del keep
+    s.close()
