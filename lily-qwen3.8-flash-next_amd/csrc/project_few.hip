@@ -166,15 +166,17 @@ hipError_t launch_project_few(hipStream_t stream, const ProjectArgs& a, bool e4m
 //   few rows     a compute unit takes in 85 GB/s through LDS: 64 x 4096 x 4096 10.1 (10.5), 64 x 16384 x 2048 19.4 (18.2)
 //   64 x 64      a line of d 0.22 where a compute unit has one tile, 0.21 a round of tiles: 256 x 4096 x 4096 17.8 (18.1),
 //                512 x 4096 x 4096 28.6 (30.9), 64 x 16384 x 2048 16.4 (16.2: memory)
-//   128 x 128    a line 0.51 a round, 0.38 where tiles are few: 1024 x 4096 x 4096 36.7 (38.6), 8192 x 4096 x 4096 271 (267)
-//   256 x 256    1.45 a tile, and 15 for every tile's epilogue, which nothing hides: 8192 x 4096 x 4096 242 (218), where
-//                128 x 128 would take 271
+//   128 x 128    a line 0.48 a round, 0.38 where tiles are few: 1024 x 4096 x 4096 36.7 (36.7), 8192 x 4096 x 4096 259 (252)
+//   256 x 256    1.45 a line, and 13 for every tile's epilogue, which nothing hides, 29 with a residual: 8192 x 4096 x 4096
+//                213 (214), with a residual 238 (246) where 128 x 128 takes 265 (264); 8192 x 8192 x 2048 248 (240) against 270
+//                (252), but with a residual 317 (304) against 300 (276)
 // Parts of d: a launch more (1.5), and the parts' sums written and read at 5.5 TB/s: 64 x 1000 x 8192 in eight 10.6 (10.5)
 // against 25.5 in one; 300 x 4096 x 4096 in two of 128 x 128 22.2 (23.3), where 64 x 64 takes 28.1 in one and 25.9 in two
 // and 128 x 128 30.4 in one; 512 x 4096 x 4096 25.9 (29.9); 100 x 10 007 x 4096 in E4M3, 79 tiles of 128 x 128, in two
 // 16.6 (16.5), in three 16.9 (16.9), in four, a second round, 20.0 (21.5).  Memory at 5.6 TB/s bounds all of them.
-// Rows that do not start at lines of 128 bytes cost 1.4 times as much a line of d, two requests: the same with rows of 4128
-// bytes 19.3 in three parts (18.9), 20.2 in two (18.9), 23.4 in one of 64 x 64 (22.8).
+// Rows that do not start at lines of 128 bytes take two requests a line, 1.4 times as long where tiles are few, 1.15 times where
+// compute units have several: the same with rows of 4128 bytes 19.3 in three parts (18.9), 20.2 in two (18.9), 23.4 in one of
+// 64 x 64 (22.8); 5000 x 7000 x 1504 bf16 125 by 128 x 128 (125), 135 by 256 x 256 (145).
 struct ProjectPlan {
     uint32_t tile = 0;     // 0: few rows
     uint32_t splits = 1;
@@ -186,7 +188,9 @@ static ProjectPlan project_plan(const ProjectArgs& a, uint64_t part_floats) {
     auto over = [](uint32_t x, uint32_t y) { return (x + y - 1u) / y; };
     auto rounds = [](uint64_t tiles) { return (double)((tiles + 255u) / 256u); };
     auto straight = [](const char* p, uint64_t stride) { return (reinterpret_cast<uintptr_t>(p) | stride) % LINE == 0u; };
-    const double crossed = straight(a.x, a.x_stride) && straight(a.w, a.w_stride) ? 1.0 : 1.4;
+    const bool crossing = !(straight(a.x, a.x_stride) && straight(a.w, a.w_stride));
+    auto crossed = [&](bool few) { return !crossing ? 1.0 : few ? 1.4 : 1.15; };
+    const double residual = a.residual == nullptr ? 0.0 : rows * n * (a.residual_bf16 ? 2.0 : 4.0) / 5.6e6;
     ProjectPlan best;
     double least = 1e30;
     auto offer = [&](uint32_t tile, uint32_t splits, double us) {
@@ -209,12 +213,12 @@ static ProjectPlan project_plan(const ProjectArgs& a, uint64_t part_floats) {
         if (k > 1u && (lines < 4u * k || (double)k * rows * part_stride(a.n) > (double)part_floats)) {
             break;
         }
-        const double each = lines * crossed / (double)k, join = k > 1u ? 1.5 + k * rows * n * 8.0 / 5.5e6 : 0.0;
-        offer(64u, k, std::max(3.0 + memory, 4.0 + each * std::max(0.22, 0.21 * rounds(t64 * k))) + join);
-        const double turns = t128 * k <= 256u ? (double)(t128 * k) / 256.0 : rounds(t128 * k);
-        offer(128u, k, std::max(3.0 + memory, 6.0 + each * std::max(0.38, 0.51 * turns)) + join);
+        const double each = lines / (double)k, join = k > 1u ? 1.5 + k * rows * n * 8.0 / 5.5e6 : 0.0;
+        const double turns64 = rounds(t64 * k), turns128 = t128 * k <= 256u ? (double)(t128 * k) / 256.0 : rounds(t128 * k);
+        offer(64u, k, std::max(3.0 + memory, 4.0 + each * crossed(turns64 <= 2.0) * std::max(0.22, 0.21 * turns64)) + residual + join);
+        offer(128u, k, std::max(3.0 + memory, 6.0 + each * crossed(turns128 <= 1.0) * std::max(0.38, 0.48 * turns128)) + residual + join);
     }
-    offer(256u, 1u, 2.0 + std::max(memory, rounds(t256) * (15.0 + lines * 1.45)));
+    offer(256u, 1u, 2.0 + std::max(memory, rounds(t256) * ((a.residual != nullptr ? 29.0 : 13.0) + lines * 1.45)));
     return best;
 }
 
