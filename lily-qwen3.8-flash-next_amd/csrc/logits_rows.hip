@@ -144,8 +144,10 @@ struct RowSum {
         }
     }
     // All the values a thread holds, in the place of what was summed before.  The exponents are formed in one operation
-    // each, v log2 e - c, c = ref log2 e rounded once: what that rounding took is the same factor for all the terms,
-    // and is given back to their sum.  (Not where the products leave the numbers.)
+    // each, v log2 e - c, c = ref log2 e rounded once: what that rounding took, 2^e, is the same factor for all the terms,
+    // and is given back to their sum.  Only for a ref below 2^24, where |e| <= 1 (half a step of c, which lies below 2^25):
+    // half a step of 1e10 log2 e is 512, and neither 2^e nor its inverse is a number then.  Elsewhere the
+    // difference comes first, as in add().
     __device__ __forceinline__ void hold(const f32x4 (&v)[HELD], float odd) {
         m = odd;
 #pragma unroll
@@ -154,7 +156,7 @@ struct RowSum {
         }
         const float ref = largest(m, F32_LOWEST);
         float part[GROUP] = {};
-        if (fabsf(ref) < 0x1p100f) {
+        if (fabsf(ref) < 0x1p24f) {
             const float c = ref * LOG2E;
 #pragma unroll
             for (int u = 0; u < HELD; ++u) {
@@ -507,8 +509,10 @@ struct LogSum {
 };
 __device__ __forceinline__ LogSum log_sum(double m, double s) {
     LogSum r;
+    // (a row with a value sums to 1 at least; one that holds +inf has no sum that means anything, and needs none)
+    const bool finite = m > (double)NEG_INF && m < (double)__builtin_huge_valf();
     r.top = m > (double)NEG_INF ? (float)m : 0.0f;
-    r.log_s = s > 0.0 ? (float)log(s) : 0.0f;   // (NaN: a row that holds +inf)
+    r.log_s = finite ? (float)log(s) : 0.0f;
     r.whole = (float)(m + (double)r.log_s);
     return r;
 }
