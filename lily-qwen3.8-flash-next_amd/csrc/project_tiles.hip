@@ -519,7 +519,8 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
         const uint32_t e = a.residual_bf16 ? 2u : 4u, lines = e;   // lines of a wave's 128 outputs of a row
         for (uint32_t k = 0; k < 2u * lines; ++k) {
             const uint32_t at = k * 64u + lane, row = m0 + wm * 128u + at / lines;
-            const char* p = static_cast<const char*>(a.residual) + ((uint64_t)row * a.residual_stride + n0 + wn * 128u) * e + at % lines * LINE;
+            // (rows may start at any element: the first whole word of what a line holds of a row)
+            const uintptr_t p = (reinterpret_cast<uintptr_t>(a.residual) + ((uint64_t)row * a.residual_stride + n0 + wn * 128u) * e + at % lines * LINE + 3u) & ~(uintptr_t)3u;
             __builtin_amdgcn_global_load_lds((gptr)p, (lptr)(lds + T::STAGES + wave * 256u), 4, 0, 0);
         }
     };
