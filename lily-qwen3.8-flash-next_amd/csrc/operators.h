@@ -21,6 +21,7 @@ hipError_t launch_rms_norm(hipStream_t stream, const lily_norm& norm);
 struct ProjectWorkspace {
     float* part;            // sums of parts of d, in 16-byte units
     uint64_t part_floats;
+    uint32_t tile = 0;      // 64, 128 or 256: what more than 16 rows get; 0: by an estimate of the time
 };
 hipError_t launch_project(hipStream_t stream, const lily_projection& p, const ProjectWorkspace& ws);
 

@@ -13,34 +13,14 @@
 #include <hip/hip_runtime.h>
 
 #include "device_common.h"
-#include "operators.h"
+#include "project_plan.h"
 
 namespace lily {
-
-constexpr uint32_t LINE = 128;   // bytes of a row that are taken at a time
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-
-struct ProjectArgs {
-    const char* x;
-    const char* w;
-    const float* x_scales;      // or null
-    const float* w_scales;      // or null
-    const void* bias;           // or null
-    const void* residual;       // or null
-    void* out;
-    uint64_t x_stride, w_stride;               // bytes
-    uint64_t residual_stride, out_stride;      // elements
-    uint32_t rows, n, d_bytes;
-    uint32_t bias_bf16, residual_bf16, out_bf16, act;
-    uint32_t splits;            // parts of d, each a workgroup's
-    float* part;                // their sums, [splits][rows][part_stride(n)]
-};
-
-__host__ __device__ constexpr uint32_t part_stride(uint32_t n) { return (n + 3u) / 4u * 4u; }
 
 // The operand of a lane: two pieces.
 struct Frag {

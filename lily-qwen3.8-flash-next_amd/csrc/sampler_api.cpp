@@ -116,6 +116,7 @@ struct lily_sampler {
     uint32_t head_library_rows_code_lines = HEAD_LIBRARY_ROWS_CODE_LINES;
     uint32_t head_library_rows_code_lines_alone = HEAD_LIBRARY_ROWS_CODE_LINES_ALONE;
     unsigned long long head_library_calls = 0;   // producer calls that went through the vendor's library
+    uint32_t project_tile = 0;  // LILY_SAMPLER_PROJECT: 0 = by an estimate, else the tile of products of more than 16 rows
     uint32_t handover = 0;  // LILY_SAMPLER_HANDOVER: 0 = by the launch's size, 1 = strict, 2 = relaxed
     // What the last lily_lm_head_bf16 call of this sampler left: where, and with which exponent
     // scale per row (tile_sum is only good for a log-probability at that scale).
@@ -1041,6 +1042,7 @@ hipStream_t sampler_stream(const lily_sampler_t* s) { return s->stream; }
 void sampler_project_workspace(const lily_sampler_t* s, ProjectWorkspace* ws) {
     ws->part = reinterpret_cast<float*>(s->ws_cand);
     ws->part_floats = (uint64_t)s->ws_slots * 2u;
+    ws->tile = s->project_tile;
 }
 
 int sample_row_with_workspace(int device, hipStream_t stream, const Workspace& ws, const float* logits,
@@ -1200,6 +1202,10 @@ int lily_sampler_create(int device, void* hip_stream, lily_sampler_t** out) {
     }
     if (const char* p = std::getenv("LILY_SAMPLER_HANDOVER")) {
         s->handover = std::strcmp(p, "strict") == 0 ? 1u : std::strcmp(p, "relaxed") == 0 ? 2u : 0u;
+    }
+    if (const char* p = std::getenv("LILY_SAMPLER_PROJECT")) {
+        const uint32_t tile = (uint32_t)std::atoi(p);
+        s->project_tile = tile == 64u || tile == 128u || tile == 256u ? tile : 0u;
     }
     const size_t slots = (size_t)WS_ROWS * MAX_SLICES;
     hipError_t err = hipMalloc(reinterpret_cast<void**>(&s->ws_cand),
