@@ -166,6 +166,7 @@ struct LogitsRows {
     bool logprobs = false;     // else the adjusted logits
     bool biased = false;       // some row has a bias list
     bool in_place = false;     // out is where the logits are
+    bool relaxed = true;       // rows in slices may hand their sums over within a launch
     float* lse = nullptr;      // [rows of out] or null
     // workspace, all of it 0 between launches
     Handed<uint64_t> word;     // [max_rows][MAX_SLICES]

@@ -16,8 +16,9 @@
 // values stay in registers: each workgroup leaves its (largest value, sum) as one word, which is the whole message,
 // looks for the words of its row's other slices, a bounded number of times, and writes.  Where a word does not
 // come (the other workgroup has no place on the chip yet) it forms the other slices' words itself, by the same
-// operations, so the result is the same.  Rows too long for that (over 524 288 ids) take a launch for the sums and one
-// that writes.
+// operations, so the result is the same.  Rows too long for that (over 524 288 ids), and rows in slices where the relaxed
+// form of the hand-over (last_to_arrive()) is taken out, take a launch for the sums and one that writes: a ticket that releases
+// and acquires writes back the outputs behind every one (1 024 rows of 151 936 1 099 us, so 305).
 //
 // Bound by memory where rows are many: 1 024 rows of 151 936 bf16 to f32 are written, adjusted, in 166 us (933 MB, 5.6
 // TB/s, what a copy reaches) and as log-probabilities in 180; under histories of 2 048 ids in 200 and 215, where the
@@ -616,7 +617,9 @@ __device__ __forceinline__ void logits_row(const RowArgs& a, uint32_t row_of_lau
             }
         };
         // Where the outputs take the logits' place, none is written before the slice's word has arrived: who forms the
-        // word itself from the logits, and still finds none behind them, has read logits.
+        // word itself from the logits, and still finds none behind them, has read logits.  (That the word is in memory
+        // when its store counts as done is the hardware's promise, as in last_to_arrive()'s relaxed form, not the memory
+        // model's; the same for the count behind which the words are cleared.)
         if (q.slices > 1u && (is_logprobs(FORM) || q.in_place != 0u)) {
             if (tid < 64u) {
                 __builtin_amdgcn_s_waitcnt(0);
@@ -724,11 +727,11 @@ hipError_t launch_form(hipStream_t stream, const RowArgs* table, const InlineRow
 
 template <int DT, int OT>
 hipError_t launch_typed(hipStream_t stream, const RowArgs* table, const InlineRows* few, uint32_t rows, const LogitsLaunch& q,
-                        bool logprobs) {
+                        bool logprobs, bool relaxed) {
     if (!logprobs && q.lse == nullptr) {
         return launch_form<DT, OT, FORM_ADJUSTED>(stream, table, few, rows, q);
     }
-    if (q.per_slice <= LOGITS_HELD) {
+    if (q.per_slice <= LOGITS_HELD && (relaxed || q.slices == 1u)) {
         return logprobs ? launch_form<DT, OT, FORM_HELD_LOGPROBS>(stream, table, few, rows, q)
                         : launch_form<DT, OT, FORM_HELD_ADJUSTED>(stream, table, few, rows, q);
     }
@@ -754,6 +757,11 @@ hipError_t launch_logits_rows(hipStream_t stream, int dtype, uint32_t rows, uint
     q.done = w.done;
     q.looks = w.looks;
     q.in_place = w.in_place;
+#ifdef LILY_STRICT_HANDOVER
+    const bool relaxed = false;
+#else
+    const bool relaxed = w.relaxed;
+#endif
     q.vocab = vocab;
     // A launch takes as many rows as the workspace has words for.
     for (uint32_t first = 0; first < rows; first += w.max_rows) {
@@ -768,11 +776,11 @@ hipError_t launch_logits_rows(hipStream_t stream, int dtype, uint32_t rows, uint
         const RowArgs* part = table != nullptr ? table + first : nullptr;
         hipError_t e;
         if (dtype == LILY_BF16) {
-            e = w.out_dtype == LILY_BF16 ? launch_typed<LILY_BF16, LILY_BF16>(stream, part, few, n, q, w.logprobs)
-                                         : launch_typed<LILY_BF16, LILY_F32>(stream, part, few, n, q, w.logprobs);
+            e = w.out_dtype == LILY_BF16 ? launch_typed<LILY_BF16, LILY_BF16>(stream, part, few, n, q, w.logprobs, relaxed)
+                                         : launch_typed<LILY_BF16, LILY_F32>(stream, part, few, n, q, w.logprobs, relaxed);
         } else {
-            e = w.out_dtype == LILY_BF16 ? launch_typed<LILY_F32, LILY_BF16>(stream, part, few, n, q, w.logprobs)
-                                         : launch_typed<LILY_F32, LILY_F32>(stream, part, few, n, q, w.logprobs);
+            e = w.out_dtype == LILY_BF16 ? launch_typed<LILY_F32, LILY_BF16>(stream, part, few, n, q, w.logprobs, relaxed)
+                                         : launch_typed<LILY_F32, LILY_F32>(stream, part, few, n, q, w.logprobs, relaxed);
         }
         if (e != hipSuccess) {
             return e;

@@ -2470,6 +2470,7 @@ static int check_logits_out(const lily_logits_out* o, const void* logits, uint64
 static LogitsRows logits_rows_of(lily_sampler* s, const lily_logits_out* o, bool biased, const void* logits) {
     LogitsRows w;
     w.in_place = o->out_dev == logits;
+    w.relaxed = s->handover != 1u;
     w.out = o->out_dev;
     w.stride = o->out_stride;
     w.out_dtype = o->out_dtype;
