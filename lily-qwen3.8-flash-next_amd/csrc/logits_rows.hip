@@ -112,7 +112,6 @@ __device__ __forceinline__ void store_one(void* row, uint32_t id, float v) {
 // What a workgroup knows of the biases of its slice.
 struct SliceBias {
     uint32_t n;        // pairs listed, in list order; more than BIAS_PAIRS: the row's own list is read
-    uint32_t total;    // scratch of the listing
     uint32_t ids[BIAS_PAIRS];
     float deltas[BIAS_PAIRS];
 };

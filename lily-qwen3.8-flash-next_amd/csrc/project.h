@@ -18,7 +18,6 @@
 namespace lily {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
@@ -49,13 +48,8 @@ __device__ __forceinline__ bf16x8 widened(uint32_t a, uint32_t b) {
 
 template <Products P>
 __device__ __forceinline__ f32x4 product(const Frag& w, const Frag& x, f32x4 c) {
-    if constexpr (P == PRODUCT_E4M3) {
-        const u32x8 a = __builtin_shufflevector(w.lo, w.hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        const u32x8 b = __builtin_shufflevector(x.lo, x.hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        // (both operands E4M3, block scales of one)
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(i32x8, a), __builtin_bit_cast(i32x8, b),
-                                                                c, 0, 0, 0, 0, 0, 0);
-    } else if constexpr (P == PRODUCT_E4M3_WIDE) {
+    static_assert(P != PRODUCT_E4M3, "few rows are read at the speed of memory: they take the exact products");
+    if constexpr (P == PRODUCT_E4M3_WIDE) {
         c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widened(w.lo[0], w.lo[1]), widened(x.lo[0], x.lo[1]), c, 0, 0, 0);
         c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widened(w.lo[2], w.lo[3]), widened(x.lo[2], x.lo[3]), c, 0, 0, 0);
         c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widened(w.hi[0], w.hi[1]), widened(x.hi[0], x.hi[1]), c, 0, 0, 0);
