@@ -511,8 +511,10 @@ int lily_lm_head_sample_rows(lily_sampler_t* s, const lily_lm_head* head, const 
  *     y = h / sqrt(mean(h^2) + eps) * (weight + weight_offset)
  * in f32.  h goes to sum_dev where that is given, y to out_dev: f32, bf16 (nearest even) or, for
  * an 8-bit product, E4M3 with one f32 scale a row: scale = max|y| / 448, q = E4M3(y / scale).  A row
- * whose largest |y| lies below 2^-116 has scale 0 and zeros; a row with a value that is not finite
- * has what the formula gives, and in 8 bits a NaN scale.
+ * whose largest |y| lies below 2^-116 has scale 0 and zeros; a row whose h holds a value that is not
+ * finite has what the formula gives, and in 8 bits a NaN scale; where only a product with the weight is
+ * infinite, so is the scale.  Squares and their sum are f32 too: a row of values from some 2^56 on is
+ * zeros (its root is infinite), and one below 2^-63 needs an eps above its squares.
  *
  * Rows hold d (1 .. LILY_NORM_MAX_D) elements, strides count elements and may be anything from d on.
  * sum_dev may be x_dev or residual_dev, and out_dev may be either, each with the same type and stride;
@@ -557,8 +559,11 @@ int lily_rms_norm(lily_sampler_t* s, const lily_norm* norm);
  * replayed one after the other.
  * E4M3 operands: with an f32 output, and always for up to 16 rows, the products and sums are as bf16 has them (each
  * E4M3 value is one of bf16).  More rows with a bf16 output may take the matrix cores' 8-bit products, at twice the rate:
- * of every eight neighbouring elements' products they drop what lies 2^-13 below the largest one, some 6e-5 of the
- * result. */
+ * of every eight neighbouring elements' products they drop what lies 2^-13 below the largest one, up to 7 * 2^-13 of
+ * that product.  The bound is relative to the sum of the groups' largest products, not to a result in which they
+ * cancel; for normally distributed operands it comes to some 6e-5 of the result's size.
+ * Which kernel a product gets, and in how many parts d is added, goes by rows, n, d and alignment: a row's last bits
+ * (and, with E4M3 operands and a bf16 output, the cut) may differ between batches of different sizes. */
 typedef enum lily_activation {
     LILY_ACT_NONE = 0,
     LILY_ACT_SILU = 1,        /* v / (1 + exp(-v)) */
@@ -618,7 +623,9 @@ typedef struct lily_logits_out {
     float* log_sum_exp_dev;   /* [rows] or NULL */
 } lily_logits_out;
 int lily_process_logits(lily_sampler_t* s, const lily_rows* batch, const lily_logits_out* out);
-/* The same of a resident batch: one or two launches, nothing staged. */
+/* The same of a resident batch, nothing staged: one launch for up to 4 096 rows (each 4 096 more take another);
+ * with sums three, the last of which clears the workspace, for vocabularies above 524 288, and where
+ * LILY_SAMPLER_HANDOVER=strict takes the sums out of the launch that writes. */
 int lily_plan_process_logits(lily_plan_t* p, const lily_logits_out* out);
 
 #ifdef __cplusplus
