@@ -399,6 +399,16 @@ struct Shared {
     double red3[4][NWAVE];
 };
 
+// The references that a sum of exponentials takes lie between these.  A term's exponent v*c - ref is formed in one
+// operation, ref being a largest v*c, rounded: what that rounding took, half a step of it, is the same for all terms and cancels in
+// the sum's logarithm, but has to stay an exponent: 64 below 2^31, 512 at 1e10 log2 e.  (The sum of a thread, a wave or a
+// slice whose every id was barred by a finite -1e10 or -1e30 was no number, and the row's with it.)  At the floor such terms
+// are 0, which is what they are beside any other.  A row whose largest value lies beyond either end is
+// known by its reference or its sum, and summed again by sum_again(); so is one beyond LSE_FAR, where values are so far
+// apart that the largest less a cut of some 26 (what the scans leave out of a sum lies below it) may be the largest itself.
+constexpr float LSE_CEIL = 0x1p31f, LSE_FLOOR = -LSE_CEIL, LSE_FAR = 0x1p28f;
+__device__ __forceinline__ float lse_ref(float largest) { return __builtin_amdgcn_fmed3f(largest, LSE_FLOOR, LSE_CEIL); }
+
 // Running sum of 2^(v*c - mc) of one thread with its own reference mc.
 struct LseAcc {
     float mc;
@@ -409,11 +419,10 @@ struct LseAcc {
     }
     // Raises the reference to cover block maximum cm; returns the reference to subtract.
     __device__ __forceinline__ float rebase(float cm, float c) {
-        const float mcn = fmaxf(mc, cm * c);
-        const float safe = fmaxf(mcn, F32_LOWEST);
-        s *= __builtin_amdgcn_exp2f(mc - safe);
+        const float mcn = lse_ref(fmaxf(mc, cm * c));
+        s *= __builtin_amdgcn_exp2f(mc - mcn);
         mc = mcn;
-        return safe;
+        return mcn;
     }
     __device__ __forceinline__ void term(float v, float c, float safe) {
         s += __builtin_amdgcn_exp2f(__builtin_fmaf(v, c, -safe));
@@ -1058,7 +1067,7 @@ struct WaveLse {
     float s;
     float booked;   // what the caller took off `s` again, kept relative to the same reference
     __device__ __forceinline__ void init() {
-        ref = F32_LOWEST;
+        ref = LSE_FLOOR;
         s = 0.0f;
         booked = 0.0f;
     }
@@ -1068,7 +1077,7 @@ struct WaveLse {
     __device__ __forceinline__ void add(const float (&v)[E], float m, float c) {
         if (__ballot(__builtin_fmaf(m, c, -ref) > LSE_RAISE) != 0ull) {
             // A term would dwarf the reference: raise it to the wave's maximum (rare).
-            const float nref = fmaxf(ref, wave_max_dpp(m * c));
+            const float nref = lse_ref(fmaxf(ref, wave_max_dpp(m * c)));
             const float down = __builtin_amdgcn_exp2f(ref - nref);
             s *= down;
             booked *= down;
@@ -1086,7 +1095,7 @@ struct WaveLse {
     __device__ __forceinline__ void add_if(const float (&v)[E], float m, float c, bool active) {
         const float d = __builtin_fmaf(active ? m : NEG_INF, c, -ref);
         if (__ballot(d > LSE_RAISE) != 0ull) {
-            const float nref = fmaxf(ref, wave_max_dpp(active ? m * c : NEG_INF));
+            const float nref = lse_ref(fmaxf(ref, wave_max_dpp(active ? m * c : NEG_INF)));
             const float down = __builtin_amdgcn_exp2f(ref - nref);
             s *= down;
             booked *= down;
@@ -1110,7 +1119,7 @@ struct WaveLse {
     float skip_below;  // loads whose maximum is not above this are left out (set by the caller)
     __device__ __forceinline__ void prepare(float block_max, float c) {
         if (__ballot(__builtin_fmaf(block_max, c, -ref) > LSE_RAISE) != 0ull) {
-            const float nref = fmaxf(ref, wave_max_dpp(block_max * c));
+            const float nref = lse_ref(fmaxf(ref, wave_max_dpp(block_max * c)));
             const float down = __builtin_amdgcn_exp2f(ref - nref);
             s *= down;
             booked *= down;

@@ -118,6 +118,39 @@ __device__ __forceinline__ void read_again(RowArgs& a, const LILY_CONST RowArgs*
     apply_selection(a);
 }
 
+// The log-probability of a row whose sum its references could not hold, by its first wave when everything else is done (`again` of its first lane; called by all
+// waves, once a kernel: a copy at every place that finishes a row took 0.5 us of 72 from the batch of 1 024).  Every
+// difference is formed first, which is right at any size of the values; a value a lane and trip to memory, some 3 ms for
+// 151 936 ids.
+template <int DT, bool LSE>
+__device__ __forceinline__ void sum_again(const LILY_CONST RowArgs* src, uint32_t vocab, const Resum& again) {
+    if (!LSE || __builtin_expect(__ballot(again.needed) == 0ull, 1)) {
+        return;
+    }
+    RowArgs a;
+    read_again(a, src);
+    const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane((int)again.id);
+    const float u = lilym_bits_f32((uint32_t)__builtin_amdgcn_readfirstlane((int)lilym_f32_bits(again.u)));
+    float top = NEG_INF;
+    double s = 0.0;
+#pragma unroll 1
+    for (uint32_t i = threadIdx.x & 63u; i < vocab; i += 64u) {
+        float v = pre_temperature_of<DT>(a, i);
+        v = i == id ? u : v;   // (it has been counted meanwhile)
+        if (v > top) {
+            s = s * (double)__builtin_amdgcn_exp2f((top - v) * a.c2) + 1.0;
+            top = v;
+        } else if (v > NEG_INF) {   // (false for a NaN: worth -inf)
+            s += (double)__builtin_amdgcn_exp2f((v - top) * a.c2);
+        }
+    }
+    const float all = wave_max_dpp(top);
+    s = wave_sum_d(top > NEG_INF ? s * (double)__builtin_amdgcn_exp2f((top - all) * a.c2) : 0.0);
+    if ((threadIdx.x & 63u) == 0u && all < __builtin_huge_valf()) {   // (one that holds +inf keeps what it has)
+        *a.out_logprob = fminf((float)(((double)(u - all) * (double)a.c2 - log2(s)) * 0.6931471805599453), 0.0f);
+    }
+}
+
 // The launch's settings once more, for the same reason.
 __device__ __forceinline__ void read_again(LaunchCfg& cfg, const LILY_CONST LaunchCfg* src) {
     static_assert(sizeof(LaunchCfg) % 8 == 0, "LaunchCfg is copied in 8-byte pieces");
@@ -296,7 +329,7 @@ __device__ __forceinline__ uint64_t merge_slices_by_wave(const LaunchCfg& cfg, s
 
 template <int DT, bool LSE, bool SPEC>
 __device__ __forceinline__ bool finish_by_wave(const RowArgs& t, const LaunchCfg& cfg, uint32_t row, uint32_t s, uint32_t n,
-                                               const uint64_t* found, uint32_t step, bool want_lse, Shared& sh) {
+                                               const uint64_t* found, uint32_t step, bool want_lse, Shared& sh, Resum& again) {
     const uint32_t lane = threadIdx.x, S = cfg.slices, vocab = cfg.vocab;
     const bool forced = (t.flags & F_FORCED) != 0u;
     const size_t slot = (size_t)row * S + s;
@@ -345,7 +378,7 @@ __device__ __forceinline__ bool finish_by_wave(const RowArgs& t, const LaunchCfg
     phase(cfg, 6);
     if (forced) {
         if (lane == 0u) {
-            finish_token<DT>(t, sh, t.forced, vocab);
+            finish_token<DT, LSE>(t, sh, t.forced, vocab, again);
         }
         return true;
     }
@@ -357,14 +390,14 @@ __device__ __forceinline__ bool finish_by_wave(const RowArgs& t, const LaunchCfg
         }
         return true;
     }
-    tail_wave<DT, SPEC>(t, vocab, step, best, have, sh, cfg, spec_d, spec_qn);
+    tail_wave<DT, LSE, SPEC>(t, vocab, step, best, have, sh, cfg, spec_d, spec_qn, again);
     return true;
 }
 
 // True in the workgroup that finishes the row (the last of its slices to arrive).
 template <int DT, int KIND, bool LSE, bool CHAIN = false, bool SPEC = false>
 __device__ __forceinline__ bool row_body(const LILY_CONST RowArgs* src, const LaunchCfg& cfg, const LILY_CONST LaunchCfg* cfg_src,
-                                         Shared& sh) {
+                                         Shared& sh, Resum& again) {
     if (cfg.served != nullptr && *(const LILY_CONST uint32_t*)(cfg.served + blockIdx.y) != 0u) {
         return false;
     }
@@ -511,7 +544,7 @@ __device__ __forceinline__ bool row_body(const LILY_CONST RowArgs* src, const La
         if (tid >= 64u) {
             return false;
         }
-        const bool finished = finish_by_wave<DT, LSE, SPEC>(t, late, row, s, n, found, step, want_lse, sh);
+        const bool finished = finish_by_wave<DT, LSE, SPEC>(t, late, row, s, n, found, step, want_lse, sh, again);
         if (finished) {
             phase(late, 7);
         }
@@ -661,7 +694,7 @@ __device__ __forceinline__ bool row_body(const LILY_CONST RowArgs* src, const La
     }
     if (t.flags & F_FORCED) {
         if (tid == 0) {
-            finish_token<DT>(t, sh, t.forced, vocab);
+            finish_token<DT, LSE>(t, sh, t.forced, vocab, again);
         }
         return true;
     }
@@ -805,7 +838,7 @@ __device__ __forceinline__ bool row_body(const LILY_CONST RowArgs* src, const La
                 r.q_ids = pre_qid + j * PRE;
                 r.q_probs = pre_qp + j * PRE;
             }
-            tail<DT, KIND != 2, true>(r, vocab, r.step + late.step_delta, n_now, ranked, cand, sh, late);
+            tail<DT, LSE, KIND != 2, true>(r, vocab, r.step + late.step_delta, n_now, ranked, cand, sh, late, again);
             // The workgroup meets over LDS only: a barrier that also waited for thread 0's stores
             // and increments to be acknowledged by memory would cost every row a round trip
             // that nothing here depends on.
@@ -843,7 +876,7 @@ __device__ __forceinline__ bool row_body(const LILY_CONST RowArgs* src, const La
         phase(late, 7);
         return true;
     }
-    tail<DT, KIND != 2, SPEC>(t, vocab, step, n, sorted, found, sh, late);
+    tail<DT, LSE, KIND != 2, SPEC>(t, vocab, step, n, sorted, found, sh, late, again);
     phase(late, 7);
     return true;
 }
@@ -869,7 +902,9 @@ __global__ __launch_bounds__(NT, KIND == 1 ? 3 : 4) void k_rows_inline(InlineRow
         tail_arrays(sh);
     }
     __syncthreads();
-    row_body<DT, KIND, LSE>(table + blockIdx.y, cfg, (const LILY_CONST LaunchCfg*)(table + INLINE_ROWS), sh);
+    Resum again;
+    row_body<DT, KIND, LSE>(table + blockIdx.y, cfg, (const LILY_CONST LaunchCfg*)(table + INLINE_ROWS), sh, again);
+    sum_again<DT, LSE>(table + blockIdx.y, cfg.vocab, again);
 }
 
 // Rows that draw in order (the verify pass under penalties): see row_body.
@@ -882,7 +917,8 @@ __global__ __launch_bounds__(NT, KIND == 1 ? 3 : 4) void k_rows_chain(InlineRows
         tail_arrays(sh);
     }
     __syncthreads();
-    row_body<DT, KIND, false, true>(table + blockIdx.y, cfg, (const LILY_CONST LaunchCfg*)(table + INLINE_ROWS), sh);
+    Resum again;
+    row_body<DT, KIND, false, true>(table + blockIdx.y, cfg, (const LILY_CONST LaunchCfg*)(table + INLINE_ROWS), sh, again);
 }
 
 // A verify pass whose rows are independent: the one-wave form of the speculative draw is compiled in,
@@ -897,7 +933,8 @@ __global__ __launch_bounds__(NT, KIND == 1 ? 3 : 4) void k_rows_verify(InlineRow
         tail_arrays(sh);
     }
     __syncthreads();
-    const bool finished = row_body<DT, KIND, false, false, true>(table + blockIdx.y, cfg, (const LILY_CONST LaunchCfg*)(table + INLINE_ROWS), sh);
+    Resum again;
+    const bool finished = row_body<DT, KIND, false, false, true>(table + blockIdx.y, cfg, (const LILY_CONST LaunchCfg*)(table + INLINE_ROWS), sh, again);
     if (!finished || threadIdx.x != 0 || cfg.accept_ctrl == nullptr) {
         return;
     }
@@ -912,7 +949,9 @@ __global__ __launch_bounds__(NT, KIND == 1 ? 3 : 4) void k_rows_table(LaunchCfg 
         tail_arrays(sh);
     }
     __syncthreads();
-    row_body<DT, KIND, LSE>(table + blockIdx.y, cfg, (const LILY_CONST LaunchCfg*)__builtin_amdgcn_kernarg_segment_ptr(), sh);
+    Resum again;
+    row_body<DT, KIND, LSE>(table + blockIdx.y, cfg, (const LILY_CONST LaunchCfg*)__builtin_amdgcn_kernarg_segment_ptr(), sh, again);
+    sum_again<DT, LSE>(table + blockIdx.y, cfg.vocab, again);
 }
 
 template <int DT, int KIND, bool LSE>

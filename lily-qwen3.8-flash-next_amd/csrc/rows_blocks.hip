@@ -55,7 +55,7 @@ static_assert(BLOCKS_LDS_BYTES >= WAVE_MERGE_SLOTS * 8, "one wave's merge works 
 
 // PEN: rows under penalties are among the launch's.  True in the wave that finished the row.
 template <int DT, bool LSE, bool PEN>
-__device__ __forceinline__ bool blocks_row(const LILY_CONST RowArgs* src, const LaunchCfg& cfg, Shared& sh) {
+__device__ __forceinline__ bool blocks_row(const LILY_CONST RowArgs* src, const LaunchCfg& cfg, Shared& sh, Resum& again) {
     if (cfg.served != nullptr && *(const LILY_CONST uint32_t*)(cfg.served + blockIdx.y) != 0u) {
         return false;
     }
@@ -137,7 +137,7 @@ __device__ __forceinline__ bool blocks_row(const LILY_CONST RowArgs* src, const 
     float lane_max = ev;        // of true values
     float T = F32_LOWEST;       // the bound, the same in every thread of a wave
     float skip = NEG_INF;       // chunks at or below it are left out of the sum
-    float ref = F32_LOWEST;     // the wave's reference: terms are 2^(x * c2 - ref)
+    float ref = LSE_FLOOR;      // the wave's reference: terms are 2^(x * c2 - ref)
     double sum = 0.0;
     uint32_t fill = 0;          // this wave's listed values
     uint32_t noted = 0;         // ... and noted ids
@@ -178,7 +178,7 @@ __device__ __forceinline__ bool blocks_row(const LILY_CONST RowArgs* src, const 
     // Terms would dwarf the wave's reference: it moves up to the wave's largest.
     auto raise = [&](float largest) {
         if (__ballot(__builtin_fmaf(largest, a.c2, -ref) > LSE_RAISE) != 0ull) {
-            const float now = fminf(fmaxf(wave_max_dpp(largest) * a.c2, -1.0e30f), 1.0e30f);
+            const float now = lse_ref(wave_max_dpp(largest) * a.c2);
             sum *= (double)__builtin_amdgcn_exp2f(ref - now);
             ref = now;
         }
@@ -582,7 +582,7 @@ __device__ __forceinline__ bool blocks_row(const LILY_CONST RowArgs* src, const 
         for (int i = 1; i < NWAVE; ++i) {
             top = fmaxf(top, sh.wthr[i]);
         }
-        mc = top > F32_LOWEST ? (double)top : 0.0;
+        mc = top > LSE_FLOOR ? (double)top : 0.0;
         for (int i = 0; i < NWAVE; ++i) {
             const double d = (double)sh.wthr[i] - mc;
             rest += d > -1000.0 ? sh.red_d[i] * pow2_d(d) : 0.0;
@@ -702,7 +702,7 @@ __device__ __forceinline__ bool blocks_row(const LILY_CONST RowArgs* src, const 
         ranked[lane] = c;
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");   // (LDS of this wave: in order already)
         __builtin_amdgcn_wave_barrier();
-        const bool finished = finish_by_wave<DT, LSE, false>(t, cfg, row, s, n, ranked, step, want_lse, sh);
+        const bool finished = finish_by_wave<DT, LSE, false>(t, cfg, row, s, n, ranked, step, want_lse, sh, again);
         if (finished) {
             phase(cfg, 7);
         }
@@ -710,14 +710,14 @@ __device__ __forceinline__ bool blocks_row(const LILY_CONST RowArgs* src, const 
     }
     if (forced) {
         if (lane == 0u) {
-            finish_token<DT>(t, sh, t.forced, vocab);
+            finish_token<DT, LSE>(t, sh, t.forced, vocab, again);
         }
     } else if (n == 0u) {
         if (lane == 0u) {
             finish_empty(t, vocab, sh, cfg);
         }
     } else {
-        tail_wave<DT, false>(t, vocab, step, c, n, sh, cfg, 0u, 0u);
+        tail_wave<DT, LSE, false>(t, vocab, step, c, n, sh, cfg, 0u, 0u, again);
     }
     phase(cfg, 7);
     return true;
@@ -726,7 +726,9 @@ __device__ __forceinline__ bool blocks_row(const LILY_CONST RowArgs* src, const 
 template <int DT, bool LSE, bool PEN>
 __global__ __launch_bounds__(NT, 4) void k_blocks_table(LaunchCfg cfg) {
     __shared__ Shared sh;
-    blocks_row<DT, LSE, PEN>((const LILY_CONST RowArgs*)cfg.table + blockIdx.y, cfg, sh);
+    Resum again;
+    blocks_row<DT, LSE, PEN>((const LILY_CONST RowArgs*)cfg.table + blockIdx.y, cfg, sh, again);
+    sum_again<DT, LSE>((const LILY_CONST RowArgs*)cfg.table + blockIdx.y, cfg.vocab, again);
 }
 
 template <int DT, bool LSE, bool PEN>

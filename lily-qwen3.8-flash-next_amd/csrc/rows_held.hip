@@ -45,7 +45,7 @@ struct HeldBias {
 
 // EXTRA: rows with a mask or a bias list are among the launch's.  True in the wave that finished the row.
 template <int DT, int NB, bool LSE, bool EXTRA, bool SPEC>
-__device__ __forceinline__ bool held_row(const LILY_CONST RowArgs* src, const LaunchCfg& cfg, Shared& sh, HeldBias* bias_lds) {
+__device__ __forceinline__ bool held_row(const LILY_CONST RowArgs* src, const LaunchCfg& cfg, Shared& sh, HeldBias* bias_lds, Resum& again) {
     if (cfg.served != nullptr && *(const LILY_CONST uint32_t*)(cfg.served + blockIdx.y) != 0u) {
         return false;
     }
@@ -313,8 +313,7 @@ __device__ __forceinline__ bool held_row(const LILY_CONST RowArgs* src, const La
     phase(cfg, 2);
 
     // ---- what reaches it is listed, the rest goes into the sum
-    // Finite and far from overflow: every term is formed as 2^(x * c2 - ref).
-    const float ref = top > NEG_INF ? fminf(fmaxf(top * a.c2, -1.0e30f), 1.0e30f) : 0.0f;
+    const float ref = top > NEG_INF ? lse_ref(top * a.c2) : 0.0f;
     uint64_t* pairs = dyn_lds;             // [NWAVE][HELD_SEG]: value's bits << 32 | id
     uint64_t* ranked = dyn_lds + HELD_CAP;
     uint32_t fill = 0;                     // this wave's
@@ -567,14 +566,14 @@ __device__ __forceinline__ bool held_row(const LILY_CONST RowArgs* src, const La
             }
         }
         __syncthreads();
-        tail<DT, false, true>(a, vocab, step, sh.n_cand, true, dyn_lds, sh, cfg);
+        tail<DT, LSE, false, true>(a, vocab, step, sh.n_cand, true, dyn_lds, sh, cfg, again);
         return w == 0u;
     }
     if (S > 1u) {
         ranked[lane] = c;
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");   // (LDS of this wave: in order already)
         __builtin_amdgcn_wave_barrier();
-        const bool finished = finish_by_wave<DT, LSE, SPEC>(a, cfg, row, s, n, ranked, step, want_lse, sh);
+        const bool finished = finish_by_wave<DT, LSE, SPEC>(a, cfg, row, s, n, ranked, step, want_lse, sh, again);
         if (finished) {
             phase(cfg, 7);
         }
@@ -582,7 +581,7 @@ __device__ __forceinline__ bool held_row(const LILY_CONST RowArgs* src, const La
     }
     if (forced) {
         if (lane == 0u) {
-            finish_token<DT>(a, sh, a.forced, vocab);
+            finish_token<DT, LSE>(a, sh, a.forced, vocab, again);
         }
     } else if (n == 0u) {
         if (lane == 0u) {
@@ -594,7 +593,7 @@ __device__ __forceinline__ bool held_row(const LILY_CONST RowArgs* src, const La
             spec_d = *a.draft;
             spec_qn = *a.q_n;
         }
-        tail_wave<DT, SPEC>(a, vocab, step, c, n, sh, cfg, spec_d, spec_qn);
+        tail_wave<DT, LSE, SPEC>(a, vocab, step, c, n, sh, cfg, spec_d, spec_qn, again);
     }
     phase(cfg, 7);
     return true;
@@ -605,14 +604,18 @@ __global__ __launch_bounds__(NT, (HELD_RESIDENT<DT, NB>)) void k_held_inline(Inl
     __shared__ Shared sh;
     __shared__ HeldBias bias[1];
     const LILY_CONST RowArgs* table = (const LILY_CONST RowArgs*)__builtin_amdgcn_kernarg_segment_ptr();
-    held_row<DT, NB, LSE, EXTRA, false>(table + blockIdx.y, cfg, sh, EXTRA ? bias : nullptr);
+    Resum again;
+    held_row<DT, NB, LSE, EXTRA, false>(table + blockIdx.y, cfg, sh, EXTRA ? bias : nullptr, again);
+    sum_again<DT, LSE>(table + blockIdx.y, cfg.vocab, again);
 }
 
 template <int DT, int NB, bool LSE, bool EXTRA>
 __global__ __launch_bounds__(NT, (HELD_RESIDENT<DT, NB>)) void k_held_table(LaunchCfg cfg) {
     __shared__ Shared sh;
     __shared__ HeldBias bias[1];
-    held_row<DT, NB, LSE, EXTRA, false>((const LILY_CONST RowArgs*)cfg.table + blockIdx.y, cfg, sh, EXTRA ? bias : nullptr);
+    Resum again;
+    held_row<DT, NB, LSE, EXTRA, false>((const LILY_CONST RowArgs*)cfg.table + blockIdx.y, cfg, sh, EXTRA ? bias : nullptr, again);
+    sum_again<DT, LSE>((const LILY_CONST RowArgs*)cfg.table + blockIdx.y, cfg.vocab, again);
 }
 
 // A verify pass whose rows are independent (see k_rows_verify).
@@ -620,7 +623,8 @@ template <int DT, int NB>
 __global__ __launch_bounds__(NT, (HELD_RESIDENT<DT, NB>)) void k_held_verify(InlineRows rows, LaunchCfg cfg) {
     __shared__ Shared sh;
     const LILY_CONST RowArgs* table = (const LILY_CONST RowArgs*)__builtin_amdgcn_kernarg_segment_ptr();
-    const bool finished = held_row<DT, NB, false, false, true>(table + blockIdx.y, cfg, sh, nullptr);
+    Resum again;
+    const bool finished = held_row<DT, NB, false, false, true>(table + blockIdx.y, cfg, sh, nullptr, again);
     if (!finished || threadIdx.x != 0u || cfg.accept_ctrl == nullptr) {
         return;
     }

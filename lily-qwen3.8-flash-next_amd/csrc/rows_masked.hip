@@ -77,10 +77,10 @@ struct MaskedSum {
         s = 0.0;
     }
     __device__ __forceinline__ float rebase(float cm, float c) {
-        const float mcn = fmaxf(mc, cm * c), safe = fmaxf(mcn, F32_LOWEST);
-        s *= (double)__builtin_amdgcn_exp2f(mc - safe);
+        const float mcn = lse_ref(fmaxf(mc, cm * c));
+        s *= (double)__builtin_amdgcn_exp2f(mc - mcn);
         mc = mcn;
-        return safe;
+        return mcn;
     }
     __device__ __forceinline__ void term(float v, float c, float safe) { s += (double)__builtin_amdgcn_exp2f(__builtin_fmaf(v, c, -safe)); }
     __device__ __forceinline__ void add_one(float v, float c) {
@@ -92,7 +92,7 @@ struct MaskedSum {
 };
 
 template <int DT, bool LSE>
-__device__ __forceinline__ void masked_row(const LILY_CONST RowArgs* src, const LaunchCfg& cfg, Shared& sh, MaskedShared& ms) {
+__device__ __forceinline__ void masked_row(const LILY_CONST RowArgs* src, const LaunchCfg& cfg, Shared& sh, MaskedShared& ms, Resum& again) {
     RowArgs a;
     load_row_args(a, src);
     apply_selection(a);
@@ -632,7 +632,7 @@ __device__ __forceinline__ void masked_row(const LILY_CONST RowArgs* src, const 
     read_again(t, src);
     if (forced) {
         if (tid == 0) {
-            finish_token<DT>(t, sh, t.forced, vocab);
+            finish_token<DT, LSE>(t, sh, t.forced, vocab, again);
         }
         return;
     }
@@ -653,7 +653,7 @@ __device__ __forceinline__ void masked_row(const LILY_CONST RowArgs* src, const 
     if (tid >= NT) {
         return;   // (the draw is four waves' work: a barrier waits for those that are left)
     }
-    tail<DT, true, false>(t, vocab, t.step + cfg.step_delta, k, true, dyn_lds, sh, cfg);
+    tail<DT, LSE, true, false>(t, vocab, t.step + cfg.step_delta, k, true, dyn_lds, sh, cfg, again);
     phase(cfg, 7);
 }
 
@@ -662,14 +662,18 @@ __global__ __launch_bounds__(MT) void k_masked_inline(InlineRows rows, LaunchCfg
     __shared__ Shared sh;
     __shared__ MaskedShared ms;
     const LILY_CONST RowArgs* table = (const LILY_CONST RowArgs*)__builtin_amdgcn_kernarg_segment_ptr();
-    masked_row<DT, LSE>(table + blockIdx.y, cfg, sh, ms);
+    Resum again;
+    masked_row<DT, LSE>(table + blockIdx.y, cfg, sh, ms, again);
+    sum_again<DT, LSE>(table + blockIdx.y, cfg.vocab, again);
 }
 
 template <int DT, bool LSE>
 __global__ __launch_bounds__(MT) void k_masked_table(LaunchCfg cfg) {
     __shared__ Shared sh;
     __shared__ MaskedShared ms;
-    masked_row<DT, LSE>((const LILY_CONST RowArgs*)cfg.table + blockIdx.y, cfg, sh, ms);
+    Resum again;
+    masked_row<DT, LSE>((const LILY_CONST RowArgs*)cfg.table + blockIdx.y, cfg, sh, ms, again);
+    sum_again<DT, LSE>((const LILY_CONST RowArgs*)cfg.table + blockIdx.y, cfg.vocab, again);
 }
 
 template <int DT, bool LSE>

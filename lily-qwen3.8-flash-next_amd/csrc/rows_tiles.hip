@@ -47,7 +47,7 @@ constexpr uint32_t REF_CAP = 2048;                       // pieces evaluated ele
 template <int DT, bool LSE, bool EXTRA>
 __device__ __forceinline__ void tiles_row(const LILY_CONST RowArgs* table, const LaunchCfg& cfg, const float* tile_max,
                                           const float* tile_sum, uint32_t tiles, const uint32_t* tile_row,
-                                          uint32_t* served) {
+                                          uint32_t* served, Resum& again) {
     __shared__ Shared sh;
     __shared__ uint16_t listed[TILES_MAX];   // tiles to read; bit 15: summed element by element
     __shared__ uint32_t refs[REF_CAP];       // pieces to evaluate: first id; bit 31: summed
@@ -242,7 +242,7 @@ __device__ __forceinline__ void tiles_row(const LILY_CONST RowArgs* table, const
             lse_reduce(sh, lse);
         }
         if (tid == 0) {
-            finish_token<DT>(a, sh, a.forced, vocab);
+            finish_token<DT, LSE>(a, sh, a.forced, vocab, again);
         }
         return;
     }
@@ -480,7 +480,7 @@ __device__ __forceinline__ void tiles_row(const LILY_CONST RowArgs* table, const
         atomicAdd(&cfg.path_stats[took], 1u);
     }
     phase(cfg, 6);
-    tail<DT, false>(a, vocab, step, n, sorted, cand, sh, cfg);
+    tail<DT, LSE, false>(a, vocab, step, n, sorted, cand, sh, cfg, again);
     phase(cfg, 7);
 }
 
@@ -488,14 +488,18 @@ template <int DT, bool LSE, bool EXTRA>
 __global__ __launch_bounds__(NT, 4) void k_rows_tiles(LaunchCfg cfg, const float* tile_max,
                                                       const float* tile_sum, uint32_t tiles,
                                                       const uint32_t* tile_row, uint32_t* served) {
-    tiles_row<DT, LSE, EXTRA>((const LILY_CONST RowArgs*)cfg.table, cfg, tile_max, tile_sum, tiles, tile_row, served);
+    Resum again;
+    tiles_row<DT, LSE, EXTRA>((const LILY_CONST RowArgs*)cfg.table, cfg, tile_max, tile_sum, tiles, tile_row, served, again);
+    sum_again<DT, LSE>((const LILY_CONST RowArgs*)cfg.table + blockIdx.y, cfg.vocab, again);
 }
 
 template <int DT, bool LSE, bool EXTRA>
 __global__ __launch_bounds__(NT, 4) void k_rows_tiles_inline(InlineRows rows, LaunchCfg cfg, const float* tile_max,
                                                              const float* tile_sum, uint32_t tiles) {
-    tiles_row<DT, LSE, EXTRA>((const LILY_CONST RowArgs*)__builtin_amdgcn_kernarg_segment_ptr(), cfg, tile_max, tile_sum, tiles,
-                              nullptr, nullptr);
+    const LILY_CONST RowArgs* table = (const LILY_CONST RowArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+    Resum again;
+    tiles_row<DT, LSE, EXTRA>(table, cfg, tile_max, tile_sum, tiles, nullptr, nullptr, again);
+    sum_again<DT, LSE>(table + blockIdx.y, cfg.vocab, again);
 }
 
 static hipError_t launch_tiles(hipStream_t stream, int dtype, bool lse, bool extra, uint32_t rows, const LaunchCfg& cfg_in,

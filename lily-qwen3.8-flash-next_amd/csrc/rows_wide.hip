@@ -539,7 +539,9 @@ __device__ __forceinline__ void wide_finish(const LILY_CONST RowArgs* src, const
     if (SIXTEEN && tid >= NT) {
         return;   // (the draw is four waves' work: a barrier waits for those that are left)
     }
-    tail<DT, true>(a, cfg.vocab, step, n, sorted, cand, sh, cfg);
+    Resum again;
+    tail<DT, LSE, true>(a, cfg.vocab, step, n, sorted, cand, sh, cfg, again);
+    sum_again<DT, LSE>(src, cfg.vocab, again);
 }
 
 // ---- second launch: the values that reach the bound, then merge, select and tail

@@ -184,17 +184,24 @@ __device__ __forceinline__ uint32_t pick_sequential(const float* prefix, uint32_
     return n - 1;
 }
 
+// A row whose sum its references could not hold (LSE_FAR): set by the one thread that finishes it, for sum_again().
+struct Resum {
+    bool needed = false;
+    uint32_t id;
+    float u;   // the id's value before the temperature
+};
+
 // log p(id) = (u*c2 - mc - log2 s) * ln 2, with the id's exponent u*c2 formed exactly as
 // the row sum formed its terms, so the two cancel when the id carries all the mass.
 // Emits `id` and, when asked, its log-probability, with the memory operations of both in one
 // round trip: the count's atomic increment returns the count the penalties used, and the logit
-// loads beside it.
-template <int DT>
-__device__ __forceinline__ void finish_token(const RowArgs& a, Shared& sh, uint32_t id, uint32_t vocab,
+// loads beside it.  LSE: false where no row of the launch asks for a log-probability.
+template <int DT, bool LSE>
+__device__ __forceinline__ void finish_token(const RowArgs& a, Shared& sh, uint32_t id, uint32_t vocab, Resum& again,
                                              bool in_order = false) {
     *a.out_id = id;
     const bool pen = (a.flags & F_PEN) != 0;
-    const bool want = a.out_logprob != nullptr;
+    const bool want = LSE && a.out_logprob != nullptr;
     if (id >= vocab) {
         if (want) {
             *a.out_logprob = NEG_INF;
@@ -223,7 +230,9 @@ __device__ __forceinline__ void finish_token(const RowArgs& a, Shared& sh, uint3
         before = atomicAdd(&a.counts[id], 1u);
         mark_listed(a.touched, words, id);
     }
-    const double base = want ? sh.lse_mc + log2(sh.lse_s) : 0.0;
+    const double mc = sh.lse_mc, s = sh.lse_s;
+    const bool sound = s > 0x1p-300 && s < 0x1p899 && __builtin_fabs(mc) < (double)LSE_FAR;   // (a term ends at 2^900)
+    const double base = want ? mc + log2(s) : 0.0;
     if (pen && !in_order && top <= before + 1u) {
         atomicMax(&a.touched[words], before + 1u);
         a.touched[words + 1u] = id;
@@ -234,6 +243,9 @@ __device__ __forceinline__ void finish_token(const RowArgs& a, Shared& sh, uint3
         if (u > NEG_INF) {
             const double e = (double)u * (double)a.c2 - base;
             lp = fminf((float)(e * 0.6931471805599453), 0.0f);  // the sum is approximate: clamp
+            again.needed = u < __builtin_huge_valf() && !(sound && e < 1.0);   // (no id is worth more than the row)
+            again.id = id;
+            again.u = u;
         }
         *a.out_logprob = lp;
     }
@@ -286,9 +298,9 @@ __device__ __forceinline__ float lane_f32(float v, uint32_t l) {
 // lane: `c` in descending order, 0 from lane k on (k >= 1 of them valid).
 // SPEC_WAVE: compile the speculative draw too (spec_d: the proposal, spec_qn: the length of the draft's
 // distribution, at most 64).
-template <int DT, bool SPEC_WAVE>
+template <int DT, bool LSE, bool SPEC_WAVE>
 __device__ __forceinline__ void tail_wave(const RowArgs& a, uint32_t vocab, uint32_t step, uint64_t c, uint32_t k_in, Shared& sh,
-                                          const LaunchCfg& cfg, uint32_t spec_d, uint32_t spec_qn) {
+                                          const LaunchCfg& cfg, uint32_t spec_d, uint32_t spec_qn, Resum& again) {
     const uint32_t k = (uint32_t)__builtin_amdgcn_readfirstlane((int)k_in);   // (the same in every lane)
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t top_key = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(c >> 32));
@@ -341,7 +353,7 @@ __device__ __forceinline__ void tail_wave(const RowArgs& a, uint32_t vocab, uint
         const float q_d = at_q != 0ull ? lane_f32(q_p, (uint32_t)__builtin_ctzll(at_q)) : 0.0f;
         if (u1 * q_d < p_d) {
             if (lane == 0) {
-                finish_token<DT>(a, sh, d, vocab, cfg.chain_rows != 0u);
+                finish_token<DT, LSE>(a, sh, d, vocab, again, cfg.chain_rows != 0u);
             }
             return;
         }
@@ -371,7 +383,7 @@ __device__ __forceinline__ void tail_wave(const RowArgs& a, uint32_t vocab, uint
         const uint32_t slot = picks != 0ull ? (uint32_t)__builtin_ctzll(picks) : kept - 1u;
         const uint32_t id = ~(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)c, (int)slot);
         if (lane == 0) {
-            finish_token<DT>(a, sh, id, vocab, cfg.chain_rows != 0u);
+            finish_token<DT, LSE>(a, sh, id, vocab, again, cfg.chain_rows != 0u);
         }
         return;
     }
@@ -379,7 +391,7 @@ __device__ __forceinline__ void tail_wave(const RowArgs& a, uint32_t vocab, uint
     const uint32_t slot = hits != 0ull ? (uint32_t)__builtin_ctzll(hits) : kept - 1u;
     const uint32_t id = ~(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)c, (int)slot);
     if (lane == 0) {
-        finish_token<DT>(a, sh, id, vocab, cfg.chain_rows != 0u);
+        finish_token<DT, LSE>(a, sh, id, vocab, again, cfg.chain_rows != 0u);
     }
 }
 
@@ -387,9 +399,9 @@ __device__ __forceinline__ void tail_wave(const RowArgs& a, uint32_t vocab, uint
 // SPEC_WAVE: compile the speculative draw of at most 64 candidates as one wave too (the kernel
 // of rows that draw in order, where every row's tail is a step of a chain; elsewhere its scalar
 // registers would be taken from the scan).
-template <int DT, bool BIG, bool SPEC_WAVE = false>
+template <int DT, bool LSE, bool BIG, bool SPEC_WAVE = false>
 __device__ __forceinline__ void tail(const RowArgs& a, uint32_t vocab, uint32_t step, uint32_t n, bool sorted,
-                     uint64_t* cand, Shared& sh, const LaunchCfg& cfg) {
+                     uint64_t* cand, Shared& sh, const LaunchCfg& cfg, Resum& again) {
 #ifdef LILY_TAIL_TRACE
 #define TAIL_MARK(i) phase(cfg, i)
 #else
@@ -417,7 +429,7 @@ __device__ __forceinline__ void tail(const RowArgs& a, uint32_t vocab, uint32_t 
     const float top = composite_value(cand[0]);
     if (k <= 64u && (a.mode != MODE_SPEC || (SPEC_WAVE && spec_qn <= 64u))) {
         if (tid < 64u) {
-            tail_wave<DT, SPEC_WAVE>(a, vocab, step, tid < k ? cand[tid] : 0ull, k, sh, cfg, spec_d, spec_qn);
+            tail_wave<DT, LSE, SPEC_WAVE>(a, vocab, step, tid < k ? cand[tid] : 0ull, k, sh, cfg, spec_d, spec_qn, again);
         }
         return;
     }
@@ -618,7 +630,7 @@ __device__ __forceinline__ void tail(const RowArgs& a, uint32_t vocab, uint32_t 
         TAIL_MARK(12);
         if (tid == 0) {
             const uint32_t id = composite_id(cand[slot]);
-            finish_token<DT>(a, sh, id, vocab, cfg.chain_rows != 0u);
+            finish_token<DT, LSE>(a, sh, id, vocab, again, cfg.chain_rows != 0u);
         }
         return;
     }
@@ -639,7 +651,7 @@ __device__ __forceinline__ void tail(const RowArgs& a, uint32_t vocab, uint32_t 
     __syncthreads();
     if (u1 * sh.q_d < sh.p_d) {
         if (tid == 0) {
-            finish_token<DT>(a, sh, d, vocab, cfg.chain_rows != 0u);
+            finish_token<DT, LSE>(a, sh, d, vocab, again, cfg.chain_rows != 0u);
         }
         return;
     }
@@ -692,7 +704,7 @@ __device__ __forceinline__ void tail(const RowArgs& a, uint32_t vocab, uint32_t 
             slot = pick_sequential(sh.cum, n_keep, u2 * mass);
         }
         const uint32_t id = composite_id(cand[slot]);
-        finish_token<DT>(a, sh, id, vocab, cfg.chain_rows != 0u);
+        finish_token<DT, LSE>(a, sh, id, vocab, again, cfg.chain_rows != 0u);
     }
 }
 
