@@ -118,10 +118,11 @@ __device__ __forceinline__ void read_again(RowArgs& a, const LILY_CONST RowArgs*
     apply_selection(a);
 }
 
-// The log-probability of a row whose sum its references could not hold, by its first wave when everything else is done (`again` of its first lane; called by all
-// waves, once a kernel: a copy at every place that finishes a row took 0.5 us of 72 from the batch of 1 024).  Every
-// difference is formed first, which is right at any size of the values; a value a lane and trip to memory, some 3 ms for
-// 151 936 ids.
+// The log-probability of a row whose sum its references could not hold, by its first wave when everything else is done
+// (`again` of its first lane; called by all waves, once a kernel: a copy at every place that finishes a row took
+// 0.5 us of 72 from the batch of 1 024).  Every difference is formed first, which is right at any size of the values; a value
+// a lane and trip to memory, 0.7 ms for 151 936 ids (eight loads in flight 0.55: such rows, all their values
+// equal as a rule, take 0.1 to 3 ms before).
 template <int DT, bool LSE>
 __device__ __forceinline__ void sum_again(const LILY_CONST RowArgs* src, uint32_t vocab, const Resum& again) {
     if (!LSE || __builtin_expect(__ballot(again.needed) == 0ull, 1)) {
