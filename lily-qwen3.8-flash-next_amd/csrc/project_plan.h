@@ -55,14 +55,14 @@ inline ProjectArgs project_args(const lily_projection& p, const ProjectWorkspace
 }
 
 // Which kernel, and how many parts of d: by an estimate of each one's time in us, from what they take on the chip
-// (rows x n x d in bf16, the estimate in brackets):
+// (rows x n x d in bf16, three sets of operands in turn, the estimate in brackets):
 //   few rows     a compute unit takes in 85 GB/s through LDS: 64 x 4096 x 4096 10.1 (10.5), 64 x 16384 x 2048 19.4 (18.2)
 //   64 x 64      a line of d 0.22 where a compute unit has one tile, 0.21 a round of tiles: 256 x 4096 x 4096 17.8 (18.1),
 //                512 x 4096 x 4096 28.6 (30.9), 64 x 16384 x 2048 16.4 (16.2: memory)
 //   128 x 128    a line 0.48 a round, 0.38 where tiles are few: 1024 x 4096 x 4096 36.7 (36.7), 8192 x 4096 x 4096 259 (252)
 //   256 x 256    1.45 a line, and 13 for every tile's epilogue, which nothing hides, 29 with a residual: 8192 x 4096 x 4096
-//                213 (214), with a residual 238 (246) where 128 x 128 takes 265 (264); 8192 x 8192 x 2048 248 (240) against 270
-//                (252), but with a residual 317 (304) against 300 (276)
+//                213 (214), with a residual 238 (246) where 128 x 128 takes 255 to 265 (264); 8192 x 8192 x 2048 240 (240) against
+//                266 (252), but with a residual 302 (304) against 292 (276)
 // Parts of d: a launch more (1.5), and the parts' sums written and read at 5.5 TB/s: 64 x 1000 x 8192 in eight 10.6 (10.5)
 // against 25.5 in one; 300 x 4096 x 4096 in two of 128 x 128 22.2 (23.3), where 64 x 64 takes 28.1 in one and 25.9 in two
 // and 128 x 128 30.4 in one; 512 x 4096 x 4096 25.9 (29.9); 100 x 10 007 x 4096 in E4M3, 79 tiles of 128 x 128, in two
@@ -70,6 +70,14 @@ inline ProjectArgs project_args(const lily_projection& p, const ProjectWorkspace
 // Rows that do not start at lines of 128 bytes take two requests a line, 1.4 times as long where tiles are few, 1.15 times where
 // compute units have several: the same with rows of 4128 bytes 19.3 in three parts (18.9), 20.2 in two (18.9), 23.4 in one of
 // 64 x 64 (22.8); 5000 x 7000 x 1504 bf16 125 by 128 x 128 (125), 135 by 256 x 256 (145).
+// Weights that come from memory every time (700 MB of them in turn, where three sets of 32 MB stay in the last-level cache) take
+// longer and change no choice above: 64 x 4096 x 4096 14.2 by few rows and by 64 x 64, 256 rows 22.4 and 23.2 by 64 x 64 and
+// 128 x 128, 1024 rows 42 by 128 x 128, 65 by 64 x 64.
+// The rates are those of bf16 and of the 8-bit products.  E4M3 with an f32 output widens its operands, four products and their
+// conversions for a line's two in bf16, which the estimate does not know: it is up to half of what these take, and its choice,
+// against the best of the others (700 MB in turn): 64 x 4096 x 4096 few rows 9.4, 64 x 64 13.1; 256 rows 64 x 64 18.6, 128 x 128 23.8;
+// 1024 rows 128 x 128 39, 64 x 64 46; 128 x 151 936 x 4096 128 x 128 181, 64 x 64 228; but 4096 rows 256 x 256 124, 128 x 128 113; 8192
+// rows 236 and 221; 8192 x 12 288 x 4096 687 and 642; and 32 x 151 936 x 4096 few rows 190, 64 x 64 144.
 struct ProjectPlan {
     uint32_t tile = 0;     // 0: few rows
     uint32_t splits = 1;
