@@ -628,6 +628,188 @@ int lily_process_logits(lily_sampler_t* s, const lily_rows* batch, const lily_lo
  * LILY_SAMPLER_HANDOVER=strict takes the sums out of the launch that writes. */
 int lily_plan_process_logits(lily_plan_t* p, const lily_logits_out* out);
 
+/* ---- Training and serving a draft head: the layer norm and its backward pass.
+ *
+ *     h = x + residual, rounded to stream_dtype (h = x where residual_dev is NULL)
+ *     mean = sum(h) / d,  rstd = 1 / sqrt(sum((h - mean)^2) / d + eps)
+ *     y = (h - mean) * rstd * weight + bias
+ * in f32.  h goes to sum_dev, mean and rstd (what the backward pass reads) to theirs, where they are given; y
+ * to out_dev: f32, bf16 (nearest even) or E4M3 with one f32 scale a row (scale_block 0) or one for each
+ * LILY_BLOCK elements of a row (scale_block LILY_BLOCK: what lily_project_blocks takes): scale = max|y| / 448,
+ * q = E4M3(y / scale).  A row or block whose largest |y| lies below 2^-116 has scale 0 and zeros; one that holds a
+ * value that is not finite has a scale that is not, too.  What is not finite in h makes its whole row a NaN.
+ *
+ * Rows hold d (1 .. LILY_NORM_MAX_D) elements, strides count elements and may be anything from d on.  What may
+ * lie where, and how many rows a call takes, is as lily_rms_norm has it.  Enqueued on the sampler's stream; no
+ * workspace. */
+#define LILY_BLOCK 128u
+typedef struct lily_layer {
+    uint32_t rows;
+    uint32_t d;
+    const void* x_dev;            /* [rows][x_stride] of x_dtype */
+    uint64_t x_stride;
+    const void* residual_dev;     /* [rows][residual_stride] of stream_dtype, or NULL */
+    uint64_t residual_stride;
+    void* sum_dev;                /* [rows][sum_stride] of stream_dtype, or NULL; only with a residual */
+    uint64_t sum_stride;
+    const void* weight_dev;       /* [d] of weight_dtype, or NULL (ones) */
+    const void* bias_dev;         /* [d] of weight_dtype, or NULL (zeros) */
+    void* out_dev;                /* [rows][out_stride] of out_dtype */
+    uint64_t out_stride;
+    float* scales_dev;            /* with LILY_E4M3 only, and required there: [rows] or [rows][scales_stride] */
+    uint64_t scales_stride;       /* scale_block LILY_BLOCK: floats, from ceil(d / LILY_BLOCK) on */
+    float* mean_dev;              /* [rows] or NULL */
+    float* rstd_dev;              /* [rows] or NULL */
+    uint32_t x_dtype;             /* LILY_F32 or LILY_BF16, as stream_dtype and weight_dtype */
+    uint32_t stream_dtype;
+    uint32_t weight_dtype;
+    uint32_t out_dtype;           /* LILY_F32, LILY_BF16 or LILY_E4M3 */
+    uint32_t scale_block;         /* 0 or LILY_BLOCK */
+    float eps;                    /* finite, >= 0 */
+} lily_layer;
+int lily_layer_norm(lily_sampler_t* s, const lily_layer* layer);
+
+/* The backward pass, from h and what the forward pass left of it.  With x = (h - mean) * rstd and g = grad * weight:
+ *     grad_x = past + rstd * (g - sum(g) / d - x * sum(g * x) / d)
+ *     grad_weight = sum over the rows of grad * x,   grad_bias = sum over the rows of grad
+ * `past` is the gradient that reaches h on the residual stream, past the norm.  Sums in f32, those over the rows in
+ * an order that rows and d alone decide (the same call gives the same bits); accumulate 1 adds them to what
+ * grad_weight_dev and grad_bias_dev hold.  A row that holds what is not finite makes its grad_x and the sums so.
+ *
+ * At least one of grad_x_dev, grad_weight_dev and grad_bias_dev is given.  grad_x_dev may be grad_dev, h_dev or
+ * past_dev, with the same type and stride; other overlaps are refused.  Rows as the forward pass takes them.
+ * Enqueued on the sampler's stream, up to three launches; sums over the rows pass through the sampler's
+ * workspace: graphs captured from one sampler are replayed one after the other. */
+typedef struct lily_layer_grad {
+    uint32_t rows;
+    uint32_t d;
+    const void* grad_dev;         /* [rows][grad_stride] of grad_dtype */
+    uint64_t grad_stride;
+    const void* h_dev;            /* [rows][h_stride] of h_dtype */
+    uint64_t h_stride;
+    const float* mean_dev;        /* [rows] */
+    const float* rstd_dev;        /* [rows] */
+    const void* weight_dev;       /* [d] of weight_dtype, or NULL (ones) */
+    const void* past_dev;         /* [rows][past_stride] of grad_x_dtype, or NULL; only with grad_x */
+    uint64_t past_stride;
+    void* grad_x_dev;             /* [rows][grad_x_stride] of grad_x_dtype, or NULL */
+    uint64_t grad_x_stride;
+    float* grad_weight_dev;       /* [d] or NULL */
+    float* grad_bias_dev;         /* [d] or NULL */
+    uint32_t grad_dtype;          /* LILY_F32 or LILY_BF16, as the other three */
+    uint32_t h_dtype;
+    uint32_t weight_dtype;
+    uint32_t grad_x_dtype;
+    uint32_t accumulate;          /* 0 or 1 */
+} lily_layer_grad;
+int lily_layer_norm_backward(lily_sampler_t* s, const lily_layer_grad* grad);
+
+/* ---- 8-bit floats with a scale for each block, and their product.
+ *
+ * lily_quantize_blocks writes a matrix as E4M3 with a scale for each LILY_BLOCK elements of a row (block_rows 1:
+ * activations) or each LILY_BLOCK rows x LILY_BLOCK elements (block_rows LILY_BLOCK: weights): scale = max|x| / 448,
+ * q = E4M3(x / scale), in f32; the last blocks of a row and of the rows may be smaller.  A block whose largest |x| lies
+ * below 2^-116 has scale 0 and zeros; where one holds a NaN the scale and every q are NaN, and an infinity as its largest value
+ * gives an infinite scale, NaN for the infinities and zeros for the rest.  Any strides from a row's length on; out may not overlap x.
+ * Up to 2^28 - 1 blocks of LILY_BLOCK elements of a row (block_rows 1), 2^24 - 1 of LILY_BLOCK x LILY_BLOCK (LILY_ERR_RANGE
+ * beyond).  Enqueued on the sampler's stream, one launch, no workspace. */
+typedef struct lily_blocks {
+    uint32_t rows;
+    uint32_t d;
+    const void* x_dev;            /* [rows][x_stride] of x_dtype */
+    uint64_t x_stride;
+    void* out_dev;                /* E4M3 [rows][out_stride] */
+    uint64_t out_stride;
+    float* scales_dev;            /* [ceil(rows / block_rows)][scales_stride] */
+    uint64_t scales_stride;       /* floats, from ceil(d / LILY_BLOCK) on */
+    uint32_t x_dtype;             /* LILY_F32 or LILY_BF16 */
+    uint32_t block_rows;          /* 1 or LILY_BLOCK */
+} lily_blocks;
+int lily_quantize_blocks(lily_sampler_t* s, const lily_blocks* blocks);
+
+/*     out[r][v] = residual[r][v] + act(sum_b x_scales[r][b] * weight_scales[v / 128][b] * sum_{i in b} x[r][i] * weight[v][i] + bias[v])
+ * b the blocks of LILY_BLOCK elements of d, the last of which may be smaller.  x and weight are E4M3, contiguous along d; a
+ * block's products and their sum on the matrix cores, the blocks' sums times their scales added in f32, the epilogue in f32, one
+ * rounding to out_dtype.  Limits, alignment, overlaps, the workspace and graphs are as lily_project has them, and so is
+ * what a product of more than 16 rows with a bf16 output drops (of every eight neighbouring products what lies 2^-13 below
+ * the largest; the bound of a block's sum is scaled with it).  A block whose scale is 0 adds zeros; one whose scale is not finite makes what it
+ * reaches so. */
+typedef struct lily_block_projection {
+    uint32_t rows;
+    uint32_t n;                       /* outputs */
+    uint32_t d;                       /* a multiple of 16 */
+    uint32_t activation;              /* lily_activation */
+    const void* x_dev;                /* E4M3 [rows][x_stride] */
+    uint64_t x_stride;                /* elements, as every stride here */
+    const float* x_scales_dev;        /* [rows][x_scales_stride] */
+    uint64_t x_scales_stride;         /* from ceil(d / LILY_BLOCK) on */
+    const void* weight_dev;           /* E4M3 [n][weight_stride] */
+    uint64_t weight_stride;
+    const float* weight_scales_dev;   /* [ceil(n / LILY_BLOCK)][weight_scales_stride] */
+    uint64_t weight_scales_stride;
+    const void* bias_dev;             /* [n] of bias_dtype, or NULL */
+    const void* residual_dev;         /* [rows][residual_stride] of residual_dtype, or NULL */
+    uint64_t residual_stride;
+    void* out_dev;                    /* [rows][out_stride] of out_dtype */
+    uint64_t out_stride;
+    uint32_t bias_dtype;              /* LILY_F32 or LILY_BF16, as residual_dtype and out_dtype */
+    uint32_t residual_dtype;
+    uint32_t out_dtype;
+    uint32_t reserved;                /* must be 0 */
+} lily_block_projection;
+int lily_project_blocks(lily_sampler_t* s, const lily_block_projection* p);
+
+/* ---- Distillation: a student's rows of logits against a teacher's top ones.
+ *
+ * The teacher's list of a row is what a draw leaves (lily_rows.dbg_*, lily_draft_dist) or its best logits: up to k ids and values.
+ * An entry counts if it lies before counts[r] (where counts are given) and its id is below vocab (LILY_NO_TOKEN pads).  With T the
+ * temperature, z the student's row, q = softmax(z / T) over the whole vocabulary:
+ *   LILY_TEACHER_LOGITS   p_j = exp(t_j / T - teacher_lse[r]) with `rest`, exp(t_j / T) over the list's sum without
+ *   LILY_TEACHER_PROBS    p_j = t_j with `rest`, t_j over the list's sum without (a value below 0 is 0)
+ *     loss = T^2 * (sum_j p_j (log p_j - log q[id_j])  [+ P (log P - log Q)])
+ * where, with `rest`, everything outside the list is one outcome more: P = max(0, 1 - sum p_j), Q the sum of q outside the
+ * list.  A term whose p is 0 is 0.  Ids that stand in a list twice add their p (and count once in Q).  With w = grad_scale *
+ * row_weights[r] (1 where NULL) the gradient of w * loss is
+ *     grad_v = w T (q_v sum p - p_v);   with `rest`, for ids outside the list, w T (q_v - P q_v / Q)
+ * A row none of whose entries count has loss 0 and a gradient of zeros, and so has the gradient of a row whose w is 0, whatever it holds.
+ * Otherwise a NaN or +inf in a student's row, or a row of -inf alone, makes its loss and whole gradient NaN, as a NaN among the values that count does;
+ * -inf in some places is a q of 0 (its gradient -w T p, a loss of +inf where p > 0).
+ *
+ * lily_distill writes the loss, stats (what the backward pass reads: the row's largest value z0 and log(sum of exp((z - z0) / T)),
+ * the same two of the ids outside the list, or zeros without `rest`) and the gradient, each where given; lily_distill_backward
+ * writes the gradient from stats.  grad_dev may be logits_dev with the same type and stride; other overlaps of an output
+ * are refused.  Vocabularies up to 2^24, lists up to LILY_SAMPLE_K_CAP, rows x vocab as far as a launch reaches
+ * (LILY_ERR_RANGE beyond).  Enqueued on the sampler's stream; a row's slices meet in the sampler's workspace: graphs captured from
+ * one sampler are replayed one after the other. */
+typedef enum lily_teacher { LILY_TEACHER_LOGITS = 0, LILY_TEACHER_PROBS = 1 } lily_teacher;
+typedef struct lily_distillation {
+    uint32_t rows;
+    uint32_t vocab;
+    const void* logits_dev;           /* [rows][logits_stride] of logits_dtype */
+    uint64_t logits_stride;
+    const uint32_t* ids_dev;          /* [rows][ids_stride] */
+    uint64_t ids_stride;
+    const void* values_dev;           /* [rows][values_stride] of values_dtype */
+    uint64_t values_stride;
+    const uint32_t* counts_dev;       /* [rows] or NULL (k) */
+    const float* teacher_lse_dev;     /* [rows]: log(sum of exp(t / T)) over the teacher's whole row; with LILY_TEACHER_LOGITS and `rest` only */
+    const float* row_weights_dev;     /* [rows] or NULL (ones) */
+    float* loss_dev;                  /* [rows] or NULL (lily_distill) */
+    float* stats_dev;                 /* [rows][4]; lily_distill: out, or NULL; lily_distill_backward: in */
+    void* grad_dev;                   /* [rows][grad_stride] of grad_dtype, or NULL (lily_distill) */
+    uint64_t grad_stride;
+    uint32_t k;                       /* entries a list holds room for, 1 .. LILY_SAMPLE_K_CAP */
+    uint32_t teacher;                 /* lily_teacher */
+    uint32_t rest;                    /* 0 or 1 */
+    uint32_t logits_dtype;            /* LILY_F32 or LILY_BF16, as values_dtype and grad_dtype */
+    uint32_t values_dtype;
+    uint32_t grad_dtype;
+    float temperature;                /* finite, > 0 */
+    float grad_scale;                 /* finite */
+} lily_distillation;
+int lily_distill(lily_sampler_t* s, const lily_distillation* d);
+int lily_distill_backward(lily_sampler_t* s, const lily_distillation* d);
+
 #ifdef __cplusplus
 }
 #endif

@@ -53,8 +53,14 @@ def units():
     out.append(("logits_rows.hip", "logits_rows.o", []))
     out.append(("project_few.hip", "project_few.o", []))
     out.append(("project_tiles.hip", "project_tiles.o", []))
+    out.append(("project_blocks.hip", "project_blocks.o", []))
+    out.append(("blocks.hip", "blocks.o", []))
+    out.append(("layer_norm.hip", "layer_norm.o", []))
+    out.append(("distill.hip", "distill.o", []))
     out.append(("sampler_api.cpp", "sampler_api.o", []))
     out.append(("operators_api.cpp", "operators_api.o", []))
+    out.append(("blocks_api.cpp", "blocks_api.o", []))
+    out.append(("learn_api.cpp", "learn_api.o", []))
     return out
 
 

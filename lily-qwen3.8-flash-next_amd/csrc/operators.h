@@ -25,4 +25,19 @@ struct ProjectWorkspace {
 };
 hipError_t launch_project(hipStream_t stream, const lily_projection& p, const ProjectWorkspace& ws);
 
+// The layer norm and its backward pass (layer_norm.hip): rows as the norm has them.
+hipError_t launch_layer_norm(hipStream_t stream, const lily_layer& layer);
+hipError_t launch_layer_norm_backward(hipStream_t stream, const lily_layer_grad& grad, const ProjectWorkspace& ws);
+
+// 8-bit floats with a scale for each block (blocks.hip), and their product (project_blocks.hip).
+hipError_t launch_quantize_blocks(hipStream_t stream, const lily_blocks& blocks);
+hipError_t launch_project_blocks(hipStream_t stream, const lily_block_projection& p, const ProjectWorkspace& ws);
+
+// Distillation (distill.hip): a workgroup takes a slice of a row.
+constexpr uint32_t DISTILL_SLICE = 8192, DISTILL_THREADS = 256;
+constexpr uint64_t distill_threads(uint32_t rows, uint32_t vocab) {
+    return (uint64_t)rows * ((vocab + DISTILL_SLICE - 1u) / DISTILL_SLICE) * DISTILL_THREADS;
+}
+hipError_t launch_distill(hipStream_t stream, const lily_distillation& d, bool backward, const ProjectWorkspace& ws);
+
 }  // namespace lily

@@ -7,26 +7,12 @@
 
 #include "../../include/lily_sampler.h"
 #include "api_internal.h"
-#include "device_scope.h"
-#include "operand_span.h"
 #include "operators.h"
+#include "operators_check.h"
 
 using namespace lily;
 
 namespace {
-
-#define HIP_TRY(call)                                                                         \
-    do {                                                                                      \
-        hipError_t e_ = (call);                                                               \
-        if (e_ != hipSuccess) {                                                               \
-            return api_fail(LILY_ERR_HIP, "%s: %s", #call, hipGetErrorString(e_));            \
-        }                                                                                     \
-    } while (0)
-#define ON_DEVICE(device)                 \
-    DeviceScope device_scope_(device);    \
-    HIP_TRY(device_scope_.err)
-
-constexpr uint32_t MAX_THREADS = 0xffffffffu;   // of a launch
 
 int check_norm(const lily_norm* n) {
     if (n == nullptr || n->x_dev == nullptr || n->out_dev == nullptr) {
@@ -70,13 +56,8 @@ int check_norm(const lily_norm* n) {
     const Span out = span(n->out_dev, n->rows, n->d, n->out_stride, n->out_dtype);
     const Span w = span(n->weight_dev, 1, n->d, n->d, n->weight_dtype);
     const Span scales = span(n->scales_dev, 1, n->rows, n->rows, LILY_F32);
-    for (const Span* s : {&x, &res, &sum, &out, &w, &scales}) {
-        if (!fits(*s)) {
-            return api_fail(LILY_ERR_RANGE, "rows and strides reach beyond the address space");
-        }
-        if (s->rows != 0u && (s->at % size_of(s->dtype) != 0u)) {
-            return api_fail(LILY_ERR_INVALID_ARG, "an array does not start at a multiple of its element's size");
-        }
+    if (int rc = check_places({&x, &res, &sum, &out, &w, &scales})) {
+        return rc;
     }
     for (const Span* o : {&sum, &out}) {
         for (const Span* i : {&x, &res}) {
@@ -143,13 +124,8 @@ int check_projection(const lily_projection* p) {
     if ((p->rows > 1u && x.stride > (1u << 23)) || (p->n > 1u && w.stride > (1u << 23))) {
         return api_fail(LILY_ERR_RANGE, "rows of x and weight lie at most 2^23 bytes apart");
     }
-    for (const Span* s : {&x, &w, &out, &res, &bias, &xs, &ws}) {
-        if (!fits(*s)) {
-            return api_fail(LILY_ERR_RANGE, "rows and strides reach beyond the address space");
-        }
-        if (s->rows != 0u && (s->at % size_of(s->dtype) != 0u)) {
-            return api_fail(LILY_ERR_INVALID_ARG, "an array does not start at a multiple of its element's size");
-        }
+    if (int rc = check_places({&x, &w, &out, &res, &bias, &xs, &ws})) {
+        return rc;
     }
     for (const Span* i : {&x, &w, &bias, &xs, &ws}) {
         if (overlap(out, *i)) {
@@ -160,10 +136,6 @@ int check_projection(const lily_projection* p) {
         return api_fail(LILY_ERR_INVALID_ARG, "out overlaps the residual without being it");
     }
     return LILY_OK;
-}
-
-int need_sampler(const lily_sampler_t* s) {
-    return s != nullptr ? LILY_OK : api_fail(LILY_ERR_INVALID_ARG, "sampler is null");
 }
 
 }  // namespace

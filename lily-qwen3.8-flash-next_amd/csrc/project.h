@@ -34,7 +34,10 @@ struct Frag {
 // exactly).  That leaves up to 7 * 2^-13 of each group's largest product, 6e-5 of the result for normal
 // data: a seventieth of the rounding of a bf16 output, and only such outputs take it.
 // PRODUCT_E4M3_WIDE turns both operands into bf16 (exact) on their way: products and sums as bf16 has them.
-enum Products { PRODUCT_BF16, PRODUCT_E4M3, PRODUCT_E4M3_WIDE };
+// PRODUCT_BLOCKS and PRODUCT_BLOCKS_WIDE are the same two for operands with a scale for each 128 elements, which are 128 bytes:
+// a line's products are summed by themselves, and their sum times both scales is added in f32.
+enum Products { PRODUCT_BF16, PRODUCT_E4M3, PRODUCT_E4M3_WIDE, PRODUCT_BLOCKS, PRODUCT_BLOCKS_WIDE };
+constexpr bool in_blocks(Products p) { return p == PRODUCT_BLOCKS || p == PRODUCT_BLOCKS_WIDE; }
 
 typedef __bf16 pj_bf16x2 __attribute__((ext_vector_type(2)));
 
@@ -48,8 +51,8 @@ __device__ __forceinline__ bf16x8 widened(uint32_t a, uint32_t b) {
 
 template <Products P>
 __device__ __forceinline__ f32x4 product(const Frag& w, const Frag& x, f32x4 c) {
-    static_assert(P != PRODUCT_E4M3, "few rows are read at the speed of memory: they take the exact products");
-    if constexpr (P == PRODUCT_E4M3_WIDE) {
+    static_assert(P != PRODUCT_E4M3 && P != PRODUCT_BLOCKS, "few rows are read at the speed of memory: they take the exact products");
+    if constexpr (P == PRODUCT_E4M3_WIDE || P == PRODUCT_BLOCKS_WIDE) {
         c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widened(w.lo[0], w.lo[1]), widened(x.lo[0], x.lo[1]), c, 0, 0, 0);
         c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widened(w.lo[2], w.lo[3]), widened(x.lo[2], x.lo[3]), c, 0, 0, 0);
         c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widened(w.hi[0], w.hi[1]), widened(x.hi[0], x.hi[1]), c, 0, 0, 0);
@@ -209,8 +212,25 @@ struct Finish {
     }
 };
 
-hipError_t launch_project_few(hipStream_t stream, const ProjectArgs& a, bool e4m3);
+// What a lane knows of the weights' scales: those of 64 lines of d, one a lane, handed out by line.  (A register that is filled in a
+// loop and read in it would be waited for, and with it everything asked for since, at every reading: it is waited for where it
+// is filled.)
+struct WeightScales {
+    const float* from;   // of the first line
+    uint32_t count;      // lines
+    float run;
+    __device__ __forceinline__ void ask(uint32_t line) {   // line: a multiple of 64 below count
+        run = gload(from + min(line + (threadIdx.x & 63u), count - 1u));
+    }
+    __device__ __forceinline__ void settle() { asm volatile("" : "+v"(run)); }
+    __device__ __forceinline__ float of(uint32_t line) const {
+        return lilym_bits_f32((uint32_t)__builtin_amdgcn_readlane((int)lilym_f32_bits(run), (int)(line & 63u)));
+    }
+};
+
+hipError_t launch_project_few(hipStream_t stream, const ProjectArgs& a, Products products);
 // `tile`: 64, 128 or 256 rows and outputs; a.splits parts of d.
 hipError_t launch_project_tiles(hipStream_t stream, const ProjectArgs& a, bool e4m3, uint32_t tile);
+hipError_t launch_project_join(hipStream_t stream, const ProjectArgs& a);
 
 }  // namespace lily

@@ -22,7 +22,9 @@ __device__ const uint4 few_zeros = {0u, 0u, 0u, 0u};   // what lies beyond d
 // RT: blocks of 16 rows of x; DEPTH: lines of a wave in flight.
 template <Products P, int RT, int WAVES, int DEPTH>
 __global__ void __launch_bounds__(WAVES * 64) k_project_few(const ProjectArgs a) {
-    constexpr uint32_t ROWS = 16 + 16 * RT, SLOT = ROWS * LINE, LOADS = ROWS / 8;
+    // (with a scale for each block a line brings its rows' scales, a lane one of them)
+    constexpr bool BLOCKS = in_blocks(P);
+    constexpr uint32_t ROWS = 16 + 16 * RT, SLOT = ROWS * LINE + (BLOCKS ? 256u : 0u), LOADS = ROWS / 8, ALL_LOADS = LOADS + (BLOCKS ? 1u : 0u);
     extern __shared__ __align__(16) char lds[];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const uint32_t g = lane >> 4, r = lane & 15u, v0 = blockIdx.x * 16u;
@@ -52,9 +54,14 @@ __global__ void __launch_bounds__(WAVES * 64) k_project_few(const ProjectArgs a)
     typedef __attribute__((address_space(1))) const void* gptr;
     typedef __attribute__((address_space(3))) void* lptr;
     char* ring = lds + wave * (DEPTH * SLOT);
+    const float* x_scale = BLOCKS ? a.x_blocks + (uint64_t)min(lane, a.rows - 1u) * a.x_blocks_stride + from : nullptr;
+    WeightScales w_scales = {BLOCKS ? a.w_blocks + (uint64_t)(v0 / LILY_BLOCK) * a.w_blocks_stride + from : nullptr, count, 0.0f};
     auto ask = [&](uint32_t l, uint32_t slot) {
         char* base = ring + slot * SLOT;
         const uint32_t at = l * LINE;
+        if constexpr (BLOCKS) {
+            __builtin_amdgcn_global_load_lds((gptr)(x_scale + l), (lptr)(base + ROWS * LINE), 4, 0, 0);
+        }
         if ((from + l + 1u) * LINE <= a.d_bytes) {
 #pragma unroll
             for (uint32_t i = 0; i < LOADS; ++i) {
@@ -70,11 +77,17 @@ __global__ void __launch_bounds__(WAVES * 64) k_project_few(const ProjectArgs a)
             }
         }
     };
+    if (BLOCKS && count != 0u) {
+        w_scales.ask(0u);
+    }
 #pragma unroll
     for (uint32_t j = 0; j < DEPTH; ++j) {
         if (j < count) {
             ask(j, j);
         }
+    }
+    if constexpr (BLOCKS) {
+        w_scales.settle();
     }
     f32x4 acc[RT];
 #pragma unroll
@@ -85,7 +98,7 @@ __global__ void __launch_bounds__(WAVES * 64) k_project_few(const ProjectArgs a)
     uint32_t slot = 0;
     for (uint32_t l = 0; l < count; ++l) {
         if (l + DEPTH <= count) {
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * LOADS) : "memory");
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * ALL_LOADS) : "memory");
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
@@ -102,14 +115,38 @@ __global__ void __launch_bounds__(WAVES * 64) k_project_few(const ProjectArgs a)
         for (int t = 0; t < RT; ++t) {
             fx[t] = frag(1u + (uint32_t)t);
         }
+        float scale[RT];
+        if constexpr (BLOCKS) {
+            const float* scales = reinterpret_cast<const float*>(ring + slot * SLOT + ROWS * LINE);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                scale[t] = scales[(uint32_t)t * 16u + r];
+            }
+        }
         __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): the slot has been read
         __builtin_amdgcn_sched_barrier(0);
         if (l + DEPTH < count) {
             ask(l + DEPTH, slot);
         }
+        if constexpr (BLOCKS) {
+            if (l != 0u && (l & 63u) == 0u) {
+                w_scales.ask(l);
+                w_scales.settle();
+            }
+            const float w = w_scales.of(l);
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            acc[t] = product<P>(fw, fx[t], acc[t]);
+            for (int t = 0; t < RT; ++t) {
+                const f32x4 line = product<P>(fw, fx[t], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    acc[t][j] = __builtin_fmaf(line[j], scale[t] * w, acc[t][j]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                acc[t] = product<P>(fw, fx[t], acc[t]);
+            }
         }
         slot = slot + 1u == DEPTH ? 0u : slot + 1u;
     }
@@ -130,33 +167,32 @@ __global__ void __launch_bounds__(WAVES * 64) k_project_few(const ProjectArgs a)
     }
 }
 
-template <int RT, int WAVES, int DEPTH>
-hipError_t launch_few(hipStream_t stream, const ProjectArgs& a, bool e4m3) {
-    constexpr uint32_t lds = WAVES * DEPTH * (16 + 16 * RT) * LINE;
+template <Products P, int RT, int WAVES, int DEPTH>
+hipError_t launch_few_of(hipStream_t stream, const ProjectArgs& a) {
+    constexpr uint32_t lds = WAVES * DEPTH * ((16 + 16 * RT) * LINE + (in_blocks(P) ? 256u : 0u));
     static_assert(lds >= WAVES * RT * 1024, "the sums' place");
-    const dim3 grid((a.n + 15u) / 16u), block(WAVES * 64);
-    static LdsAllowed allowed[2];
-    const void* kernel = e4m3 ? (const void*)k_project_few<PRODUCT_E4M3_WIDE, RT, WAVES, DEPTH>
-                              : (const void*)k_project_few<PRODUCT_BF16, RT, WAVES, DEPTH>;
-    if (const hipError_t e = allowed[e4m3 ? 1 : 0].say(kernel, lds); e != hipSuccess) {
+    static LdsAllowed allowed;
+    if (const hipError_t e = allowed.say((const void*)k_project_few<P, RT, WAVES, DEPTH>, lds); e != hipSuccess) {
         return e;
     }
-    if (e4m3) {
-        hipLaunchKernelGGL((k_project_few<PRODUCT_E4M3_WIDE, RT, WAVES, DEPTH>), grid, block, lds, stream, a);
-    } else {
-        hipLaunchKernelGGL((k_project_few<PRODUCT_BF16, RT, WAVES, DEPTH>), grid, block, lds, stream, a);
-    }
+    hipLaunchKernelGGL((k_project_few<P, RT, WAVES, DEPTH>), dim3((a.n + 15u) / 16u), dim3(WAVES * 64), lds, stream, a);
     return hipGetLastError();
+}
+template <int RT, int WAVES, int DEPTH>
+hipError_t launch_few(hipStream_t stream, const ProjectArgs& a, Products products) {
+    return products == PRODUCT_BF16        ? launch_few_of<PRODUCT_BF16, RT, WAVES, DEPTH>(stream, a)
+           : products == PRODUCT_E4M3_WIDE ? launch_few_of<PRODUCT_E4M3_WIDE, RT, WAVES, DEPTH>(stream, a)
+                                           : launch_few_of<PRODUCT_BLOCKS_WIDE, RT, WAVES, DEPTH>(stream, a);
 }
 
 }  // namespace
 
 // (waves x lines of a wave in flight, d = 4096 bf16, n = 4096 / 151 936 in E4M3, us: 8 x 2 7.5 / 105, 8 x 4 7.7 / 150, 4 x 4
 // 7.8 / 103; 64 rows 4 x 2 10.1, 8 x 1 10.3, 4 x 4 10.4)
-hipError_t launch_project_few(hipStream_t stream, const ProjectArgs& a, bool e4m3) {
-    return a.rows <= 16u   ? launch_few<1, 8, 2>(stream, a, e4m3)
-           : a.rows <= 32u ? launch_few<2, 8, 2>(stream, a, e4m3)
-                           : launch_few<4, 4, 2>(stream, a, e4m3);
+hipError_t launch_project_few(hipStream_t stream, const ProjectArgs& a, Products products) {
+    return a.rows <= 16u   ? launch_few<1, 8, 2>(stream, a, products)
+           : a.rows <= 32u ? launch_few<2, 8, 2>(stream, a, products)
+                           : launch_few<4, 4, 2>(stream, a, products);
 }
 
 hipError_t launch_project(hipStream_t stream, const lily_projection& p, const ProjectWorkspace& ws) {
@@ -164,7 +200,7 @@ hipError_t launch_project(hipStream_t stream, const lily_projection& p, const Pr
     const bool e4m3 = p.dtype == LILY_E4M3;
     const ProjectPlan plan = project_plan(a, ws);
     a.splits = plan.splits;
-    return plan.tile == 0u ? launch_project_few(stream, a, e4m3) : launch_project_tiles(stream, a, e4m3, plan.tile);
+    return plan.tile == 0u ? launch_project_few(stream, a, e4m3 ? PRODUCT_E4M3_WIDE : PRODUCT_BF16) : launch_project_tiles(stream, a, e4m3, plan.tile);
 }
 
 }  // namespace lily

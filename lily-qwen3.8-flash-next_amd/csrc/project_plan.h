@@ -24,6 +24,10 @@ struct ProjectArgs {
     uint32_t bias_bf16, residual_bf16, out_bf16, act;
     uint32_t splits;            // parts of d, each a workgroup's
     float* part;                // their sums, [splits][rows][part_stride(n)]
+    // scales of blocks: of 128 elements of a row of x, of 128 x 128 weights
+    const float* x_blocks;      // [rows][x_blocks_stride]
+    const float* w_blocks;      // [over(n, 128)][w_blocks_stride]
+    uint32_t x_blocks_stride, w_blocks_stride;   // floats
 };
 
 constexpr uint32_t part_stride(uint32_t n) { return (n + 3u) / 4u * 4u; }

@@ -129,6 +129,66 @@ class _Projection(C.Structure):
                 ("activation", C.c_uint32)]
 
 
+class _Layer(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("d", C.c_uint32),
+                ("x_dev", C.c_void_p), ("x_stride", C.c_uint64),
+                ("residual_dev", C.c_void_p), ("residual_stride", C.c_uint64),
+                ("sum_dev", C.c_void_p), ("sum_stride", C.c_uint64),
+                ("weight_dev", C.c_void_p), ("bias_dev", C.c_void_p),
+                ("out_dev", C.c_void_p), ("out_stride", C.c_uint64),
+                ("scales_dev", C.c_void_p), ("scales_stride", C.c_uint64),
+                ("mean_dev", C.c_void_p), ("rstd_dev", C.c_void_p),
+                ("x_dtype", C.c_uint32), ("stream_dtype", C.c_uint32), ("weight_dtype", C.c_uint32),
+                ("out_dtype", C.c_uint32), ("scale_block", C.c_uint32), ("eps", C.c_float)]
+
+
+class _LayerGrad(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("d", C.c_uint32),
+                ("grad_dev", C.c_void_p), ("grad_stride", C.c_uint64),
+                ("h_dev", C.c_void_p), ("h_stride", C.c_uint64),
+                ("mean_dev", C.c_void_p), ("rstd_dev", C.c_void_p), ("weight_dev", C.c_void_p),
+                ("past_dev", C.c_void_p), ("past_stride", C.c_uint64),
+                ("grad_x_dev", C.c_void_p), ("grad_x_stride", C.c_uint64),
+                ("grad_weight_dev", C.c_void_p), ("grad_bias_dev", C.c_void_p),
+                ("grad_dtype", C.c_uint32), ("h_dtype", C.c_uint32), ("weight_dtype", C.c_uint32),
+                ("grad_x_dtype", C.c_uint32), ("accumulate", C.c_uint32)]
+
+
+class _Blocks(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("d", C.c_uint32),
+                ("x_dev", C.c_void_p), ("x_stride", C.c_uint64),
+                ("out_dev", C.c_void_p), ("out_stride", C.c_uint64),
+                ("scales_dev", C.c_void_p), ("scales_stride", C.c_uint64),
+                ("x_dtype", C.c_uint32), ("block_rows", C.c_uint32)]
+
+
+class _BlockProjection(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("n", C.c_uint32), ("d", C.c_uint32), ("activation", C.c_uint32),
+                ("x_dev", C.c_void_p), ("x_stride", C.c_uint64),
+                ("x_scales_dev", C.c_void_p), ("x_scales_stride", C.c_uint64),
+                ("weight_dev", C.c_void_p), ("weight_stride", C.c_uint64),
+                ("weight_scales_dev", C.c_void_p), ("weight_scales_stride", C.c_uint64),
+                ("bias_dev", C.c_void_p), ("residual_dev", C.c_void_p), ("residual_stride", C.c_uint64),
+                ("out_dev", C.c_void_p), ("out_stride", C.c_uint64),
+                ("bias_dtype", C.c_uint32), ("residual_dtype", C.c_uint32), ("out_dtype", C.c_uint32),
+                ("reserved", C.c_uint32)]
+
+
+class _Distillation(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("vocab", C.c_uint32),
+                ("logits_dev", C.c_void_p), ("logits_stride", C.c_uint64),
+                ("ids_dev", C.c_void_p), ("ids_stride", C.c_uint64),
+                ("values_dev", C.c_void_p), ("values_stride", C.c_uint64),
+                ("counts_dev", C.c_void_p), ("teacher_lse_dev", C.c_void_p), ("row_weights_dev", C.c_void_p),
+                ("loss_dev", C.c_void_p), ("stats_dev", C.c_void_p),
+                ("grad_dev", C.c_void_p), ("grad_stride", C.c_uint64),
+                ("k", C.c_uint32), ("teacher", C.c_uint32), ("rest", C.c_uint32),
+                ("logits_dtype", C.c_uint32), ("values_dtype", C.c_uint32), ("grad_dtype", C.c_uint32),
+                ("temperature", C.c_float), ("grad_scale", C.c_float)]
+
+
+TEACHERS = {"logits": 0, "probs": 1}
+BLOCK = 128
 ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4}
 
 
@@ -219,6 +279,12 @@ def _load():
     }
     sigs["lily_rms_norm"] = [vp, C.POINTER(_Norm)]
     sigs["lily_project"] = [vp, C.POINTER(_Projection)]
+    sigs["lily_layer_norm"] = [vp, C.POINTER(_Layer)]
+    sigs["lily_layer_norm_backward"] = [vp, C.POINTER(_LayerGrad)]
+    sigs["lily_quantize_blocks"] = [vp, C.POINTER(_Blocks)]
+    sigs["lily_project_blocks"] = [vp, C.POINTER(_BlockProjection)]
+    sigs["lily_distill"] = [vp, C.POINTER(_Distillation)]
+    sigs["lily_distill_backward"] = [vp, C.POINTER(_Distillation)]
     sigs["lily_process_logits"] = [vp, C.POINTER(_Rows), C.POINTER(_LogitsOut)]
     sigs["lily_plan_process_logits"] = [vp, C.POINTER(_LogitsOut)]
     L.lily_insertions_create.restype = C.c_int
@@ -646,6 +712,149 @@ class Sampler:
         _check(_lib.lily_project(self._h, C.byref(_Projection(
             rows, n, d, xt, xp, xs, wp, ws, self._scales(x_scales, rows, "x_scales"),
             self._scales(weight_scales, n, "weight_scales"), bp, rp, rs, op, os_, bt, rt, ot, act))))
+
+    # -- training and serving a draft head
+    def _floats(self, t, shape, name):
+        """(address, stride) of an f32 matrix whose rows are contiguous."""
+        at, stride, code = self._matrix(t, shape, name)
+        self._must(code == F32, name, "F32")
+        return at, stride
+
+    def _words(self, t, shape, name):
+        """(address, stride) of int32 rows, or of an int32 vector."""
+        if t is None:
+            return None, 0
+        self._must(t.dtype == torch.int32 and tuple(t.shape) == tuple(shape) and (t.stride(-1) == 1 or shape[-1] <= 1), name,
+                   f"int32 {list(shape)}, contiguous")
+        self._must(t.get_device() == self.device, name, "on the sampler's device")
+        return t.data_ptr(), t.stride(0)
+
+    @staticmethod
+    def _blocks(n):
+        return (n + BLOCK - 1) // BLOCK
+
+    def layer_norm(self, x, weight, bias, out, eps=1e-5, residual=None, summed=None, scales=None, mean=None, rstd=None):
+        """lily_layer_norm: out = (h - mean) * rstd * weight + bias, h = x + residual, h to `summed`, each row's mean and
+        1 / sqrt(var + eps) to `mean` and `rstd`.  out: f32, bf16, or float8_e4m3fn with `scales`: [rows] f32, or
+        [rows, ceil(d / 128)] f32 for a scale for each 128 elements."""
+        shape = x.shape
+        if len(shape) != 2:
+            raise SamplerError(-1, "x must be [rows, d], rows contiguous")
+        rows, d = shape
+        xp, xs, xt = self._matrix(x, shape, "x")
+        op, os_, ot = self._matrix(out, shape, "out")
+        wp, wt = self._vector(weight, d, "weight")
+        bp, bt = self._vector(bias, d, "bias")
+        if weight is not None and bias is not None and wt != bt:
+            raise SamplerError(-1, "weight and bias must have one type")
+        rp, rs, rt = self._matrix(residual, shape, "residual") if residual is not None else (None, 0, F32)
+        sp, ss, st = self._matrix(summed, shape, "summed") if summed is not None else (None, 0, rt)
+        if st != rt:
+            raise SamplerError(-1, "summed must have the residual's type")
+        block, stride = 0, 0
+        if scales is not None and scales.dim() == 2:
+            block = BLOCK
+            cp, stride = self._floats(scales, (rows, self._blocks(d)), "scales")
+        else:
+            cp = self._scales(scales, rows, "scales")
+        _check(_lib.lily_layer_norm(self._h, C.byref(_Layer(
+            rows, d, xp, xs, rp, rs, sp, ss, wp, bp, op, os_, cp, stride, self._scales(mean, rows, "mean"),
+            self._scales(rstd, rows, "rstd"), xt, rt, wt if weight is not None else bt, ot, block, eps))))
+
+    def layer_norm_backward(self, grad, h, mean, rstd, weight, grad_x=None, grad_weight=None, grad_bias=None, past=None,
+                            accumulate=False):
+        """lily_layer_norm_backward: from the gradient of the norm's output and the forward pass's h, mean and rstd, the gradient
+        of h (`past`, what reaches h past the norm, joins) and, f32, of weight and bias (added to what is there with
+        `accumulate`)."""
+        shape = grad.shape
+        if len(shape) != 2:
+            raise SamplerError(-1, "grad must be [rows, d], rows contiguous")
+        rows, d = shape
+        gp, gs, gt = self._matrix(grad, shape, "grad")
+        hp, hs, ht = self._matrix(h, shape, "h")
+        wp, wt = self._vector(weight, d, "weight")
+        xp, xs, xt = self._matrix(grad_x, shape, "grad_x") if grad_x is not None else (None, 0, F32)
+        pp, ps, pt = self._matrix(past, shape, "past") if past is not None else (None, 0, xt)
+        if grad_x is not None and pt != xt:
+            raise SamplerError(-1, "past must have grad_x's type")
+        _check(_lib.lily_layer_norm_backward(self._h, C.byref(_LayerGrad(
+            rows, d, gp, gs, hp, hs, self._scales(mean, rows, "mean"), self._scales(rstd, rows, "rstd"), wp, pp, ps, xp, xs,
+            self._scales(grad_weight, d, "grad_weight"), self._scales(grad_bias, d, "grad_bias"), gt, ht, wt, xt,
+            1 if accumulate else 0))))
+
+    def quantize_blocks(self, x, out, scales):
+        """lily_quantize_blocks: x as float8_e4m3fn in `out` with f32 `scales` [rows, ceil(d / 128)] (a scale for each 128 elements)
+        or [ceil(rows / 128), ceil(d / 128)] (for each 128 x 128)."""
+        shape = x.shape
+        if len(shape) != 2:
+            raise SamplerError(-1, "x must be [rows, d], rows contiguous")
+        rows, d = shape
+        xp, xs, xt = self._matrix(x, shape, "x")
+        op, os_, ot = self._matrix(out, shape, "out")
+        if ot != E4M3:
+            raise SamplerError(-1, "out must be E4M3")
+        by_row = scales.dim() == 2 and scales.shape[0] == rows
+        cp, cs = self._floats(scales, (rows if by_row else self._blocks(rows), self._blocks(d)), "scales")
+        _check(_lib.lily_quantize_blocks(self._h, C.byref(_Blocks(rows, d, xp, xs, op, os_, cp, cs, xt, 1 if by_row else BLOCK))))
+
+    def project_blocks(self, x, x_scales, weight, weight_scales, out, bias=None, activation="none", residual=None):
+        """lily_project_blocks: out = residual + activation(x @ weight.T + bias) of operands in float8_e4m3fn with f32 scales, x
+        [rows, d] with [rows, ceil(d / 128)], weight [n, d] with [ceil(n / 128), ceil(d / 128)]."""
+        if x.dim() != 2 or weight.dim() != 2:
+            raise SamplerError(-1, "x must be [rows, d] and weight [n, d], rows contiguous")
+        rows, d = x.shape
+        n = weight.shape[0]
+        xp, xs, xt = self._matrix(x, (rows, d), "x")
+        wp, ws, wt = self._matrix(weight, (n, d), "weight")
+        op, os_, ot = self._matrix(out, (rows, n), "out")
+        if xt != E4M3 or wt != E4M3:
+            raise SamplerError(-1, "x and weight must be E4M3")
+        act = ACTIVATIONS.get(activation)
+        if act is None:
+            raise SamplerError(-1, f"activation must be one of {', '.join(ACTIVATIONS)}")
+        xcp, xcs = self._floats(x_scales, (rows, self._blocks(d)), "x_scales")
+        wcp, wcs = self._floats(weight_scales, (self._blocks(n), self._blocks(d)), "weight_scales")
+        bp, bt = self._vector(bias, n, "bias")
+        rp, rs, rt = self._matrix(residual, (rows, n), "residual") if residual is not None else (None, 0, F32)
+        _check(_lib.lily_project_blocks(self._h, C.byref(_BlockProjection(
+            rows, n, d, act, xp, xs, xcp, xcs, wp, ws, wcp, wcs, bp, rp, rs, op, os_, bt, rt, ot, 0))))
+
+    def _distillation(self, logits, ids, values, loss, temperature, teacher, rest, teacher_lse, counts, stats, grad, row_weights,
+                      grad_scale):
+        if logits.dim() != 2 or values.dim() != 2:
+            raise SamplerError(-1, "logits must be [rows, vocab] and values [rows, k], rows contiguous")
+        rows, vocab = logits.shape
+        k = values.shape[1]
+        kind = TEACHERS.get(teacher)
+        if kind is None:
+            raise SamplerError(-1, f"teacher must be one of {', '.join(TEACHERS)}")
+        zp, zs, zt = self._matrix(logits, (rows, vocab), "logits")
+        ip, is_ = self._words(ids, (rows, k), "ids")
+        vp, vs, vt = self._matrix(values, (rows, k), "values")
+        gp, gs, gt = self._matrix(grad, (rows, vocab), "grad") if grad is not None else (None, 0, F32)
+        sp = None
+        if stats is not None:
+            sp, ss = self._floats(stats, (rows, 4), "stats")
+            self._must(ss == 4 or rows == 1, "stats", "contiguous")
+        return _Distillation(
+            rows, vocab, zp, zs, ip, is_, vp, vs, self._words(counts, (rows,), "counts")[0],
+            self._scales(teacher_lse, rows, "teacher_lse"), self._scales(row_weights, rows, "row_weights"),
+            self._scales(loss, rows, "loss"), sp, gp, gs, k, kind, 1 if rest else 0, zt, vt, gt, temperature, grad_scale)
+
+    def distill(self, logits, ids, values, loss, temperature=1.0, teacher="logits", rest=False, teacher_lse=None, counts=None,
+                stats=None, grad=None, row_weights=None, grad_scale=1.0):
+        """lily_distill: the loss [rows] of a student's logits [rows, vocab] against a teacher's lists of ids (int32, -1 pads) and
+        values [rows, k] (teacher "logits" or "probs"), `counts` of them a row; with `rest` everything outside a list is one
+        outcome more (and "logits" come with `teacher_lse`, log(sum of exp(t / T)) over the teacher's row).  `stats` [rows, 4]
+        for distill_backward, and `grad` of sum(grad_scale * row_weights * loss) (`logits` itself too), where given."""
+        _check(_lib.lily_distill(self._h, C.byref(self._distillation(
+            logits, ids, values, loss, temperature, teacher, rest, teacher_lse, counts, stats, grad, row_weights, grad_scale))))
+
+    def distill_backward(self, logits, ids, values, temperature=1.0, teacher="logits", rest=False, teacher_lse=None, counts=None,
+                         stats=None, grad=None, row_weights=None, grad_scale=1.0):
+        """lily_distill_backward: the gradient that distill writes, from the `stats` it left."""
+        _check(_lib.lily_distill_backward(self._h, C.byref(self._distillation(
+            logits, ids, values, None, temperature, teacher, rest, teacher_lse, counts, stats, grad, row_weights, grad_scale))))
 
     def _logits_out(self, rows, vocab, out, log_sum_exp, logprobs):
         at, stride, code = self._matrix(out, (rows, vocab), "out")
