@@ -778,9 +778,9 @@ int lily_project_blocks(lily_sampler_t* s, const lily_block_projection* p);
  * lily_distill writes the loss, stats (what the backward pass reads: the row's largest value z0 and log(sum of exp((z - z0) / T)),
  * the same two of the ids outside the list, or zeros without `rest`) and the gradient, each where given; lily_distill_backward
  * writes the gradient from stats.  grad_dev may be logits_dev with the same type and stride; other overlaps of an output
- * are refused.  Vocabularies up to 2^24, lists up to LILY_SAMPLE_K_CAP, rows x vocab as far as a launch reaches
- * (LILY_ERR_RANGE beyond).  Enqueued on the sampler's stream; a row's slices meet in the sampler's workspace: graphs captured from
- * one sampler are replayed one after the other. */
+ * are refused.  Vocabularies up to 2^24, lists up to LILY_SAMPLE_K_CAP (LILY_ERR_RANGE beyond).
+ * Enqueued on the sampler's stream; a row's slices meet in the sampler's workspace: graphs captured from one sampler are
+ * replayed one after the other. */
 typedef enum lily_teacher { LILY_TEACHER_LOGITS = 0, LILY_TEACHER_PROBS = 1 } lily_teacher;
 typedef struct lily_distillation {
     uint32_t rows;

@@ -174,9 +174,6 @@ int check_distillation(const lily_distillation* d, bool backward) {
     if (d->k > LILY_SAMPLE_K_CAP) {
         return api_fail(LILY_ERR_RANGE, "a teacher's list holds up to %u entries", LILY_SAMPLE_K_CAP);
     }
-    if (distill_threads(d->rows, d->vocab) > MAX_THREADS) {
-        return api_fail(LILY_ERR_RANGE, "rows x vocab is more than a launch reaches");
-    }
     if (d->logits_dtype > LILY_BF16 || d->values_dtype > LILY_BF16 || d->grad_dtype > LILY_BF16) {
         return api_fail(LILY_ERR_INVALID_ARG, "logits, values and grad are LILY_F32 or LILY_BF16");
     }

@@ -22,6 +22,7 @@ struct ProjectWorkspace {
     float* part;            // sums of parts of d, in 16-byte units
     uint64_t part_floats;
     uint32_t tile = 0;      // 64, 128 or 256: what more than 16 rows get; 0: by an estimate of the time
+    uint32_t looks = 4096;  // of a distillation's workgroups for the sums of their row's other slices
 };
 hipError_t launch_project(hipStream_t stream, const lily_projection& p, const ProjectWorkspace& ws);
 
@@ -33,11 +34,8 @@ hipError_t launch_layer_norm_backward(hipStream_t stream, const lily_layer_grad&
 hipError_t launch_quantize_blocks(hipStream_t stream, const lily_blocks& blocks);
 hipError_t launch_project_blocks(hipStream_t stream, const lily_block_projection& p, const ProjectWorkspace& ws);
 
-// Distillation (distill.hip): a workgroup takes a slice of a row.
-constexpr uint32_t DISTILL_SLICE = 8192, DISTILL_THREADS = 256;
-constexpr uint64_t distill_threads(uint32_t rows, uint32_t vocab) {
-    return (uint64_t)rows * ((vocab + DISTILL_SLICE - 1u) / DISTILL_SLICE) * DISTILL_THREADS;
-}
+// Distillation (distill.hip): workgroups of this many threads take slices of a row, of this many ids at most.
+constexpr uint32_t DISTILL_SLICE = 16384, DISTILL_THREADS = 512;
 hipError_t launch_distill(hipStream_t stream, const lily_distillation& d, bool backward, const ProjectWorkspace& ws);
 
 }  // namespace lily

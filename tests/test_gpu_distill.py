@@ -218,15 +218,16 @@ def test_temperatures(sampler, temperature, teacher, rest):
 
 
 @pytest.mark.parametrize("teacher, rest", KINDS)
-@pytest.mark.parametrize("rows, vocab", [(600, 5000), (300, 40000), (2100, 130)])
+@pytest.mark.parametrize("rows, vocab", [(600, 5000), (300, 40000), (2100, 130), (257, 70001), (260, 153607), (256, 248320)])
 def test_many_rows(sampler, teacher, rest, rows, vocab):
     check(sampler, Case(rows, vocab, 40, "bf16", "f32", "bf16", teacher, rest, 1.5, lambda r: r % 45, weights=True))
 
 
 @pytest.mark.parametrize("teacher, rest", KINDS)
-def test_lists_of_every_length(sampler, teacher, rest):
+@pytest.mark.parametrize("rows", [40, 280])
+def test_lists_of_every_length(sampler, teacher, rest, rows):
     """Counts from none to more than there is room for, and ids that pad."""
-    c = Case(40, 9000, 33, "f32", "f32", "f32", teacher, rest, 1.0, lambda r: r if r < 39 else -1)
+    c = Case(rows, 9000, 33, "f32", "f32", "f32", teacher, rest, 1.0, lambda r: r if r < 39 else -1)
     c.ids[:, 5] = -1
     c.ids[:, 6] = 9000            # the first id beyond the vocabulary
     c.ids[::3, 7:] = -1
@@ -236,8 +237,9 @@ def test_lists_of_every_length(sampler, teacher, rest):
 
 @pytest.mark.parametrize("teacher, rest", KINDS)
 @pytest.mark.parametrize("k", [4, 70, 1000])
-def test_an_id_that_stands_there_twice(sampler, teacher, rest, k):
-    c = Case(8, 20000, k, "f32", "f32", "f32", teacher, rest, 1.0)
+@pytest.mark.parametrize("rows", [8, 300])
+def test_an_id_that_stands_there_twice(sampler, teacher, rest, k, rows):
+    c = Case(rows, 20000, k, "f32", "f32", "f32", teacher, rest, 1.0)
     c.ids[0, :] = 17                           # every entry the same id
     c.ids[1, 1] = c.ids[1, 0]
     c.ids[2, k - 1] = c.ids[2, 0]
@@ -248,9 +250,10 @@ def test_an_id_that_stands_there_twice(sampler, teacher, rest, k):
 
 
 @pytest.mark.parametrize("teacher, rest", KINDS)
-def test_masked_logits(sampler, teacher, rest):
+@pytest.mark.parametrize("rows", [6, 260])
+def test_masked_logits(sampler, teacher, rest, rows):
     """-inf in the student's rows, outside its list, in it where the teacher has nothing and where it has something."""
-    c = Case(6, 12000, 16, "f32", "f32", "f32", teacher, rest, 1.0)
+    c = Case(rows, 12000, 16, "f32", "f32", "f32", teacher, rest, 1.0)
     none = -INF if teacher == "logits" else 0.0
     outside = torch.ones(12000, dtype=torch.bool, device=dev())
     outside[c.ids[0].long()] = False
@@ -266,10 +269,10 @@ def test_masked_logits(sampler, teacher, rest):
 
 
 @pytest.mark.parametrize("teacher, rest", KINDS)
-@pytest.mark.parametrize("vocab", [300, 20000])
-def test_what_is_not_finite(sampler, teacher, rest, vocab):
+@pytest.mark.parametrize("rows, vocab", [(9, 300), (9, 20000), (270, 60000), (270, 200000)])
+def test_what_is_not_finite(sampler, teacher, rest, rows, vocab):
     """NaN, +inf and rows of -inf make their row a NaN and no other; rows without an entry that counts or without weight stay zeros."""
-    c = Case(9, vocab, 8, "f32", "f32", "f32", teacher, rest, 1.0, lambda r: 0 if r in (6, 7) else 8, weights=True)
+    c = Case(rows, vocab, 8, "f32", "f32", "f32", teacher, rest, 1.0, lambda r: 0 if r in (6, 7) else 8, weights=True)
     free = next(i for i in range(vocab) if i not in set(c.ids[0].tolist()))
     c.logits[0, free] = float("nan")
     c.logits[1, c.ids[1, 2].long()] = float("nan")
@@ -288,8 +291,9 @@ def test_what_is_not_finite(sampler, teacher, rest, vocab):
     sampler.synchronize()
     for grad in (c.grad, again):
         assert bool(torch.isnan(grad[:5]).all()), [bool(torch.isnan(grad[r]).all()) for r in range(5)]
-        assert bool(torch.isfinite(grad[5]).all()) and bool((grad[6:] == 0).all())
+        assert bool(torch.isfinite(grad[5]).all()) and bool((grad[6:9] == 0).all()) and bool(torch.isfinite(grad[9:]).all())
     assert bool(torch.isnan(c.loss[:5]).all()) and bool(torch.isfinite(c.loss[5])) and bool((c.loss[6:8] == 0).all())
+    assert bool(torch.isfinite(c.loss[9:]).all())
 
 
 def test_a_list_without_mass(sampler):
@@ -302,7 +306,7 @@ def test_a_list_without_mass(sampler):
 
 
 @pytest.mark.parametrize("x", ["f32", "bf16"])
-@pytest.mark.parametrize("rows, vocab, k", [(3, 20000, 50), (700, 3001, 17), (2, 200, 190)])
+@pytest.mark.parametrize("rows, vocab, k", [(3, 20000, 50), (700, 3001, 17), (2, 200, 190), (300, 50001, 60)])
 @pytest.mark.parametrize("teacher, rest", KINDS)
 def test_in_place(sampler, x, rows, vocab, k, teacher, rest):
     c = Case(rows, vocab, k, x, "f32", x, teacher, rest, 1.0)
@@ -377,7 +381,7 @@ def test_rows_that_lie_further_apart_than_32_bits(sampler):
     near(wide, want[4], want[5])
 
 
-@pytest.mark.parametrize("rows, vocab", [(3, 30000), (400, 3000)])
+@pytest.mark.parametrize("rows, vocab", [(3, 30000), (400, 3000), (300, 9000)])
 def test_a_captured_graph(rows, vocab):
     stream = torch.cuda.Stream()
     s = LS.Sampler(0, stream)
@@ -427,3 +431,26 @@ def test_what_the_python_mirror_refuses(sampler):
     for bad in (dict(stats=None), dict(grad=None)):
         with pytest.raises(LS.SamplerError):
             sampler.distill_backward(**{**good, **bad})
+
+
+@pytest.mark.parametrize("looks", [0, 1, 3])
+@pytest.mark.parametrize("teacher, rest", KINDS)
+def test_slices_whose_neighbours_are_not_seen(monkeypatch, looks, teacher, rest):
+    """A workgroup that does not find its row's other sums forms them itself: by the same operations, so the bits are the same."""
+    monkeypatch.setenv("LILY_SAMPLER_DISTILL_LOOKS", str(looks))
+    s, usual = LS.Sampler(0), None
+    for rows, vocab, k, x in ((3, 40003, 30, "f32"), (200, 33001, 60, "bf16"), (2, 100000, 1000, "bf16"), (150, 70001, 5, "f32")):
+        c = Case(rows, vocab, k, x, "f32", x, teacher, rest, 1.0, weights=True)
+        c.ids[1, 1] = c.ids[1, 0]
+        c.logits[0, ::3] = -INF
+        check(s, c)
+        monkeypatch.delenv("LILY_SAMPLER_DISTILL_LOOKS", raising=False)
+        usual = usual or LS.Sampler(0)
+        loss, grad, stats = torch.empty_like(c.loss), torch.empty_like(c.grad), torch.empty_like(c.stats)
+        torch.cuda.synchronize()
+        s.distill(c.logits, c.ids, c.values, c.loss, stats=c.stats, grad=c.grad, **c.lists(), **c.grads())
+        usual.distill(c.logits, c.ids, c.values, loss, stats=stats, grad=grad, **c.lists(), **c.grads())
+        torch.cuda.synchronize()
+        assert torch.equal(loss, c.loss) and torch.equal(stats, c.stats) and torch.equal(grad, c.grad)
+    s.close()
+    usual.close()
