@@ -293,15 +293,15 @@ __device__ __forceinline__ Gradient gradient_of(const DistillArgs& a, const RowS
     g.ref = reference(a.rest != 0u ? r.out.m : r.all.m);
     g.factor = g.zeros        ? 0.0f
                : a.rest == 0u ? g.wt * r.inv_all
-               : r.nothing    ? (r.log_all != r.log_all ? r.log_all : 0.0f)
+               : r.nothing    ? (r.inv_all != r.inv_all ? r.inv_all : 0.0f)
                               : g.wt * (r.q_out - l.left) * r.inv_out;
     return g;
 }
 
 // The list as the workgroup sees it.
 struct SliceList {
-    uint32_t ids[LILY_SAMPLE_K_CAP];   // LILY_NO_TOKEN: not in this slice
-    float p[LILY_SAMPLE_K_CAP];
+    uint32_t ids[LILY_SAMPLE_K_CAP];   // LILY_NO_TOKEN: does not count
+    float z[LILY_SAMPLE_K_CAP], p[LILY_SAMPLE_K_CAP];   // of what lies in the slice: logit, probability
     uint32_t bits[DISTILL_SLICE / 32u];
     uint32_t twice;                    // an id stands there twice
 };
@@ -399,8 +399,10 @@ __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at)
     const uint32_t last_at = whole * 8u >= lo && whole * 8u + tid < hi ? whole * 8u + tid : LILY_NO_TOKEN;
     const float last = last_at != LILY_NO_TOKEN ? load1(z, last_at, BF16) : NEG_INF;   // the id behind the pieces
     auto there = [&](uint32_t c) { return whole != 0u && first + c * NT_DISTILL + tid < whole; };
-    list.bits[tid] = 0u;
-    static_assert(DISTILL_SLICE / 32u == NT_DISTILL, "a word of the bitmap a thread");
+    for (uint32_t w = tid; w < SLICE / 32u; w += NT_DISTILL) {
+        list.bits[w] = 0u;
+    }
+    static_assert(SLICE <= DISTILL_SLICE, "a bit for every id of a slice");
     if (tid == 0u) {
         list.twice = 0u;
     }
@@ -428,31 +430,39 @@ __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at)
     __syncthreads();
     const bool twice = list.twice != 0u;
     Listed l = {};
-    float p[ENTRIES] = {};
     if constexpr (FORM != FORM_SUM) {
         l = a.listed[in_launch];
         const float lse = a.teacher_lse != nullptr ? gload(a.teacher_lse + row) : 0.0f;
 #pragma unroll
         for (uint32_t e = 0; e < ENTRIES; ++e) {
-            p[e] = here[e] ? entry_probability(a, value[e], l, lse) : 0.0f;
-        }
-        if (twice) {
-#pragma unroll
-            for (uint32_t e = 0; e < ENTRIES; ++e) {
-                if (here[e]) {
-                    list.p[e * NT_DISTILL + tid] = p[e];
-                }
+            if (here[e]) {
+                list.p[e * NT_DISTILL + tid] = entry_probability(a, value[e], l, lse);
             }
-            __syncthreads();
         }
     }
-    if (twice) {
+    if (twice) {   // the first of an id speaks for all of them
+        __syncthreads();
+        float p[ENTRIES];
 #pragma unroll
         for (uint32_t e = 0; e < ENTRIES; ++e) {
             here[e] = here[e] && speaks(list, e * NT_DISTILL + tid);
-            if (here[e] && FORM != FORM_SUM) {
-                p[e] = added_up(list, e * NT_DISTILL + tid, a.k);
+            p[e] = here[e] && FORM != FORM_SUM ? added_up(list, e * NT_DISTILL + tid, a.k) : 0.0f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t e = 0; e < ENTRIES; ++e) {
+            if (here[e]) {
+                list.p[e * NT_DISTILL + tid] = p[e];
             }
+        }
+    }
+    // (from here on a thread's entries are its own places in LDS: the slice needs the registers)
+#pragma unroll
+    for (uint32_t e = 0; e < ENTRIES; ++e) {
+        const uint32_t j = e * NT_DISTILL + tid;
+        if (j < a.k) {
+            list.ids[j] = here[e] ? id[e] : LILY_NO_TOKEN;
+            list.z[j] = mine[e];
         }
     }
 
@@ -493,10 +503,10 @@ __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at)
         }
         s[0] = {own, sum};
         if (SUMS && a.rest != 0u) {
-#pragma unroll
-            for (uint32_t e = 0; e < ENTRIES; ++e) {
-                if (here[e]) {
-                    s[1] = joined(s[1], {mine[e], term(mine[e], mine[e], a.c2)}, a.c2);
+            for (uint32_t j = tid; j < a.k; j += NT_DISTILL) {
+                if (list.ids[j] != LILY_NO_TOKEN) {
+                    const float v = list.z[j];
+                    s[1] = joined(s[1], {v, term(v, v, a.c2)}, a.c2);
                 }
             }
         }
@@ -604,16 +614,15 @@ __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at)
     }
     // The list's ids anew, behind the stores above.
     __syncthreads();
-#pragma unroll
-    for (uint32_t e = 0; e < ENTRIES; ++e) {
-        if (here[e]) {
-            store1(grad, id[e], g.wt * (term(mine[e], r.all.m, a.c2) * r.inv_all - p[e]), dtype);
+    for (uint32_t j = tid; j < a.k; j += NT_DISTILL) {
+        if (list.ids[j] != LILY_NO_TOKEN) {
+            store1(grad, list.ids[j], g.wt * (term(list.z[j], r.all.m, a.c2) * r.inv_all - list.p[j]), dtype);
         }
     }
 }
 
 template <uint32_t TURNS, bool BF16, int FORM>
-__global__ void __launch_bounds__(NT_DISTILL, 6) k_distill(const DistillArgs a) {
+__global__ void __launch_bounds__(NT_DISTILL, TURNS > 4 ? 4 : 6) k_distill(const DistillArgs a) {
     if constexpr (FORM != FORM_AFTER) {
         distill_slice<TURNS, BF16, FORM>(a, blockIdx.x);
     } else {
@@ -634,17 +643,30 @@ __global__ void __launch_bounds__(NT_DISTILL, 6) k_distill(const DistillArgs a) 
     }
 }
 
-template <uint32_t TURNS, int FORM>
-void launch_turns(hipStream_t stream, const DistillArgs& a, uint32_t groups) {
-    if (a.logits_bf16 != 0u) {
-        hipLaunchKernelGGL((k_distill<TURNS, true, FORM>), dim3(groups), dim3(NT_DISTILL), 0, stream, a);
-    } else {
-        hipLaunchKernelGGL((k_distill<TURNS, false, FORM>), dim3(groups), dim3(NT_DISTILL), 0, stream, a);
-    }
-}
+// Turns of a slice: where rows are many, as many as a thread holds exponentials of (two workgroups a compute unit in bf16: 2048 rows of
+// 151 936 in bf16 266 us by eight, 301 by four, 295 by six, 457 by two; in f32, 1024 rows, 253 by four, 263 by eight), and three for the
+// backward pass, which holds nothing (219 against 233 by four and 218 by two; lists of 1000 entries 94, 98 and 100).
+constexpr uint32_t TURNS_BACK = 3;
+constexpr uint32_t turns_held(bool bf16) { return bf16 ? 8u : 4u; }
 template <int FORM>
 void launch_form(hipStream_t stream, const DistillArgs& a, uint32_t turns, uint32_t groups) {
-    turns == 1u ? launch_turns<1, FORM>(stream, a, groups) : turns == 2u ? launch_turns<2, FORM>(stream, a, groups) : launch_turns<4, FORM>(stream, a, groups);
+    const dim3 grid(groups), block(NT_DISTILL);
+#define LILY_DISTILL(TURNS, BF16)                                                                       \
+    if (turns == TURNS && (a.logits_bf16 != 0u) == BF16) {                                              \
+        hipLaunchKernelGGL((k_distill<TURNS, BF16, FORM>), grid, block, 0, stream, a);                  \
+    }
+    if constexpr (FORM == FORM_BACK) {
+        LILY_DISTILL(TURNS_BACK, true)
+        LILY_DISTILL(TURNS_BACK, false)
+    } else {
+        LILY_DISTILL(turns_held(true), true)
+        LILY_DISTILL(turns_held(false), false)
+    }
+    LILY_DISTILL(1u, true)
+    LILY_DISTILL(1u, false)
+    LILY_DISTILL(2u, true)
+    LILY_DISTILL(2u, false)
+#undef LILY_DISTILL
 }
 
 }  // namespace
@@ -679,7 +701,7 @@ hipError_t launch_distill(hipStream_t stream, const lily_distillation& d, bool b
     // Few rows are cut finer, as long as every workgroup has a place on the chip.
     auto slices = [&](uint64_t turns) { return (d.vocab + turns * TURN - 1u) / (turns * TURN); };
     auto fits = [&](uint64_t turns) { return slices(turns) <= WORD_SLICES && slices(turns) * d.rows <= 768u; };
-    const uint32_t turns = fits(1u) ? 1u : fits(2u) ? 2u : 4u;
+    const uint32_t turns = fits(1u) ? 1u : fits(2u) ? 2u : backward ? TURNS_BACK : turns_held(a.logits_bf16 != 0u);
     a.slices = (d.vocab + turns * TURN - 1u) / (turns * TURN);
     const bool held = d.grad_dev != nullptr && a.slices <= WORD_SLICES;
     // As many rows at a time as the workspace holds words, lists' sums and lists of slices of.

@@ -35,7 +35,7 @@ hipError_t launch_quantize_blocks(hipStream_t stream, const lily_blocks& blocks)
 hipError_t launch_project_blocks(hipStream_t stream, const lily_block_projection& p, const ProjectWorkspace& ws);
 
 // Distillation (distill.hip): workgroups of this many threads take slices of a row, of this many ids at most.
-constexpr uint32_t DISTILL_SLICE = 16384, DISTILL_THREADS = 512;
+constexpr uint32_t DISTILL_SLICE = 32768, DISTILL_THREADS = 512;
 hipError_t launch_distill(hipStream_t stream, const lily_distillation& d, bool backward, const ProjectWorkspace& ws);
 
 }  // namespace lily
