@@ -102,25 +102,6 @@ __device__ __forceinline__ void group_sums(Sum (&t)[N], float c2, float* part) {
     }
 }
 
-// Eight logits of a row as they lie in memory.
-template <bool BF16>
-struct Eight;
-template <>
-struct Eight<true> {
-    u32x4 a;
-    __device__ __forceinline__ void load(const void* row, uint32_t i) { a = *(const LILY_GLOBAL u32x4_at2*)(static_cast<const uint16_t*>(row) + i); }
-    __device__ __forceinline__ void widened(float (&v)[8]) const { widen({a, a}, true, v); }
-};
-template <>
-struct Eight<false> {
-    u32x4 a, b;
-    __device__ __forceinline__ void load(const void* row, uint32_t i) {
-        a = *(const LILY_GLOBAL u32x4_at4*)(static_cast<const uint32_t*>(row) + i);
-        b = *(const LILY_GLOBAL u32x4_at4*)(static_cast<const uint32_t*>(row) + i + 4);
-    }
-    __device__ __forceinline__ void widened(float (&v)[8]) const { widen({a, b}, false, v); }
-};
-
 __device__ __forceinline__ const void* at_row(const void* p, uint64_t row, uint64_t stride, bool bf16) {
     return static_cast<const char*>(p) + row * stride * (bf16 ? 2u : 4u);
 }

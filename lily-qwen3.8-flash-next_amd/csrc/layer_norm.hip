@@ -303,6 +303,170 @@ __global__ void __launch_bounds__(1024) k_layer_grad(const LayerGradArgs a) {
     }
 }
 
+// Both at once, for rows of up to 8192 elements: a workgroup takes `groups` rows at a time, `threads` threads and eight elements a
+// thread each, and keeps what its rows add to the gradients of weight and bias in registers; the next rows (in bf16 the next
+// two) are on their way while a row's two sums go through LDS.
+enum LayerTypes { LAYER_F32, LAYER_BF16, LAYER_MIXED };   // of grad, h, past and grad_x
+template <int TYPES>
+struct LayerPiece : Eight<TYPES == LAYER_BF16> {
+    __device__ __forceinline__ void ask(const void* row, uint32_t i, bool) { this->load(row, i); }
+    __device__ __forceinline__ void take(bool, float (&v)[8]) const { this->widened(v); }
+};
+template <>
+struct LayerPiece<LAYER_MIXED> {
+    Raw raw;
+    __device__ __forceinline__ void ask(const void* row, uint32_t i, bool bf16) { raw = load8(row, i, bf16); }
+    __device__ __forceinline__ void take(bool bf16, float (&v)[8]) const { widen(raw, bf16, v); }
+};
+template <bool RAGGED, int TYPES>
+__global__ void __launch_bounds__(1024) k_layer_grad_all(const LayerGradArgs a, uint32_t threads, uint32_t groups) {
+    constexpr uint32_t AHEAD = TYPES == LAYER_BF16 ? 2u : 1u;   // (registers)
+    __shared__ float part[2][2][16];
+    extern __shared__ float share[];   // [groups - 1][16][threads]
+    const uint32_t tid = threadIdx.x;
+    const uint32_t group = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid / threads)), in_row = tid - group * threads, i = in_row * 8u;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), from = group * (threads >> 6), to = from + (threads >> 6);   // waves of the group
+    const bool whole = i + 8u <= a.d;
+    const bool grad_bf16 = TYPES == LAYER_MIXED ? a.grad_bf16 != 0u : TYPES == LAYER_BF16, h_bf16 = TYPES == LAYER_MIXED ? a.h_bf16 != 0u : grad_bf16,
+               x_bf16 = TYPES == LAYER_MIXED ? a.grad_x_bf16 != 0u : grad_bf16;
+    struct Next {
+        LayerPiece<TYPES> grad, h, past;
+        float mean, rstd;
+    } next[AHEAD];
+    // (what lies behind the last whole piece of a row is not asked for; the loads stand outside of every branch)
+    const uint32_t at = a.d >= 8u ? min(i, a.d - 8u) : 0u;
+    const void* past_or_grad = a.past != nullptr ? a.past : a.grad;
+    const uint64_t past_stride = a.past != nullptr ? a.past_stride : a.grad_stride;
+    const bool past_bf16 = a.past != nullptr ? x_bf16 : grad_bf16;
+    auto ask = [&](Next& n, uint64_t row) {
+        const uint64_t r = min(row, (uint64_t)a.rows - 1u);
+        if (!RAGGED || a.d >= 8u) {
+            n.grad.ask(row_at(a.grad, r, a.grad_stride, grad_bf16), at, grad_bf16);
+            n.h.ask(row_at(a.h, r, a.h_stride, h_bf16), at, h_bf16);
+            if (a.past != nullptr) {
+                n.past.ask(row_at(past_or_grad, r, past_stride, past_bf16), at, past_bf16);
+            }
+        }
+        n.mean = gload(a.mean + r);
+        n.rstd = gload(a.rstd + r);
+    };
+    // (the piece that a row ends in goes element by element)
+    auto take = [&](const LayerPiece<TYPES>& piece, const void* p, uint64_t row, uint64_t stride, bool bf16, float (&v)[8]) {
+        if (!RAGGED || whole) {
+            piece.take(bf16, v);
+        } else {
+            const char* from_row = row_at(p, min(row, (uint64_t)a.rows - 1u), stride, bf16);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = i + (uint32_t)j < a.d ? load1(from_row, i + (uint32_t)j, bf16) : 0.0f;
+            }
+        }
+    };
+    const uint64_t step = (uint64_t)gridDim.x * groups;
+    uint64_t row = (uint64_t)blockIdx.x * groups + group;
+#pragma unroll
+    for (uint32_t q = 0; q < AHEAD; ++q) {
+        ask(next[q], row + q * step);
+    }
+    float w[8], gw[8] = {}, gb[8] = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        w[j] = a.weight != nullptr && i + (uint32_t)j < a.d ? load1(a.weight, i + (uint32_t)j, a.weight_bf16) : 1.0f;
+    }
+    const float over_d = 1.0f / (float)a.d;
+    auto one = [&](Next& n, uint32_t turn) {
+        const bool there = row < a.rows && (RAGGED || whole);   // (a piece behind the row's end is nothing)
+        const float mean = n.mean, rstd = n.rstd;
+        float g[8], x[8], past[8], sg = 0.0f, sx = 0.0f;
+        take(n.grad, a.grad, row, a.grad_stride, grad_bf16, g);
+        take(n.h, a.h, row, a.h_stride, h_bf16, x);
+        if (a.past != nullptr) {
+            take(n.past, a.past, row, a.past_stride, x_bf16, past);
+        }
+        ask(n, row + AHEAD * step);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const bool in = there && (!RAGGED || i + (uint32_t)j < a.d);
+            g[j] = in ? g[j] : 0.0f;
+            x[j] = in ? (x[j] - mean) * rstd : 0.0f;
+            gb[j] += g[j];
+            gw[j] = __builtin_fmaf(g[j], x[j], gw[j]);
+            g[j] *= w[j];
+            sg += g[j];
+            sx = __builtin_fmaf(g[j], x[j], sx);
+        }
+        sg = wave_sum_f(sg);
+        sx = wave_sum_f(sx);
+        if ((tid & 63u) == 0u) {
+            part[turn][0][wave] = sg;
+            part[turn][1][wave] = sx;
+        }
+        __syncthreads();
+        sg = sx = 0.0f;
+        for (uint32_t q = from; q < to; ++q) {
+            sg += part[turn][0][q];
+            sx += part[turn][1][q];
+        }
+        sg *= over_d;
+        sx *= over_d;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float v = rstd * (g[j] - sg - x[j] * sx);
+            g[j] = a.past != nullptr ? v + past[j] : v;
+        }
+        char* out = const_cast<char*>(row_at(a.grad_x, row, a.grad_x_stride, x_bf16));
+        if (there && whole) {
+            if (x_bf16) {
+                store8(out, i, g, LILY_BF16);
+            } else {
+                store8(out, i, g, LILY_F32);
+            }
+        } else if (RAGGED && there) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (i + (uint32_t)j < a.d) {
+                    store1(out, i + (uint32_t)j, g[j], x_bf16 ? LILY_BF16 : LILY_F32);
+                }
+            }
+        }
+        row += step;
+    };
+    if constexpr (AHEAD == 2u) {
+        // (two turns at a time: the registers of what comes next take turns; a turn behind the last row adds nothing)
+        for (uint64_t first = (uint64_t)blockIdx.x * groups; first < a.rows; first += 2u * step) {
+            one(next[0], 0u);
+            __builtin_amdgcn_sched_barrier(0);
+            one(next[AHEAD - 1u], 1u);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    } else {
+        uint32_t turn = 0u;
+        for (uint64_t first = (uint64_t)blockIdx.x * groups; first < a.rows; first += step, turn ^= 1u) {
+            one(next[0], turn);
+        }
+    }
+    if (group != 0u) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            share[((group - 1u) * 16u + (uint32_t)j) * threads + in_row] = gw[j];
+            share[((group - 1u) * 16u + 8u + (uint32_t)j) * threads + in_row] = gb[j];
+        }
+    }
+    __syncthreads();
+    if (group == 0u && i < a.wide) {
+        float* out = a.part + (uint64_t)blockIdx.x * 2u * a.wide + i;
+        for (uint32_t q = 0; q + 1u < groups; ++q) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                gw[j] += share[(q * 16u + (uint32_t)j) * threads + in_row];
+                gb[j] += share[(q * 16u + 8u + (uint32_t)j) * threads + in_row];
+            }
+        }
+        store8(out, 0u, gw, LILY_F32);
+        store8(out + a.wide, 0u, gb, LILY_F32);
+    }
+}
+
 // Sums over the rows of a part (blockIdx.y, every a.parts-th row), 64 lanes of eight elements by four rows at a time.
 template <bool RAGGED>
 __global__ void __launch_bounds__(256) k_layer_columns(const LayerGradArgs a) {
@@ -361,6 +525,7 @@ __global__ void __launch_bounds__(256) k_layer_join(const LayerGradArgs a) {
     float* to = blockIdx.y == 0u ? a.grad_weight : a.grad_bias;
     const uint32_t per = (a.parts + 7u) / 8u, last = min((run + 1u) * per, a.parts);
     float sum = 0.0f;
+#pragma unroll 8
     for (uint32_t p = run * per; p < last; ++p) {
         sum += gload(a.part + ((uint64_t)p * 2u + blockIdx.y) * a.wide + min(i, a.wide - 1u));
     }
@@ -442,8 +607,30 @@ hipError_t launch_layer_norm_backward(hipStream_t stream, const lily_layer_grad&
     a.grad_x_bf16 = n.grad_x_dtype == LILY_BF16;
     a.accumulate = n.accumulate;
     a.part = ws.part;
+    const bool sums = n.grad_weight_dev != nullptr || n.grad_bias_dev != nullptr;
+    auto join = [&] { hipLaunchKernelGGL(k_layer_join, dim3((n.d + 31u) / 32u, 2), dim3(256), 0, stream, a); };
+    if (sums && n.grad_x_dev != nullptr && n.d <= 8192u) {
+        const uint32_t threads = norm_shape(n.d).threads, groups = 1024u / threads;
+        a.parts = std::min({(n.rows + groups - 1u) / groups, 256u, (uint32_t)(ws.part_floats / (2ull * a.wide))});
+        const uint32_t lds = (groups - 1u) * 16u * threads * 4u;
+        const bool mixed = a.grad_bf16 != a.h_bf16 || a.grad_bf16 != a.grad_x_bf16;
+#define LILY_LAYER(RAGGED, TYPES) \
+    hipLaunchKernelGGL((k_layer_grad_all<RAGGED, TYPES>), dim3(a.parts), dim3(threads * groups), lds, stream, a, threads, groups)
+        if (n.d % 8u != 0u) {
+            LILY_LAYER(true, LAYER_MIXED);
+        } else if (mixed) {
+            LILY_LAYER(false, LAYER_MIXED);
+        } else if (a.grad_bf16 != 0u) {
+            LILY_LAYER(false, LAYER_BF16);
+        } else {
+            LILY_LAYER(false, LAYER_F32);
+        }
+#undef LILY_LAYER
+        join();
+        return hipGetLastError();
+    }
     // (the columns' sums first: grad_x may lie where an operand lies)
-    if (n.grad_weight_dev != nullptr || n.grad_bias_dev != nullptr) {
+    if (sums) {
         const uint32_t strips = (n.d + 511u) / 512u;
         a.parts = std::min({(n.rows + 3u) / 4u, (2048u + strips - 1u) / strips, (uint32_t)(ws.part_floats / (2ull * a.wide))});
         if (n.d % 8u != 0u) {
@@ -451,7 +638,7 @@ hipError_t launch_layer_norm_backward(hipStream_t stream, const lily_layer_grad&
         } else {
             hipLaunchKernelGGL(k_layer_columns<false>, dim3(strips, a.parts), dim3(256), 0, stream, a);
         }
-        hipLaunchKernelGGL(k_layer_join, dim3((n.d + 31u) / 32u, 2), dim3(256), 0, stream, a);
+        join();
     }
     if (n.grad_x_dev != nullptr) {
         const NormShape shape = norm_shape(n.d);

@@ -52,6 +52,24 @@ __device__ __forceinline__ void widen(const Raw& r, bool bf16, float (&v)[8]) {
         }
     }
 }
+// The same of one type.
+template <bool BF16>
+struct Eight;
+template <>
+struct Eight<true> {
+    u32x4 a;
+    __device__ __forceinline__ void load(const void* row, uint32_t i) { a = *(const LILY_GLOBAL u32x4_at2*)(static_cast<const uint16_t*>(row) + i); }
+    __device__ __forceinline__ void widened(float (&v)[8]) const { widen({a, a}, true, v); }
+};
+template <>
+struct Eight<false> {
+    u32x4 a, b;
+    __device__ __forceinline__ void load(const void* row, uint32_t i) {
+        a = *(const LILY_GLOBAL u32x4_at4*)(static_cast<const uint32_t*>(row) + i);
+        b = *(const LILY_GLOBAL u32x4_at4*)(static_cast<const uint32_t*>(row) + i + 4);
+    }
+    __device__ __forceinline__ void widened(float (&v)[8]) const { widen({a, b}, false, v); }
+};
 __device__ __forceinline__ float load1(const void* row, uint32_t i, bool bf16) {
     return bf16 ? load_logit<LILY_BF16>(row, i) : load_logit<LILY_F32>(row, i);
 }
