@@ -19,7 +19,7 @@ hipError_t launch_tile_of(hipStream_t stream, const ProjectArgs& a) {
     if (const hipError_t e = allowed.say((const void*)k_project_tiles<P, T>, T::LDS_BYTES); e != hipSuccess) {
         return e;
     }
-    hipLaunchKernelGGL((k_project_tiles<P, T>), dim3(m_tiles * n_tiles * a.splits), dim3(256), T::LDS_BYTES, stream, a, m_tiles, n_tiles);
+    hipLaunchKernelGGL((k_project_tiles<P, T>), dim3(m_tiles * n_tiles * a.splits), dim3(64 * T::WAVES), T::LDS_BYTES, stream, a, m_tiles, n_tiles);
     return a.splits > 1u ? launch_project_join(stream, a) : hipGetLastError();
 }
 template <class T>

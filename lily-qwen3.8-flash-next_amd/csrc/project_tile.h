@@ -80,24 +80,28 @@ __device__ __forceinline__ typename Block<S>::Sums step(const Block<S>& w, const
 
 template <int S_, int WM_, int WN_, int MT_, int NT_, int RESIDENT_, int DEPTH_, bool BLOCKS_ = false>
 struct Tile {
-    // BLOCKS: a unit brings the scales of its rows of x too, 64 for each wave
+    // BLOCKS: the scales of the rows of x lie behind the stages, those of RUN stages and of the RUN stages that follow
     static constexpr bool BLOCKS = BLOCKS_;
-    static constexpr int SCALES = BLOCKS ? 4 * 256 : 0;                // bytes
+    static constexpr int RUN = 8;
     // DEPTH: stages in LDS (an even number), RESIDENT: workgroups a compute unit is to hold
     static constexpr int S = S_, WM = WM_, WN = WN_, MT = MT_, NT = NT_, RESIDENT = RESIDENT_, DEPTH = DEPTH_;
     static constexpr int MH = MT / 2, NH = NT / 2;                     // blocks of a half
     static constexpr int BM = WM * MT * S, BN = WN * NT * S;
     static constexpr int XR = WM * MH * S, WR = WN * NH * S;           // rows of a unit: of x, of the weights
-    static constexpr int UNIT = (XR + WR) * (int)LINE + SCALES;
-    static constexpr int XL = XR / 32, WL = WR / 32, LOADS = XL + WL + (BLOCKS ? 1 : 0);  // loads of a wave and unit
+    static constexpr int UNIT = (XR + WR) * (int)LINE, WAVES = WM * WN;
+    static constexpr int XL = XR / (8 * WAVES), WL = WR / (8 * WAVES), LOADS = XL + WL;  // loads of a wave and unit
+    static constexpr int SCALES = BLOCKS ? BM * RUN * 4 : 0, SCALE_LOADS = BM / WAVES / 8;   // bytes of a run; loads of a wave, eight rows each
     // The epilogue's: a wave's rows that lie in LDS at once (half of the large tile's), and floats of a row there (a step of
     // four banks from row to row).
     static constexpr int PARTS = S == 32 ? 2 : 1, PART_ROWS = MT * S / PARTS, ROW = NT * S + 4;
-    static constexpr int STAGES = 2 * DEPTH * UNIT, SPREAD = 4 * PART_ROWS * ROW * 4;   // bytes
-    static constexpr int LDS_BYTES = SPREAD > STAGES ? SPREAD : STAGES;
+    static constexpr int STAGES = 2 * DEPTH * UNIT, SPREAD = WAVES * PART_ROWS * ROW * 4;   // bytes
+    static constexpr int TOUCHED = STAGES + 2 * SCALES, USED = TOUCHED + (S == 32 ? WAVES * 256 : 0);
+    static constexpr int LDS_BYTES = SPREAD > USED ? SPREAD : USED;
     static_assert(DEPTH % 2 == 0 && (2 * DEPTH - 1) * LOADS < 64, "loads in flight are counted in six bits");
-    static_assert(!BLOCKS || (MH * S <= 64 && NT * S <= (int)LILY_BLOCK), "a wave's rows of a unit are 64 at most, its outputs one block");
-    static_assert(WM * WN == 4 && XR % 32 == 0 && WR % 32 == 0, "whole loads a wave");
+    static_assert(!BLOCKS || NT * S <= (int)LILY_BLOCK, "a wave's outputs are of one block");
+    static_assert(!BLOCKS || (SCALE_LOADS >= 1 && SCALE_LOADS <= RUN - DEPTH), "a run's scales are asked for in time");
+    static_assert(XR % (8 * WAVES) == 0 && WR % (8 * WAVES) == 0, "whole loads a wave");
+    static_assert(LDS_BYTES <= 160 * 1024, "a compute unit's");
 };
 
 template <int V>
@@ -304,7 +308,7 @@ __device__ __forceinline__ void give_out(const ProjectArgs& a, const typename Bl
 }
 
 template <Products P, class T>
-__global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const ProjectArgs a, uint32_t m_tiles, uint32_t n_tiles) {
+__global__ void __launch_bounds__(64 * T::WAVES, T::RESIDENT * T::WAVES / 4) k_project_tiles(const ProjectArgs a, uint32_t m_tiles, uint32_t n_tiles) {
     constexpr int MH = T::MH, NH = T::NH, S = T::S, DEPTH = T::DEPTH;
     typedef Block<S> Operand;
     typedef typename Operand::Sums Sums;
@@ -331,9 +335,9 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
     const char* w_rows = a.w + (uint64_t)n0 * a.w_stride;
     uint32_t x_at[2][T::XL], w_at[2][T::WL];
 #pragma unroll
-    for (int i = 0; i < T::XL + T::WL; ++i) {
+    for (int i = 0; i < T::LOADS; ++i) {
         const bool is_x = i < T::XL;
-        const uint32_t row = (uint32_t)((is_x ? i : i - T::XL) * 32) + wave * 8u + (lane >> 3);   // of the unit's part
+        const uint32_t row = (uint32_t)((is_x ? i : i - T::XL) * 8 * T::WAVES) + wave * 8u + (lane >> 3);   // of the unit's part
         const uint32_t piece = (lane & 7u) ^ ((row >> 1) & 7u);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -353,31 +357,24 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
     // are a raw buffer's, and nothing is ever asked beyond the rows)
     auto x_buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(x_rows), 0, -1, 0x00020000);
     auto w_buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(w_rows), 0, -1, 0x00020000);
-    // (scales: a lane's row of the wave's own half hx, the rows again where there are fewer than lanes)
-    const float* x_scales[2];
+    // Scales of the rows of x: a load brings those of eight rows for a run of stages, eight neighbouring floats a row (a load of
+    // one stage's, a line of memory for every lane, takes as long as all of the stage's operands).  A row's eight change places by the
+    // row's number, so that lanes that read one stage's of neighbouring rows meet different banks.
     WeightScales w_scales = {};
     if constexpr (T::BLOCKS) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t row = m0 + wm * (uint32_t)(T::MT * S) + (uint32_t)h * (uint32_t)(MH * S) + lane % (uint32_t)(MH * S);
-            x_scales[h] = a.x_blocks + (uint64_t)min(row, a.rows - 1u) * a.x_blocks_stride + first;
-        }
         const uint32_t block = min((n0 + wn * (uint32_t)(T::NT * S)) / LILY_BLOCK, (a.n - 1u) / LILY_BLOCK);
         w_scales = {a.w_blocks + (uint64_t)block * a.w_blocks_stride + first, steps, 0.0f};
         w_scales.ask(0u);
     }
-    auto load_scales = [&](uint32_t s, int hx, int unit) {
-        __builtin_amdgcn_global_load_lds((gptr)(x_scales[hx] + s), (lptr)(lds + unit * T::UNIT + (T::XR + T::WR) * (int)LINE + wave * 256u), 4, 0, 0);
+    auto load_scales = [&](uint32_t run, int k) {
+        const uint32_t row = wave * (uint32_t)(T::SCALE_LOADS * 8) + (uint32_t)k * 8u, in = row + (lane >> 3);
+        const uint32_t stage = min(run * (uint32_t)T::RUN + ((lane & 7u) ^ ((in >> 3) & 7u)), steps - 1u);
+        const float* from = a.x_blocks + (uint64_t)min(m0 + in, a.rows - 1u) * a.x_blocks_stride + first + stage;
+        __builtin_amdgcn_global_load_lds((gptr)from, (lptr)(lds + T::STAGES + (run & 1u) * (uint32_t)T::SCALES + row * (uint32_t)(T::RUN * 4)), 4, 0, 0);
     };
     auto load = [&](uint32_t s, int hx, int hw, int unit, int i) {
-        if constexpr (T::BLOCKS) {
-            if (i == T::XL + T::WL) {
-                load_scales(s, hx, unit);
-                return;
-            }
-        }
         const uint32_t k0 = (first + s) * LINE;
-        char* base = lds + unit * T::UNIT + wave * 1024u + i * 4096;
+        char* base = lds + unit * T::UNIT + wave * 1024u + i * (1024 * T::WAVES);
         if (i < T::XL) {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(x_buffer, (lptr)base, 16, (int)x_at[hx][i < T::XL ? i : 0], (int)k0, 0, 0);
         } else {
@@ -396,16 +393,13 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
         // the stage that d ends in: pieces beyond it are zeros
         char* base = lds + unit * T::UNIT + wave * 1024u;
         const char* zeros = reinterpret_cast<const char*>(&line_of_zeros);
-        if constexpr (T::BLOCKS) {
-            load_scales(s, hx, unit);
-        }
 #pragma unroll
-        for (int i = 0; i < T::XL + T::WL; ++i) {
+        for (int i = 0; i < T::LOADS; ++i) {
             const char* from = i < T::XL ? x_rows + k0 + (uint64_t)x_at[hx][i < T::XL ? i : 0]
                                          : w_rows + k0 + (uint64_t)w_at[hw][i < T::XL ? 0 : i - T::XL];
-            const uint32_t row = (uint32_t)((i < T::XL ? i : i - T::XL) * 32) + wave * 8u + (lane >> 3);
+            const uint32_t row = (uint32_t)((i < T::XL ? i : i - T::XL) * 8 * T::WAVES) + wave * 8u + (lane >> 3);
             from = k0 + ((lane & 7u) ^ ((row >> 1) & 7u)) * 16u < a.d_bytes ? from : zeros;
-            __builtin_amdgcn_global_load_lds((gptr)from, (lptr)(base + i * 4096), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((gptr)from, (lptr)(base + i * (1024 * T::WAVES)), 16, 0, 0);
         }
     };
     // A lane's operands out of a unit.
@@ -419,11 +413,12 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
         const int i = k / Operand::PIECES, q = k % Operand::PIECES;
         f[i].p[q] = *reinterpret_cast<const u32x4*>(lds + ((from + (uint32_t)(i * S * (int)LINE)) ^ ((uint32_t)q * Operand::NEXT_PIECE)));
     };
-    auto read_x = [&](int h, int unit, int k) {
+    auto read_x = [&](int h, int unit, int k, uint32_t s) {   // (s: the stage that they are of)
         if constexpr (T::BLOCKS) {
             if (k >= XPIECES) {
-                scale[h][k - XPIECES] = *reinterpret_cast<const float*>(lds + unit * T::UNIT + (T::XR + T::WR) * (int)LINE + wave * 256u +
-                                                                        ((uint32_t)((k - XPIECES) * S) + r_in) * 4u);
+                const uint32_t row = wm * (uint32_t)(T::MT * S) + (uint32_t)(h * MH * S + (k - XPIECES) * S) + r_in;
+                scale[h][k - XPIECES] = *reinterpret_cast<const float*>(lds + T::STAGES + (s / (uint32_t)T::RUN & 1u) * (uint32_t)T::SCALES +
+                                                                        (row * (uint32_t)T::RUN + ((s & 7u) ^ ((row >> 3) & 7u))) * 4u);
                 return;
             }
         }
@@ -449,24 +444,36 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
     clear();
     // A quarter's products, one by one, `reads` reads and `loads` loads spread between the first of them: the
     // matrix pipe is never without work while they are issued.
-    auto quarter = [&](int hx, int hw, int reads, auto&& read_one, int loads, auto&& load_one, float w = 1.0f) {
+    // (With scales a line's sums are formed by themselves, and scaled into the tile's while the next quarter's are: what waits
+    // for a product's sums waits for the matrix pipe.  `turn`: the places of both.)
+    Sums line[2][T::BLOCKS ? MH * NH : 1];
+    float by[MH];      // of the line that waits
+    auto add = [&](int hx, int hw, int turn, int b) {
+        const int i = b / NH, j = b % NH;
+#pragma unroll
+        for (int e = 0; e < (int)(sizeof(Sums) / 4); ++e) {
+            acc[hx][i][hw][j][e] = __builtin_fmaf(line[turn][b][e], by[i], acc[hx][i][hw][j][e]);
+        }
+    };
+    if constexpr (T::BLOCKS) {
+#pragma unroll
+        for (int i = 0; i < MH; ++i) {
+            by[i] = 0.0f;
+        }
+#pragma unroll
+        for (int b = 0; b < MH * NH; ++b) {
+            line[1][b] = Sums(0.0f);
+        }
+    }
+    auto quarter = [&](int hx, int hw, int reads, auto&& read_one, int loads, auto&& load_one, int turn, int waits_x, int waits_w, float w) {
         constexpr int STEP = STEPS<P, S>, ALL = STEP * MH * NH;
-        // a line's sums by themselves, then scaled into the tile's
-        Sums line[T::BLOCKS ? MH * NH : 1];
-        float by[MH];
+        float next_by[MH];
         if constexpr (T::BLOCKS) {
 #pragma unroll
             for (int i = 0; i < MH; ++i) {
-                by[i] = scale[hx][i] * w;
+                next_by[i] = scale[hx][i] * w;
             }
         }
-        auto add = [&](int b) {
-            const int i = b / NH, j = b % NH;
-#pragma unroll
-            for (int e = 0; e < (int)(sizeof(Sums) / 4); ++e) {
-                acc[hx][i][hw][j][e] = __builtin_fmaf(line[b][e], by[i], acc[hx][i][hw][j][e]);
-            }
-        };
 #pragma unroll
         for (int t = 0; t < ALL; ++t) {
             const int q = t / (MH * NH), i = t / NH % MH, j = t % NH;
@@ -483,21 +490,19 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
                 }
             }
             if constexpr (T::BLOCKS) {
-                constexpr int BEHIND = 2;   // a sum is used two products after its last one
-                line[i * NH + j] = step<P, S>(fw[hw][j], fx[hx][i], q == 0 ? Sums(0.0f) : line[i * NH + j], q);
-                if (q == STEP - 1 && i * NH + j >= BEHIND) {
-                    add(i * NH + j - BEHIND);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                if (t == ALL - 1) {
-#pragma unroll
-                    for (int b = MH * NH > BEHIND ? MH * NH - BEHIND : 0; b < MH * NH; ++b) {
-                        add(b);
-                    }
+                line[turn][i * NH + j] = step<P, S>(fw[hw][j], fx[hx][i], q == 0 ? Sums(0.0f) : line[turn][i * NH + j], q);
+                if (q == 0) {
+                    add(waits_x, waits_w, 1 - turn, t);
                 }
             } else {
                 acc[hx][i][hw][j] = step<P, S>(fw[hw][j], fx[hx][i], acc[hx][i][hw][j], q);
-                __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (T::BLOCKS) {
+#pragma unroll
+            for (int i = 0; i < MH; ++i) {
+                by[i] = next_by[i];
             }
         }
     };
@@ -529,21 +534,27 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
             w = w_scales.of(s);
         }
         meet(INNER || s + D <= steps);              // X of this stage has landed; Y's place is free
+        if constexpr (T::BLOCKS) {   // (so is that of the scales of the run before; the waits count these as loads, and so wait for more)
+            const uint32_t run = s / (uint32_t)T::RUN + 1u, k = s % (uint32_t)T::RUN;
+            if (k < (uint32_t)T::SCALE_LOADS && run * (uint32_t)T::RUN < steps) {
+                load_scales(run, (int)k);
+            }
+        }
         if constexpr (!INNER) {
             if (s + D < steps) {
                 ask(s + D, 0, p, Y);
             }
         }
-        quarter(0, p, WREADS, [&](int k) { read_w(1 - p, X, k); }, LOADS, [&](int k) { load(s + D, 0, p, Y, k); }, w);
-        quarter(0, 1 - p, XREADS, [&](int k) { read_x(1, X, k); }, 0, nothing, w);
+        quarter(0, p, WREADS, [&](int k) { read_w(1 - p, X, k); }, LOADS, [&](int k) { load(s + D, 0, p, Y, k); }, 0, 1, 1 - p, w);
+        quarter(0, 1 - p, XREADS, [&](int k) { read_x(1, X, k, s); }, 0, nothing, 1, 0, p, w);
         meet(INNER || s + D < steps);               // Y of the next stage has landed; X's place is free
         if constexpr (!INNER) {
             if (s + D < steps) {
                 ask(s + D, 1, 1 - p, X);
             }
         }
-        quarter(1, 1 - p, XREADS, [&](int k) { read_x(0, Y_NEXT, k); }, LOADS, [&](int k) { load(s + D, 1, 1 - p, X, k); }, w);
-        quarter(1, p, WREADS, [&](int k) { read_w(1 - p, Y_NEXT, k); }, 0, nothing, w);
+        quarter(1, 1 - p, XREADS, [&](int k) { read_x(0, Y_NEXT, k, s + 1u); }, LOADS, [&](int k) { load(s + D, 1, 1 - p, X, k); }, 0, 0, 1 - p, w);
+        quarter(1, p, WREADS, [&](int k) { read_w(1 - p, Y_NEXT, k); }, 0, nothing, 1, 1, 1 - p, w);
     };
     // (everything that has to be a constant of a stage is one: DEPTH stages one after the other)
     auto stages = [&](uint32_t s, auto inner) {
@@ -562,6 +573,12 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
         one(Constant<5>{});
     };
     static_assert(DEPTH <= 6, "stages() lists six");
+    if constexpr (T::BLOCKS) {
+#pragma unroll
+        for (int k = 0; k < T::SCALE_LOADS; ++k) {
+            load_scales(0u, k);
+        }
+    }
 #pragma unroll
     for (int j = 0; j < DEPTH; ++j) {
         if ((uint32_t)j < steps) {
@@ -576,7 +593,7 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
     }
 #pragma unroll
     for (int k = 0; k < XREADS; ++k) {
-        read_x(0, 0, k);
+        read_x(0, 0, k, 0u);
     }
 #pragma unroll
     for (int k = 0; k < WREADS; ++k) {
@@ -593,13 +610,12 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
     constexpr uint32_t TOUCH = 10;
     const bool touches = a.residual != nullptr && m0 + (uint32_t)T::BM <= a.rows && n0 + (uint32_t)T::BN <= a.n;
     auto touch = [&] {
-        static_assert(T::STAGES + 1024 <= T::LDS_BYTES || S != 32, "a place for them");
-        const uint32_t e = a.residual_bf16 ? 2u : 4u, lines = e;   // lines of a wave's 128 outputs of a row
-        for (uint32_t k = 0; k < 2u * lines; ++k) {
-            const uint32_t at = k * 64u + lane, row = m0 + wm * 128u + at / lines;
+        const uint32_t e = a.residual_bf16 ? 2u : 4u, lines = (uint32_t)(T::NT * S) * e / LINE;   // lines of a wave's outputs of a row
+        for (uint32_t k = 0; k < (uint32_t)(T::MT * S) / 64u * lines; ++k) {
+            const uint32_t at = k * 64u + lane, row = m0 + wm * (uint32_t)(T::MT * S) + at / lines;
             // (rows may start at any element: the first whole word of what a line holds of a row)
-            const uintptr_t p = (reinterpret_cast<uintptr_t>(a.residual) + ((uint64_t)row * a.residual_stride + n0 + wn * 128u) * e + at % lines * LINE + 3u) & ~(uintptr_t)3u;
-            __builtin_amdgcn_global_load_lds((gptr)p, (lptr)(lds + T::STAGES + wave * 256u), 4, 0, 0);
+            const uintptr_t p = (reinterpret_cast<uintptr_t>(a.residual) + ((uint64_t)row * a.residual_stride + n0 + wn * (uint32_t)(T::NT * S)) * e + at % lines * LINE + 3u) & ~(uintptr_t)3u;
+            __builtin_amdgcn_global_load_lds((gptr)p, (lptr)(lds + T::TOUCHED + wave * 256u), 4, 0, 0);
         }
     };
     const uint32_t touch_at = steps > TOUCH ? (steps - TOUCH) / DEPTH * DEPTH : 0u;
@@ -613,6 +629,19 @@ __global__ void __launch_bounds__(256, T::RESIDENT) k_project_tiles(const Projec
     }
     for (; s < steps; s += DEPTH) {
         stages(s, Constant<0>{});
+    }
+    if constexpr (T::BLOCKS) {   // what still waits: the last stage's last quarter
+        auto rest = [&](auto p) {
+#pragma unroll
+            for (int b = 0; b < MH * NH; ++b) {
+                add(1, decltype(p)::value, 1, b);
+            }
+        };
+        if ((steps & 1u) != 0u) {
+            rest(Constant<0>{});
+        } else {
+            rest(Constant<1>{});
+        }
     }
     give_out<T>(a, acc, lds, m0 + wm * (uint32_t)(T::MT * S), n0 + wn * (uint32_t)(T::NT * S), wave, lane, split);
 }
