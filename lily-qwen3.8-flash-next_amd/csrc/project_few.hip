@@ -22,9 +22,8 @@ __device__ const uint4 few_zeros = {0u, 0u, 0u, 0u};   // what lies beyond d
 // RT: blocks of 16 rows of x; DEPTH: lines of a wave in flight.
 template <Products P, int RT, int WAVES, int DEPTH>
 __global__ void __launch_bounds__(WAVES * 64) k_project_few(const ProjectArgs a) {
-    // (with a scale for each block a line brings its rows' scales, a lane one of them)
     constexpr bool BLOCKS = in_blocks(P);
-    constexpr uint32_t ROWS = 16 + 16 * RT, SLOT = ROWS * LINE + (BLOCKS ? 256u : 0u), LOADS = ROWS / 8, ALL_LOADS = LOADS + (BLOCKS ? 1u : 0u);
+    constexpr uint32_t ROWS = 16 + 16 * RT, SLOT = ROWS * LINE, LOADS = ROWS / 8;
     extern __shared__ __align__(16) char lds[];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const uint32_t g = lane >> 4, r = lane & 15u, v0 = blockIdx.x * 16u;
@@ -54,14 +53,22 @@ __global__ void __launch_bounds__(WAVES * 64) k_project_few(const ProjectArgs a)
     typedef __attribute__((address_space(1))) const void* gptr;
     typedef __attribute__((address_space(3))) void* lptr;
     char* ring = lds + wave * (DEPTH * SLOT);
-    const float* x_scale = BLOCKS ? a.x_blocks + (uint64_t)min(lane, a.rows - 1u) * a.x_blocks_stride + from : nullptr;
+    // With a scale for each block: a row's scales of eight lines at a time (one line's would be a request for each of the rows), a run's
+    // behind the rings, the next one's on their way.  A row's eight lie from place row / 8 on, so that 16 rows meet 16 banks.
+    constexpr uint32_t RUN_LOADS = 2u * RT, RUN_BYTES = RT * 16u * 32u;
+    char* const runs = lds + WAVES * DEPTH * SLOT + wave * (2u * RUN_BYTES);
+    auto ask_scales = [&](uint32_t run) {
+#pragma unroll
+        for (uint32_t i = 0; i < RUN_LOADS; ++i) {
+            const uint32_t row = i * 8u + (lane >> 3), l = min(run * 8u + ((lane & 7u) ^ (i & 7u)), count - 1u);
+            __builtin_amdgcn_global_load_lds((gptr)(a.x_blocks + (uint64_t)min(row, a.rows - 1u) * a.x_blocks_stride + from + l),
+                                             (lptr)(runs + (run & 1u) * RUN_BYTES + i * 256u), 4, 0, 0);
+        }
+    };
     WeightScales w_scales = {BLOCKS ? a.w_blocks + (uint64_t)(v0 / LILY_BLOCK) * a.w_blocks_stride + from : nullptr, count, 0.0f};
     auto ask = [&](uint32_t l, uint32_t slot) {
         char* base = ring + slot * SLOT;
         const uint32_t at = l * LINE;
-        if constexpr (BLOCKS) {
-            __builtin_amdgcn_global_load_lds((gptr)(x_scale + l), (lptr)(base + ROWS * LINE), 4, 0, 0);
-        }
         if ((from + l + 1u) * LINE <= a.d_bytes) {
 #pragma unroll
             for (uint32_t i = 0; i < LOADS; ++i) {
@@ -79,6 +86,7 @@ __global__ void __launch_bounds__(WAVES * 64) k_project_few(const ProjectArgs a)
     };
     if (BLOCKS && count != 0u) {
         w_scales.ask(0u);
+        ask_scales(0u);
     }
 #pragma unroll
     for (uint32_t j = 0; j < DEPTH; ++j) {
@@ -97,8 +105,10 @@ __global__ void __launch_bounds__(WAVES * 64) k_project_few(const ProjectArgs a)
     const uint32_t off = r * LINE + ((g ^ (r >> 1)) << 4);
     uint32_t slot = 0;
     for (uint32_t l = 0; l < count; ++l) {
-        if (l + DEPTH <= count) {
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * ALL_LOADS) : "memory");
+        if (BLOCKS && l + DEPTH <= count && (l & 7u) == 1u && l + 7u < count) {   // (a run's scales were asked for in between)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * LOADS + RUN_LOADS) : "memory");
+        } else if (l + DEPTH <= count) {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * LOADS) : "memory");
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
@@ -117,14 +127,17 @@ __global__ void __launch_bounds__(WAVES * 64) k_project_few(const ProjectArgs a)
         }
         float scale[RT];
         if constexpr (BLOCKS) {
-            const float* scales = reinterpret_cast<const float*>(ring + slot * SLOT + ROWS * LINE);
+            const float* scales = reinterpret_cast<const float*>(runs + (l >> 3 & 1u) * RUN_BYTES);
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-                scale[t] = scales[(uint32_t)t * 16u + r];
+                scale[t] = scales[((uint32_t)t * 16u + r) * 8u + ((l ^ ((uint32_t)t * 2u + (r >> 3))) & 7u)];
             }
         }
         __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): the slot has been read
         __builtin_amdgcn_sched_barrier(0);
+        if (BLOCKS && (l & 7u) == 0u && l + 8u < count) {
+            ask_scales(l / 8u + 1u);
+        }
         if (l + DEPTH < count) {
             ask(l + DEPTH, slot);
         }
@@ -169,7 +182,7 @@ __global__ void __launch_bounds__(WAVES * 64) k_project_few(const ProjectArgs a)
 
 template <Products P, int RT, int WAVES, int DEPTH>
 hipError_t launch_few_of(hipStream_t stream, const ProjectArgs& a) {
-    constexpr uint32_t lds = WAVES * DEPTH * ((16 + 16 * RT) * LINE + (in_blocks(P) ? 256u : 0u));
+    constexpr uint32_t lds = WAVES * (DEPTH * (16 + 16 * RT) * LINE + (in_blocks(P) ? 2 * RT * 16 * 32 : 0));
     static_assert(lds >= WAVES * RT * 1024, "the sums' place");
     static LdsAllowed allowed;
     if (const hipError_t e = allowed.say((const void*)k_project_few<P, RT, WAVES, DEPTH>, lds); e != hipSuccess) {

@@ -86,7 +86,16 @@ struct ProjectPlan {
     uint32_t tile = 0;     // 0: few rows
     uint32_t splits = 1;
 };
-inline ProjectPlan project_plan(const ProjectArgs& a, const ProjectWorkspace& ws) {
+// What the estimate goes by, us: a round of tiles and a line of d, and a round's epilogue.
+struct ProjectRates {
+    double few = 85e3;                                      // bytes a compute unit takes in
+    double line64_one = 0.22, line64 = 0.21, tile64 = 0.0;  // (`one`: the least that a line takes)
+    double line128_one = 0.38, line128 = 0.48, tile128 = 0.0;
+    double line256 = 1.45, tile256 = 13.0, tile256_residual = 29.0;
+    uint32_t outputs128 = 128;                              // of a tile of 128 rows
+    bool large = true;                                      // is there a tile of 256?
+};
+inline ProjectPlan project_plan(const ProjectArgs& a, const ProjectWorkspace& ws, const ProjectRates& rate = ProjectRates()) {
     const double rows = a.rows, n = a.n, bytes = a.d_bytes;
     const uint32_t lines = (a.d_bytes + LINE - 1u) / LINE;
     const double memory = ((rows + n) * bytes + rows * n * (a.out_bf16 ? 2.0 : 4.0)) / 5.6e6;
@@ -107,12 +116,12 @@ inline ProjectPlan project_plan(const ProjectArgs& a, const ProjectWorkspace& ws
     };
     if (a.rows <= 64u) {
         const double blocks = a.rows <= 16u ? 2.0 : a.rows <= 32u ? 3.0 : 5.0;   // of 16 rows a workgroup takes in
-        offer(0u, 1u, 2.8 + std::max(memory, rounds(over(a.n, 16u)) * blocks * 16.0 * bytes / 85e3));
+        offer(0u, 1u, 2.8 + std::max(memory, rounds(over(a.n, 16u)) * blocks * 16.0 * bytes / rate.few));
         if (a.rows <= 16u) {
             return best;   // (nothing else reads the weights once)
         }
     }
-    const uint64_t t64 = (uint64_t)over(a.rows, 64u) * over(a.n, 64u), t128 = (uint64_t)over(a.rows, 128u) * over(a.n, 128u),
+    const uint64_t t64 = (uint64_t)over(a.rows, 64u) * over(a.n, 64u), t128 = (uint64_t)over(a.rows, 128u) * over(a.n, rate.outputs128),
                    t256 = (uint64_t)over(a.rows, 256u) * over(a.n, 256u);
     for (uint32_t k = 1; k <= 16u; ++k) {
         if (k > 1u && (lines < 4u * k || (double)k * rows * part_stride(a.n) > (double)ws.part_floats)) {
@@ -120,10 +129,14 @@ inline ProjectPlan project_plan(const ProjectArgs& a, const ProjectWorkspace& ws
         }
         const double each = lines / (double)k, join = k > 1u ? 1.5 + k * rows * n * 8.0 / 5.5e6 : 0.0;
         const double turns64 = rounds(t64 * k), turns128 = t128 * k <= 256u ? (double)(t128 * k) / 256.0 : rounds(t128 * k);
-        offer(64u, k, std::max(3.0 + memory, 4.0 + each * crossed(turns64 <= 2.0) * std::max(0.22, 0.21 * turns64)) + residual + join);
-        offer(128u, k, std::max(3.0 + memory, 6.0 + each * crossed(turns128 <= 1.0) * std::max(0.38, 0.48 * turns128)) + residual + join);
+        offer(64u, k, std::max(3.0 + memory, 4.0 + each * crossed(turns64 <= 2.0) * std::max(rate.line64_one, rate.line64 * turns64) + rate.tile64 * turns64) +
+                          residual + join);
+        offer(128u, k, std::max(3.0 + memory, 6.0 + each * crossed(turns128 <= 1.0) * std::max(rate.line128_one, rate.line128 * turns128) + rate.tile128 * turns128) +
+                           residual + join);
     }
-    offer(256u, 1u, 2.0 + std::max(memory, rounds(t256) * ((a.residual != nullptr ? 29.0 : 13.0) + lines * 1.45)));
+    if (rate.large) {
+        offer(256u, 1u, 2.0 + std::max(memory, rounds(t256) * ((a.residual != nullptr ? rate.tile256_residual : rate.tile256) + lines * rate.line256)));
+    }
     return best;
 }
 

@@ -93,7 +93,7 @@ struct Tile {
     static constexpr int SCALES = BLOCKS ? BM * RUN * 4 : 0, SCALE_LOADS = BM / WAVES / 8;   // bytes of a run; loads of a wave, eight rows each
     // The epilogue's: a wave's rows that lie in LDS at once (half of the large tile's), and floats of a row there (a step of
     // four banks from row to row).
-    static constexpr int PARTS = S == 32 ? 2 : 1, PART_ROWS = MT * S / PARTS, ROW = NT * S + 4;
+    static constexpr int PARTS = S == 32 || WM * WN == 8 ? 2 : 1, PART_ROWS = MT * S / PARTS, ROW = NT * S + 4;
     static constexpr int STAGES = 2 * DEPTH * UNIT, SPREAD = WAVES * PART_ROWS * ROW * 4;   // bytes
     static constexpr int TOUCHED = STAGES + 2 * SCALES, USED = TOUCHED + (S == 32 ? WAVES * 256 : 0);
     static constexpr int LDS_BYTES = SPREAD > USED ? SPREAD : USED;
@@ -307,6 +307,23 @@ __device__ __forceinline__ void give_out(const ProjectArgs& a, const typename Bl
     }
 }
 
+// A workgroup's tile and part of d.  Consecutive workgroups go to consecutive XCDs: each XCD gets a run of tiles of its own (they
+// share its L2), in groups of four tiles of rows.
+struct TilePlace {
+    uint32_t m0, n0, split;
+};
+template <class T>
+__device__ __forceinline__ TilePlace place_of(const ProjectArgs& a, uint32_t m_tiles, uint32_t n_tiles) {
+    const uint32_t tiles = m_tiles * n_tiles, all = tiles * a.splits;
+    const uint32_t xcd = blockIdx.x & 7u, slot = blockIdx.x >> 3, each = all / 8u, more = all % 8u;
+    const uint32_t job = xcd * each + min(xcd, more) + slot;
+    const uint32_t split = job / tiles, tile = job % tiles;
+    constexpr uint32_t GROUP_M = 4;
+    const uint32_t band = tile / (GROUP_M * n_tiles), in_band = tile % (GROUP_M * n_tiles);
+    const uint32_t band_m = min(GROUP_M, m_tiles - band * GROUP_M);
+    return {(band * GROUP_M + in_band % band_m) * (uint32_t)T::BM, in_band / band_m * (uint32_t)T::BN, split};
+}
+
 template <Products P, class T>
 __global__ void __launch_bounds__(64 * T::WAVES, T::RESIDENT * T::WAVES / 4) k_project_tiles(const ProjectArgs a, uint32_t m_tiles, uint32_t n_tiles) {
     constexpr int MH = T::MH, NH = T::NH, S = T::S, DEPTH = T::DEPTH;
@@ -315,16 +332,8 @@ __global__ void __launch_bounds__(64 * T::WAVES, T::RESIDENT * T::WAVES / 4) k_p
     extern __shared__ __align__(16) char lds[];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const uint32_t wm = wave / T::WN, wn = wave % T::WN, r_in = lane % (uint32_t)S;
-    // Consecutive workgroups go to consecutive XCDs: each XCD gets a run of tiles of its own (they share
-    // its L2), in groups of four tiles of rows.
-    const uint32_t tiles = m_tiles * n_tiles, all = tiles * a.splits;
-    const uint32_t xcd = blockIdx.x & 7u, slot = blockIdx.x >> 3, each = all / 8u, more = all % 8u;
-    const uint32_t job = xcd * each + min(xcd, more) + slot;
-    const uint32_t split = job / tiles, tile = job % tiles;
-    constexpr uint32_t GROUP_M = 4;
-    const uint32_t band = tile / (GROUP_M * n_tiles), in_band = tile % (GROUP_M * n_tiles);
-    const uint32_t band_m = min(GROUP_M, m_tiles - band * GROUP_M);
-    const uint32_t m0 = (band * GROUP_M + in_band % band_m) * T::BM, n0 = in_band / band_m * T::BN;
+    const TilePlace place = place_of<T>(a, m_tiles, n_tiles);
+    const uint32_t split = place.split, m0 = place.m0, n0 = place.n0;
 
     const uint32_t stages_all = (a.d_bytes + LINE - 1u) / LINE;
     const uint32_t per = stages_all / a.splits, over = stages_all % a.splits;

@@ -204,6 +204,17 @@ def test_each_tile(monkeypatch, tile, rows, n, d, out):
     s.close()
 
 
+@pytest.mark.parametrize("lines", [1, 2, 3, 4, 8, 9, 17, 63, 64, 65, 129])
+@pytest.mark.parametrize("rows, n", [(1, 1), (255, 257), (256, 512), (600, 300)])
+def test_whole_lines_of_the_largest_tile(monkeypatch, rows, n, lines):
+    """Stages that follow each other in two places of shared memory, eight stages' scales, sixty-four stages' scales of the weights."""
+    monkeypatch.setenv("LILY_SAMPLER_PROJECT", "256")
+    s = LS.Sampler(0)
+    run(s, rows, n, 128 * lines, "bf16")
+    run(s, rows, n, 128 * lines, "bf16", "silu", "f32", "bf16", 1, 3)
+    s.close()
+
+
 @pytest.mark.parametrize("rows", [4, 40, 300])
 def test_scales_of_zero_infinite_scales_and_values_that_are_not_finite(sampler, rows):
     g = torch.Generator(device=dev()).manual_seed(8)
