@@ -3,12 +3,20 @@
 // With p the teacher's list and q = softmax(z / T):
 //     loss = T^2 (sum_j p_j (log p_j - log q_j) [+ P (log P - log Q)]),  grad_v = w T (q_v sum p - p_v) [outside: w T (q_v - P q_v / Q)]
 //
-// A small launch adds up every row's list.  Then a workgroup takes a slice of a row and keeps it in registers, up to 32 values
-// a thread, while the row's slices exchange their sums: a sum is one word (largest value, sum of exponentials), which is the
-// whole message, stored and looked for by relaxed atomics at device scope; a second one holds the list's ids, which stand apart where the
-// rest counts as one outcome.  So rows are read once and written once.  Whoever misses a word after a number of looks (a neighbour has no
-// place on the chip yet) enters its slice into a list and ends; a last launch, which finds every word, does the slices of that list,
-// and the losses.  Rows of more than 64 slices go that way altogether.
+// A workgroup takes a slice of a row and keeps it in registers, up to 64 values a thread, while the row's slices exchange their sums: a sum
+// is one word (largest value, sum of exponentials), which is the whole message, stored and looked for by relaxed atomics at device scope;
+// a second one holds the list's ids, which stand apart where the rest counts as one outcome, a third what the list adds to the loss.  So
+// rows are read once and written once.
+//
+// Few rows, whose slices all have a place on the chip, are one launch.  Every workgroup adds up its row's list itself.  One that misses a
+// word after a number of looks forms that slice's sums itself, by the same operations.  The words lie in a place of their own that is zeros
+// between two calls: the last of a row's workgroups clears them.  37 rows of 151 936 in f32 18.5 us, 24.5 by the three launches that
+// more rows take; 8 of them are the memory's, the others trips to it that wait for each other: the list's ids, the logits they name, the
+// words, and the gradient.
+//
+// Of more rows a small launch adds up the lists and clears the words.  Whoever misses a word (a neighbour has no place on the chip yet) enters
+// its slice into a list and ends; a last launch, which finds every word, does the slices of that list, and the losses.  Rows of more than 64
+// slices go that way altogether.  2048 rows of 151 936 in bf16 254 us (4.9 TB/s), 1024 in f32 256 (4.8).
 //
 // The gradient is written as an id outside the list has it, everywhere, and then anew for the list's ids, by the thread that
 // holds the entry: of an id that the list names twice the first one, found by a bitmap of the slice.  Nothing is added by atomics: the
@@ -27,8 +35,10 @@ namespace {
 constexpr uint32_t NT_DISTILL = DISTILL_THREADS, DISTILL_WAVES = NT_DISTILL / 64u, TURN = NT_DISTILL * 8u;   // ids of a turn
 constexpr uint32_t ENTRIES = LILY_SAMPLE_K_CAP / NT_DISTILL;
 constexpr uint32_t WORD_SLICES = 64u;   // slices of a row that a wave looks for
+constexpr uint32_t WORDS = 3u;          // of a slice
 
 enum Form {
+    FORM_ALONE,   // everything, by slices that wait for each other: few rows
     FORM_HELD,    // sums, and the gradient by slices that wait for each other
     FORM_SUM,     // the sums alone
     FORM_AFTER,   // the gradient from the sums of a launch before, of all slices or of those that are left; losses and stats
@@ -41,7 +51,7 @@ struct Listed {
     float left;        // P
     float weight;      // of the row's gradient
     uint32_t live;     // some entry counts, and has a probability
-    double known;      // of the loss, what does not wait for the row's sum: sum_j p_j (log p_j - z_j / T)
+    double entropy;    // sum_j p_j log p_j
 };
 
 struct DistillArgs {
@@ -54,8 +64,11 @@ struct DistillArgs {
     float* loss;
     float* stats;
     void* grad;
-    uint64_t* words;    // [rows][slices][2]: of a slice, (largest value << 32 | sum) outside the list, and in it; 0 = not there
+    // [rows][slices][WORDS]: of a slice, (largest value << 32 | sum) outside the list, and in it, and the sum of p_j z_j of the entries
+    // that lie in it, in 64 bits (-0.0 for zero); 0 = not there
+    uint64_t* words;
     Listed* listed;     // [rows]
+    uint32_t* done;     // [rows] (of few rows): how many slices need the row's words no more
     uint32_t* late;     // [0]: how many slices are left to the last launch, then which; null: all of them
     uint32_t rows;      // of the launch
     uint64_t logits_stride, ids_stride, values_stride, grad_stride;   // elements
@@ -89,16 +102,10 @@ __device__ __forceinline__ void group_sums(Sum (&t)[N], float c2, float* part) {
     }
     __syncthreads();
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-        float m = NEG_INF, s = 0.0f;
-        for (uint32_t q = 0; q < WAVES; ++q) {
-            m = fmaxf(m, part[(q * N + (uint32_t)n) * 2u]);
-        }
-        for (uint32_t q = 0; q < WAVES; ++q) {
-            const float mq = part[(q * N + (uint32_t)n) * 2u];
-            s += part[(q * N + (uint32_t)n) * 2u + 1u] * term(mq == NEG_INF ? reference(m) : mq, m, c2);
-        }
-        t[n] = {m, s};
+    for (int n = 0; n < N; ++n) {   // (a lane a wave's)
+        const uint32_t q = (threadIdx.x % WAVES) * N + (uint32_t)n;
+        const float mq = part[q * 2u], m = wave_max_dpp(mq), sq = part[q * 2u + 1u] * term(mq == NEG_INF ? reference(m) : mq, m, c2);
+        t[n] = {m, wave_sum_f((threadIdx.x & 63u) < WAVES ? sq : 0.0f)};
     }
 }
 
@@ -131,16 +138,80 @@ __device__ __forceinline__ float entry_probability(const DistillArgs& a, float t
     return entry_mass(a, t, l.top, lse) * (a.rest != 0u ? 1.0f : 1.0f / l.sum);
 }
 
+__device__ __forceinline__ double wave_sum_of(double d) {
+    for (int off = 32; off > 0; off >>= 1) {
+        d += __shfl_xor(d, off);
+    }
+    return d;
+}
+// A wave's parts together, behind a barrier.
+template <uint32_t WAVES>
+__device__ __forceinline__ double together(const double* part) {
+    double d = 0.0;
+#pragma unroll
+    for (uint32_t q = 0; q < WAVES; ++q) {
+        d += part[q];
+    }
+    return d;
+}
+
+// A row's list added up, by a workgroup of WAVES waves: a thread has entries e * 64 WAVES + tid.
+template <uint32_t WAVES, uint32_t E>
+__device__ __forceinline__ Listed add_up(const DistillArgs& a, uint64_t row, const uint32_t (&id)[E], const float (&t)[E], float lse, float* part) {
+    const bool relative = a.probs == 0u && a.rest == 0u;
+    Sum mass[1] = {{NEG_INF, 0.0f}};   // (relative to 0, where it is not to the largest value: -inf where no entry counts)
+#pragma unroll
+    for (uint32_t e = 0; e < E; ++e) {
+        if (id[e] != LILY_NO_TOKEN) {
+            mass[0].m = relative ? fmaxf(mass[0].m, t[e]) : 0.0f;
+        }
+    }
+    const float own = mass[0].m;
+#pragma unroll
+    for (uint32_t e = 0; e < E; ++e) {
+        mass[0].s += id[e] != LILY_NO_TOKEN ? entry_mass(a, t[e], own, lse) : 0.0f;
+    }
+    group_sums<WAVES>(mass, a.c2, part);
+    Listed l = {};
+    l.sum = mass[0].s;
+    l.top = mass[0].m;
+    l.left = a.rest == 0u ? 0.0f : l.sum < 1.0f || l.sum != l.sum ? 1.0f - l.sum : 0.0f;
+    l.weight = a.grad_scale * (a.row_weights != nullptr ? gload(a.row_weights + row) : 1.0f);
+    l.live = (a.rest != 0u ? l.top == 0.0f : l.sum > 0.0f || l.sum != l.sum) ? 1u : 0u;
+    return l;
+}
+// Of its entropy, a wave's part in part[wave] (in 64 bits: a loss near zero is a difference of large logarithms).
+template <uint32_t WAVES, uint32_t E>
+__device__ __forceinline__ void entropy_of(const DistillArgs& a, const uint32_t (&id)[E], const float (&t)[E], const Listed& l, float lse, double* part) {
+    double d = 0.0;
+    if ((threadIdx.x & ~63u) < a.k) {   // (a wave without entries has nothing to add up)
+        const double log_sum = a.rest != 0u ? 0.0 : log((double)l.sum);
+#pragma unroll
+        for (uint32_t e = 0; e < E; ++e) {
+            if (id[e] != LILY_NO_TOKEN) {
+                const float p = entry_probability(a, t[e], l, lse);
+                const double log_p = a.probs != 0u  ? log((double)t[e]) - log_sum
+                                     : a.rest != 0u ? (double)t[e] * a.over_t - (double)lse
+                                                    : ((double)t[e] - (double)l.top) * a.over_t - log_sum;
+                d += p == 0.0f ? 0.0 : (double)p * log_p;
+            }
+        }
+        d = wave_sum_of(d);
+    }
+    if ((threadIdx.x & 63u) == 0u) {
+        part[threadIdx.x >> 6] = d;
+    }
+}
+
 // A row's list added up, its words cleared: a workgroup a row.
 __global__ void __launch_bounds__(256) k_distill_lists(const DistillArgs a) {
-    __shared__ float part[4 * 2 * 2];
+    __shared__ float part[4 * 2];
     __shared__ double part_d[4];
     constexpr uint32_t E = LILY_SAMPLE_K_CAP / 256u;
     const uint32_t tid = threadIdx.x, in_launch = blockIdx.x;
     const uint64_t row = a.row0 + in_launch;
     const uint32_t count = list_length(a, row);
     const float lse = a.teacher_lse != nullptr ? gload(a.teacher_lse + row) : 0.0f;
-    const bool relative = a.probs == 0u && a.rest == 0u;
     uint32_t id[E];
     float t[E];
 #pragma unroll
@@ -156,55 +227,16 @@ __global__ void __launch_bounds__(256) k_distill_lists(const DistillArgs a) {
     if (in_launch == 0u && tid == 0u && a.late != nullptr) {
         a.late[0] = 0u;
     }
-    for (uint32_t q = tid; q < a.slices * 2u; q += 256u) {
-        store_through(a.words + (uint64_t)in_launch * a.slices * 2u + q, (uint64_t)0);
+    for (uint32_t q = tid; q < a.slices * WORDS; q += 256u) {
+        store_through(a.words + (uint64_t)in_launch * a.slices * WORDS + q, (uint64_t)0);
     }
-    Sum mass[2] = {{relative ? NEG_INF : 0.0f, 0.0f}, {NEG_INF, 0.0f}};   // of the list; [1].m: whether any entry counts
-#pragma unroll
-    for (uint32_t e = 0; e < E; ++e) {
-        if (id[e] != LILY_NO_TOKEN) {
-            mass[0].m = relative ? fmaxf(mass[0].m, t[e]) : 0.0f;
-            mass[1].m = 0.0f;
-        }
-    }
-    const float own = mass[0].m;
-#pragma unroll
-    for (uint32_t e = 0; e < E; ++e) {
-        mass[0].s += id[e] != LILY_NO_TOKEN ? entry_mass(a, t[e], own, lse) : 0.0f;
-    }
-    group_sums<4u>(mass, a.c2, part);
-    const float sum = mass[0].s;
-    Listed l = {};
-    l.sum = sum;
-    l.top = mass[0].m;
-    double d = 0.0;   // (in 64 bits: a loss near zero is a difference of large logarithms)
+    Listed l = add_up<4u>(a, row, id, t, lse, part);
     if (a.loss != nullptr) {
-        const void* z = at_row(a.logits, row, a.logits_stride, a.logits_bf16);
-        const double log_sum = a.rest != 0u ? 0.0 : log((double)sum);
-#pragma unroll
-        for (uint32_t e = 0; e < E; ++e) {
-            if (id[e] != LILY_NO_TOKEN) {
-                const float p = entry_probability(a, t[e], l, lse);
-                const double log_p = a.probs != 0u  ? log((double)t[e]) - log_sum
-                                     : a.rest != 0u ? (double)t[e] * a.over_t - (double)lse
-                                                    : ((double)t[e] - (double)l.top) * a.over_t - log_sum;
-                d += p == 0.0f ? 0.0 : (double)p * (log_p - (double)load1(z, id[e], a.logits_bf16) * a.over_t);
-            }
-        }
-        for (int off = 32; off > 0; off >>= 1) {
-            d += __shfl_xor(d, off);
-        }
-        if ((tid & 63u) == 0u) {
-            part_d[tid >> 6] = d;
-        }
+        entropy_of<4u>(a, id, t, l, lse, part_d);
         __syncthreads();
-        d = part_d[0] + part_d[1] + part_d[2] + part_d[3];
+        l.entropy = together<4u>(part_d);
     }
     if (tid == 0u) {
-        l.left = a.rest == 0u ? 0.0f : sum < 1.0f || sum != sum ? 1.0f - sum : 0.0f;
-        l.weight = a.grad_scale * (a.row_weights != nullptr ? gload(a.row_weights + row) : 1.0f);
-        l.live = mass[1].m == 0.0f && (a.rest != 0u || sum > 0.0f || sum != sum) ? 1u : 0u;
-        l.known = d;
         a.listed[in_launch] = l;
     }
 }
@@ -233,12 +265,16 @@ __device__ __forceinline__ RowSums of_sums(const DistillArgs& a, Sum out, Sum in
     r.out = out;
     r.all = joined(out, in, a.c2);
     const float m = r.all.m;
-    r.log_all = m == NEG_INF ? __builtin_nanf("") : logf(r.all.s);
     r.nothing = out.m == NEG_INF && out.s == 0.0f;
-    r.log_out = r.nothing ? 0.0f : logf(out.s);
+    r.log_all = r.log_out = 0.0f;   // (with_logarithms: the gradient needs none)
     r.inv_all = m == NEG_INF ? __builtin_nanf("") : 1.0f / r.all.s;
     r.inv_out = 1.0f / out.s;
     r.q_out = term(out.m == NEG_INF ? reference(m) : out.m, m, a.c2) * out.s * r.inv_all;
+    return r;
+}
+__device__ __forceinline__ RowSums with_logarithms(RowSums r) {
+    r.log_all = r.all.m == NEG_INF ? __builtin_nanf("") : logf(r.all.s);
+    r.log_out = r.nothing ? 0.0f : logf(r.out.s);
     return r;
 }
 __device__ __forceinline__ RowSums of_stats(const DistillArgs& a, uint64_t row) {
@@ -308,9 +344,13 @@ __device__ __forceinline__ uint64_t word_of(Sum s) { return (uint64_t)lilym_f32_
 __device__ __forceinline__ Sum sum_of(uint64_t w) { return {lilym_bits_f32((uint32_t)(w >> 32)), lilym_bits_f32((uint32_t)w)}; }
 
 // A row's sums from its slices' words, the same in every lane of a wave.
-__device__ __forceinline__ RowSums of_words(const DistillArgs& a, uint32_t lane, const uint64_t (*words)[2]) {
+__device__ __forceinline__ RowSums of_words(const DistillArgs& a, uint32_t lane, const uint64_t (*words)[WORDS]) {
     Sum o = {NEG_INF, 0.0f}, i = {NEG_INF, 0.0f};
-    for (uint32_t q = lane; q < a.slices; q += 64u) {
+    if (lane < a.slices) {
+        o = sum_of(words[lane][0]);
+        i = sum_of(words[lane][1]);
+    }
+    for (uint32_t q = lane + 64u; q < a.slices; q += 64u) {
         o = joined(o, sum_of(words[q][0]), a.c2);
         i = joined(i, sum_of(words[q][1]), a.c2);
     }
@@ -322,26 +362,254 @@ __device__ __forceinline__ RowSums of_words(const DistillArgs& a, uint32_t lane,
     return of_sums(a, all_o, all_i);
 }
 
-// A row's loss and stats, by a wave.
-__device__ __forceinline__ void finish_row(const DistillArgs& a, uint32_t in_launch, uint32_t lane) {
-    const uint64_t row = a.row0 + in_launch;
-    const RowSums r = of_words(a, lane, reinterpret_cast<const uint64_t (*)[2]>(a.words) + (uint64_t)in_launch * a.slices);
-    if (lane != 0u) {
-        return;
+// Their third words together, the same in every lane of a wave.
+__device__ __forceinline__ double products_of_words(const DistillArgs& a, uint32_t lane, const uint64_t (*words)[WORDS]) {
+    double d = 0.0;
+    for (uint32_t q = lane; q < a.slices; q += 64u) {
+        d += __longlong_as_double((long long)words[q][2]);
     }
+    return wave_sum_of(d);
+}
+
+// From the wave that formed them to the workgroup.
+constexpr uint32_t ROW_SUMS = 8;
+__device__ __forceinline__ void hand_over(float* to, const RowSums& r) {
+    const float v[ROW_SUMS] = {r.all.m, r.all.s, r.out.m, r.out.s, r.inv_all, r.inv_out, r.q_out, r.nothing ? 1.0f : 0.0f};
+#pragma unroll
+    for (uint32_t i = 0; i < ROW_SUMS; ++i) {
+        to[i] = v[i];
+    }
+}
+__device__ __forceinline__ RowSums handed(const float* from) {
+    return {{from[0], from[1]}, {from[2], from[3]}, 0.0f, 0.0f, from[4], from[5], from[6], from[7] != 0.0f};
+}
+
+// (FORM_ALONE) A workgroup that needs its row's words no more, and has stored its own, says so; the last one clears them for the next call.
+__device__ __forceinline__ uint32_t leave_row(const DistillArgs& a, uint32_t in_launch) {
+    return threadIdx.x == 0u ? atomicAdd(a.done + in_launch, 1u) : 0u;
+}
+__device__ __forceinline__ void clear_row(const DistillArgs& a, uint32_t in_launch, uint64_t* words, uint32_t before) {
+    if (threadIdx.x < 64u && (uint32_t)__builtin_amdgcn_readfirstlane((int)before) == a.slices - 1u) {
+        for (uint32_t q = threadIdx.x; q < a.slices * WORDS; q += 64u) {
+            store_through(words + q, (uint64_t)0);
+        }
+        if (threadIdx.x == 0u) {
+            store_through(a.done + in_launch, 0u);
+        }
+    }
+}
+
+// A row's loss and stats, by a thread.
+__device__ __forceinline__ void finish_row(const DistillArgs& a, uint64_t row, const RowSums& sums, const Listed& l, double products) {
+    const RowSums r = with_logarithms(sums);
     if (a.stats != nullptr) {
         store_stats(a, row, r);
     }
     if (a.loss != nullptr) {
         // (the sums' part of it: log q = z / T - z0 / T - log(sum); a row of -inf alone has no sum, its logarithm is no number)
-        const Listed l = a.listed[in_launch];
         const double log_all = r.log_all != r.log_all ? (double)r.log_all : log((double)r.all.s), top = (double)r.all.m * a.over_t;
-        double d = l.known + (double)l.sum * (a.rest != 0u ? 1.0 : 1.0 / (double)l.sum) * (top + log_all);
+        double d = l.entropy - products * a.over_t + (double)l.sum * (a.rest != 0u ? 1.0 : 1.0 / (double)l.sum) * (top + log_all);
         if (a.rest != 0u && l.left != 0.0f) {
             const double log_q = r.nothing ? -INFINITY : (double)reference(r.out.m) * a.over_t - top + log((double)r.out.s) - log_all;
             d += (double)l.left * (log((double)l.left) - log_q);
         }
         a.loss[row] = l.live != 0u ? (float)(d * (double)a.temperature * (double)a.temperature) + (r.log_all != r.log_all ? r.log_all : 0.0f) : 0.0f;
+    }
+}
+
+// A thread's part of a slice: pieces of eight ids, and an id behind the row's last whole piece.
+template <uint32_t TURNS, bool BF16>
+struct Part {
+    Eight<BF16> raw[TURNS];
+    uint32_t lo, hi, whole, last_at;
+    float last;
+
+    __device__ __forceinline__ void load(const DistillArgs& a, const void* z, uint32_t slice) {
+        const uint32_t tid = threadIdx.x;
+        whole = a.vocab / 8u;   // pieces of a row
+        lo = slice * (TURNS * TURN);
+        hi = min(lo + TURNS * TURN, a.vocab);
+        if (whole != 0u) {
+#pragma unroll
+            for (uint32_t c = 0; c < TURNS; ++c) {
+                raw[c].load(z, min(lo / 8u + c * NT_DISTILL + tid, whole - 1u) * 8u);
+            }
+        }
+        last_at = whole * 8u >= lo && whole * 8u + tid < hi ? whole * 8u + tid : LILY_NO_TOKEN;
+        last = last_at != LILY_NO_TOKEN ? load1(z, last_at, BF16) : NEG_INF;
+    }
+    __device__ __forceinline__ bool there(uint32_t c) const { return whole != 0u && lo / 8u + c * NT_DISTILL + threadIdx.x < whole; }
+};
+
+// The ids that stand in a slice, in LDS (a thread's entries in its own places) and marked; a thread's entries' logits.  The caller's next
+// barrier stands behind it.  `id`: as loaded; of those that do not count LILY_NO_TOKEN afterwards.
+template <uint32_t TURNS, bool BF16>
+__device__ __forceinline__ void enter(const DistillArgs& a, const void* z, const Part<TURNS, BF16>& part, uint32_t count, SliceList& list,
+                                      uint32_t (&id)[ENTRIES], bool (&here)[ENTRIES], float (&mine)[ENTRIES]) {
+    const uint32_t tid = threadIdx.x;
+    for (uint32_t w = tid; w < TURNS * TURN / 32u; w += NT_DISTILL) {
+        list.bits[w] = 0u;
+    }
+    static_assert(TURNS * TURN <= DISTILL_SLICE, "a bit for every id of a slice");
+    if (tid == 0u) {
+        list.twice = 0u;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t e = 0; e < ENTRIES; ++e) {
+        const uint32_t j = e * NT_DISTILL + tid, off = id[e] - part.lo;
+        id[e] = j < count && id[e] < a.vocab ? id[e] : LILY_NO_TOKEN;
+        here[e] = id[e] >= part.lo && id[e] < part.hi;
+        mine[e] = NEG_INF;
+        if (j < a.k) {
+            list.ids[j] = here[e] ? id[e] : LILY_NO_TOKEN;
+        }
+        if (here[e]) {
+            mine[e] = load1(z, id[e], BF16);
+            if ((atomicOr(&list.bits[off >> 5], 1u << (off & 31u)) >> (off & 31u) & 1u) != 0u) {
+                list.twice = 1u;
+            }
+        }
+    }
+}
+// Of an id that stands there twice the first entry speaks for all of them.
+__device__ __forceinline__ void make_unique(const DistillArgs& a, SliceList& list, bool probabilities) {
+    if (list.twice == 0u) {
+        return;
+    }
+    __syncthreads();
+    bool first[ENTRIES];
+    float p[ENTRIES];
+#pragma unroll
+    for (uint32_t e = 0; e < ENTRIES; ++e) {
+        const uint32_t j = e * NT_DISTILL + threadIdx.x;
+        first[e] = j < a.k && list.ids[j] != LILY_NO_TOKEN && speaks(list, j);
+        p[e] = first[e] && probabilities ? added_up(list, j, a.k) : 0.0f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t e = 0; e < ENTRIES; ++e) {
+        const uint32_t j = e * NT_DISTILL + threadIdx.x;
+        if (first[e]) {
+            list.p[j] = p[e];
+        } else if (j < a.k) {
+            list.ids[j] = LILY_NO_TOKEN;
+        }
+    }
+}
+// A slice's entries' logits and probabilities, kept in the thread's own places in LDS, and a wave's part of the sum of their products in
+// part[wave].
+__device__ __forceinline__ void keep(const DistillArgs& a, const Listed& l, float lse, SliceList& list, const bool (&here)[ENTRIES],
+                                     const float (&z)[ENTRIES], const float (&t)[ENTRIES], double* part) {
+    double d = 0.0;
+    if ((threadIdx.x & ~63u) < a.k) {
+#pragma unroll
+        for (uint32_t e = 0; e < ENTRIES; ++e) {
+            if (here[e]) {
+                const float p = entry_probability(a, t[e], l, lse);
+                list.z[e * NT_DISTILL + threadIdx.x] = z[e];
+                list.p[e * NT_DISTILL + threadIdx.x] = p;
+                d += p == 0.0f ? 0.0 : (double)p * (double)z[e];
+            }
+        }
+        if (a.loss != nullptr) {
+            d = wave_sum_of(d);
+        }
+    }
+    if ((threadIdx.x & 63u) == 0u) {
+        part[threadIdx.x >> 6] = d;
+    }
+}
+__device__ __forceinline__ uint64_t word_of(double d) { return (uint64_t)__double_as_longlong(d == 0.0 ? -0.0 : d); }
+
+// A thread's exponentials of a slice, relative to its largest value `own`, and its sums: outside the list, and in it.
+template <uint32_t TURNS, bool BF16>
+__device__ __forceinline__ void exponentials(const DistillArgs& a, const Part<TURNS, BF16>& part, const SliceList& list, bool sums, float (&x)[TURNS][8],
+                                             float& last_x, float& own, Sum (&s)[2]) {
+    const uint8_t* named = reinterpret_cast<const uint8_t*>(list.bits);
+    const uint32_t tid = threadIdx.x, behind = part.last_at - part.lo;
+    const bool counts = part.last_at != LILY_NO_TOKEN && (a.rest == 0u || (list.bits[behind >> 5] >> (behind & 31u) & 1u) == 0u);
+    own = counts ? part.last : NEG_INF;
+#pragma unroll
+    for (uint32_t c = 0; c < TURNS; ++c) {
+        part.raw[c].widened(x[c]);
+        // What the list names is not outside it (its gradient is formed elsewhere), and what is not there is nothing.
+        const uint32_t out = !part.there(c) ? 255u : a.rest != 0u ? named[c * NT_DISTILL + tid] : 0u;
+        if (out != 0u) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[c][j] = (out >> j & 1u) != 0u ? NEG_INF : x[c][j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            own = fmaxf(own, x[c][j]);
+        }
+    }
+    const float ref = reference(own);
+    last_x = counts ? __builtin_amdgcn_exp2f((part.last - ref) * a.c2) : 0.0f;
+    float sum = last_x;
+#pragma unroll
+    for (uint32_t c = 0; c < TURNS; ++c) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[c][j] = __builtin_amdgcn_exp2f((x[c][j] - ref) * a.c2);
+            sum += x[c][j];
+        }
+    }
+    s[0] = {own, sum};
+    s[1] = {NEG_INF, 0.0f};
+    if (sums && a.rest != 0u) {
+        for (uint32_t j = tid; j < a.k; j += NT_DISTILL) {
+            if (list.ids[j] != LILY_NO_TOKEN) {
+                const float v = list.z[j];
+                s[1] = joined(s[1], {v, term(v, v, a.c2)}, a.c2);
+            }
+        }
+    }
+}
+
+
+// (FORM_ALONE) The words of the slices `left` of the row that slice `at` belongs to, which have not come: from the logits, by the operations
+// of their own workgroups.  What has come by then stands: that workgroup may have stored its gradient over the logits since, and has
+// stored the words first.  Not a part of its caller: that keeps its own slice in registers.  `of`: the kernel's arguments.
+template <uint32_t TURNS, bool BF16>
+__device__ __attribute__((noinline)) void words_of_slices(const DistillArgs* of, uint32_t at, uint64_t left, uint64_t* words) {
+    __shared__ SliceList list;
+    __shared__ float sums[DISTILL_WAVES * 4];
+    __shared__ double products[DISTILL_WAVES];
+    const DistillArgs a = *of;
+    const uint32_t tid = threadIdx.x, in_launch = at / a.slices;
+    const uint64_t row = a.row0 + in_launch;
+    const void* z = at_row(a.logits, row, a.logits_stride, BF16);
+    const uint32_t count = list_length(a, row);
+    const float lse = a.teacher_lse != nullptr ? gload(a.teacher_lse + row) : 0.0f;
+    for (; left != 0ull; left &= left - 1ull) {
+        const uint32_t slice = (uint32_t)__builtin_ctzll(left);
+        uint32_t id[ENTRIES];
+        float value[ENTRIES], mine[ENTRIES];
+        bool here[ENTRIES];
+#pragma unroll
+        for (uint32_t e = 0; e < ENTRIES; ++e) {
+            id[e] = gload(a.ids + row * a.ids_stride + min(e * NT_DISTILL + tid, a.k - 1u));
+            value[e] = entry_value(a, row, min(e * NT_DISTILL + tid, a.k - 1u));
+        }
+        Part<TURNS, BF16> part;
+        part.load(a, z, slice);
+        enter(a, z, part, count, list, id, here, mine);
+        const Listed l = add_up<DISTILL_WAVES>(a, row, id, value, lse, sums);
+        __syncthreads();
+        keep(a, l, lse, list, here, mine, value, products);
+        make_unique(a, list, false);
+        Sum s[2];
+        float x[TURNS][8], last_x, own;
+        exponentials(a, part, list, true, x, last_x, own, s);
+        group_sums<DISTILL_WAVES>(s, a.c2, sums);
+        if (tid < WORDS) {
+            const uint64_t come = load_through(a.words + ((uint64_t)in_launch * a.slices + slice) * WORDS + tid);
+            words[slice * WORDS + tid] = come != 0ull ? come : tid == 2u ? word_of(together<DISTILL_WAVES>(products)) : word_of(tid == 0u ? s[0] : s[1]);
+        }
+        __syncthreads();   // (the list and the sums' places have been read)
     }
 }
 
@@ -351,190 +619,145 @@ __device__ __forceinline__ void finish_row(const DistillArgs& a, uint32_t in_lau
 template <uint32_t TURNS, bool BF16, int FORM>
 __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at) {
     __shared__ SliceList list;
-    __shared__ float part[DISTILL_WAVES * 4];
-    __shared__ uint64_t words[WORD_SLICES][2];
-    __shared__ uint32_t missing;
-    constexpr uint32_t SLICE = TURNS * TURN;
+    __shared__ float sums[DISTILL_WAVES * 4];
+    __shared__ double entropy[FORM == FORM_ALONE ? DISTILL_WAVES : 1];
+    __shared__ uint64_t words[WORD_SLICES][WORDS];
+    __shared__ double products[DISTILL_WAVES];
+    __shared__ uint64_t missing;
+    __shared__ float come[ROW_SUMS];
     // (the backward pass has sums and needs none; a slice that was left is done as it would have been)
-    constexpr bool EXPS = FORM != FORM_BACK, SUMS = FORM == FORM_HELD || FORM == FORM_SUM;
+    constexpr bool EXPS = FORM != FORM_BACK, SUMS = FORM == FORM_ALONE || FORM == FORM_HELD || FORM == FORM_SUM;
+    constexpr bool ADDS = FORM == FORM_ALONE || FORM == FORM_BACK;   // adds up its row's list itself
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
     const uint32_t slice = at % a.slices, in_launch = at / a.slices;
     const uint64_t row = a.row0 + in_launch;
     const void* z = at_row(a.logits, row, a.logits_stride, BF16);
-    const uint32_t whole = a.vocab / 8u;   // whole pieces of a row; the ids behind them are an id a thread
-    const uint32_t lo = slice * SLICE, hi = min(lo + SLICE, a.vocab), first = lo / 8u;
     const uint32_t count = list_length(a, row);
 
+    const float lse = a.teacher_lse != nullptr ? gload(a.teacher_lse + row) : 0.0f;
+    uint64_t* out = a.words + (uint64_t)in_launch * a.slices * WORDS;
+    const bool finishes = FORM == FORM_ALONE && slice == 0u && a.loss != nullptr;   // (the others have no use for the third words)
+
     uint32_t id[ENTRIES];
+    float value[ENTRIES];
 #pragma unroll
     for (uint32_t e = 0; e < ENTRIES; ++e) {
         id[e] = gload(a.ids + row * a.ids_stride + min(e * NT_DISTILL + tid, a.k - 1u));
+        value[e] = ADDS ? entry_value(a, row, min(e * NT_DISTILL + tid, a.k - 1u)) : 0.0f;
     }
-    Eight<BF16> raw[TURNS];
-    if (whole != 0u) {
-#pragma unroll
-        for (uint32_t c = 0; c < TURNS; ++c) {
-            raw[c].load(z, min(first + c * NT_DISTILL + tid, whole - 1u) * 8u);
-        }
-    }
-    const uint32_t last_at = whole * 8u >= lo && whole * 8u + tid < hi ? whole * 8u + tid : LILY_NO_TOKEN;
-    const float last = last_at != LILY_NO_TOKEN ? load1(z, last_at, BF16) : NEG_INF;   // the id behind the pieces
-    auto there = [&](uint32_t c) { return whole != 0u && first + c * NT_DISTILL + tid < whole; };
-    for (uint32_t w = tid; w < SLICE / 32u; w += NT_DISTILL) {
-        list.bits[w] = 0u;
-    }
-    static_assert(SLICE <= DISTILL_SLICE, "a bit for every id of a slice");
-    if (tid == 0u) {
-        list.twice = 0u;
-    }
-    __syncthreads();
-    bool here[ENTRIES];                        // entries of the slice: of an id that stands there twice, the first
-    float mine[ENTRIES], value[ENTRIES];       // their logits, and their values
-#pragma unroll
-    for (uint32_t e = 0; e < ENTRIES; ++e) {
-        const uint32_t j = e * NT_DISTILL + tid, off = id[e] - lo;
-        id[e] = j < count && id[e] < a.vocab ? id[e] : LILY_NO_TOKEN;
-        here[e] = id[e] >= lo && id[e] < hi;
-        mine[e] = NEG_INF;
-        value[e] = 0.0f;
-        if (j < a.k) {
-            list.ids[j] = id[e];
-        }
-        if (here[e]) {
-            mine[e] = load1(z, id[e], BF16);
-            value[e] = entry_value(a, row, j);
-            if ((atomicOr(&list.bits[off >> 5], 1u << (off & 31u)) >> (off & 31u) & 1u) != 0u) {
-                list.twice = 1u;
-            }
-        }
-    }
-    __syncthreads();
-    const bool twice = list.twice != 0u;
+    Part<TURNS, BF16> part;
+    part.load(a, z, slice);
+    bool here[ENTRIES];   // entries of the slice
+    float mine[ENTRIES];
+    enter(a, z, part, count, list, id, here, mine);
     Listed l = {};
-    if constexpr (FORM != FORM_SUM) {
+    if constexpr (ADDS) {
+        l = add_up<DISTILL_WAVES>(a, row, id, value, lse, sums);
+    } else {
+#pragma unroll
+        for (uint32_t e = 0; e < ENTRIES; ++e) {
+            if (here[e]) {
+                value[e] = entry_value(a, row, e * NT_DISTILL + tid);
+            }
+        }
         l = a.listed[in_launch];
-        const float lse = a.teacher_lse != nullptr ? gload(a.teacher_lse + row) : 0.0f;
-#pragma unroll
-        for (uint32_t e = 0; e < ENTRIES; ++e) {
-            if (here[e]) {
-                list.p[e * NT_DISTILL + tid] = entry_probability(a, value[e], l, lse);
-            }
-        }
     }
-    if (twice) {   // the first of an id speaks for all of them
-        __syncthreads();
-        float p[ENTRIES];
-#pragma unroll
-        for (uint32_t e = 0; e < ENTRIES; ++e) {
-            here[e] = here[e] && speaks(list, e * NT_DISTILL + tid);
-            p[e] = here[e] && FORM != FORM_SUM ? added_up(list, e * NT_DISTILL + tid, a.k) : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (uint32_t e = 0; e < ENTRIES; ++e) {
-            if (here[e]) {
-                list.p[e * NT_DISTILL + tid] = p[e];
-            }
-        }
-    }
+    __syncthreads();
     // (from here on a thread's entries are its own places in LDS: the slice needs the registers)
-#pragma unroll
-    for (uint32_t e = 0; e < ENTRIES; ++e) {
-        const uint32_t j = e * NT_DISTILL + tid;
-        if (j < a.k) {
-            list.ids[j] = here[e] ? id[e] : LILY_NO_TOKEN;
-            list.z[j] = mine[e];
-        }
-    }
+    keep(a, l, lse, list, here, mine, value, products);
+    make_unique(a, list, FORM != FORM_SUM);
 
-    // The slice's sums, in every thread; its exponentials, relative to the thread's largest value, stay for the gradient.
-    Sum s[2] = {{NEG_INF, 0.0f}, {NEG_INF, 0.0f}};
+    Sum s[2];   // the slice's, in every thread; its exponentials stay for the gradient
     float x[TURNS][8], last_x = 0.0f, own = NEG_INF;
     if constexpr (EXPS) {
-        const uint8_t* named = reinterpret_cast<const uint8_t*>(list.bits);
-        const uint32_t behind = last_at - lo;
-        const bool counts = last_at != LILY_NO_TOKEN && (a.rest == 0u || (list.bits[behind >> 5] >> (behind & 31u) & 1u) == 0u);
-        own = counts ? last : NEG_INF;
-#pragma unroll
-        for (uint32_t c = 0; c < TURNS; ++c) {
-            raw[c].widened(x[c]);
-            // What the list names is not outside it (its gradient is formed elsewhere), and what is not there is nothing.
-            const uint32_t out = !there(c) ? 255u : a.rest != 0u ? named[c * NT_DISTILL + tid] : 0u;
-            if (out != 0u) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    x[c][j] = (out >> j & 1u) != 0u ? NEG_INF : x[c][j];
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                own = fmaxf(own, x[c][j]);
-            }
-        }
-        const float ref = reference(own);
-        last_x = counts ? __builtin_amdgcn_exp2f((last - ref) * a.c2) : 0.0f;
-        float sum = last_x;
-#pragma unroll
-        for (uint32_t c = 0; c < TURNS; ++c) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[c][j] = __builtin_amdgcn_exp2f((x[c][j] - ref) * a.c2);
-                sum += x[c][j];
-            }
-        }
-        s[0] = {own, sum};
-        if (SUMS && a.rest != 0u) {
-            for (uint32_t j = tid; j < a.k; j += NT_DISTILL) {
-                if (list.ids[j] != LILY_NO_TOKEN) {
-                    const float v = list.z[j];
-                    s[1] = joined(s[1], {v, term(v, v, a.c2)}, a.c2);
-                }
-            }
-        }
+        exponentials(a, part, list, SUMS, x, last_x, own, s);
         if constexpr (SUMS) {
-            group_sums<DISTILL_WAVES>(s, a.c2, part);
+            group_sums<DISTILL_WAVES>(s, a.c2, sums);
         }
     }
-
-    uint64_t* out = a.words + (uint64_t)in_launch * a.slices * 2u;
+    const uint64_t word = !SUMS ? 0ull : tid == 2u ? word_of(together<DISTILL_WAVES>(products)) : word_of(tid == 0u ? s[0] : s[1]);
     RowSums r;
     if constexpr (FORM == FORM_SUM) {
-        if (tid < 2u) {
-            out[slice * 2u + tid] = word_of(tid == 0u ? s[0] : s[1]);
+        if (tid < WORDS) {
+            out[slice * WORDS + tid] = word;
         }
         return;
     } else if constexpr (FORM == FORM_BACK) {
         r = of_stats(a, row);
     } else if constexpr (FORM == FORM_AFTER) {
-        r = of_words(a, lane, reinterpret_cast<const uint64_t (*)[2]>(out));
+        r = of_words(a, lane, reinterpret_cast<const uint64_t (*)[WORDS]>(out));
     } else {
-        if (tid < 2u) {
-            store_through(out + slice * 2u + tid, word_of(tid == 0u ? s[0] : s[1]));
+        if (tid < WORDS) {
+            store_through(out + slice * WORDS + tid, word);
+            words[slice][tid] = word;
+        }
+        if constexpr (FORM == FORM_ALONE) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the words have arrived before anything of the gradient has)
+            if (a.grad == nullptr && slice != 0u) {
+                clear_row(a, in_launch, out, leave_row(a, in_launch));
+                return;
+            }
+        }
+        if (finishes) {   // (while the words are on their way)
+            entropy_of<DISTILL_WAVES>(a, id, value, l, lse, entropy);
         }
         if (tid < 64u) {
-            uint64_t seen[2] = {lane == slice ? word_of(s[0]) : 0ull, lane == slice || a.rest == 0u ? word_of(s[1]) : 0ull};
-            bool all = a.slices == 1u;
-            for (uint32_t n = 0; n < a.looks && !all; ++n) {
-                if (lane < a.slices) {
-                    seen[0] = seen[0] == 0ull ? load_through(out + lane * 2u) : seen[0];
-                    seen[1] = seen[1] == 0ull ? load_through(out + lane * 2u + 1u) : seen[1];
+            const bool asks = lane < a.slices && lane != slice;
+            uint64_t seen[3] = {0ull, a.rest == 0u ? word_of(Sum{NEG_INF, 0.0f}) : 0ull, finishes ? 0ull : word_of(0.0)};
+            uint64_t left = __ballot(asks);
+            for (uint32_t n = 0; n < a.looks && left != 0ull; ++n) {
+                if (asks) {
+#pragma unroll
+                    for (uint32_t w = 0; w < WORDS; ++w) {
+                        seen[w] = seen[w] == 0ull ? load_through(out + lane * WORDS + w) : seen[w];
+                    }
                 }
-                all = __ballot(lane < a.slices && (seen[0] == 0ull || seen[1] == 0ull)) == 0ull;
+                left = __ballot(asks && (seen[0] == 0ull || seen[1] == 0ull || seen[2] == 0ull));
             }
-            words[lane][0] = seen[0];
-            words[lane][1] = seen[1];
+            if (asks) {
+#pragma unroll
+                for (uint32_t w = 0; w < WORDS; ++w) {
+                    words[lane][w] = seen[w];
+                }
+            }
+            const RowSums w = of_words(a, lane, words);
             if (lane == 0u) {
-                missing = all ? 0u : 1u;
+                missing = left;
+                hand_over(come, w);
             }
         }
         __syncthreads();
-        if (missing != 0u) {
-            if (tid == 0u) {
-                a.late[1u + atomicAdd(a.late, 1u)] = at;
+        if constexpr (FORM == FORM_HELD) {
+            if (missing != 0ull) {
+                if (tid == 0u) {
+                    a.late[1u + atomicAdd(a.late, 1u)] = at;
+                }
+                return;
             }
+        } else if (missing != 0ull) {
+            words_of_slices<TURNS, BF16>(reinterpret_cast<const DistillArgs*>((const void*)__builtin_amdgcn_kernarg_segment_ptr()), at, missing, &words[0][0]);
+            const RowSums w = of_words(a, lane, words);
+            if (tid == 0u) {
+                hand_over(come, w);
+            }
+            __syncthreads();
+        }
+        r = handed(come);
+    }
+    uint32_t left_before = 0u;
+    if constexpr (FORM == FORM_ALONE) {
+        if (a.grad == nullptr) {
+            if (tid >= NT_DISTILL - 64u) {
+                const double d = products_of_words(a, lane, words);
+                l.entropy = together<DISTILL_WAVES>(entropy);
+                if (lane == 0u) {
+                    finish_row(a, row, r, l, d);
+                }
+            }
+            clear_row(a, in_launch, out, leave_row(a, in_launch));
             return;
         }
-        r = of_words(a, lane, words);
+        left_before = leave_row(a, in_launch);
     }
     const Gradient g = gradient_of(a, r, l);
     const uint32_t dtype = a.grad_bf16 != 0u ? LILY_BF16 : LILY_F32;
@@ -561,7 +784,7 @@ __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at)
             }
         }
     } else {
-        last_x = g.zeros ? 0.0f : g.factor * term(last, g.ref, a.c2);
+        last_x = g.zeros ? 0.0f : g.factor * term(part.last, g.ref, a.c2);
     }
 #pragma unroll
     for (uint32_t c = 0; c < TURNS; ++c) {
@@ -572,14 +795,14 @@ __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at)
                 v[j] = x[c][j];
             }
         } else if (!g.zeros) {
-            raw[c].widened(v);
+            part.raw[c].widened(v);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 v[j] = g.factor * __builtin_amdgcn_exp2f((v[j] - g.ref) * a.c2);
             }
         }
-        if (there(c)) {
-            const uint32_t at = (first + c * NT_DISTILL + tid) * 8u;
+        if (part.there(c)) {
+            const uint32_t at = part.lo + (c * NT_DISTILL + tid) * 8u;
             if (a.grad_bf16 != 0u) {
                 store8(grad, at, v, LILY_BF16);
             } else {
@@ -587,18 +810,26 @@ __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at)
             }
         }
     }
-    if (last_at != LILY_NO_TOKEN) {
-        store1(grad, last_at, last_x, dtype);
+    if (part.last_at != LILY_NO_TOKEN) {
+        store1(grad, part.last_at, last_x, dtype);
     }
-    if (g.zeros) {
-        return;
-    }
-    // The list's ids anew, behind the stores above.
-    __syncthreads();
-    for (uint32_t j = tid; j < a.k; j += NT_DISTILL) {
-        if (list.ids[j] != LILY_NO_TOKEN) {
-            store1(grad, list.ids[j], g.wt * (term(list.z[j], r.all.m, a.c2) * r.inv_all - list.p[j]), dtype);
+    if (!g.zeros) {   // the list's ids anew, behind the stores above
+        __syncthreads();
+        for (uint32_t j = tid; j < a.k; j += NT_DISTILL) {
+            if (list.ids[j] != LILY_NO_TOKEN) {
+                store1(grad, list.ids[j], g.wt * (term(list.z[j], r.all.m, a.c2) * r.inv_all - list.p[j]), dtype);
+            }
         }
+    }
+    if constexpr (FORM == FORM_ALONE) {
+        if (slice == 0u && tid >= NT_DISTILL - 64u) {
+            const double d = products_of_words(a, lane, words);
+            l.entropy = together<DISTILL_WAVES>(entropy);
+            if (lane == 0u) {
+                finish_row(a, row, r, l, d);
+            }
+        }
+        clear_row(a, in_launch, out, left_before);
     }
 }
 
@@ -612,7 +843,13 @@ __global__ void __launch_bounds__(NT_DISTILL, TURNS > 4 ? 4 : 6) k_distill(const
         if (blockIdx.x < finishers) {
             const uint32_t in_launch = blockIdx.x * DISTILL_WAVES + (threadIdx.x >> 6);
             if (in_launch < a.rows) {
-                finish_row(a, in_launch, threadIdx.x & 63u);
+                const uint32_t lane = threadIdx.x & 63u;
+                const auto words = reinterpret_cast<const uint64_t (*)[WORDS]>(a.words) + (uint64_t)in_launch * a.slices;
+                const RowSums r = of_words(a, lane, words);
+                const double d = products_of_words(a, lane, words);
+                if (lane == 0u) {
+                    finish_row(a, a.row0 + in_launch, r, a.listed[in_launch], d);
+                }
             }
             return;
         }
@@ -626,7 +863,9 @@ __global__ void __launch_bounds__(NT_DISTILL, TURNS > 4 ? 4 : 6) k_distill(const
 
 // Turns of a slice: where rows are many, as many as a thread holds exponentials of (two workgroups a compute unit in bf16: 2048 rows of
 // 151 936 in bf16 266 us by eight, 301 by four, 295 by six, 457 by two; in f32, 1024 rows, 253 by four, 263 by eight), and three for the
-// backward pass, which holds nothing (219 against 233 by four and 218 by two; lists of 1000 entries 94, 98 and 100).
+// backward pass, which holds nothing (219 against 233 by four and 218 by two; lists of 1000 entries 94, 98 and 100).  The backward pass adds
+// up the lists itself, in every slice: 300 rows of 248 320 with lists of 1000 89 against 94 with a launch for them, 2048 of 151 936 with
+// lists of 64 221 against 219.
 constexpr uint32_t TURNS_BACK = 3;
 constexpr uint32_t turns_held(bool bf16) { return bf16 ? 8u : 4u; }
 template <int FORM>
@@ -639,14 +878,16 @@ void launch_form(hipStream_t stream, const DistillArgs& a, uint32_t turns, uint3
     if constexpr (FORM == FORM_BACK) {
         LILY_DISTILL(TURNS_BACK, true)
         LILY_DISTILL(TURNS_BACK, false)
+    }
+    if constexpr (FORM == FORM_BACK || FORM == FORM_ALONE) {
+        LILY_DISTILL(1u, true)
+        LILY_DISTILL(1u, false)
+        LILY_DISTILL(2u, true)
+        LILY_DISTILL(2u, false)
     } else {
         LILY_DISTILL(turns_held(true), true)
         LILY_DISTILL(turns_held(false), false)
     }
-    LILY_DISTILL(1u, true)
-    LILY_DISTILL(1u, false)
-    LILY_DISTILL(2u, true)
-    LILY_DISTILL(2u, false)
 #undef LILY_DISTILL
 }
 
@@ -679,27 +920,39 @@ hipError_t launch_distill(hipStream_t stream, const lily_distillation& d, bool b
     a.over_t = 1.0 / (double)d.temperature;
     a.logits_bf16 = d.logits_dtype == LILY_BF16;
     a.grad_scale = d.grad_scale;
-    // Few rows are cut finer, as long as every workgroup has a place on the chip.
+    // Few rows are cut finer, as long as every workgroup has a place on the chip; then one launch does everything.
     auto slices = [&](uint64_t turns) { return (d.vocab + turns * TURN - 1u) / (turns * TURN); };
-    auto fits = [&](uint64_t turns) { return slices(turns) <= WORD_SLICES && slices(turns) * d.rows <= 768u; };
-    const uint32_t turns = fits(1u) ? 1u : fits(2u) ? 2u : backward ? TURNS_BACK : turns_held(a.logits_bf16 != 0u);
-    a.slices = (d.vocab + turns * TURN - 1u) / (turns * TURN);
+    auto fits = [&](uint64_t turns) { return slices(turns) <= WORD_SLICES && slices(turns) * d.rows <= DISTILL_ALONE; };
+    const bool few = fits(2u);
+    const uint32_t turns = fits(1u) ? 1u : few ? 2u : backward ? TURNS_BACK : turns_held(a.logits_bf16 != 0u);
+    a.slices = (uint32_t)slices(turns);
+    if (few || backward) {
+        a.words = ws.exchange;
+        a.done = reinterpret_cast<uint32_t*>(ws.exchange + WORDS * DISTILL_ALONE);
+        const uint64_t most = 0xffffffffull / ((uint64_t)a.slices * NT_DISTILL) - 1u;   // rows of a launch
+        for (uint64_t row = 0; row < d.rows; row += most) {
+            const uint32_t rows = (uint32_t)std::min<uint64_t>(most, d.rows - row);
+            a.row0 = row;
+            if (backward) {
+                launch_form<FORM_BACK>(stream, a, turns, rows * a.slices);
+            } else {
+                launch_form<FORM_ALONE>(stream, a, turns, rows * a.slices);
+            }
+        }
+        return hipGetLastError();
+    }
     const bool held = d.grad_dev != nullptr && a.slices <= WORD_SLICES;
     // As many rows at a time as the workspace holds words, lists' sums and lists of slices of.
-    const uint64_t each = a.slices * 5ull + sizeof(Listed) / 4u;   // floats
+    const uint64_t each = a.slices * (WORDS * 2ull + 1u) + sizeof(Listed) / 4u;   // floats
     const uint64_t most = std::min<uint64_t>((ws.part_floats - 4u) / each, 0xffffffffull / ((uint64_t)a.slices * NT_DISTILL) - 1u);
     for (uint64_t row = 0; row < d.rows; row += most) {
         const uint32_t rows = (uint32_t)std::min<uint64_t>(most, d.rows - row), groups = rows * a.slices;
         a.row0 = row;
         a.rows = rows;
         a.words = reinterpret_cast<uint64_t*>(ws.part);
-        a.listed = reinterpret_cast<Listed*>(ws.part + (uint64_t)groups * 4u);
-        a.late = held && !backward ? reinterpret_cast<uint32_t*>(a.listed + rows) : nullptr;
+        a.listed = reinterpret_cast<Listed*>(ws.part + (uint64_t)groups * (WORDS * 2u));
+        a.late = held ? reinterpret_cast<uint32_t*>(a.listed + rows) : nullptr;
         hipLaunchKernelGGL(k_distill_lists, dim3(rows), dim3(256), 0, stream, a);
-        if (backward) {
-            launch_form<FORM_BACK>(stream, a, turns, groups);
-            continue;
-        }
         if (held) {
             launch_form<FORM_HELD>(stream, a, turns, groups);
         } else {

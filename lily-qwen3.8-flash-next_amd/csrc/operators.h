@@ -23,6 +23,7 @@ struct ProjectWorkspace {
     uint64_t part_floats;
     uint32_t tile = 0;      // 64, 128 or 256: what more than 16 rows get; 0: by an estimate of the time
     uint32_t looks = 4096;  // of a distillation's workgroups for the sums of their row's other slices
+    uint64_t* exchange;     // of a distillation of few rows: those sums, and counters, zeros between two calls
 };
 hipError_t launch_project(hipStream_t stream, const lily_projection& p, const ProjectWorkspace& ws);
 
@@ -36,6 +37,8 @@ hipError_t launch_project_blocks(hipStream_t stream, const lily_block_projection
 
 // Distillation (distill.hip): workgroups of this many threads take slices of a row, of this many ids at most.
 constexpr uint32_t DISTILL_SLICE = 32768, DISTILL_THREADS = 512;
+constexpr uint32_t DISTILL_ALONE = 768;   // workgroups of few rows: three a compute unit
+constexpr uint64_t DISTILL_EXCHANGE = DISTILL_ALONE * 28ull;   // bytes: three words and a counter each
 hipError_t launch_distill(hipStream_t stream, const lily_distillation& d, bool backward, const ProjectWorkspace& ws);
 
 }  // namespace lily

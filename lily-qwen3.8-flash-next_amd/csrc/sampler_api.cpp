@@ -84,6 +84,7 @@ struct lily_sampler {
     uint64_t* ws_cand = nullptr;
     double* ws_lse = nullptr;
     uint32_t* ws_ticket = nullptr;
+    uint64_t* ws_exchange = nullptr;  // of a distillation of few rows
     uint64_t* chain_cand = nullptr;   // [LILY_MAX_VERIFY_ROWS][CHAIN_CAP], then the rows' counts and
     uint32_t* chain_n = nullptr;      // the ticket of a chained launch
     uint32_t* chain_ticket = nullptr;
@@ -1045,6 +1046,7 @@ void sampler_project_workspace(const lily_sampler_t* s, ProjectWorkspace* ws) {
     ws->part_floats = (uint64_t)s->ws_slots * 2u;
     ws->tile = s->project_tile;
     ws->looks = s->distill_looks;
+    ws->exchange = s->ws_exchange;
 }
 
 int sample_row_with_workspace(int device, hipStream_t stream, const Workspace& ws, const float* logits,
@@ -1218,6 +1220,8 @@ int lily_sampler_create(int device, void* hip_stream, lily_sampler_t** out) {
     if (err == hipSuccess) err = hipMalloc(reinterpret_cast<void**>(&s->ws_lse), slots * 16);
     if (err == hipSuccess) err = hipMalloc(reinterpret_cast<void**>(&s->ws_ticket), WS_ROWS * 4);
     if (err == hipSuccess) err = hipMemset(s->ws_ticket, 0, WS_ROWS * 4);
+    if (err == hipSuccess) err = hipMalloc(reinterpret_cast<void**>(&s->ws_exchange), DISTILL_EXCHANGE);
+    if (err == hipSuccess) err = hipMemset(s->ws_exchange, 0, DISTILL_EXCHANGE);
     if (err == hipSuccess) err = hipMalloc(reinterpret_cast<void**>(&s->wide_max), (size_t)WIDE_FLOATS * 4);
     if (err == hipSuccess) err = hipMalloc(reinterpret_cast<void**>(&s->wide_count), WS_ROWS * 4);
     if (err == hipSuccess) err = hipMemset(s->wide_count, 0, WS_ROWS * 4);
@@ -1254,6 +1258,7 @@ void lily_sampler_destroy(lily_sampler_t* s) {
     (void)hipFree(s->ws_cand);
     (void)hipFree(s->ws_lse);
     (void)hipFree(s->ws_ticket);
+    (void)hipFree(s->ws_exchange);
     (void)hipFree(s->wide_max);
     (void)hipFree(s->wide_count);
     (void)hipFree(s->wide_bounds);

@@ -3,7 +3,8 @@
 Bars (u = 2^-24), a = (z - z0) / T a value's distance from its row's largest, q = softmax:
   * an exponential: its argument's difference and product with log2(e) / T round three times (3 u |a|), the exponential 2 u;
     values meet their row's reference in two steps whose distances add up to |a|;
-  * a sum of them: sum q (3 |a| + 6) u, and up to 32 + 8 + 16 + 31 additions: (3 E + 100) u relative, E = sum q |a|;
+  * a sum of them: sum q (3 |a| + 6) u, and up to 65 additions in a thread, 8 in its wave, 8 of waves and 8 of slices: (3 E + 100) u
+    relative, E = sum q |a|;
     a stored logarithm rounds u |log sum| more, and what is formed of it so much again: (3 E + 140) u in all, call it s;
   * q: (3 |a| + 8) u + s relative; r, the same outside the list; a probability of the list: (3 |t - t0| / T + 140) u + its own
     sum's (3 E_t + 140) u, or from the teacher's sum one exponential of an argument in 64 bits, 4 u (a probability given as such: 130 u with
@@ -454,3 +455,26 @@ def test_slices_whose_neighbours_are_not_seen(monkeypatch, looks, teacher, rest)
         assert torch.equal(loss, c.loss) and torch.equal(stats, c.stats) and torch.equal(grad, c.grad)
     s.close()
     usual.close()
+
+
+@pytest.mark.parametrize("looks", [0, 2, 4096])
+@pytest.mark.parametrize("x", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [2, 30])
+def test_in_place_whether_neighbours_are_seen_or_not(monkeypatch, looks, x, rows):
+    """A workgroup that adds up a neighbour's slice itself takes no gradient for a logit; what a call leaves is what the next one finds."""
+    monkeypatch.setenv("LILY_SAMPLER_DISTILL_LOOKS", str(looks))
+    s = LS.Sampler(0)
+    c = Case(rows, 100003, 40, x, "f32", x, "logits", True, 1.0, weights=True)
+    kept = c.logits.clone()
+    check(s, c)
+    first = c.grad.clone(), c.loss.clone()
+    for _ in range(20):
+        z, loss = kept.clone(), torch.empty_like(c.loss)
+        torch.cuda.synchronize()
+        s.distill(z, c.ids, c.values, loss, grad=z, **c.lists(), **c.grads())
+        torch.cuda.synchronize()
+        assert torch.equal(z, first[0]) and torch.equal(loss, first[1])
+        s.distill(kept, c.ids, c.values, loss, **c.lists())      # the loss alone, the same way
+        torch.cuda.synchronize()
+        assert torch.equal(loss, first[1])
+    s.close()
