@@ -51,7 +51,8 @@ struct Listed {
     float left;        // P
     float weight;      // of the row's gradient
     uint32_t live;     // some entry counts, and has a probability
-    double entropy;    // sum_j p_j log p_j
+    double mass;       // what its entries' masses m_j come to, in 64 bits
+    double entropy;    // sum_j m_j log m_j
 };
 
 struct DistillArgs {
@@ -64,7 +65,7 @@ struct DistillArgs {
     float* loss;
     float* stats;
     void* grad;
-    // [rows][slices][WORDS]: of a slice, (largest value << 32 | sum) outside the list, and in it, and the sum of p_j z_j of the entries
+    // [rows][slices][WORDS]: of a slice, (largest value << 32 | sum) outside the list, and in it, and the sum of m_j z_j of the entries
     // that lie in it, in 64 bits (-0.0 for zero); 0 = not there
     uint64_t* words;
     Listed* listed;     // [rows]
@@ -134,9 +135,6 @@ __device__ __forceinline__ float exp_of(double x) {
 __device__ __forceinline__ float entry_mass(const DistillArgs& a, float t, float top, float lse) {
     return a.probs != 0u ? t : a.rest != 0u ? exp_of((double)t * a.over_t - (double)lse) : term(t, top, a.c2);
 }
-__device__ __forceinline__ float entry_probability(const DistillArgs& a, float t, const Listed& l, float lse) {
-    return entry_mass(a, t, l.top, lse) * (a.rest != 0u ? 1.0f : 1.0f / l.sum);
-}
 
 __device__ __forceinline__ double wave_sum_of(double d) {
     for (int off = 32; off > 0; off >>= 1) {
@@ -180,33 +178,37 @@ __device__ __forceinline__ Listed add_up(const DistillArgs& a, uint64_t row, con
     l.live = (a.rest != 0u ? l.top == 0.0f : l.sum > 0.0f || l.sum != l.sum) ? 1u : 0u;
     return l;
 }
-// Of its entropy, a wave's part in part[wave] (in 64 bits: a loss near zero is a difference of large logarithms).
+// Its mass and entropy, a wave's parts in part[0][wave] and part[1][wave].  In 64 bits: a loss near zero is a difference of large logarithms,
+// and a mass that is off by a rounding is off by that much of the row's largest logit.
 template <uint32_t WAVES, uint32_t E>
-__device__ __forceinline__ void entropy_of(const DistillArgs& a, const uint32_t (&id)[E], const float (&t)[E], const Listed& l, float lse, double* part) {
-    double d = 0.0;
+__device__ __forceinline__ void entropy_of(const DistillArgs& a, const uint32_t (&id)[E], const float (&t)[E], const Listed& l, float lse,
+                                           double (*part)[WAVES]) {
+    double mass = 0.0, entropy = 0.0;
     if ((threadIdx.x & ~63u) < a.k) {   // (a wave without entries has nothing to add up)
-        const double log_sum = a.rest != 0u ? 0.0 : log((double)l.sum);
 #pragma unroll
         for (uint32_t e = 0; e < E; ++e) {
             if (id[e] != LILY_NO_TOKEN) {
-                const float p = entry_probability(a, t[e], l, lse);
-                const double log_p = a.probs != 0u  ? log((double)t[e]) - log_sum
+                const double m = (double)entry_mass(a, t[e], l.top, lse);
+                const double log_m = a.probs != 0u  ? log((double)t[e])
                                      : a.rest != 0u ? (double)t[e] * a.over_t - (double)lse
-                                                    : ((double)t[e] - (double)l.top) * a.over_t - log_sum;
-                d += p == 0.0f ? 0.0 : (double)p * log_p;
+                                                    : ((double)t[e] - (double)reference(l.top)) * a.over_t;
+                mass += m;
+                entropy += m == 0.0 ? 0.0 : m * log_m;
             }
         }
-        d = wave_sum_of(d);
+        mass = wave_sum_of(mass);
+        entropy = wave_sum_of(entropy);
     }
     if ((threadIdx.x & 63u) == 0u) {
-        part[threadIdx.x >> 6] = d;
+        part[0][threadIdx.x >> 6] = mass;
+        part[1][threadIdx.x >> 6] = entropy;
     }
 }
 
 // A row's list added up, its words cleared: a workgroup a row.
 __global__ void __launch_bounds__(256) k_distill_lists(const DistillArgs a) {
     __shared__ float part[4 * 2];
-    __shared__ double part_d[4];
+    __shared__ double part_d[2][4];
     constexpr uint32_t E = LILY_SAMPLE_K_CAP / 256u;
     const uint32_t tid = threadIdx.x, in_launch = blockIdx.x;
     const uint64_t row = a.row0 + in_launch;
@@ -234,7 +236,8 @@ __global__ void __launch_bounds__(256) k_distill_lists(const DistillArgs a) {
     if (a.loss != nullptr) {
         entropy_of<4u>(a, id, t, l, lse, part_d);
         __syncthreads();
-        l.entropy = together<4u>(part_d);
+        l.mass = together<4u>(part_d[0]);
+        l.entropy = together<4u>(part_d[1]);
     }
     if (tid == 0u) {
         a.listed[in_launch] = l;
@@ -317,27 +320,31 @@ __device__ __forceinline__ Gradient gradient_of(const DistillArgs& a, const RowS
 
 // The list as the workgroup sees it.
 struct SliceList {
-    uint32_t ids[LILY_SAMPLE_K_CAP];   // LILY_NO_TOKEN: does not count
+    alignas(16) uint32_t ids[LILY_SAMPLE_K_CAP];   // LILY_NO_TOKEN: does not count, or not in the slice
     float z[LILY_SAMPLE_K_CAP], p[LILY_SAMPLE_K_CAP];   // of what lies in the slice: logit, probability
     uint32_t bits[DISTILL_SLICE / 32u];
     uint32_t twice;                    // an id stands there twice
 };
-// Whether entry j is the first of its id.
-__device__ __forceinline__ bool speaks(const SliceList& l, uint32_t j) {
-    for (uint32_t q = 0; q < j; ++q) {
-        if (l.ids[q] == l.ids[j]) {
-            return false;
+// The first entry of an id, and the probabilities of all of its entries, in their order.
+struct Speaker {
+    uint32_t j;
+    float p;
+};
+__device__ __forceinline__ Speaker speaker_of(const SliceList& l, uint32_t id, uint32_t k) {
+    Speaker s = {LILY_NO_TOKEN, 0.0f};
+#pragma unroll 4
+    for (uint32_t q = 0; q < k; q += 4u) {   // (a match is rare, and nothing else waits for the one before)
+        const uint4 v = *reinterpret_cast<const uint4*>(l.ids + q);
+        if (v.x == id || v.y == id || v.z == id || v.w == id) {
+            for (uint32_t i = q; i < q + 4u; ++i) {
+                if (l.ids[i] == id) {
+                    s.j = min(s.j, i);
+                    s.p += l.p[i];
+                }
+            }
         }
     }
-    return true;
-}
-// The probabilities of entry j's id, from its first entry on.
-__device__ __forceinline__ float added_up(const SliceList& l, uint32_t j, uint32_t k) {
-    float p = l.p[j];
-    for (uint32_t q = j + 1u; q < k; ++q) {
-        p += l.ids[q] == l.ids[j] ? l.p[q] : 0.0f;
-    }
-    return p;
+    return s;
 }
 
 __device__ __forceinline__ uint64_t word_of(Sum s) { return (uint64_t)lilym_f32_bits(s.m) << 32 | lilym_f32_bits(s.s); }
@@ -408,10 +415,16 @@ __device__ __forceinline__ void finish_row(const DistillArgs& a, uint64_t row, c
     if (a.loss != nullptr) {
         // (the sums' part of it: log q = z / T - z0 / T - log(sum); a row of -inf alone has no sum, its logarithm is no number)
         const double log_all = r.log_all != r.log_all ? (double)r.log_all : log((double)r.all.s), top = (double)r.all.m * a.over_t;
-        double d = l.entropy - products * a.over_t + (double)l.sum * (a.rest != 0u ? 1.0 : 1.0 / (double)l.sum) * (top + log_all);
-        if (a.rest != 0u && l.left != 0.0f) {
+        double d = l.entropy - products * a.over_t, left = 0.0;
+        if (a.rest != 0u) {
+            d += l.mass * (top + log_all);
+            left = l.mass < 1.0 || l.mass != l.mass ? 1.0 - l.mass : 0.0;
+        } else {
+            d = d / l.mass - log(l.mass) + (top + log_all);
+        }
+        if (left != 0.0) {
             const double log_q = r.nothing ? -INFINITY : (double)reference(r.out.m) * a.over_t - top + log((double)r.out.s) - log_all;
-            d += (double)l.left * (log((double)l.left) - log_q);
+            d += left * (log(left) - log_q);
         }
         a.loss[row] = l.live != 0u ? (float)(d * (double)a.temperature * (double)a.temperature) + (r.log_all != r.log_all ? r.log_all : 0.0f) : 0.0f;
     }
@@ -450,6 +463,7 @@ __device__ __forceinline__ void enter(const DistillArgs& a, const void* z, const
     for (uint32_t w = tid; w < TURNS * TURN / 32u; w += NT_DISTILL) {
         list.bits[w] = 0u;
     }
+    static_assert(ENTRIES * NT_DISTILL == LILY_SAMPLE_K_CAP, "every entry a place");
     static_assert(TURNS * TURN <= DISTILL_SLICE, "a bit for every id of a slice");
     if (tid == 0u) {
         list.twice = 0u;
@@ -461,9 +475,7 @@ __device__ __forceinline__ void enter(const DistillArgs& a, const void* z, const
         id[e] = j < count && id[e] < a.vocab ? id[e] : LILY_NO_TOKEN;
         here[e] = id[e] >= part.lo && id[e] < part.hi;
         mine[e] = NEG_INF;
-        if (j < a.k) {
-            list.ids[j] = here[e] ? id[e] : LILY_NO_TOKEN;
-        }
+        list.ids[j] = here[e] ? id[e] : LILY_NO_TOKEN;
         if (here[e]) {
             mine[e] = load1(z, id[e], BF16);
             if ((atomicOr(&list.bits[off >> 5], 1u << (off & 31u)) >> (off & 31u) & 1u) != 0u) {
@@ -473,32 +485,34 @@ __device__ __forceinline__ void enter(const DistillArgs& a, const void* z, const
     }
 }
 // Of an id that stands there twice the first entry speaks for all of them.
-__device__ __forceinline__ void make_unique(const DistillArgs& a, SliceList& list, bool probabilities) {
+__device__ __forceinline__ void make_unique(const DistillArgs& a, SliceList& list) {
     if (list.twice == 0u) {
         return;
     }
     __syncthreads();
-    bool first[ENTRIES];
-    float p[ENTRIES];
+    Speaker speaker[ENTRIES];
 #pragma unroll
     for (uint32_t e = 0; e < ENTRIES; ++e) {
-        const uint32_t j = e * NT_DISTILL + threadIdx.x;
-        first[e] = j < a.k && list.ids[j] != LILY_NO_TOKEN && speaks(list, j);
-        p[e] = first[e] && probabilities ? added_up(list, j, a.k) : 0.0f;
+        const uint32_t j = e * NT_DISTILL + threadIdx.x, id = j < a.k ? list.ids[j] : LILY_NO_TOKEN;
+        speaker[e] = {LILY_NO_TOKEN, 0.0f};
+        if (id != LILY_NO_TOKEN) {
+            speaker[e] = speaker_of(list, id, a.k);
+        }
     }
     __syncthreads();
 #pragma unroll
     for (uint32_t e = 0; e < ENTRIES; ++e) {
         const uint32_t j = e * NT_DISTILL + threadIdx.x;
-        if (first[e]) {
-            list.p[j] = p[e];
+        if (speaker[e].j == j) {
+            list.p[j] = speaker[e].p;
         } else if (j < a.k) {
             list.ids[j] = LILY_NO_TOKEN;
         }
     }
 }
-// A slice's entries' logits and probabilities, kept in the thread's own places in LDS, and a wave's part of the sum of their products in
-// part[wave].
+
+// A slice's entries' logits and probabilities, kept in the thread's own places in LDS, and a wave's part of the sum of logits times masses
+// in part[wave].
 __device__ __forceinline__ void keep(const DistillArgs& a, const Listed& l, float lse, SliceList& list, const bool (&here)[ENTRIES],
                                      const float (&z)[ENTRIES], const float (&t)[ENTRIES], double* part) {
     double d = 0.0;
@@ -506,10 +520,10 @@ __device__ __forceinline__ void keep(const DistillArgs& a, const Listed& l, floa
 #pragma unroll
         for (uint32_t e = 0; e < ENTRIES; ++e) {
             if (here[e]) {
-                const float p = entry_probability(a, t[e], l, lse);
+                const float m = entry_mass(a, t[e], l.top, lse);
                 list.z[e * NT_DISTILL + threadIdx.x] = z[e];
-                list.p[e * NT_DISTILL + threadIdx.x] = p;
-                d += p == 0.0f ? 0.0 : (double)p * (double)z[e];
+                list.p[e * NT_DISTILL + threadIdx.x] = m * (a.rest != 0u ? 1.0f : 1.0f / l.sum);
+                d += m == 0.0f ? 0.0 : (double)m * (double)z[e];
             }
         }
         if (a.loss != nullptr) {
@@ -600,7 +614,7 @@ __device__ __attribute__((noinline)) void words_of_slices(const DistillArgs* of,
         const Listed l = add_up<DISTILL_WAVES>(a, row, id, value, lse, sums);
         __syncthreads();
         keep(a, l, lse, list, here, mine, value, products);
-        make_unique(a, list, false);
+        make_unique(a, list);
         Sum s[2];
         float x[TURNS][8], last_x, own;
         exponentials(a, part, list, true, x, last_x, own, s);
@@ -620,7 +634,7 @@ template <uint32_t TURNS, bool BF16, int FORM>
 __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at) {
     __shared__ SliceList list;
     __shared__ float sums[DISTILL_WAVES * 4];
-    __shared__ double entropy[FORM == FORM_ALONE ? DISTILL_WAVES : 1];
+    __shared__ double entropy[2][DISTILL_WAVES];   // (FORM_ALONE)
     __shared__ uint64_t words[WORD_SLICES][WORDS];
     __shared__ double products[DISTILL_WAVES];
     __shared__ uint64_t missing;
@@ -665,7 +679,7 @@ __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at)
     __syncthreads();
     // (from here on a thread's entries are its own places in LDS: the slice needs the registers)
     keep(a, l, lse, list, here, mine, value, products);
-    make_unique(a, list, FORM != FORM_SUM);
+    make_unique(a, list);
 
     Sum s[2];   // the slice's, in every thread; its exponentials stay for the gradient
     float x[TURNS][8], last_x = 0.0f, own = NEG_INF;
@@ -749,7 +763,8 @@ __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at)
         if (a.grad == nullptr) {
             if (tid >= NT_DISTILL - 64u) {
                 const double d = products_of_words(a, lane, words);
-                l.entropy = together<DISTILL_WAVES>(entropy);
+                l.mass = together<DISTILL_WAVES>(entropy[0]);
+                l.entropy = together<DISTILL_WAVES>(entropy[1]);
                 if (lane == 0u) {
                     finish_row(a, row, r, l, d);
                 }
@@ -824,7 +839,8 @@ __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at)
     if constexpr (FORM == FORM_ALONE) {
         if (slice == 0u && tid >= NT_DISTILL - 64u) {
             const double d = products_of_words(a, lane, words);
-            l.entropy = together<DISTILL_WAVES>(entropy);
+            l.mass = together<DISTILL_WAVES>(entropy[0]);
+                l.entropy = together<DISTILL_WAVES>(entropy[1]);
             if (lane == 0u) {
                 finish_row(a, row, r, l, d);
             }

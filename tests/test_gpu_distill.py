@@ -478,3 +478,16 @@ def test_in_place_whether_neighbours_are_seen_or_not(monkeypatch, looks, x, rows
         torch.cuda.synchronize()
         assert torch.equal(loss, first[1])
     s.close()
+
+
+@pytest.mark.parametrize("rows", [3, 700])
+@pytest.mark.parametrize("teacher, rest", KINDS)
+def test_lists_of_one_id_and_of_pairs(sampler, rows, teacher, rest):
+    """The first entry of an id speaks for all of them: lists that name one id throughout, and every id twice, apart and side by side."""
+    c = Case(rows, 30011, 1000, "bf16", "f32", "f32", teacher, rest, 1.0, weights=True)
+    c.ids[0] = 17
+    c.ids[1, 500:] = c.ids[1, :500]
+    c.ids[2, 1::2] = c.ids[2, ::2]
+    if teacher == "probs":
+        c.values.mul_(0.9 / c.values.sum(1, keepdim=True))
+    check(sampler, c)
