@@ -211,24 +211,26 @@ hipError_t launch_large(hipStream_t stream, const ProjectArgs& a) {
 // What the estimate of the plan (project_plan.h) goes by, from what the kernels take here (rows x n x d, three sets of operands in turn,
 // the estimate in brackets):
 //   few rows     the widened products, not the loads, bound it: 32 x 4096 x 4096 8.6 (7.7), 64 rows 10.6 to 12.6 (11.0), but
-//                32 x 151 936 x 4096 202 (189) where 64 x 64 takes 123 (114)
-//   64 x 64      256 x 4096 x 4096 14.6 (16.2) against 19.6 by 128 x 128, 100 x 10 007 x 4096 17.2 (19.4) against 17.8, 512 x 4096 x 4096
-//                18.7 (19.4) against 21.9
-//   128 x 128    256 x 12 288 x 4096 24.2 (24.6) against 28.7 by 64 x 64, 1024 x 4096 x 4096 25.1 (25.8) against 33.6 and 52.9 by 256 x 256,
-//                1024 x 12 288 x 4096 57.1 (59.5) against 58.4
-//   256 x 256    8192 x 12 288 x 4096 385 to 392 (390) against 441, 8192 x 8192 x 2048 143 to 150 (145) against 158, 4096 x 4096 x 14 336 208 (211)
-//                against 247; with a residual 8192 x 12 288 x 4096 455 (432) against 487, 4096 x 4096 x 4096 72 (74) against 82
+//                32 x 151 936 x 4096 202 (189) where 64 x 64 takes 123 (118)
+//   64 x 64      256 x 4096 x 4096 14.2 (14.5) against 19.7 by 128 x 128, 100 x 10 007 x 4096 17.2 (20.2) against 17.8, 512 x 4096 x 4096
+//                19.6 (20.2) against 22, 128 x 4096 x 4096 in two parts 13.5 (13.8), in four 16 (15.1)
+//   128 x 128    256 x 12 288 x 4096 24.4 (23.3) against 28.8 by 64 x 64, 1024 x 4096 x 4096 25.6 (26.2) against 34 and 53 by 256 x 256,
+//                1024 x 12 288 x 4096 57.5 (60.6) against 61
+//   256 x 256    8192 x 12 288 x 4096 385 to 396 (390) against 444, 8192 x 8192 x 2048 143 to 150 (145) against 162, 4096 x 4096 x 14 336 210 (211)
+//                against 249; with a residual 8192 x 12 288 x 4096 456 (432) against 490, 4096 x 4096 x 4096 72 (74) against 81
 // An f32 output's widened products: 64 x 64 up to 512 x 4096 x 4096 (28.2, where 128 x 64 takes 30), then 128 x 64, whose waves widen six
-// blocks for eight blocks' products, where 64 x 64 widens eight: 1024 x 4096 x 4096 42.9 against 50.5, 8192 x 12 288 x 4096 895 against 1066.
+// blocks for eight blocks' products, where 64 x 64 widens eight: 1024 x 4096 x 4096 43 against 51, 8192 x 12 288 x 4096 900 against 1066.
 // (128 x 128 by four waves, eight widened for sixteen, has no registers for it and took 1650; 128 x 128 by eight waves 913.)
 ProjectRates block_rates(const ProjectArgs& a) {
     ProjectRates rate;
     rate.few = 40e3;
-    rate.line64_one = a.out_bf16 ? 0.35 : 0.55;
-    rate.line64 = a.out_bf16 ? 0.21 : 0.34;
-    rate.tile64 = 1.0;
-    rate.line128_one = 0.58;
-    rate.line128 = 0.52;
+    rate.start64 = 6.8;
+    rate.line64_one = a.out_bf16 ? 0.23 : 0.45;
+    rate.line64 = a.out_bf16 ? 0.20 : 0.33;
+    rate.tile64 = 0.3;
+    rate.start128 = 9.0;
+    rate.line128_one = a.out_bf16 ? 0.42 : 0.6;
+    rate.line128 = 0.50;
     rate.tile128 = 1.2;
     rate.line256 = 1.8;
     rate.tile256 = 7.0;

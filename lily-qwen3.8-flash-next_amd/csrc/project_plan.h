@@ -86,11 +86,11 @@ struct ProjectPlan {
     uint32_t tile = 0;     // 0: few rows
     uint32_t splits = 1;
 };
-// What the estimate goes by, us: a round of tiles and a line of d, and a round's epilogue.
+// What the estimate goes by, us: what a launch takes before and behind its lines, a line of d for a round of tiles, a round's epilogue.
 struct ProjectRates {
     double few = 85e3;                                      // bytes a compute unit takes in
-    double line64_one = 0.22, line64 = 0.21, tile64 = 0.0;  // (`one`: the least that a line takes)
-    double line128_one = 0.38, line128 = 0.48, tile128 = 0.0;
+    double start64 = 4.0, line64_one = 0.22, line64 = 0.21, tile64 = 0.0;   // (`one`: the least that a line takes)
+    double start128 = 6.0, line128_one = 0.38, line128 = 0.48, tile128 = 0.0;
     double line256 = 1.45, tile256 = 13.0, tile256_residual = 29.0;
     uint32_t outputs128 = 128;                              // of a tile of 128 rows
     bool large = true;                                      // is there a tile of 256?
@@ -129,9 +129,9 @@ inline ProjectPlan project_plan(const ProjectArgs& a, const ProjectWorkspace& ws
         }
         const double each = lines / (double)k, join = k > 1u ? 1.5 + k * rows * n * 8.0 / 5.5e6 : 0.0;
         const double turns64 = rounds(t64 * k), turns128 = t128 * k <= 256u ? (double)(t128 * k) / 256.0 : rounds(t128 * k);
-        offer(64u, k, std::max(3.0 + memory, 4.0 + each * crossed(turns64 <= 2.0) * std::max(rate.line64_one, rate.line64 * turns64) + rate.tile64 * turns64) +
+        offer(64u, k, std::max(3.0 + memory, rate.start64 + each * crossed(turns64 <= 2.0) * std::max(rate.line64_one, rate.line64 * turns64) + rate.tile64 * turns64) +
                           residual + join);
-        offer(128u, k, std::max(3.0 + memory, 6.0 + each * crossed(turns128 <= 1.0) * std::max(rate.line128_one, rate.line128 * turns128) + rate.tile128 * turns128) +
+        offer(128u, k, std::max(3.0 + memory, rate.start128 + each * crossed(turns128 <= 1.0) * std::max(rate.line128_one, rate.line128 * turns128) + rate.tile128 * turns128) +
                            residual + join);
     }
     if (rate.large) {
