@@ -939,8 +939,14 @@ hipError_t launch_distill(hipStream_t stream, const lily_distillation& d, bool b
     // Few rows are cut finer, as long as every workgroup has a place on the chip; then one launch does everything.
     auto slices = [&](uint64_t turns) { return (d.vocab + turns * TURN - 1u) / (turns * TURN); };
     auto fits = [&](uint64_t turns) { return slices(turns) <= WORD_SLICES && slices(turns) * d.rows <= DISTILL_ALONE; };
-    const bool few = fits(2u);
-    const uint32_t turns = fits(1u) ? 1u : few ? 2u : backward ? TURNS_BACK : turns_held(a.logits_bf16 != 0u);
+    // (what one launch rests on beside whole words is the hardware's: that a workgroup's words have arrived when it counts them so, before its
+    // gradient and before it is counted out)
+#ifdef LILY_STRICT_HANDOVER
+    const bool few = backward && fits(2u);
+#else
+    const bool few = fits(2u) && (backward || !ws.strict);
+#endif
+    const uint32_t turns = few && fits(1u) ? 1u : few ? 2u : backward ? TURNS_BACK : turns_held(a.logits_bf16 != 0u);
     a.slices = (uint32_t)slices(turns);
     if (few || backward) {
         a.words = ws.exchange;

@@ -23,6 +23,7 @@ struct ProjectWorkspace {
     uint64_t part_floats;
     uint32_t tile = 0;      // 64, 128 or 256: what more than 16 rows get; 0: by an estimate of the time
     uint32_t looks = 4096;  // of a distillation's workgroups for the sums of their row's other slices
+    bool strict = false;    // nothing is to rest on the order in which the hardware counts stores
     uint64_t* exchange;     // of a distillation of few rows: those sums, and counters, zeros between two calls
 };
 hipError_t launch_project(hipStream_t stream, const lily_projection& p, const ProjectWorkspace& ws);

@@ -1047,6 +1047,7 @@ void sampler_project_workspace(const lily_sampler_t* s, ProjectWorkspace* ws) {
     ws->tile = s->project_tile;
     ws->looks = s->distill_looks;
     ws->exchange = s->ws_exchange;
+    ws->strict = s->handover == 1u;
 }
 
 int sample_row_with_workspace(int device, hipStream_t stream, const Workspace& ws, const float* logits,

@@ -491,3 +491,22 @@ def test_lists_of_one_id_and_of_pairs(sampler, rows, teacher, rest):
     if teacher == "probs":
         c.values.mul_(0.9 / c.values.sum(1, keepdim=True))
     check(sampler, c)
+
+
+@pytest.mark.parametrize("looks", ["4096", "0"])
+@pytest.mark.parametrize("teacher, rest", KINDS)
+def test_few_rows_by_three_launches(monkeypatch, looks, teacher, rest):
+    """LILY_SAMPLER_HANDOVER=strict: sums that pass between launches, or as whole words."""
+    monkeypatch.setenv("LILY_SAMPLER_HANDOVER", "strict")
+    monkeypatch.setenv("LILY_SAMPLER_DISTILL_LOOKS", looks)
+    s = LS.Sampler(0)
+    for rows, vocab, k, x in ((3, 40003, 30, "f32"), (2, 100000, 1000, "bf16"), (30, 7, 3, "f32")):
+        c = Case(rows, vocab, k, x, "f32", x, teacher, rest, 1.0, weights=True)
+        check(s, c)
+        want = c.grad.clone()
+        z = c.logits.clone()
+        torch.cuda.synchronize()
+        s.distill(z, c.ids, c.values, c.loss, grad=z, **c.lists(), **c.grads())
+        s.synchronize()
+        assert torch.equal(z, want)
+    s.close()
