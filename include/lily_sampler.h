@@ -673,7 +673,7 @@ int lily_layer_norm(lily_sampler_t* s, const lily_layer* layer);
  *     grad_x = past + rstd * (g - sum(g) / d - x * sum(g * x) / d)
  *     grad_weight = sum over the rows of grad * x,   grad_bias = sum over the rows of grad
  * `past` is the gradient that reaches h on the residual stream, past the norm.  Sums in f32, those over the rows in
- * an order that rows and d alone decide (the same call gives the same bits); accumulate 1 adds them to what
+ * an order that the call's sizes, types and outputs decide (the same call gives the same bits); accumulate 1 adds them to what
  * grad_weight_dev and grad_bias_dev hold.  A row that holds what is not finite makes its grad_x and the sums so.
  *
  * At least one of grad_x_dev, grad_weight_dev and grad_bias_dev is given.  grad_x_dev may be grad_dev, h_dev or

@@ -16,7 +16,7 @@
 //
 // Of more rows a small launch adds up the lists and clears the words.  Whoever misses a word (a neighbour has no place on the chip yet) enters
 // its slice into a list and ends; a last launch, which finds every word, does the slices of that list, and the losses.  Rows of more than 64
-// slices go that way altogether.  2048 rows of 151 936 in bf16 254 us (4.9 TB/s), 1024 in f32 256 (4.8).
+// slices go that way altogether.  2048 rows of 151 936 in bf16 254 us (4.9 TB/s), 1024 in f32 258 (4.8).
 //
 // The gradient is written as an id outside the list has it, everywhere, and then anew for the list's ids, by the thread that
 // holds the entry: of an id that the list names twice the first one, found by a bitmap of the slice.  Nothing is added by atomics: the
@@ -323,30 +323,10 @@ struct SliceList {
     alignas(16) uint32_t ids[LILY_SAMPLE_K_CAP];   // LILY_NO_TOKEN: does not count, or not in the slice
     float z[LILY_SAMPLE_K_CAP], p[LILY_SAMPLE_K_CAP];   // of what lies in the slice: logit, probability
     uint32_t bits[DISTILL_SLICE / 32u];
-    uint32_t twice;                    // an id stands there twice
+    uint32_t twice;                    // entries whose id another one had marked before
+    uint16_t which[LILY_SAMPLE_K_CAP];
+    uint32_t marked[LILY_SAMPLE_K_CAP / 32u], silent[LILY_SAMPLE_K_CAP / 32u];   // a bit for each of these; for each that another one speaks for
 };
-// The first entry of an id, and the probabilities of all of its entries, in their order.
-struct Speaker {
-    uint32_t j;
-    float p;
-};
-__device__ __forceinline__ Speaker speaker_of(const SliceList& l, uint32_t id, uint32_t k) {
-    Speaker s = {LILY_NO_TOKEN, 0.0f};
-#pragma unroll 4
-    for (uint32_t q = 0; q < k; q += 4u) {   // (a match is rare, and nothing else waits for the one before)
-        const uint4 v = *reinterpret_cast<const uint4*>(l.ids + q);
-        if (v.x == id || v.y == id || v.z == id || v.w == id) {
-            for (uint32_t i = q; i < q + 4u; ++i) {
-                if (l.ids[i] == id) {
-                    s.j = min(s.j, i);
-                    s.p += l.p[i];
-                }
-            }
-        }
-    }
-    return s;
-}
-
 __device__ __forceinline__ uint64_t word_of(Sum s) { return (uint64_t)lilym_f32_bits(s.m) << 32 | lilym_f32_bits(s.s); }
 __device__ __forceinline__ Sum sum_of(uint64_t w) { return {lilym_bits_f32((uint32_t)(w >> 32)), lilym_bits_f32((uint32_t)w)}; }
 
@@ -465,6 +445,9 @@ __device__ __forceinline__ void enter(const DistillArgs& a, const void* z, const
     }
     static_assert(ENTRIES * NT_DISTILL == LILY_SAMPLE_K_CAP, "every entry a place");
     static_assert(TURNS * TURN <= DISTILL_SLICE, "a bit for every id of a slice");
+    if (tid < LILY_SAMPLE_K_CAP / 32u) {
+        list.marked[tid] = list.silent[tid] = 0u;
+    }
     if (tid == 0u) {
         list.twice = 0u;
     }
@@ -479,33 +462,63 @@ __device__ __forceinline__ void enter(const DistillArgs& a, const void* z, const
         if (here[e]) {
             mine[e] = load1(z, id[e], BF16);
             if ((atomicOr(&list.bits[off >> 5], 1u << (off & 31u)) >> (off & 31u) & 1u) != 0u) {
-                list.twice = 1u;
+                list.which[atomicAdd(&list.twice, 1u)] = (uint16_t)j;
+                atomicOr(&list.marked[j >> 5], 1u << (j & 31u));
             }
         }
     }
 }
-// Of an id that stands there twice the first entry speaks for all of them.
+__device__ __forceinline__ uint32_t wave_min(uint32_t v) {
+    for (int off = 32; off > 0; off >>= 1) {
+        v = min(v, (uint32_t)__shfl_xor((int)v, off));
+    }
+    return v;
+}
+// Of an id that stands there twice the first entry speaks for all of them, with their probabilities added up in their order.  A wave looks
+// at the whole list for one marked entry at a time; the first marked one of an id (which of them are marked, the atomics decide) does the rest.
 __device__ __forceinline__ void make_unique(const DistillArgs& a, SliceList& list) {
-    if (list.twice == 0u) {
+    const uint32_t n = list.twice;
+    if (n == 0u) {
         return;
     }
     __syncthreads();
-    Speaker speaker[ENTRIES];
-#pragma unroll
-    for (uint32_t e = 0; e < ENTRIES; ++e) {
-        const uint32_t j = e * NT_DISTILL + threadIdx.x, id = j < a.k ? list.ids[j] : LILY_NO_TOKEN;
-        speaker[e] = {LILY_NO_TOKEN, 0.0f};
-        if (id != LILY_NO_TOKEN) {
-            speaker[e] = speaker_of(list, id, a.k);
+    constexpr uint32_t ROUNDS = LILY_SAMPLE_K_CAP / 64u;
+    const uint32_t lane = threadIdx.x & 63u;
+    for (uint32_t d = threadIdx.x >> 6; d < n; d += DISTILL_WAVES) {
+        const uint32_t j = (uint32_t)__builtin_amdgcn_readfirstlane((int)list.which[d]);
+        const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane((int)list.ids[j]);
+        uint32_t first = LILY_NO_TOKEN, first_marked = LILY_NO_TOKEN;
+#pragma unroll 4
+        for (uint32_t i = 0; i < ROUNDS; ++i) {
+            const bool is = list.ids[i * 64u + lane] == id, marked = (list.marked[i * 2u + (lane >> 5)] >> (lane & 31u) & 1u) != 0u;
+            const uint32_t q = i * 64u + lane;
+            first = min(first, is ? q : LILY_NO_TOKEN);
+            first_marked = min(first_marked, is && marked ? q : LILY_NO_TOKEN);
+        }
+        first = wave_min(first);
+        if (wave_min(first_marked) != j) {
+            continue;
+        }
+        float p = 0.0f;
+#pragma clang loop unroll(disable)
+        for (uint32_t i = 0; i < ROUNDS; ++i) {   // (the masks once more: 32 registers that hold them leave the chip a workgroup less)
+            const bool is = list.ids[i * 64u + lane] == id;
+            for (uint64_t left = __ballot(is); left != 0ull; left &= left - 1ull) {
+                p += list.p[i * 64u + (uint32_t)__builtin_ctzll(left)];
+            }
+            if (is && i * 64u + lane != first) {
+                atomicOr(&list.silent[(i * 64u + lane) >> 5], 1u << (lane & 31u));
+            }
+        }
+        if (lane == 0u) {
+            list.p[first] = p;
         }
     }
     __syncthreads();
 #pragma unroll
     for (uint32_t e = 0; e < ENTRIES; ++e) {
         const uint32_t j = e * NT_DISTILL + threadIdx.x;
-        if (speaker[e].j == j) {
-            list.p[j] = speaker[e].p;
-        } else if (j < a.k) {
+        if ((list.silent[j >> 5] >> (j & 31u) & 1u) != 0u) {
             list.ids[j] = LILY_NO_TOKEN;
         }
     }
@@ -849,8 +862,9 @@ __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at)
     }
 }
 
+// (waves of a SIMD: held in f32 four workgroups a compute unit take 258 us where three, of 67 registers, take 268)
 template <uint32_t TURNS, bool BF16, int FORM>
-__global__ void __launch_bounds__(NT_DISTILL, TURNS > 4 ? 4 : 6) k_distill(const DistillArgs a) {
+__global__ void __launch_bounds__(NT_DISTILL, TURNS > 4 ? 4 : FORM == FORM_HELD ? 8 : 6) k_distill(const DistillArgs a) {
     if constexpr (FORM != FORM_AFTER) {
         distill_slice<TURNS, BF16, FORM>(a, blockIdx.x);
     } else {

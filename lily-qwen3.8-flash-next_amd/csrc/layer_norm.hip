@@ -5,6 +5,9 @@
 // One workgroup per row: a thread keeps its part of the row in registers through both sums (the values', then that of the
 // squared distances from their mean, which does not cancel) and the outputs, so a row is read once and written once.  A
 // block of 128 elements with a scale of its own is a row of 16 lanes: its largest value takes no memory and no barrier.
+//
+// Bound by memory: 8192 x 4096, bf16 rows, residual and sum, E4M3 blocks, 52 to 55 us (4.3 to 4.5 TB/s; the RMS norm to E4M3 rows the same on
+// the same chip).  4 rows 4.5 us, a launch, a trip to memory and two sums.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -305,7 +308,10 @@ __global__ void __launch_bounds__(1024) k_layer_grad(const LayerGradArgs a) {
 
 // Both at once, for rows of up to 8192 elements: a workgroup takes `groups` rows at a time, `threads` threads and eight elements a
 // thread each, and keeps what its rows add to the gradients of weight and bias in registers; the next rows (in bf16 the next
-// two) are on their way while a row's two sums go through LDS.
+// two) are on their way while a row's two sums go through LDS.  So grad and h are read once: 16 384 x 4096 in bf16 with `past` 104 us
+// and 4 of joining 256 workgroups' parts (537 MB, 5.0 TB/s) against 161 by the two kernels below, which read them twice; 2049 x 2560 in
+// f32 17 + 4 against 43, of which the memory's are 11: eight rows a workgroup, each a trip to memory, two barriers and its stores.
+// Longer rows, of which a thread would have to keep more, and calls for one of the outputs alone go by those two.
 enum LayerTypes { LAYER_F32, LAYER_BF16, LAYER_MIXED };   // of grad, h, past and grad_x
 template <int TYPES>
 struct LayerPiece : Eight<TYPES == LAYER_BF16> {

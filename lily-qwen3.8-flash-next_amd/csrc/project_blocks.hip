@@ -4,8 +4,12 @@
 //
 // The kernels are the plain product's (project_few.hip, project_tile.h): what they take of a row at a time, 128 bytes, is
 // one block.  Its products are summed on the matrix cores from zero, and the sum joins the tile's by a multiplication
-// with both scales and an addition in f32.  The scales of x arrive in LDS beside the rows they belong to, those of
-// the weights are one a wave and line.
+// with both scales and an addition in f32, behind the next products.  The scales of x arrive in LDS eight blocks at a time (a load for
+// each block of each row took as long as the rows: 8192 x 12 288 x 4096 507 us, 437 so); those of the weights are one a wave and line,
+// 64 lines' in a lane each.
+//
+// 4 x 151 936 x 4096 to f32 100 to 102 us (622 MB, 6.2 TB/s), 100 x 10 007 x 4096 17 us where the memory takes 7.5, 8192 x 12 288 x
+// 4096 at 2.1 PFLOP/s, two thirds of what the matrix cores reach in E4M3.
 #include "project_tile.h"
 
 namespace lily {

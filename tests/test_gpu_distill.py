@@ -510,3 +510,8 @@ def test_few_rows_by_three_launches(monkeypatch, looks, teacher, rest):
         s.synchronize()
         assert torch.equal(z, want)
     s.close()
+
+
+@pytest.mark.parametrize("rows, vocab, x", [(2, 1 << 24, "bf16"), (3, 1100003, "f32"), (1, 2097160, "bf16")])
+def test_vocabularies_of_more_slices_than_a_wave_looks_for(sampler, rows, vocab, x):
+    check(sampler, Case(rows, vocab, 64, x, "f32", x, "logits", True, 1.0, weights=True))
