@@ -804,7 +804,7 @@ typedef struct lily_distillation {
     uint32_t logits_dtype;            /* LILY_F32 or LILY_BF16, as values_dtype and grad_dtype */
     uint32_t values_dtype;
     uint32_t grad_dtype;
-    float temperature;                /* finite, > 0 */
+    float temperature;                /* finite, from 2^-126 on */
     float grad_scale;                 /* finite */
 } lily_distillation;
 int lily_distill(lily_sampler_t* s, const lily_distillation* d);

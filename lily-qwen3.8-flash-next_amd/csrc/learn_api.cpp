@@ -183,8 +183,9 @@ int check_distillation(const lily_distillation* d, bool backward) {
     if ((d->teacher == LILY_TEACHER_LOGITS && d->rest != 0u) != (d->teacher_lse_dev != nullptr)) {
         return api_fail(LILY_ERR_INVALID_ARG, "teacher_lse comes with logits and rest, and only there");
     }
-    if (!(std::isfinite(d->temperature) && d->temperature > 0.0f) || !std::isfinite(d->grad_scale)) {
-        return api_fail(LILY_ERR_INVALID_ARG, "temperature must be finite and > 0, grad_scale finite");
+    // (below 2^-126 log2(e) / T is none of f32's)
+    if (!(std::isfinite(d->temperature) && d->temperature >= 0x1p-126f) || !std::isfinite(d->grad_scale)) {
+        return api_fail(LILY_ERR_INVALID_ARG, "temperature must be finite and at least 2^-126, grad_scale finite");
     }
     if (d->rows > 1u && (d->logits_stride < d->vocab || d->ids_stride < d->k || d->values_stride < d->k ||
                          (d->grad_dev != nullptr && d->grad_stride < d->vocab))) {

@@ -49,6 +49,7 @@ class Case:
     def __init__(self, rows, vocab, k, x="f32", t="f32", out="f32", teacher="logits", rest=False, temperature=1.0, counts=None, pad=0, start=0,
                  weights=False, seed=0, spread=3.0):
         g = torch.Generator(device=dev()).manual_seed(rows * 17 + vocab + k + seed)
+        temperature = float(torch.tensor(temperature, dtype=torch.float32))   # what the call is given: 1e-6 is 2.5e-9 of itself off, of z / T some hundredths
         self.rows, self.vocab, self.k, self.T, self.teacher, self.rest = rows, vocab, k, temperature, teacher, rest
         self.pad, self.start, self.out = pad, start, out
         z = spread * torch.randn(rows, vocab, generator=g, device=dev())
@@ -137,10 +138,11 @@ class Case:
             zr = z.masked_fill(member, -INF)
             some = (~member & (z > -INF)).any(1, keepdim=True)
             r0, rs, r, ar, sr = whole(torch.where(some, zr, torch.zeros_like(zr)))
-            r, Q = torch.where(some, r, 0.0), torch.where(some, torch.exp(r0 + rs - z0 - ls), 0.0)
-            term = torch.where(P > 0, P * (torch.log(P) - torch.log(Q)), 0.0 * P)
+            logQ = torch.where(some, r0 + rs - z0 - ls, -INF)   # (where exp(logQ) is below what 64 bits hold, log of it is not it)
+            r, Q = torch.where(some, r, 0.0), torch.exp(logQ)
+            term = torch.where(P > 0, P * (torch.log(P) - logQ), 0.0 * P)
             loss = loss + term[:, 0]
-            gap = torch.where((P > 0) & some, (torch.log(P) - torch.log(Q)).abs(), 0.0 * P)
+            gap = torch.where((P > 0) & some, (torch.log(P) - logQ).abs(), 0.0 * P)
             loss_tol = loss_tol + (dP * (gap + 1) + P * (s + sr))[:, 0]
             stats[:, 2:] = torch.where(some, torch.cat([raw.masked_fill(member, -INF).amax(1, keepdim=True), rs], 1), torch.tensor([-INF, 0.0], device=dev(), dtype=torch.float64))
             stats_tol[:, 3:] = torch.where(some, sr, 0.0)
@@ -515,3 +517,10 @@ def test_few_rows_by_three_launches(monkeypatch, looks, teacher, rest):
 @pytest.mark.parametrize("rows, vocab, x", [(2, 1 << 24, "bf16"), (3, 1100003, "f32"), (1, 2097160, "bf16")])
 def test_vocabularies_of_more_slices_than_a_wave_looks_for(sampler, rows, vocab, x):
     check(sampler, Case(rows, vocab, 64, x, "f32", x, "logits", True, 1.0, weights=True))
+
+
+@pytest.mark.parametrize("temperature", [2.0 ** -100, 1e-6, 1e6])
+@pytest.mark.parametrize("teacher, rest", KINDS)
+@pytest.mark.parametrize("rows", [3, 900])
+def test_temperatures_that_leave_one_outcome_or_all_alike(sampler, temperature, teacher, rest, rows):
+    check(sampler, Case(rows, 9001, 40, "f32", "f32", "f32", teacher, rest, temperature, weights=True))

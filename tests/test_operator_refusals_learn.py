@@ -124,6 +124,7 @@ FAULTS = [
     ("distill", dict(teacher=2), INVALID, "teacher is"), ("distill", dict(rest=2), INVALID, "rest 0 or 1"), ("distill", dict(rest=1), INVALID, "teacher_lse"),
     ("distill", dict(teacher_lse_dev=0x42000), INVALID, "teacher_lse"), ("distill", dict(rest=1, teacher=1, teacher_lse_dev=0x42000), INVALID, "teacher_lse"),
     ("distill", dict(temperature=0.0), INVALID, "temperature"), ("distill", dict(temperature=-1.0), INVALID, "temperature"), ("distill", dict(temperature=NAN), INVALID, "temperature"),
+    ("distill", dict(temperature=1e-38), INVALID, "temperature"), ("distill", dict(temperature=1e-40), INVALID, "temperature"),
     ("distill", dict(temperature=INF), INVALID, "temperature"), ("distill", dict(grad_scale=INF), INVALID, "grad_scale"), ("distill", dict(logits_stride=99), INVALID, "shorter"),
     ("distill", dict(ids_stride=7), INVALID, "shorter"), ("distill", dict(values_stride=7), INVALID, "shorter"), ("distill", dict(grad_stride=99), INVALID, "shorter"),
     ("distill", dict(ids_dev=0x20002), INVALID, "multiple"), ("distill", dict(stats_dev=0x51002), INVALID, "multiple"), ("distill", dict(logits_stride=1 << 62), RANGE, "address"),
