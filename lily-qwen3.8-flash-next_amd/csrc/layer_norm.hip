@@ -306,11 +306,12 @@ __global__ void __launch_bounds__(1024) k_layer_grad(const LayerGradArgs a) {
     }
 }
 
-// Both at once, for rows of up to 8192 elements: a workgroup takes `groups` rows at a time, `threads` threads and eight elements a
+// Both at once, for rows of 8 to 8192 elements: a workgroup takes `groups` rows at a time, `threads` threads and eight elements a
 // thread each, and keeps what its rows add to the gradients of weight and bias in registers; the next rows (in bf16 the next
 // two) are on their way while a row's two sums go through LDS.  So grad and h are read once: 16 384 x 4096 in bf16 with `past` 104 us
 // and 4 of joining 256 workgroups' parts (537 MB, 5.0 TB/s) against 161 by the two kernels below, which read them twice; 2049 x 2560 in
 // f32 17 + 4 against 43, of which the memory's are 11: eight rows a workgroup, each a trip to memory, two barriers and its stores.
+// Rows of 4001, 8000 of them in bf16 with `past`, 65 us (134 where the piece that a row ends in was read an element at a time).
 // Longer rows, of which a thread would have to keep more, and calls for one of the outputs alone go by those two.
 enum LayerTypes { LAYER_F32, LAYER_BF16, LAYER_MIXED };   // of grad, h, past and grad_x
 template <int TYPES>
@@ -340,31 +341,39 @@ __global__ void __launch_bounds__(1024) k_layer_grad_all(const LayerGradArgs a, 
         float mean, rstd;
     } next[AHEAD];
     // (what lies behind the last whole piece of a row is not asked for; the loads stand outside of every branch)
-    const uint32_t at = a.d >= 8u ? min(i, a.d - 8u) : 0u;
+    const uint32_t at = min(i, a.d - 8u);
     const void* past_or_grad = a.past != nullptr ? a.past : a.grad;
     const uint64_t past_stride = a.past != nullptr ? a.past_stride : a.grad_stride;
     const bool past_bf16 = a.past != nullptr ? x_bf16 : grad_bf16;
     auto ask = [&](Next& n, uint64_t row) {
         const uint64_t r = min(row, (uint64_t)a.rows - 1u);
-        if (!RAGGED || a.d >= 8u) {
-            n.grad.ask(row_at(a.grad, r, a.grad_stride, grad_bf16), at, grad_bf16);
-            n.h.ask(row_at(a.h, r, a.h_stride, h_bf16), at, h_bf16);
-            if (a.past != nullptr) {
-                n.past.ask(row_at(past_or_grad, r, past_stride, past_bf16), at, past_bf16);
-            }
+        n.grad.ask(row_at(a.grad, r, a.grad_stride, grad_bf16), at, grad_bf16);
+        n.h.ask(row_at(a.h, r, a.h_stride, h_bf16), at, h_bf16);
+        if (a.past != nullptr) {
+            n.past.ask(row_at(past_or_grad, r, past_stride, past_bf16), at, past_bf16);
         }
         n.mean = gload(a.mean + r);
         n.rstd = gload(a.rstd + r);
     };
-    // (the piece that a row ends in goes element by element)
-    auto take = [&](const LayerPiece<TYPES>& piece, const void* p, uint64_t row, uint64_t stride, bool bf16, float (&v)[8]) {
-        if (!RAGGED || whole) {
-            piece.take(bf16, v);
-        } else {
-            const char* from_row = row_at(p, min(row, (uint64_t)a.rows - 1u), stride, bf16);
+    // (the piece that a row ends in: of the row's last eight elements, which it has asked for, the last ones)
+    const bool one_on = (a.d & 1u) != 0u, two_on = ((8u - a.d % 8u) & 2u) != 0u, four_on = ((8u - a.d % 8u) & 4u) != 0u;
+    auto take = [&](const LayerPiece<TYPES>& piece, bool bf16, float (&v)[8]) {
+        piece.take(bf16, v);
+        if (RAGGED && !whole) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[j] = i + (uint32_t)j < a.d ? load1(from_row, i + (uint32_t)j, bf16) : 0.0f;
+            for (int j = 0; j < 7; ++j) {
+                const float here = v[j], behind = v[j + 1];
+                v[j] = one_on ? behind : here;
+            }
+#pragma unroll
+            for (int j = 0; j < 6; ++j) {
+                const float here = v[j], behind = v[j + 2];
+                v[j] = two_on ? behind : here;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float here = v[j], behind = v[j + 4];
+                v[j] = four_on ? behind : here;
             }
         }
     };
@@ -384,10 +393,10 @@ __global__ void __launch_bounds__(1024) k_layer_grad_all(const LayerGradArgs a, 
         const bool there = row < a.rows && (RAGGED || whole);   // (a piece behind the row's end is nothing)
         const float mean = n.mean, rstd = n.rstd;
         float g[8], x[8], past[8], sg = 0.0f, sx = 0.0f;
-        take(n.grad, a.grad, row, a.grad_stride, grad_bf16, g);
-        take(n.h, a.h, row, a.h_stride, h_bf16, x);
+        take(n.grad, grad_bf16, g);
+        take(n.h, h_bf16, x);
         if (a.past != nullptr) {
-            take(n.past, a.past, row, a.past_stride, x_bf16, past);
+            take(n.past, x_bf16, past);
         }
         ask(n, row + AHEAD * step);
 #pragma unroll
@@ -615,19 +624,24 @@ hipError_t launch_layer_norm_backward(hipStream_t stream, const lily_layer_grad&
     a.part = ws.part;
     const bool sums = n.grad_weight_dev != nullptr || n.grad_bias_dev != nullptr;
     auto join = [&] { hipLaunchKernelGGL(k_layer_join, dim3((n.d + 31u) / 32u, 2), dim3(256), 0, stream, a); };
-    if (sums && n.grad_x_dev != nullptr && n.d <= 8192u) {
+    if (sums && n.grad_x_dev != nullptr && n.d >= 8u && n.d <= 8192u) {
         const uint32_t threads = norm_shape(n.d).threads, groups = 1024u / threads;
         a.parts = std::min({(n.rows + groups - 1u) / groups, 256u, (uint32_t)(ws.part_floats / (2ull * a.wide))});
         const uint32_t lds = (groups - 1u) * 16u * threads * 4u;
         const bool mixed = a.grad_bf16 != a.h_bf16 || a.grad_bf16 != a.grad_x_bf16;
 #define LILY_LAYER(RAGGED, TYPES) \
     hipLaunchKernelGGL((k_layer_grad_all<RAGGED, TYPES>), dim3(a.parts), dim3(threads * groups), lds, stream, a, threads, groups)
-        if (n.d % 8u != 0u) {
+        const bool ragged = n.d % 8u != 0u;
+        if (mixed && ragged) {
             LILY_LAYER(true, LAYER_MIXED);
         } else if (mixed) {
             LILY_LAYER(false, LAYER_MIXED);
+        } else if (a.grad_bf16 != 0u && ragged) {
+            LILY_LAYER(true, LAYER_BF16);
         } else if (a.grad_bf16 != 0u) {
             LILY_LAYER(false, LAYER_BF16);
+        } else if (ragged) {
+            LILY_LAYER(true, LAYER_F32);
         } else {
             LILY_LAYER(false, LAYER_F32);
         }

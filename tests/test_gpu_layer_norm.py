@@ -248,6 +248,29 @@ def test_backward_against_the_formula(sampler, rows, d, gt, ht, wt, ot, with_pas
     check_grad(alone, want[0], want[1])
 
 
+@pytest.mark.parametrize("d", list(range(8, 25)) + list(range(1025, 1032)))
+@pytest.mark.parametrize("gt, ht, ot", [("bf16", "bf16", "bf16"), ("f32", "f32", "f32"), ("f32", "bf16", "f32"), ("bf16", "f32", "bf16")])
+@pytest.mark.parametrize("pad, start", [(0, 0), (5, 1)])
+def test_backward_where_a_row_ends_in_every_place_of_a_piece(sampler, d, gt, ht, ot, pad, start):
+    """In place of its operands too: the piece that a row ends in is read with elements of the one before."""
+    rng = np.random.default_rng(d + pad)
+    rows = 777
+    grad, h = matrix(rng, rows, d, gt, pad, 1.0, start)[1], matrix(rng, rows, d, ht, pad, 2.0, start, 0.5)[1]
+    past = matrix(rng, rows, d, ot, pad, 1.0, start)[1]
+    mean, rstd = statistics(h)
+    weight = torch.from_numpy(rng.normal(0, 1, d).astype(np.float32)).to(dev())
+    want = backward(grad, h, mean, rstd, weight, past)
+    for place in ("past", "grad") if gt == ot else ("past",):
+        t = dict(grad=grad.clone(), past=past.clone())
+        gx = t[place]
+        gw, gb = torch.empty(d, device=dev()), torch.empty(d, device=dev())
+        torch.cuda.synchronize()
+        sampler.layer_norm_backward(t["grad"], h, mean, rstd, weight, grad_x=gx, grad_weight=gw, grad_bias=gb, past=t["past"])
+        sampler.synchronize()
+        for got, k in ((gx, 0), (gw, 2), (gb, 4)):
+            check_grad(got, want[k], want[k + 1])
+
+
 @pytest.mark.parametrize("rows, d", [(5, 640), (40, 1001), (3, 12000)])
 @pytest.mark.parametrize("where", ["grad", "h", "past"])
 def test_backward_in_place(sampler, rows, d, where):
