@@ -10,16 +10,16 @@
 //
 // Few rows, whose slices all have a place on the chip, are one launch.  Every workgroup adds up its row's list itself.  One that misses a
 // word after a number of looks forms that slice's sums itself, by the same operations.  The words lie in a place of their own that is zeros
-// between two calls: the last of a row's workgroups clears them.  37 rows of 151 936 in f32 18.5 us, 24.5 by the three launches that
+// between two calls: the last of a row's workgroups clears them.  37 rows of 151 936 in f32 18 us, 24.5 by the three launches that
 // more rows take; 8 of them are the memory's, the others trips to it that wait for each other: the list's ids, the logits they name, the
 // words, and the gradient.
 //
 // Of more rows a small launch adds up the lists and clears the words.  Whoever misses a word (a neighbour has no place on the chip yet) enters
 // its slice into a list and ends; a last launch, which finds every word, does the slices of that list, and the losses.  Rows of more than 64
-// slices go that way altogether.  2048 rows of 151 936 in bf16 254 us (4.9 TB/s), 1024 in f32 258 (4.8).
+// slices go that way altogether.  2048 rows of 151 936 in bf16 251 us (5.0 TB/s), 1024 in f32 258 (4.8).
 //
 // The gradient is written as an id outside the list has it, everywhere, and then anew for the list's ids, by the thread that
-// holds the entry: of an id that the list names twice the first one, found by a bitmap of the slice.  Nothing is added by atomics: the
+// holds the entry: of an id that the list names twice (a bitmap of the slice says so) the first one.  Nothing is added by atomics: the
 // same call gives the same bits.
 #include <hip/hip_runtime.h>
 
@@ -131,7 +131,7 @@ __device__ __forceinline__ float exp_of(double x) {
     const double y = x * 1.4426950408889634, n = rint(y);
     return y > -200.0 && y < 200.0 ? ldexpf(__builtin_amdgcn_exp2f((float)(y - n)), (int)n) : y != y ? __builtin_nanf("") : y < 0.0 ? 0.0f : __builtin_huge_valf();
 }
-// Its probability up to the list's mass (logits without `rest`: relative to `top`), and as it is.
+// Its probability, without `rest` times the list's mass (logits then: relative to `top`).
 __device__ __forceinline__ float entry_mass(const DistillArgs& a, float t, float top, float lse) {
     return a.probs != 0u ? t : a.rest != 0u ? exp_of((double)t * a.over_t - (double)lse) : term(t, top, a.c2);
 }
@@ -476,7 +476,7 @@ __device__ __forceinline__ uint32_t wave_min(uint32_t v) {
 }
 // Of an id that stands there twice the first entry speaks for all of them, with their probabilities added up in their order.  A wave looks
 // at the whole list for one marked entry at a time; the first marked one of an id (which of them are marked, the atomics decide) does the rest.
-__device__ __forceinline__ void make_unique(const DistillArgs& a, SliceList& list) {
+__device__ __forceinline__ void make_unique(SliceList& list) {
     const uint32_t n = list.twice;
     if (n == 0u) {
         return;
@@ -627,7 +627,7 @@ __device__ __attribute__((noinline)) void words_of_slices(const DistillArgs* of,
         const Listed l = add_up<DISTILL_WAVES>(a, row, id, value, lse, sums);
         __syncthreads();
         keep(a, l, lse, list, here, mine, value, products);
-        make_unique(a, list);
+        make_unique(list);
         Sum s[2];
         float x[TURNS][8], last_x, own;
         exponentials(a, part, list, true, x, last_x, own, s);
@@ -692,7 +692,7 @@ __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at)
     __syncthreads();
     // (from here on a thread's entries are its own places in LDS: the slice needs the registers)
     keep(a, l, lse, list, here, mine, value, products);
-    make_unique(a, list);
+    make_unique(list);
 
     Sum s[2];   // the slice's, in every thread; its exponentials stay for the gradient
     float x[TURNS][8], last_x = 0.0f, own = NEG_INF;

@@ -12,6 +12,7 @@
 
 #include <algorithm>
 
+#include "launch.h"
 #include "operators.h"
 #include "row_pieces.h"
 
@@ -312,7 +313,7 @@ __global__ void __launch_bounds__(1024) k_layer_grad(const LayerGradArgs a) {
 // and 4 of joining 256 workgroups' parts (537 MB, 5.0 TB/s) against 161 by the two kernels below, which read them twice; 2049 x 2560 in
 // f32 17 + 4 against 43, of which the memory's are 11: eight rows a workgroup, each a trip to memory, two barriers and its stores.
 // Rows of 4001, 8000 of them in bf16 with `past`, 65 us (134 where the piece that a row ends in was read an element at a time).
-// Longer rows, of which a thread would have to keep more, and calls for one of the outputs alone go by those two.
+// Longer rows go by k_layer_grad_long or by those two, calls for one of the outputs alone by those two.
 enum LayerTypes { LAYER_F32, LAYER_BF16, LAYER_MIXED };   // of grad, h, past and grad_x
 template <int TYPES>
 struct LayerPiece : Eight<TYPES == LAYER_BF16> {
@@ -325,6 +326,26 @@ struct LayerPiece<LAYER_MIXED> {
     __device__ __forceinline__ void ask(const void* row, uint32_t i, bool bf16) { raw = load8(row, i, bf16); }
     __device__ __forceinline__ void take(bool bf16, float (&v)[8]) const { widen(raw, bf16, v); }
 };
+// The piece that a row of d elements ends in: of the row's last eight elements, which stand in v, the last ones.
+__device__ __forceinline__ void ends_in(uint32_t d, float (&v)[8]) {
+    const uint32_t shift = 8u - d % 8u;
+    const bool one = (shift & 1u) != 0u, two = (shift & 2u) != 0u, four = (shift & 4u) != 0u;
+#pragma unroll
+    for (int j = 0; j < 7; ++j) {
+        const float here = v[j], behind = v[j + 1];
+        v[j] = one ? behind : here;
+    }
+#pragma unroll
+    for (int j = 0; j < 6; ++j) {
+        const float here = v[j], behind = v[j + 2];
+        v[j] = two ? behind : here;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float here = v[j], behind = v[j + 4];
+        v[j] = four ? behind : here;
+    }
+}
 template <bool RAGGED, int TYPES>
 __global__ void __launch_bounds__(1024) k_layer_grad_all(const LayerGradArgs a, uint32_t threads, uint32_t groups) {
     constexpr uint32_t AHEAD = TYPES == LAYER_BF16 ? 2u : 1u;   // (registers)
@@ -355,26 +376,10 @@ __global__ void __launch_bounds__(1024) k_layer_grad_all(const LayerGradArgs a, 
         n.mean = gload(a.mean + r);
         n.rstd = gload(a.rstd + r);
     };
-    // (the piece that a row ends in: of the row's last eight elements, which it has asked for, the last ones)
-    const bool one_on = (a.d & 1u) != 0u, two_on = ((8u - a.d % 8u) & 2u) != 0u, four_on = ((8u - a.d % 8u) & 4u) != 0u;
     auto take = [&](const LayerPiece<TYPES>& piece, bool bf16, float (&v)[8]) {
         piece.take(bf16, v);
         if (RAGGED && !whole) {
-#pragma unroll
-            for (int j = 0; j < 7; ++j) {
-                const float here = v[j], behind = v[j + 1];
-                v[j] = one_on ? behind : here;
-            }
-#pragma unroll
-            for (int j = 0; j < 6; ++j) {
-                const float here = v[j], behind = v[j + 2];
-                v[j] = two_on ? behind : here;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float here = v[j], behind = v[j + 4];
-                v[j] = four_on ? behind : here;
-            }
+            ends_in(a.d, v);
         }
     };
     const uint64_t step = (uint64_t)gridDim.x * groups;
@@ -482,6 +487,155 @@ __global__ void __launch_bounds__(1024) k_layer_grad_all(const LayerGradArgs a, 
     }
 }
 
+// The same for rows of up to 16 384 elements: a row a workgroup, two pieces a thread, whose sums over the rows lie in LDS, 128 bytes a
+// thread.  `past` is asked for when its row's turn comes.  3068 x 10 336 in bf16 with `past` 81 us against 94.5 by the two kernels below,
+// 3000 x 12 345 115 against 132, 2000 x 16 384 in f32 114 against 145, with `past` 141 against 157.  Rows of f32 that are no multiple of 8 long, and
+// of mixed types, have no registers for it and go by those two: 2000 x 14 835 in f32 192 so, 155 by them; mixed 3451 x 14 835 324 and 227.
+constexpr uint32_t LONG_THREADS = 1024, LONG_PIECES = 2, LONG_LDS = LONG_THREADS * LONG_PIECES * 64;
+template <bool RAGGED, bool BF16>
+__global__ void __launch_bounds__(LONG_THREADS) k_layer_grad_long(const LayerGradArgs a) {
+    __shared__ float part[2][2][16];
+    extern __shared__ f32x4 long_sums[];   // [pieces][weight's, bias's][halves][threads]
+    const uint32_t tid = threadIdx.x, wave = tid >> 6;
+    uint32_t i[LONG_PIECES], at[LONG_PIECES];
+    bool whole[LONG_PIECES];
+#pragma unroll
+    for (uint32_t c = 0; c < LONG_PIECES; ++c) {
+        i[c] = (c * LONG_THREADS + tid) * 8u;
+        whole[c] = i[c] + 8u <= a.d;
+        at[c] = min(i[c], a.d - 8u);
+#pragma unroll
+        for (uint32_t q = 0; q < 4u; ++q) {
+            long_sums[(c * 4u + q) * LONG_THREADS + tid] = f32x4(0.0f);
+        }
+    }
+    Eight<BF16> grad[LONG_PIECES], h[LONG_PIECES];
+    float next_mean, next_rstd;
+    auto ask = [&](uint64_t row) {
+        const uint64_t r = min(row, (uint64_t)a.rows - 1u);
+#pragma unroll
+        for (uint32_t c = 0; c < LONG_PIECES; ++c) {
+            grad[c].load(row_at(a.grad, r, a.grad_stride, BF16), at[c]);
+            h[c].load(row_at(a.h, r, a.h_stride, BF16), at[c]);
+        }
+        next_mean = gload(a.mean + r);
+        next_rstd = gload(a.rstd + r);
+    };
+    auto take = [&](const Eight<BF16>& piece, uint32_t c, float (&v)[8]) {
+        piece.widened(v);
+        if (RAGGED && !whole[c]) {
+            ends_in(a.d, v);
+        }
+    };
+    const float over_d = 1.0f / (float)a.d;
+    ask(blockIdx.x);
+    uint32_t turn = 0u;
+    for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1u) {
+        float g[LONG_PIECES][8], x[LONG_PIECES][8], sg = 0.0f, sx = 0.0f;
+        const float mean = next_mean, rstd = next_rstd;
+        Eight<BF16> past[LONG_PIECES];
+        Raw weight[LONG_PIECES];   // (from the L2)
+#pragma unroll
+        for (uint32_t c = 0; c < LONG_PIECES; ++c) {
+            take(grad[c], c, g[c]);
+            take(h[c], c, x[c]);
+            if (a.weight != nullptr) {
+                weight[c] = load8(a.weight, at[c], a.weight_bf16);
+            }
+        }
+        if (a.past != nullptr) {
+#pragma unroll
+            for (uint32_t c = 0; c < LONG_PIECES; ++c) {
+                past[c].load(row_at(a.past, row, a.past_stride, BF16), at[c]);
+            }
+        }
+        ask(row + gridDim.x);
+#pragma unroll
+        for (uint32_t c = 0; c < LONG_PIECES; ++c) {
+            float w[8] = {};
+            if (a.weight != nullptr) {
+                widen(weight[c], a.weight_bf16, w);
+                if (RAGGED && !whole[c]) {
+                    ends_in(a.d, w);
+                }
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                f32x4& gw = long_sums[(c * 4u + (uint32_t)half) * LONG_THREADS + tid];
+                f32x4& gb = long_sums[(c * 4u + 2u + (uint32_t)half) * LONG_THREADS + tid];
+                f32x4 new_gw = gw, new_gb = gb;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int j = half * 4 + e;
+                    const bool in = RAGGED ? i[c] + (uint32_t)j < a.d : whole[c];   // (a piece behind the row's end is nothing)
+                    g[c][j] = in ? g[c][j] : 0.0f;
+                    x[c][j] = in ? (x[c][j] - mean) * rstd : 0.0f;
+                    new_gb[e] += g[c][j];
+                    new_gw[e] = __builtin_fmaf(g[c][j], x[c][j], new_gw[e]);
+                    g[c][j] *= a.weight != nullptr && in ? w[j] : 1.0f;
+                    sg += g[c][j];
+                    sx = __builtin_fmaf(g[c][j], x[c][j], sx);
+                }
+                gw = new_gw;
+                gb = new_gb;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        sg = wave_sum_f(sg);
+        sx = wave_sum_f(sx);
+        if ((tid & 63u) == 0u) {
+            part[turn][0][wave] = sg;
+            part[turn][1][wave] = sx;
+        }
+        if (RAGGED && a.past != nullptr) {   // (a piece that lies over its neighbour's has to be there before that is stored)
+            __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+        }
+        __syncthreads();
+        sg = sx = 0.0f;
+        for (uint32_t q = 0; q < LONG_THREADS / 64u; ++q) {
+            sg += part[turn][0][q];
+            sx += part[turn][1][q];
+        }
+        sg *= over_d;
+        sx *= over_d;
+        char* out = const_cast<char*>(row_at(a.grad_x, row, a.grad_x_stride, BF16));
+#pragma unroll
+        for (uint32_t c = 0; c < LONG_PIECES; ++c) {
+            float v[8] = {};
+            if (a.past != nullptr) {
+                take(past[c], c, v);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float own = rstd * (g[c][j] - sg - x[c][j] * sx);
+                v[j] = a.past != nullptr ? own + v[j] : own;
+            }
+            if (whole[c]) {
+                store8(out, i[c], v, BF16 ? LILY_BF16 : LILY_F32);
+            } else if (RAGGED) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (i[c] + (uint32_t)j < a.d) {
+                        store1(out, i[c] + (uint32_t)j, v[j], BF16 ? LILY_BF16 : LILY_F32);
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+#pragma unroll
+    for (uint32_t c = 0; c < LONG_PIECES; ++c) {
+        if (i[c] < a.wide) {
+            float* out = a.part + (uint64_t)blockIdx.x * 2u * a.wide + i[c];
+#pragma unroll
+            for (uint32_t half = 0; half < 2u; ++half) {
+                *reinterpret_cast<f32x4*>(out + half * 4u) = long_sums[(c * 4u + half) * LONG_THREADS + tid];
+                *reinterpret_cast<f32x4*>(out + a.wide + half * 4u) = long_sums[(c * 4u + 2u + half) * LONG_THREADS + tid];
+            }
+        }
+    }
+}
+
 // Sums over the rows of a part (blockIdx.y, every a.parts-th row), 64 lanes of eight elements by four rows at a time.
 template <bool RAGGED>
 __global__ void __launch_bounds__(256) k_layer_columns(const LayerGradArgs a) {
@@ -554,6 +708,16 @@ __global__ void __launch_bounds__(256) k_layer_join(const LayerGradArgs a) {
     }
 }
 
+template <bool RAGGED, bool BF16>
+hipError_t launch_long(hipStream_t stream, const LayerGradArgs& a) {
+    static LdsAllowed allowed;
+    if (const hipError_t e = allowed.say((const void*)k_layer_grad_long<RAGGED, BF16>, LONG_LDS); e != hipSuccess) {
+        return e;
+    }
+    hipLaunchKernelGGL((k_layer_grad_long<RAGGED, BF16>), dim3(a.parts), dim3(LONG_THREADS), LONG_LDS, stream, a);
+    return hipGetLastError();
+}
+
 }  // namespace
 
 hipError_t launch_layer_norm(hipStream_t stream, const lily_layer& n) {
@@ -624,14 +788,13 @@ hipError_t launch_layer_norm_backward(hipStream_t stream, const lily_layer_grad&
     a.part = ws.part;
     const bool sums = n.grad_weight_dev != nullptr || n.grad_bias_dev != nullptr;
     auto join = [&] { hipLaunchKernelGGL(k_layer_join, dim3((n.d + 31u) / 32u, 2), dim3(256), 0, stream, a); };
+    const bool mixed = a.grad_bf16 != a.h_bf16 || a.grad_bf16 != a.grad_x_bf16, ragged = n.d % 8u != 0u;
     if (sums && n.grad_x_dev != nullptr && n.d >= 8u && n.d <= 8192u) {
         const uint32_t threads = norm_shape(n.d).threads, groups = 1024u / threads;
         a.parts = std::min({(n.rows + groups - 1u) / groups, 256u, (uint32_t)(ws.part_floats / (2ull * a.wide))});
         const uint32_t lds = (groups - 1u) * 16u * threads * 4u;
-        const bool mixed = a.grad_bf16 != a.h_bf16 || a.grad_bf16 != a.grad_x_bf16;
 #define LILY_LAYER(RAGGED, TYPES) \
     hipLaunchKernelGGL((k_layer_grad_all<RAGGED, TYPES>), dim3(a.parts), dim3(threads * groups), lds, stream, a, threads, groups)
-        const bool ragged = n.d % 8u != 0u;
         if (mixed && ragged) {
             LILY_LAYER(true, LAYER_MIXED);
         } else if (mixed) {
@@ -646,6 +809,17 @@ hipError_t launch_layer_norm_backward(hipStream_t stream, const lily_layer_grad&
             LILY_LAYER(false, LAYER_F32);
         }
 #undef LILY_LAYER
+        join();
+        return hipGetLastError();
+    }
+    if (sums && n.grad_x_dev != nullptr && !mixed && (a.grad_bf16 != 0u || !ragged) && n.d > 8192u && n.d <= LONG_THREADS * LONG_PIECES * 8u) {
+        a.parts = std::min({n.rows, 256u, (uint32_t)(ws.part_floats / (2ull * a.wide))});
+        const hipError_t e = a.grad_bf16 == 0u ? launch_long<false, false>(stream, a)
+                             : ragged          ? launch_long<true, true>(stream, a)
+                                               : launch_long<false, true>(stream, a);
+        if (e != hipSuccess) {
+            return e;
+        }
         join();
         return hipGetLastError();
     }
