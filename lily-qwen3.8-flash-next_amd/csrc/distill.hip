@@ -891,13 +891,14 @@ __global__ void __launch_bounds__(NT_DISTILL, TURNS > 4 ? 4 : FORM == FORM_HELD 
     }
 }
 
-// Turns of a slice: where rows are many, as many as a thread holds exponentials of (two workgroups a compute unit in bf16: 2048 rows of
-// 151 936 in bf16 266 us by eight, 301 by four, 295 by six, 457 by two; in f32, 1024 rows, 253 by four, 263 by eight), and three for the
-// backward pass, which holds nothing (219 against 233 by four and 218 by two; lists of 1000 entries 94, 98 and 100).  The backward pass adds
-// up the lists itself, in every slice: 300 rows of 248 320 with lists of 1000 89 against 94 with a launch for them, 2048 of 151 936 with
-// lists of 64 221 against 219.
-constexpr uint32_t TURNS_BACK = 3;
-constexpr uint32_t turns_held(bool bf16) { return bf16 ? 8u : 4u; }
+// Turns of a slice.  Four fill the chip best, 32 exponentials a thread; from some 700 rows on in bf16 eight (two workgroups a compute unit)
+// have fewer lists to look through and words to wait for: 128 rows of 151 936 31.4 us by four and 33 by eight, 256 51.8 and 55, 512 81 and 82.5, 700
+// 103 both, 1024 141 and 139, 2048 with `rest` 271 and 251; 300 of 248 320 with lists of 1000 128 and 134.  (By six 87 and 151 at 512 and 1024; in f32,
+// 1024 rows, 253 by four and 263 by eight.)  Three for the backward pass, which holds nothing (219 against 233 by four and 218 by two; lists
+// of 1000 entries 94, 98 and 100); it adds up the lists itself, in every slice: 300 rows of 248 320 with lists of 1000 89 against 94 with a launch
+// for them, 2048 of 151 936 with lists of 64 221 against 219.
+constexpr uint32_t TURNS_BACK = 3, TURNS_HELD = 4, TURNS_MANY = 8;
+constexpr uint64_t MANY_GROUPS = 7168;   // by four
 template <int FORM>
 void launch_form(hipStream_t stream, const DistillArgs& a, uint32_t turns, uint32_t groups) {
     const dim3 grid(groups), block(NT_DISTILL);
@@ -915,8 +916,9 @@ void launch_form(hipStream_t stream, const DistillArgs& a, uint32_t turns, uint3
         LILY_DISTILL(2u, true)
         LILY_DISTILL(2u, false)
     } else {
-        LILY_DISTILL(turns_held(true), true)
-        LILY_DISTILL(turns_held(false), false)
+        LILY_DISTILL(TURNS_MANY, true)
+        LILY_DISTILL(TURNS_HELD, true)
+        LILY_DISTILL(TURNS_HELD, false)
     }
 #undef LILY_DISTILL
 }
@@ -960,7 +962,8 @@ hipError_t launch_distill(hipStream_t stream, const lily_distillation& d, bool b
 #else
     const bool few = fits(2u) && (backward || !ws.strict);
 #endif
-    const uint32_t turns = few && fits(1u) ? 1u : few ? 2u : backward ? TURNS_BACK : turns_held(a.logits_bf16 != 0u);
+    const bool many = a.logits_bf16 != 0u && (slices(TURNS_HELD) > WORD_SLICES || slices(TURNS_HELD) * d.rows > MANY_GROUPS);
+    const uint32_t turns = few && fits(1u) ? 1u : few ? 2u : backward ? TURNS_BACK : many ? TURNS_MANY : TURNS_HELD;
     a.slices = (uint32_t)slices(turns);
     if (few || backward) {
         a.words = ws.exchange;

@@ -442,7 +442,7 @@ def test_slices_whose_neighbours_are_not_seen(monkeypatch, looks, teacher, rest)
     """A workgroup that does not find its row's other sums forms them itself: by the same operations, so the bits are the same."""
     monkeypatch.setenv("LILY_SAMPLER_DISTILL_LOOKS", str(looks))
     s, usual = LS.Sampler(0), None
-    for rows, vocab, k, x in ((3, 40003, 30, "f32"), (200, 33001, 60, "bf16"), (2, 100000, 1000, "bf16"), (150, 70001, 5, "f32")):
+    for rows, vocab, k, x in ((3, 40003, 30, "f32"), (200, 33001, 60, "bf16"), (2, 100000, 1000, "bf16"), (150, 70001, 5, "f32"), (2400, 33001, 20, "bf16")):
         c = Case(rows, vocab, k, x, "f32", x, teacher, rest, 1.0, weights=True)
         c.ids[1, 1] = c.ids[1, 0]
         c.logits[0, ::3] = -INF
