@@ -375,3 +375,25 @@ def test_what_the_python_mirror_refuses(sampler):
         kw.update(bad)
         with pytest.raises(LS.SamplerError):
             sampler.layer_norm_backward(**kw)
+
+
+@pytest.mark.parametrize("rows, d", [(1, 140), (3, 8), (3, 2560), (16, 64), (17, 64), (2, 8191), (300, 1001), (5, 10000)])
+@pytest.mark.parametrize("leave", [None, "grad_weight", "grad_bias"])
+def test_all_gradients_added_to_what_is_there(sampler, rows, d, leave):
+    """With one part of the rows and with several; what is not asked for is not touched."""
+    rng = np.random.default_rng(rows * 7 + d)
+    grad, h = matrix(rng, rows, d, "bf16")[1], matrix(rng, rows, d, "bf16", 0, 2.0)[1]
+    mean, rstd = statistics(h)
+    gx = torch.empty(rows, d, dtype=torch.bfloat16, device=dev())
+    sums = dict(grad_weight=torch.full((d,), 3.0, device=dev()), grad_bias=torch.full((d,), -2.0, device=dev()))
+    want = backward(grad, h, mean, rstd, None, None)
+    torch.cuda.synchronize()
+    given = {k: v for k, v in sums.items() if k != leave}
+    sampler.layer_norm_backward(grad, h, mean, rstd, None, grad_x=gx, accumulate=True, **given)
+    sampler.synchronize()
+    check_grad(gx, want[0], want[1])
+    for name, k, start in (("grad_weight", 2, 3.0), ("grad_bias", 4, -2.0)):
+        if name == leave:
+            assert bool((sums[name] == start).all())
+        else:
+            check_grad(sums[name], want[k] + start, want[k + 1] + U * (want[k].abs() + abs(start)))
