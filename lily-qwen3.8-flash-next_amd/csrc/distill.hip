@@ -791,8 +791,9 @@ __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at)
     const uint32_t dtype = a.grad_bf16 != 0u ? LILY_BF16 : LILY_F32;
     void* grad = const_cast<void*>(at_row(a.grad, row, a.grad_stride, a.grad_bf16 != 0u));
     if constexpr (EXPS) {
-        // (an infinite or undefined reference has made the sums, and with them the factor, a NaN)
-        const float factor = g.zeros ? 0.0f : g.factor * __builtin_amdgcn_exp2f((reference(own) - g.ref) * a.c2);
+        // (an infinite or undefined reference has made the sums, and with them the factor, a NaN.  Where there is nothing above -inf the
+        // exponentials are zeros: nothing is to be made of a distance from 0, exp of which may be infinite)
+        const float factor = g.zeros ? 0.0f : g.factor * term(own == NEG_INF ? g.ref : own, g.ref, a.c2);
 #pragma unroll
         for (uint32_t c = 0; c < TURNS; ++c) {
 #pragma unroll
