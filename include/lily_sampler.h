@@ -768,9 +768,9 @@ int lily_project_blocks(lily_sampler_t* s, const lily_block_projection* p);
  *   LILY_TEACHER_PROBS    p_j = t_j with `rest`, t_j over the list's sum without (a value below 0 is 0)
  *     loss = T^2 * (sum_j p_j (log p_j - log q[id_j])  [+ P (log P - log Q)])
  * where, with `rest`, everything outside the list is one outcome more: P = max(0, 1 - sum p_j), Q the sum of q outside the
- * list.  A term whose p is 0 is 0.  Ids that stand in a list twice add their p (and count once in Q).  With w = grad_scale *
- * row_weights[r] (1 where NULL) the gradient of w * loss is
- *     grad_v = w T (q_v sum p - p_v);   with `rest`, for ids outside the list, w T (q_v - P q_v / Q)
+ * list.  A term whose p is 0 is 0.  Ids that stand in a list twice add their terms here and their p below (and count once in Q).  With
+ * w = grad_scale * row_weights[r] (1 where NULL) and S = sum p_j [+ P], which is 1 but with `rest` and a list of more, the gradient of w * loss is
+ *     grad_v = w T (S q_v - p_v);   with `rest`, for ids outside the list, w T (S q_v - P q_v / Q)
  * A row none of whose entries count has loss 0 and a gradient of zeros, and so has the gradient of a row whose w is 0, whatever it holds.
  * Otherwise a NaN or +inf in a student's row, or a row of -inf alone, makes its loss and whole gradient NaN, as a NaN among the values that count does;
  * -inf in some places is a q of 0 (its gradient -w T p, a loss of +inf where p > 0).

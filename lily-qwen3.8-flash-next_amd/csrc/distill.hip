@@ -1,7 +1,7 @@
 // distill.hip - a student's rows of logits against a teacher's top ones: loss, and gradient.
 //
-// With p the teacher's list and q = softmax(z / T):
-//     loss = T^2 (sum_j p_j (log p_j - log q_j) [+ P (log P - log Q)]),  grad_v = w T (q_v sum p - p_v) [outside: w T (q_v - P q_v / Q)]
+// With p the teacher's list, q = softmax(z / T) and S = sum p [+ P], which is 1 but where a list has more than 1 beside the rest:
+//     loss = T^2 (sum_j p_j (log p_j - log q_j) [+ P (log P - log Q)]),  grad_v = w T (S q_v - p_v) [outside: w T (S q_v - P q_v / Q)]
 //
 // A workgroup takes a slice of a row and keeps it in registers, up to 64 values a thread, while the row's slices exchange their sums: a sum
 // is one word (largest value, sum of exponentials), which is the whole message, stored and looked for by relaxed atomics at device scope;
@@ -301,20 +301,23 @@ __device__ __forceinline__ void store_stats(const DistillArgs& a, uint64_t row, 
     to[3] = a.rest != 0u ? r.log_out : 0.0f;
 }
 
-// The gradient of an id outside the list, factor * exp((z - ref) / T), and of one in it, wt * (q - p).
+// The gradient of an id outside the list, factor * exp((z - ref) / T), and of one in it, wt * (inv * exp((z - z0) / T) - p).
 struct Gradient {
     bool zeros;
     float wt, ref, factor;
+    float inv;   // S over the row's sum of exponentials (a list has more than 1 where its rounded logits meet the sum over the exact row)
 };
 __device__ __forceinline__ Gradient gradient_of(const DistillArgs& a, const RowSums& r, const Listed& l) {
     Gradient g;
     g.zeros = l.live == 0u || l.weight == 0.0f;
-    g.wt = l.weight * a.temperature * (l.sum != l.sum ? l.sum : 1.0f);
+    g.wt = l.weight * a.temperature;
+    const float total = l.sum != l.sum || (a.rest != 0u && l.sum > 1.0f) ? l.sum : 1.0f;
+    g.inv = r.inv_all * total;
     g.ref = reference(a.rest != 0u ? r.out.m : r.all.m);
     g.factor = g.zeros        ? 0.0f
-               : a.rest == 0u ? g.wt * r.inv_all
+               : a.rest == 0u ? g.wt * g.inv
                : r.nothing    ? (r.inv_all != r.inv_all ? r.inv_all : 0.0f)
-                              : g.wt * (r.q_out - l.left) * r.inv_out;
+                              : g.wt * (r.q_out * total - l.left) * r.inv_out;
     return g;
 }
 
@@ -846,7 +849,7 @@ __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at)
         __syncthreads();
         for (uint32_t j = tid; j < a.k; j += NT_DISTILL) {
             if (list.ids[j] != LILY_NO_TOKEN) {
-                store1(grad, list.ids[j], g.wt * (term(list.z[j], r.all.m, a.c2) * r.inv_all - list.p[j]), dtype);
+                store1(grad, list.ids[j], g.wt * (term(list.z[j], r.all.m, a.c2) * g.inv - list.p[j]), dtype);
             }
         }
     }
