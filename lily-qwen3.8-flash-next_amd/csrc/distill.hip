@@ -316,7 +316,7 @@ __device__ __forceinline__ Gradient gradient_of(const DistillArgs& a, const RowS
     g.ref = reference(a.rest != 0u ? r.out.m : r.all.m);
     g.factor = g.zeros        ? 0.0f
                : a.rest == 0u ? g.wt * g.inv
-               : r.nothing    ? (r.inv_all != r.inv_all ? r.inv_all : 0.0f)
+               : r.nothing    ? (g.inv != g.inv ? g.inv : 0.0f)   // (a NaN in the row or in its list reaches what is 0, too)
                               : g.wt * (r.q_out * total - l.left) * r.inv_out;
     return g;
 }

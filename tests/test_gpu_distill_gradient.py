@@ -1,5 +1,5 @@
 """The gradient of a distillation, against its formula in 64 bits, where a row's largest logit lies far below zero and much of the row is
-masked, and where a list's probabilities come to more than 1.
+masked, where nothing is left outside the list, and where a list's probabilities come to more than 1.
 
 Bars are those of test_gpu_distill.py: they count distances from the row's largest value, wherever that lies.  With S = sum p + P, 1 unless the
 list has more, the gradient of the loss is
@@ -71,6 +71,24 @@ def test_masked_rows_far_below_zero_by_the_other_ways(monkeypatch, name, value, 
         torch.cuda.synchronize()
         assert torch.equal(z, want)
     s.close()
+
+
+@pytest.mark.parametrize("rows, vocab", [(4, 300), (5, 24581), (300, 40000), (4, 1100003)])
+@pytest.mark.parametrize("teacher, rest", D.KINDS)
+def test_a_value_that_is_no_number_where_nothing_is_left_outside_the_list(sampler, rows, vocab, teacher, rest):
+    """It makes the row's loss and whole gradient a NaN there too, and no other row's."""
+    c = D.Case(rows, vocab, 12, "f32", "f32", "f32", teacher, rest, 1.0)
+    c.logits[:2].masked_fill_(~members(c)[:2], -INF)
+    c.values[0, 3] = float("nan")
+    c.outputs()
+    again = torch.empty_like(c.grad)
+    torch.cuda.synchronize()
+    sampler.distill(c.logits, c.ids, c.values, c.loss, stats=c.stats, grad=c.grad, **c.lists(), **c.grads())
+    sampler.distill_backward(c.logits, c.ids, c.values, stats=c.stats, grad=again, **c.lists(), **c.grads())
+    sampler.synchronize()
+    assert bool(torch.isnan(c.loss[0])) and bool(torch.isfinite(c.loss[2:]).all())
+    for grad in (c.grad, again):
+        assert bool(torch.isnan(grad[0]).all()) and bool(torch.isfinite(grad[1:]).all())
 
 
 class Heavy(D.Case):
