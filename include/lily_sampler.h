@@ -711,8 +711,8 @@ int lily_layer_norm_backward(lily_sampler_t* s, const lily_layer_grad* grad);
  * q = E4M3(x / scale), in f32; the last blocks of a row and of the rows may be smaller.  A block whose largest |x| lies
  * below 2^-116 has scale 0 and zeros; where one holds a NaN the scale and every q are NaN, and an infinity as its largest value
  * gives an infinite scale, NaN for the infinities and zeros for the rest.  Any strides from a row's length on; out may not overlap x.
- * Up to 2^28 - 1 blocks of LILY_BLOCK elements of a row (block_rows 1), 2^24 - 1 of LILY_BLOCK x LILY_BLOCK (LILY_ERR_RANGE
- * beyond).  Enqueued on the sampler's stream, one launch, no workspace. */
+ * Rows of up to 2^32 - 128 elements, up to 2^28 - 1 blocks of LILY_BLOCK elements of a row (block_rows 1), 2^24 - 1 of LILY_BLOCK x
+ * LILY_BLOCK (LILY_ERR_RANGE beyond).  Enqueued on the sampler's stream, one launch, no workspace. */
 typedef struct lily_blocks {
     uint32_t rows;
     uint32_t d;

@@ -27,6 +27,10 @@ int check_blocks(const lily_blocks* q) {
     if (q->block_rows != 1u && q->block_rows != LILY_BLOCK) {
         return api_fail(LILY_ERR_INVALID_ARG, "block_rows is 1 or LILY_BLOCK");
     }
+    // (what the kernels add to an element's place stays below 2^32)
+    if (q->d > 0xffffff80u) {
+        return api_fail(LILY_ERR_RANGE, "a call takes rows of up to 2^32 - 128 elements");
+    }
     const uint64_t down = q->block_rows == 1u ? q->rows : blocks_of(q->rows), across = blocks_of(q->d);
     // (16 threads a block of a row, 256 a block of rows)
     if (down * across > MAX_THREADS / (q->block_rows == 1u ? 16u : 256u)) {

@@ -156,3 +156,12 @@ def test_the_most_blocks(rows, d, block_rows, sound):
     far = 1 << 48
     rc, text = _call(*ENTRIES["blocks"], dict(rows=rows, d=d, block_rows=block_rows, x_dev=far, out_dev=2 * far, scales_dev=3 * far, x_stride=d, out_stride=d))
     assert (rc, text) == (INVALID, "sampler is null") if sound else rc == RANGE and "up to" in text, (rc, text)
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("d, sound", [(0xffffff80, True), (0xffffff81, False), (0xffffff82, False), (0xffffffff, False)])
+def test_the_longest_rows_of_blocks(d, sound, block_rows):
+    """Blocks of a row are counted, and its pieces of eight looked at, in 32 bits.  (2^25 blocks of rows are more than a call takes.)"""
+    far = 1 << 48
+    rc, text = _call(*ENTRIES["blocks"], dict(rows=1, d=d, block_rows=block_rows, x_dev=far, out_dev=2 * far, scales_dev=3 * far))
+    assert (rc, text) == (INVALID, "sampler is null") if sound and block_rows == 1 else rc == RANGE and "up to" in text, (rc, text)
