@@ -361,17 +361,14 @@ __global__ void __launch_bounds__(1024) k_layer_grad_all(const LayerGradArgs a, 
         LayerPiece<TYPES> grad, h, past;
         float mean, rstd;
     } next[AHEAD];
-    // (what lies behind the last whole piece of a row is not asked for; the loads stand outside of every branch)
+    // (what lies behind the last whole piece of a row is not asked for; the loads of grad and h stand outside of every branch)
     const uint32_t at = min(i, a.d - 8u);
-    const void* past_or_grad = a.past != nullptr ? a.past : a.grad;
-    const uint64_t past_stride = a.past != nullptr ? a.past_stride : a.grad_stride;
-    const bool past_bf16 = a.past != nullptr ? x_bf16 : grad_bf16;
     auto ask = [&](Next& n, uint64_t row) {
         const uint64_t r = min(row, (uint64_t)a.rows - 1u);
         n.grad.ask(row_at(a.grad, r, a.grad_stride, grad_bf16), at, grad_bf16);
         n.h.ask(row_at(a.h, r, a.h_stride, h_bf16), at, h_bf16);
         if (a.past != nullptr) {
-            n.past.ask(row_at(past_or_grad, r, past_stride, past_bf16), at, past_bf16);
+            n.past.ask(row_at(a.past, r, a.past_stride, x_bf16), at, x_bf16);
         }
         n.mean = gload(a.mean + r);
         n.rstd = gload(a.rstd + r);
