@@ -636,7 +636,7 @@ int lily_plan_process_logits(lily_plan_t* p, const lily_logits_out* out);
  * in f32.  h goes to sum_dev, mean and rstd (what the backward pass reads) to theirs, where they are given; y
  * to out_dev: f32, bf16 (nearest even) or E4M3 with one f32 scale a row (scale_block 0) or one for each
  * LILY_BLOCK elements of a row (scale_block LILY_BLOCK: what lily_project_blocks takes): scale = max|y| / 448,
- * q = E4M3(y / scale).  A row or block whose largest |y| lies below 2^-116 has scale 0 and zeros; one that holds a
+ * q = E4M3(y / scale), the quotient as y times 448 / max|y|, within 1.5 ulp of it.  A row or block whose largest |y| lies below 2^-116 has scale 0 and zeros; one that holds a
  * value that is not finite has a scale that is not, too.  What is not finite in h makes its whole row a NaN.
  *
  * Rows hold d (1 .. LILY_NORM_MAX_D) elements, strides count elements and may be anything from d on.  What may
@@ -708,7 +708,7 @@ int lily_layer_norm_backward(lily_sampler_t* s, const lily_layer_grad* grad);
  *
  * lily_quantize_blocks writes a matrix as E4M3 with a scale for each LILY_BLOCK elements of a row (block_rows 1:
  * activations) or each LILY_BLOCK rows x LILY_BLOCK elements (block_rows LILY_BLOCK: weights): scale = max|x| / 448,
- * q = E4M3(x / scale), in f32; the last blocks of a row and of the rows may be smaller.  A block whose largest |x| lies
+ * q = E4M3(x / scale), in f32 (the quotient as x times 448 / max|x|, within 1.5 ulp of it); the last blocks of a row and of the rows may be smaller.  A block whose largest |x| lies
  * below 2^-116 has scale 0 and zeros; where one holds a NaN the scale and every q are NaN, and an infinity as its largest value
  * gives an infinite scale, NaN for the infinities and zeros for the rest.  Any strides from a row's length on; out may not overlap x.
  * Rows of up to 2^32 - 128 elements, up to 2^28 - 1 blocks of LILY_BLOCK elements of a row (block_rows 1), 2^24 - 1 of LILY_BLOCK x

@@ -857,7 +857,7 @@ __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at)
         if (slice == 0u && tid >= NT_DISTILL - 64u) {
             const double d = products_of_words(a, lane, words);
             l.mass = together<DISTILL_WAVES>(entropy[0]);
-                l.entropy = together<DISTILL_WAVES>(entropy[1]);
+            l.entropy = together<DISTILL_WAVES>(entropy[1]);
             if (lane == 0u) {
                 finish_row(a, row, r, l, d);
             }
@@ -866,7 +866,8 @@ __device__ __forceinline__ void distill_slice(const DistillArgs& a, uint32_t at)
     }
 }
 
-// (waves of a SIMD: held in f32 four workgroups a compute unit take 258 us where three, of 67 registers, take 268)
+// (waves of a SIMD: held in f32 four workgroups a compute unit take 258 us where three, of 67 registers, take 268.  Few rows in one launch have 104 to
+// 184 bytes of scratch a lane, the call's of words_of_slices and, of two turns, six registers spilled)
 template <uint32_t TURNS, bool BF16, int FORM>
 __global__ void __launch_bounds__(NT_DISTILL, TURNS > 4 ? 4 : FORM == FORM_HELD ? 8 : 6) k_distill(const DistillArgs a) {
     if constexpr (FORM != FORM_AFTER) {

@@ -7,7 +7,8 @@
 // block of 128 elements with a scale of its own is a row of 16 lanes: its largest value takes no memory and no barrier.
 //
 // Bound by memory: 8192 x 4096, bf16 rows, residual and sum, E4M3 blocks, 52 to 55 us (4.3 to 4.5 TB/s; the RMS norm to E4M3 rows the same on
-// the same chip).  4 rows 4.5 us, a launch, a trip to memory and two sums.
+// the same chip).  4 rows 4.5 us, a launch, a trip to memory and two sums.  Rows of more than 16 384 elements, four pieces a thread with all their
+// operands, spill 49 registers (74 where they are no multiple of 8 long).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -311,7 +312,8 @@ __global__ void __launch_bounds__(1024) k_layer_grad(const LayerGradArgs a) {
 // thread each, and keeps what its rows add to the gradients of weight and bias in registers; the next rows (in bf16 the next
 // two) are on their way while a row's two sums go through LDS.  So grad and h are read once: 16 384 x 4096 in bf16 with `past` 104 us
 // and 4 of joining 256 workgroups' parts (537 MB, 5.0 TB/s) against 161 by the two kernels below, which read them twice; 2049 x 2560 in
-// f32 17 + 4 against 43, of which the memory's are 11: eight rows a workgroup, each a trip to memory, two barriers and its stores.
+// f32 17 + 4 against 43, of which the memory's are 11: three turns of three rows a workgroup, each a barrier, its stores and, since f32 has
+// registers for one turn ahead, a trip to memory (120 to 126 of 128; of bf16's whole rows one is spilled).
 // Rows of 4001, 8000 of them in bf16 with `past`, 65 us (134 where the piece that a row ends in was read an element at a time).
 // Longer rows go by k_layer_grad_long or by those two, calls for one of the outputs alone by those two.
 enum LayerTypes { LAYER_F32, LAYER_BF16, LAYER_MIXED };   // of grad, h, past and grad_x
@@ -502,8 +504,9 @@ __global__ void __launch_bounds__(1024) k_layer_grad_all(const LayerGradArgs a, 
 
 // The same for rows of up to 16 384 elements: a row a workgroup, two pieces a thread, whose sums over the rows lie in LDS, 128 bytes a
 // thread.  `past` is asked for when its row's turn comes.  3068 x 10 336 in bf16 with `past` 81 us against 94.5 by the two kernels below,
-// 3000 x 12 345 115 against 132, 2000 x 16 384 in f32 114 against 145, with `past` 141 against 157.  Rows of f32 that are no multiple of 8 long, and
-// of mixed types, have no registers for it and go by those two: 2000 x 14 835 in f32 192 so, 155 by them; mixed 3451 x 14 835 324 and 227.
+// 3000 x 12 345 115 against 132, 2000 x 16 384 in f32 114 against 145, with `past` 141 against 157.  That is with 13 registers spilled in bf16 and 23 in
+// f32 (56 and 96 bytes a lane).  Rows of f32 that are no multiple of 8 long, and of mixed types, spill more than one reading saves and go by those
+// two: 2000 x 14 835 in f32 192 so, 155 by them; mixed 3451 x 14 835 324 and 227.
 constexpr uint32_t LONG_THREADS = 1024, LONG_PIECES = 2, LONG_LDS = LONG_THREADS * LONG_PIECES * 64;
 template <bool RAGGED, bool BF16>
 __global__ void __launch_bounds__(LONG_THREADS) k_layer_grad_long(const LayerGradArgs a) {

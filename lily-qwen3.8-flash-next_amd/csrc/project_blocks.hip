@@ -26,9 +26,10 @@ namespace {
 // stage is conditional, its loads beyond the last line are the last line's again: a branch in the middle of a stage made the compiler
 // move additions across it, 112 registers of sums waiting (312 bytes of scratch).
 //
-// 8192 x 12 288 x 4096 385 to 392 us, 2.1 PFLOP/s; the product with a scale a row, which has nothing to scale between two lines,
-// takes 349 on the same chip.  The matrix cores are busy 49% of its cycles (63% there): an addition's four multiplications stand
-// beside every product.  A third product between a sum and its addition, or waves of two priorities, change nothing (389 to 391).
+// 8192 x 12 288 x 4096 385 to 398 us by the chip, 2.1 PFLOP/s; the product with a scale a row, which has nothing to scale between two lines,
+// takes 349 on the same chip.  The matrix cores are busy 49% of its cycles (63% there), the vector unit with 96 000 instructions a SIMD about
+// as long: neither bounds it, they stand behind one another.  Both waves of a SIMD pass the same two barriers a stage, and so read, multiply and
+// add at much the same time.  A third product between a sum and its addition, or waves of two priorities, change nothing (389 to 391).
 template <class T>
 __global__ void __launch_bounds__(512, 2) k_blocks_large(const ProjectArgs a, uint32_t m_tiles, uint32_t n_tiles) {
     constexpr int S = 16, MB = 8, NB = 4, XL = 2, WL = 4;   // blocks of a wave; loads of a wave: half of the rows', all of the weights'
